@@ -99,7 +99,7 @@ int rh_memcpy_d2h(rh_context *ctx, void *host_dst, const void *dev_src, size_t b
  * 3 = attention, 4 = bf16 split of GEMM activations (weight-only int8 and
  * fp32 GEMMs on bf16 planes), 5 = full-int8 GEMM with the GELU +
  * QuantizeRowU8 row pass in its epilogue (the one-pass FFN1; ops count the
- * GEMM only). Reading syncs the stream. */
+ * GEMM only), 6 = e4m3 GEMM. Reading syncs the stream. */
 typedef struct {
   int64_t launches;
   double total_ms;    /* sum of per-launch event durations */
@@ -157,6 +157,9 @@ int rh_attention_planes(rh_context *ctx, const void *qkv_hi, const void *qkv_lo,
 #define RH_MODE_F32 0
 #define RH_MODE_W8 1
 #define RH_MODE_A8W8 2
+/* e4m3 weights, one power-of-two scale for each 128 x 128 block (below, "8-bit
+ * floating point"); no counterpart in the reference. */
+#define RH_MODE_FP8 3
 typedef struct rh_weight rh_weight;
 
 int rh_pack_weight(rh_context *ctx, int mode, const float *bT, const float *bias,
@@ -179,8 +182,9 @@ int rh_pack_weight_gated(rh_context *ctx, int mode, const float *gate, const flo
 /* Shape and mode of a packed weight. */
 int rh_weight_info(const rh_weight *w, int *mode, int *k, int *n);
 /* Host copies of the quantization results, for parity checks: q is
- * [n][k] row-major (RH_MODE_W8 / RH_MODE_A8W8), scales [n], colsum [n]
- * (RH_MODE_A8W8 only). Any output may be NULL. */
+ * [n][k] row-major (RH_MODE_W8 / RH_MODE_A8W8; RH_MODE_FP8: e4m3 codes),
+ * scales [n] (RH_MODE_FP8: [n][ceil(k/128)]), colsum [n] (RH_MODE_A8W8 only).
+ * Any output may be NULL. */
 int rh_weight_export(const rh_weight *w, int8_t *q, float *scales, int32_t *colsum);
 
 /* ---- activations and GEMMs (tensor level, dev pointers) ---------------------
@@ -225,7 +229,8 @@ int rh_gemm_u8s8_i32(rh_context *ctx, int32_t *acc, const uint8_t *qa, int ldq,
  * fused into the GEMM epilogue: dst = act(a·Wᵀ + bias). act: 0 none,
  * 1 erf-GELU (geluScalar, internal/tensor/tensor.go:508-538). For
  * RH_MODE_A8W8 the quantization scratch comes from qa/row_scales as in
- * rh_matmul_packed_vnni (both may be NULL for the other modes). */
+ * rh_matmul_packed_vnni (both may be NULL for the other modes; RH_MODE_FP8
+ * stages its e4m3 rows in the context's workspace). */
 #define RH_ACT_NONE 0
 #define RH_ACT_GELU 1
 #define RH_ACT_SWIGLU 2 /* silu(gate)*up, tensor.SiLU (tensor.go:477-481)       */
@@ -256,7 +261,8 @@ int rh_linear_u8(rh_context *ctx, const uint8_t *qa, int ldq, const float *row_s
  * the process ends, instead of caller scratch or a workspace it allocates.
  * It calls no hipMalloc/hipFree and times no launches. Sizes whose staging
  * exceeds the array (full int8: m*round_up(k,16) + 4m bytes; planes:
- * m*round_up(k,64)*2 bytes per plane) return RH_ERR_INVALID. Every call on
+ * m*round_up(k,64)*2 bytes per plane; e4m3: m*round_up(k,128) bytes and
+ * rh_fp8_scale_bytes) return RH_ERR_INVALID. Every call on
  * one GPU shares that GPU's array: calls that overlap on one GPU (from
  * different contexts or threads) race and must be ordered by the caller. */
 #define RH_NOALLOC_SCRATCH_BYTES (64u * 1024u * 1024u)
@@ -270,6 +276,116 @@ int rh_gelu(rh_context *ctx, float *x, size_t n);          /* tensor.go:508-538 
  * pointers; other shapes reduce across a wave (within float32 rounding). */
 int rh_layernorm(rh_context *ctx, float *x, const float *gamma,
                  const float *beta, int m, int n, float eps);
+
+/* ---- 8-bit floating point ------------------------------------------------------
+ * e4m3 values with power-of-two scales. A block of values is held as e4m3 codes
+ * times 2^(x - 127), x one byte: the smallest with which the block's largest
+ * magnitude is at most 448 (0 for anything below). Scaling by it is exact, so a
+ * code is the e4m3 value nearest to its input, ties to even. Blocks are 128 values
+ * of an activation row (the last one of a row may be shorter), 128 x 128 of a
+ * weight (gate and up each by blocks of their own), 64 tokens of one kv head of
+ * the cache below. No counterpart in the reference.
+ *
+ * None of these calls allocates or waits, and each may be captured into a HIP
+ * graph; buffers named scratch belong to the calls that share them, in stream
+ * order. Products of one 64-value step are summed by the matrix cores with 13 bits
+ * below the largest of them, steps in fp32: about 1.5e-5 of a result.
+ *
+ * The bytes sa of the scales of m rows of k values; block j of row r lies at byte
+ * ((j * ceil(m / 128) + r / 128) * 32 + r % 32) * 4 + r % 128 / 32. */
+size_t rh_fp8_scale_bytes(int m, int k);
+/* a: fp32 (a_bf16 0) or bf16 rows [m][lda] -> codes qa [m][ldq], ldq = k rounded up
+ * to 128 (zeros past k), and sa. Infinities and NaN set no scale and become NaN, and
+ * so does every output of their row. qa 16-byte, sa 4-byte aligned; lda and a's
+ * alignment are free (rows of 16-byte aligned groups of 8 are read faster). */
+int rh_quantize_rows_fp8(rh_context *ctx, const void *a, int a_bf16, int lda, int m, int k,
+                         uint8_t *qa, int ldq, uint8_t *sa);
+/* dst = act(rows . W^T + bias) of rows that are e4m3 already, to fp32 or bf16 rows
+ * [m][ldd] (ldd a multiple of 4; dst 16-byte, bf16 8-byte aligned). w is a
+ * RH_MODE_FP8 weight; a gated weight takes a gated act and writes n / 2 columns. */
+int rh_matmul_fp8(rh_context *ctx, void *dst, int dst_bf16, int ldd, const uint8_t *qa, int ldq,
+                  const uint8_t *sa, const rh_weight *w, int m, int act);
+/* Both: a's rows become e4m3 in the scratch qa [m][ldq] and sa (whose contents
+ * afterwards are unspecified), then rh_matmul_fp8. rh_linear does the same for fp32
+ * rows through the context's workspace. */
+int rh_linear_fp8(rh_context *ctx, void *dst, int dst_bf16, int ldd, const void *a, int a_bf16,
+                  int lda, const rh_weight *w, int m, int act, uint8_t *qa, int ldq, uint8_t *sa);
+
+/* ---- paged e4m3 key/value cache ---------------------------------------------------
+ * For decoder embedders whose texts share a beginning (an instruction before every
+ * query) or come in parts: keys and values of what has been seen stay in pages, and a
+ * forward runs only what is new. A page holds one block of RH_CACHE_BLOCK tokens for
+ * all kv heads. Texts may share whole pages: they list the same ones in their tables.
+ * All buffers are the caller's, on the context's device:
+ *   k, v          [pages][kv_heads][64 * dh] e4m3 codes, 16-byte aligned
+ *   k_exp, v_exp  [pages][kv_heads] scale bytes
+ * Inside a head's block, value d of token t lies at
+ *   k: ((d/64*2 + t/32)*2 + d%32/16)*1024 + (d%64/32*32 + t%32)*16 + d%16
+ *   v: (d/32*2 + t/32)*1024 + (t%8/4*32 + d%32)*16 + t%32/8*4 + t%4
+ * dh in {64, 128, 256}. Nothing needs to be cleared before its first use. */
+#define RH_CACHE_BLOCK 64
+typedef struct {
+  int pages;
+  int kv_heads;
+  int dh;
+  int reserved; /* zero */
+  uint8_t *k;
+  uint8_t *v;
+  uint8_t *k_exp;
+  uint8_t *v_exp;
+} rh_kv_cache;
+
+/* Tables and maps of a batch, from its lengths, on the device. Request b has past[b]
+ * tokens in the cache and fresh[b] new ones (either may be 0); its blocks are the
+ * pages table[b*ldt ..], of which the first ceil(past/64) are there. The others get
+ * pages from free_pages [n_free], in request order. Where past % 64 != 0 the last
+ * page is written on by rh_cache_append: it must not be shared. Outputs:
+ *   table   the new entries (the rest is left as it is)
+ *   cu      [batch+1] rows of the new tokens: request b owns cu[b] .. cu[b+1]-1
+ *   blocks  [batch+1] the same over the blocks that new tokens touch
+ *   lens    [batch] past + fresh (another buffer than past and fresh)
+ *   slots   [rows] page * 64 + position % 64 of each row, -1 behind the last one
+ *           and where the table's page is negative
+ *   pos     [rows] position of each row in its text (RoPE), 0 behind the last one
+ *   status  [4] 0, rows used, pages taken, blocks touched
+ * A plan that does not fit changes no table: status[0] is then a sum of 1 (a negative
+ * length), 2 (a text longer than ldt blocks), 4 (more than `rows` new tokens), 8
+ * (fewer free pages than needed), status[1..3], cu and blocks are 0, lens = past and
+ * every slot -1, so the calls below do nothing. All are device pointers. */
+int rh_cache_plan(rh_context *ctx, const int32_t *past, const int32_t *fresh, int batch,
+                  const int32_t *free_pages, int n_free, int32_t *table, int ldt, int32_t *cu,
+                  int32_t *blocks, int32_t *lens, int64_t *slots, int32_t *pos, int rows,
+                  int32_t *status);
+/* New K and V rows into their slots. kv holds fp32 (kv_bf16 0) or bf16 rows [rows][ldkv]
+ * with kv head h at columns k_off + h*dh and v_off + h*dh (ldkv and the offsets multiples
+ * of 8, kv 16-byte aligned); cu, blocks and slots are a plan's. A block that new tokens
+ * open is written whole, zeros behind them. In one that holds tokens already the scale
+ * becomes the larger of its own and the new tokens', and the codes kept are rescaled
+ * (exact but for values that fall below e4m3's normal range). A token with an infinity
+ * or NaN in a head's K or V is kept as K = NaN, V = 0 there: queries that see it get NaN,
+ * others are not touched. Rows whose slot is negative or behind the last page are
+ * skipped. */
+int rh_cache_append(rh_context *ctx, const rh_kv_cache *cache, const void *kv, int kv_bf16,
+                    int ldkv, int k_off, int v_off, const int32_t *cu, const int32_t *blocks,
+                    const int64_t *slots, int batch, int rows);
+/* rh_attention of the rows cu[b] .. cu[b+1]-1 over the cache: those are the last tokens of
+ * the lens[b] that request b has there (positions lens[b] - count ..), or, without causal
+ * and window, queries of any kind (attention to an encoder's states of another length).
+ * q head h starts at column q_off + h*dh of q [rows][ldq], fp32 (rounded to 8 significant
+ * bits here) or bf16, its kv head is h / (heads/kv_heads); causal and window as in
+ * rh_attention; scale > 0. P is held to 8 significant bits and the sums in fp32. out is fp32
+ * or bf16 [rows][ldout], head h at h*dh. A row that sees no key is 0; rows behind cu[batch]
+ * are left as they are. Table entries that are no page of the cache hold no keys. max_q
+ * must be >= every request's rows; max_len should be >= every lens (it only chooses how the
+ * work is split). ldq and q_off multiples of 8, ldout of 4, q 16-byte, out 16-byte (bf16:
+ * 8-byte) aligned; scratch: rh_cache_attention_scratch bytes, 16-byte aligned. */
+size_t rh_cache_attention_scratch(int batch, int max_q, int max_len, int heads, int kv_heads,
+                                  int dh);
+int rh_cache_attention(rh_context *ctx, const void *q, int q_bf16, int ldq, int q_off,
+                       const rh_kv_cache *cache, const int32_t *table, int ldt, const int32_t *cu,
+                       const int32_t *lens, int batch, int max_q, int max_len, int heads,
+                       float scale, int causal, int window, void *out, int out_bf16, int ldout,
+                       void *scratch, size_t scratch_bytes);
 
 /* ---- encoder model ------------------------------------------------------------
  * Replaces model.Load + Model.Forward/ForwardTokens + the Embed batch loop

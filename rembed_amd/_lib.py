@@ -22,7 +22,7 @@ RH_ERR_VOCAB = 7
 RH_ERR_SEQ = 8
 RH_ERR_MISSING = 9
 
-RH_MODE_F32, RH_MODE_W8, RH_MODE_A8W8 = 0, 1, 2
+RH_MODE_F32, RH_MODE_W8, RH_MODE_A8W8, RH_MODE_FP8 = 0, 1, 2, 3
 RH_QUANT_NONE, RH_QUANT_WEIGHTS, RH_QUANT_FULL = 0, 1, 2
 RH_POOL_MEAN, RH_POOL_CLS, RH_POOL_LAST = 0, 1, 2
 RH_ACT_NONE, RH_ACT_GELU, RH_ACT_SWIGLU, RH_ACT_GEGLU = 0, 1, 2, 3
@@ -41,6 +41,7 @@ RH_OPT_GRAPH = 9
 RH_CTX_F32_ALGO, RH_CTX_W8_TERMS, RH_CTX_I8_TILE, RH_CTX_BF_ALGO, RH_CTX_BF_TILE = 1, 2, 3, 4, 5
 RH_CTX_TILE_GROUP = 6
 RH_NOALLOC_SCRATCH_BYTES = 64 * 1024 * 1024
+RH_CACHE_BLOCK = 64
 
 # Symbols the header declares (checked by the CPU test suite).
 EXPORTS = [
@@ -53,7 +54,9 @@ EXPORTS = [
     "rh_quantize_rows_u8", "rh_gelu_quantize_rows_u8", "rh_matmul", "rh_matmul_packed", "rh_matmul_packed8",
     "rh_matmul_packed_vnni", "rh_gemm_u8s8_i32", "rh_linear", "rh_linear_u8",
     "rh_linear_noalloc", "rh_gelu",
-    "rh_layernorm", "rh_model_create", "rh_model_set_tensor",
+    "rh_layernorm", "rh_fp8_scale_bytes", "rh_quantize_rows_fp8", "rh_matmul_fp8",
+    "rh_linear_fp8", "rh_cache_plan", "rh_cache_append", "rh_cache_attention_scratch",
+    "rh_cache_attention", "rh_model_create", "rh_model_set_tensor",
     "rh_model_finalize", "rh_model_share", "rh_model_destroy", "rh_model_set_option",
     "rh_model_quantized", "rh_model_quantized_activations", "rh_model_embed",
     "rh_model_embed_tokens", "rh_model_embed_device", "rh_model_check",
@@ -85,6 +88,13 @@ class ModelConfig(ctypes.Structure):
         ("query_pre_attn_scalar", ctypes.c_int), ("dense_hidden", ctypes.c_int),
         ("rel_buckets", ctypes.c_int), ("reserved", ctypes.c_int * 7),
     ]
+
+
+class KVCacheDesc(ctypes.Structure):
+    """rh_kv_cache."""
+    _fields_ = [("pages", ctypes.c_int), ("kv_heads", ctypes.c_int), ("dh", ctypes.c_int),
+                ("reserved", ctypes.c_int), ("k", ctypes.c_void_p), ("v", ctypes.c_void_p),
+                ("k_exp", ctypes.c_void_p), ("v_exp", ctypes.c_void_p)]
 
 
 class ProfileStat(ctypes.Structure):
@@ -138,6 +148,15 @@ def _load():
         "rh_linear_noalloc": (I, [P, P, P, P, I, I]),
         "rh_gelu": (I, [P, P, S]),
         "rh_layernorm": (I, [P, P, P, P, I, I, F]),
+        "rh_fp8_scale_bytes": (S, [I, I]),
+        "rh_quantize_rows_fp8": (I, [P, P, I, I, I, I, P, I, P]),
+        "rh_matmul_fp8": (I, [P, P, I, I, P, I, P, P, I, I]),
+        "rh_linear_fp8": (I, [P, P, I, I, P, I, I, P, I, I, P, I, P]),
+        "rh_cache_plan": (I, [P, P, P, I, P, I, P, I, P, P, P, P, P, I, P]),
+        "rh_cache_append": (I, [P, ctypes.POINTER(KVCacheDesc), P, I, I, I, I, P, P, P, I, I]),
+        "rh_cache_attention_scratch": (S, [I, I, I, I, I, I]),
+        "rh_cache_attention": (I, [P, P, I, I, I, ctypes.POINTER(KVCacheDesc), P, I, P, P, I, I,
+                                   I, I, F, I, I, P, I, I, P, S]),
         "rh_model_create": (I, [P, ctypes.POINTER(ModelConfig), I, ctypes.POINTER(P)]),
         "rh_model_set_tensor": (I, [P, ctypes.c_char_p, P, P, I]),
         "rh_model_finalize": (I, [P]),

@@ -28,7 +28,8 @@ FLAGS = [
 # Per-file code generation: the attention kernels keep their MFMA
 # accumulators in VGPRs (no AGPR round trips for the online-softmax rescale,
 # two waves per SIMD at head dim 128).
-FILE_FLAGS = {"attention.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"]}
+FILE_FLAGS = {f: ["-mllvm", "-amdgpu-mfma-vgpr-form=1"]
+              for f in ("attention.hip", "cache_attention.hip")}
 
 
 def sources():

@@ -255,7 +255,7 @@ static int check_raw_shape(int k, int n) {
 }
 
 int pack_check(int mode, const float* bT, int k, int n, bool raw_ok) {
-  static const char* names[] = {"PackB", "PackB8", "PackB8VNNI"};
+  static const char* names[] = {"PackB", "PackB8", "PackB8VNNI", "PackFP8"};
   int st = raw_ok && mode == RH_MODE_F32 ? check_raw_shape(k, n)
                                          : check_pack_shape(names[mode], k, n);
   if (st != RH_OK || mode == RH_MODE_F32) return st;
@@ -271,10 +271,11 @@ int pack_check(int mode, const float* bT, int k, int n, bool raw_ok) {
 
 int pack_weight(Context* ctx, int mode, const float* bT, const float* bias, int k,
                 int n, rh_weight** out, bool raw_ok) {
-  static const char* names[] = {"PackB", "PackB8", "PackB8VNNI"};
+  static const char* names[] = {"PackB", "PackB8", "PackB8VNNI", "PackFP8"};
   int st = raw_ok && mode == RH_MODE_F32 ? check_raw_shape(k, n)
                                          : check_pack_shape(names[mode], k, n);
   if (st != RH_OK) return st;
+  if (mode == RH_MODE_FP8) return pack_weight_fp8(ctx, bT, bias, k, n, out);
   // owned here until the upload succeeds (a throw or a failed upload frees it)
   std::unique_ptr<rh_weight, void (*)(rh_weight*)> w(new rh_weight(), destroy_weight);
   w->ctx = ctx;
@@ -333,6 +334,7 @@ void destroy_weight(rh_weight* w) {
   if (w->d_bf) (void)hipFree(w->d_bf);
   if (w->d_bf_lo) (void)hipFree(w->d_bf_lo);
   if (w->d_frag) (void)hipFree(w->d_frag);
+  if (w->d_exp) (void)hipFree(w->d_exp);
   delete w;
 }
 
@@ -359,6 +361,7 @@ int pack_weight_gated(Context* ctx, int mode, const float* gate, const float* up
   int st0 = raw_ok && mode == RH_MODE_F32 ? check_raw_shape(k, i)
                                           : check_pack_shape("gated PackB", k, i);
   if (st0 != RH_OK) return st0;
+  if (mode == RH_MODE_FP8) return pack_weight_fp8_gated(ctx, gate, up, k, i, out);
   std::vector<float> inter((size_t)2 * i * k);
   for (int t = 0; t < i / kGluGroup; t++)
     for (int r = 0; r < kGluGroup; r++) {
@@ -456,7 +459,7 @@ int run_gemm_i8_ln(Context* ctx, const rh_weight* w, const uint8_t* qa, int ldq,
 // into the context workspace, then the planes GEMM. Rows go in chunks that
 // keep the kernel's 32-bit element offsets in range.
 bool linear_on_planes(const Context* ctx, const rh_weight* w) {
-  return w->mode != RH_MODE_A8W8 && ctx->bf_algo == 0 &&
+  return w->mode != RH_MODE_A8W8 && w->mode != RH_MODE_FP8 && ctx->bf_algo == 0 &&
          !(w->mode == RH_MODE_F32 && ctx->f32_algo == F32_NATIVE);
 }
 
@@ -604,6 +607,14 @@ int run_linear(Context* ctx, const rh_weight* w, const float* a, int lda, int m,
     return run_gemm_i8(ctx, w, qa, ldq, rs, m, EPI_F32, dst, ldc, act, bias, nullptr,
                        nullptr, ops);
   }
+  if (w->mode == RH_MODE_FP8 && !pin && !pout) {
+    const int ldq = (int)round_up(w->k, kFp8Block);
+    const size_t rows = round_up((size_t)m * ldq, 256);
+    hipError_t e = ctx->ensure_ws(rows + rh_fp8_scale_bytes(m, w->k));
+    if (e != hipSuccess) return hip_fail(e, "fp8 linear workspace", __FILE__, __LINE__);
+    uint8_t* codes = static_cast<uint8_t*>(ctx->ws);
+    return run_linear_fp8(ctx, w, a, 0, lda, m, dst, 0, ldc, act, bias, codes, ldq, codes + rows);
+  }
   if (linear_on_planes(ctx, w))
     return run_linear_planes(ctx, w, a, lda, m, dst, ldc, act, bias, pin, pout);
   if (pin || pout) return fail(RH_ERR_INVALID, "planes given to a linear that does not use them");
@@ -675,11 +686,6 @@ static void* scratch_addr(int device) {
 using namespace rh;
 
 // ---- C ABI ---------------------------------------------------------------------
-
-#define CTX_GUARD(ctx)                                               \
-  if (!(ctx)) return fail(RH_ERR_INVALID, "null context");           \
-  std::lock_guard<std::mutex> lk_((ctx)->mu);                         \
-  RH_HIP(hipSetDevice((ctx)->device))
 
 extern "C" {
 
@@ -934,7 +940,7 @@ int rh_pack_weight_gated(rh_context* ctx, int mode, const float* gate,
                                     const float* up, int k, int i, rh_weight** out) {
   return api_call([&]() -> int {
     if (!out || !gate || !up) return fail(RH_ERR_INVALID, "null argument");
-    if (mode < RH_MODE_F32 || mode > RH_MODE_A8W8) return fail(RH_ERR_INVALID, "unknown mode");
+    if (mode < RH_MODE_F32 || mode > RH_MODE_FP8) return fail(RH_ERR_INVALID, "unknown mode");
     CTX_GUARD(ctx);
     return pack_weight_gated(ctx, mode, gate, up, k, i, out);
   });
@@ -944,7 +950,7 @@ int rh_pack_weight(rh_context* ctx, int mode, const float* bT, const float* bias
                    int k, int n, rh_weight** out) {
   return api_call([&]() -> int {
     if (!out || !bT) return fail(RH_ERR_INVALID, "null argument");
-    if (mode < RH_MODE_F32 || mode > RH_MODE_A8W8) return fail(RH_ERR_INVALID, "unknown mode");
+    if (mode < RH_MODE_F32 || mode > RH_MODE_FP8) return fail(RH_ERR_INVALID, "unknown mode");
     CTX_GUARD(ctx);
     return pack_weight(ctx, mode, bT, bias, k, n, out);
   });
@@ -988,6 +994,7 @@ int rh_weight_export(const rh_weight* w, int8_t* q, float* scales, int32_t* cols
         memcpy(q + (size_t)j * w->k, img.data() + (size_t)j * w->kp, w->k);
     }
     if (scales) {
+      if (w->mode == RH_MODE_FP8) return export_fp8_scales(w, scales, colsum);
       if (!w->d_scales) return fail(RH_ERR_INVALID, "weight has no scales");
       RH_HIP(hipMemcpy(scales, w->d_scales, w->n * sizeof(float), hipMemcpyDeviceToHost));
     }
@@ -1042,8 +1049,8 @@ static int check_gemm(const rh_context* ctx, const rh_weight* w, int mode, const
   if (mode >= 0 && w->glu) return fail(RH_ERR_INVALID, "gated weight: use rh_linear with a gated act");
   if (m < 0) return fail(RH_ERR_INVALID, "negative m");
   if (m > 0 && (!a || !dst)) return fail(RH_ERR_INVALID, "null argument");
-  // the int8 epilogue writes 16-byte vectors
-  if (w->mode == RH_MODE_A8W8 && !aligned16(dst))
+  // the int8 and e4m3 epilogues write 16-byte vectors
+  if ((w->mode == RH_MODE_A8W8 || w->mode == RH_MODE_FP8) && !aligned16(dst))
     return fail(RH_ERR_INVALID, "output must be 16-byte aligned");
   return RH_OK;
 }
@@ -1216,6 +1223,8 @@ int rh_linear_u8(rh_context* ctx, const uint8_t* qa, int ldq, const float* row_s
 static size_t noalloc_bytes(const rh_context* ctx, const rh_weight* w, int m) {
   if (w->mode == RH_MODE_A8W8)
     return round_up((size_t)m * round_up(w->k, 16), 256) + (size_t)m * 4;
+  if (w->mode == RH_MODE_FP8)
+    return round_up((size_t)m * round_up(w->k, kFp8Block), 256) + rh_fp8_scale_bytes(m, w->k);
   if (linear_on_planes(ctx, w))
     return round_up((size_t)m * round_up(w->k, 64) * 2, 256) * linear_a_terms(ctx, w);
   return 0;
@@ -1254,6 +1263,11 @@ int rh_linear_noalloc(rh_context* ctx, float* dst, const float* a, const rh_weig
       uint8_t* qa = base;
       float* rs = reinterpret_cast<float*>(base + round_up((size_t)m * ldq, 256));
       return run_linear(ctx, w, a, w->k, m, dst, ldc, act, w->d_bias, qa, ldq, rs, true);
+    }
+    if (w->mode == RH_MODE_FP8) {
+      const int ldq = (int)round_up(w->k, kFp8Block);
+      return run_linear_fp8(ctx, w, a, 0, w->k, m, dst, 0, ldc, act, w->d_bias, base, ldq,
+                            base + round_up((size_t)m * ldq, 256));
     }
     if (linear_on_planes(ctx, w)) {
       const int ldk = (int)round_up(w->k, 64);

@@ -7,6 +7,12 @@
 
 #include "rh_internal.h"
 
+// Every call on a context holds its mutex and runs with its device current.
+#define CTX_GUARD(ctx)                                               \
+  if (!(ctx)) return fail(RH_ERR_INVALID, "null context");           \
+  std::lock_guard<std::mutex> lk_((ctx)->mu);                         \
+  RH_HIP(hipSetDevice((ctx)->device))
+
 // rh_context: one device, one stream (default priority), a mutex that
 // serializes the calls made on it, GEMM strategy switches, and the optional
 // per-launch event timing used by the benchmark.
@@ -69,6 +75,8 @@ struct rh_weight {
   // l's 16 bytes (column nb*32 + l%32, k bytes ks*32 + (l/32)*16 ..) at l*16,
   // so a wave's fragment is one coalesced 16-byte load per lane
   void* d_frag = nullptr;
+  // FP8: scale bytes of the packed rows (fp8_scale_at, np / 128 groups)
+  uint8_t* d_exp = nullptr;
 };
 
 namespace rh {
@@ -135,6 +143,19 @@ int run_gemm_i8(Context* ctx, const rh_weight* w, const uint8_t* qa, int ldq,
 // run_gemm_i8 with the residual + LayerNorm finish (launch_gemm_i8_ln).
 int run_gemm_i8_ln(Context* ctx, const rh_weight* w, const uint8_t* qa, int ldq,
                    const float* rs, int m, const I8LnArgs& f, double ops);
+// The FP8 mode (capi_fp8.cpp). The packers' shapes and values are checked by the
+// caller (pack_weight, pack_weight_gated).
+constexpr int kFp8Block = 128;
+int pack_weight_fp8(Context* ctx, const float* bT, const float* bias, int k, int n,
+                    rh_weight** out);
+int pack_weight_fp8_gated(Context* ctx, const float* gate, const float* up, int k, int i,
+                          rh_weight** out);
+int export_fp8_scales(const rh_weight* w, float* scales, int32_t* colsum);
+// a (fp32 or bf16 rows [m][lda]) to codes and scale bytes in qa [m][ldq] / sa, then
+// the GEMM to fp32 or bf16 rows [m][ldd]; a null: qa and sa hold the rows already.
+int run_linear_fp8(Context* ctx, const rh_weight* w, const void* a, int a_bf16, int lda, int m,
+                   void* dst, int dst_bf16, int ldd, int act, const float* bias, uint8_t* qa,
+                   int ldq, uint8_t* sa);
 // The capacity that a staging buffer of `have` bytes takes to hold `need`, never
 // past `most` unless `need` is: at least twice the old one, so that calls whose
 // outputs grow a little at a time do not each pin memory anew (59 calls of 8 texts,

@@ -118,11 +118,14 @@ class PackedWeight:
         self.ctx, self.h, self.mode, self.K, self.N = ctx, h, mode, k, n
 
     def export(self):
-        """Host copies: (q [n][k] int8 or None, scales [n] or None, colsum or None)."""
+        """Host copies: (q [n][k] int8 or None, scales [n] or None, colsum or None).
+        RH_MODE_FP8: q holds e4m3 codes, scales [n][ceil(k/128)]."""
         q = sc = cs = None
         if self.mode != _lib.RH_MODE_F32:
             q = np.empty((self.N, self.K), np.int8)
             sc = np.empty(self.N, np.float32)
+        if self.mode == _lib.RH_MODE_FP8:  # a scale for each row and 128 columns
+            sc = np.empty((self.N, (self.K + 127) // 128), np.float32)
         if self.mode == _lib.RH_MODE_A8W8:
             cs = np.empty(self.N, np.int32)
         check(lib.rh_weight_export(self.h, None if q is None else q.ctypes.data,
@@ -157,6 +160,12 @@ def PackB8(ctx, bT, k, n, bias=None):
 def PackB8VNNI(ctx, bT, k, n, bias=None):
     """internal/tensor/pack_vnni.go:28 — int8 weights for u8 x s8 GEMM."""
     return PackedWeight(ctx, _lib.RH_MODE_A8W8, bT, k, n, bias)
+
+
+def PackFP8(ctx, bT, k, n, bias=None):
+    """e4m3 weights, a power-of-two scale for each 128 x 128 block (no counterpart
+    in the reference)."""
+    return PackedWeight(ctx, _lib.RH_MODE_FP8, bT, k, n, bias)
 
 
 class PackedGated(PackedWeight):
@@ -251,6 +260,83 @@ def LinearU8(ctx, qa, ldq, row_scales, pb, m, act, qa_out, ldq_out, rs_out, absm
     """applyDense + QuantizeRowU8 of the output rows (rh_linear_u8)."""
     check(lib.rh_linear_u8(ctx.h, qa.ptr, ldq, row_scales.ptr, pb.h, m, act, qa_out.ptr,
                            ldq_out, rs_out.ptr, absmax.ptr))
+
+
+# ---- 8-bit floating point -------------------------------------------------------
+
+def _ptr(buf):
+    return None if buf is None else buf.ptr
+
+
+def ldq_fp8(k):
+    """Row stride of e4m3 activations: k rounded up to 128 bytes."""
+    return (k + 127) // 128 * 128
+
+
+def fp8_scale_bytes(m, k):
+    """Bytes of the scales of m e4m3 rows of k values (rh_fp8_scale_bytes)."""
+    return lib.rh_fp8_scale_bytes(m, k)
+
+
+def QuantizeRowsFP8(ctx, a, a_bf16, lda, m, k, qa, ldq, sa):
+    """fp32 or bf16 rows to e4m3 codes and scale bytes (rh_quantize_rows_fp8)."""
+    check(lib.rh_quantize_rows_fp8(ctx.h, a.ptr, int(a_bf16), lda, m, k, qa.ptr, ldq, sa.ptr))
+
+
+def MatMulFP8(ctx, dst, dst_bf16, ldd, qa, ldq, sa, pb, m, act=_lib.RH_ACT_NONE):
+    """act(rows . W^T + bias) of e4m3 rows (rh_matmul_fp8)."""
+    check(lib.rh_matmul_fp8(ctx.h, dst.ptr, int(dst_bf16), ldd, qa.ptr, ldq, sa.ptr, pb.h, m, act))
+
+
+def LinearFP8(ctx, dst, dst_bf16, ldd, a, a_bf16, lda, pb, m, act, qa, ldq, sa):
+    """applyDense (bert.go:282-301) on an e4m3 weight: fp32 or bf16 rows in, fp32 or bf16
+    rows out, the e4m3 rows staged in qa and sa (rh_linear_fp8)."""
+    check(lib.rh_linear_fp8(ctx.h, dst.ptr, int(dst_bf16), ldd, a.ptr, int(a_bf16), lda, pb.h, m,
+                            act, qa.ptr, ldq, sa.ptr))
+
+
+class KVCache:
+    """A paged e4m3 key/value cache (rh_kv_cache): pages of RH_CACHE_BLOCK tokens. Its
+    buffers are allocated here, or given (k, v, k_exp, v_exp with a .ptr)."""
+
+    def __init__(self, ctx, pages, kv_heads, dh, k=None, v=None, k_exp=None, v_exp=None):
+        codes = pages * kv_heads * _lib.RH_CACHE_BLOCK * dh
+        self.ctx, self.pages, self.kv_heads, self.dh = ctx, pages, kv_heads, dh
+        self.k = ctx.alloc(codes) if k is None else k
+        self.v = ctx.alloc(codes) if v is None else v
+        self.k_exp = ctx.alloc(pages * kv_heads) if k_exp is None else k_exp
+        self.v_exp = ctx.alloc(pages * kv_heads) if v_exp is None else v_exp
+        self.desc = _lib.KVCacheDesc(pages, kv_heads, dh, 0, self.k.ptr, self.v.ptr,
+                                     self.k_exp.ptr, self.v_exp.ptr)
+
+
+def CachePlan(ctx, past, fresh, batch, free_pages, n_free, table, ldt, cu, blocks, lens, slots,
+              pos, rows, status):
+    """Block table, slot map, row and block offsets of a batch (rh_cache_plan)."""
+    check(lib.rh_cache_plan(ctx.h, past.ptr, fresh.ptr, batch, _ptr(free_pages), n_free,
+                            table.ptr, ldt, cu.ptr, blocks.ptr, lens.ptr, _ptr(slots), _ptr(pos),
+                            rows, status.ptr))
+
+
+def CacheAppend(ctx, cache, kv, kv_bf16, ldkv, k_off, v_off, cu, blocks, slots, batch, rows):
+    """New K and V rows into the cache (rh_cache_append)."""
+    check(lib.rh_cache_append(ctx.h, cache.desc, kv.ptr, int(kv_bf16), ldkv, k_off, v_off, cu.ptr,
+                              blocks.ptr, slots.ptr, batch, rows))
+
+
+def cache_attention_scratch(batch, max_q, max_len, heads, kv_heads, dh):
+    """Scratch bytes of CacheAttention (rh_cache_attention_scratch)."""
+    return lib.rh_cache_attention_scratch(batch, max_q, max_len, heads, kv_heads, dh)
+
+
+def CacheAttention(ctx, out, out_bf16, ldout, q, q_bf16, ldq, q_off, cache, table, ldt, cu, lens,
+                   batch, max_q, max_len, heads, scale, causal=True, window=0, scratch=None,
+                   scratch_bytes=0):
+    """Attention of new rows over the cache (rh_cache_attention)."""
+    check(lib.rh_cache_attention(ctx.h, q.ptr, int(q_bf16), ldq, q_off, cache.desc, table.ptr,
+                                 ldt, cu.ptr, lens.ptr, batch, max_q, max_len, heads,
+                                 float(scale), int(causal), window, out.ptr, int(out_bf16), ldout,
+                                 _ptr(scratch), scratch_bytes))
 
 
 # ---- host-array conveniences used by tests and the bench -----------------------

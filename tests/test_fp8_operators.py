@@ -1,0 +1,845 @@
+"""e4m3 linears, block tables, the paged e4m3 cache and attention over it, against numpy in
+64 bits (fp8_oracle).
+
+Tolerances. A rounding is off by at most half a step: bf16 2^-8 of the value, e4m3 2^-4; codes,
+scale bytes and whole numbers are equal. The matrix cores add the products of one 64-value
+step with 13 bits below the largest of them, so a step is off by at most 64 * 2^-13 = 2^-7
+of its largest product; on normal values, where those errors are independent and a step's
+largest product is about 4.5 standard deviations, 2^-13 * 4.5 / sqrt(12) = 1.6e-4 of the
+result's norm.
+"""
+import ctypes
+
+import numpy as np
+import pytest
+
+import fp8_oracle as O
+
+STEP = 2.0 ** -7
+NORM = 2.0 ** -13 * 4.5 / 12 ** 0.5
+BF16 = 2.0 ** -8
+
+
+def bf16(x):
+    """float32 values rounded to bf16 (nearest even), and their bits."""
+    u = np.ascontiguousarray(x, np.float32).view(np.uint32).astype(np.uint64)
+    r = (u + 0x7FFF + (u >> 16 & 1)) >> 16
+    r = np.where((u & 0x7FFFFFFF) > 0x7F800000, u >> 16 | 64, r).astype(np.uint16)
+    return (r.astype(np.uint32) << 16).view(np.float32), r
+
+
+def from_bf16(bits):
+    return (bits.astype(np.uint32) << 16).view(np.float32)
+
+
+def typed(x, dtype):
+    """The device image of x and the values it holds."""
+    if dtype == "bf16":
+        v, bits = bf16(x)
+        return bits, v
+    x = np.ascontiguousarray(x, np.float32)
+    return x, x
+
+
+# ---- CPU: the oracle, the refusals ----------------------------------------------------
+
+def test_oracle_codes_are_torch_codes():
+    torch = pytest.importorskip("torch")
+    rng = np.random.default_rng(0)
+    x = np.concatenate([rng.uniform(-448, 448, 4096), rng.standard_normal(4096),
+                        rng.standard_normal(4096) * 0.01, O.CODES[:127], -O.CODES[:127],
+                        (O.CODES[:126] + O.CODES[1:127]) / 2]).astype(np.float32)
+    want = torch.from_numpy(x).to(torch.float8_e4m3fn).view(torch.uint8).numpy()
+    assert np.array_equal(O.encode(x), want)
+
+
+def test_oracle_exponents_are_the_smallest():
+    rng = np.random.default_rng(1)
+    top = np.concatenate([rng.uniform(0, 1e4, 999), 2.0 ** rng.uniform(-100, 100, 999),
+                          448 * 2.0 ** np.arange(-20, 20), 449 * 2.0 ** np.arange(-20, 20)])
+    e = O.exponent(top)
+    assert (top <= 448 * O.two(e)).all() and (top > 448 * O.two(e - 1)).all()
+    assert O.exponent(np.array([0.0, 2.0 ** -149]))[0] == 0
+
+
+def test_oracle_layouts_are_permutations():
+    for dh in (64, 128, 256):
+        for at in (O.k_at, O.v_at):
+            assert np.array_equal(np.sort(O.places(at, dh).ravel()), np.arange(64 * dh))
+
+
+P = ctypes.c_void_p(4096)  # a pointer that no refused call may follow
+
+
+def refused(code, fn, *args):
+    from rembed_amd import _lib
+    assert getattr(_lib.lib, fn)(*args) == code, _lib.lib.rh_last_error()
+    assert _lib.lib.rh_last_error()
+
+
+def test_quantize_refusals():
+    from rembed_amd import _lib as L
+    ok = [None, P, 0, 256, 4, 256, P, 256, P]
+
+    def no(code, **kw):
+        a = list(ok)
+        for i, v in kw.items():
+            a[int(i[1:])] = v
+        refused(code, "rh_quantize_rows_fp8", *a)
+
+    no(L.RH_ERR_INVALID)                      # no context
+    no(L.RH_ERR_INVALID, a4=-1)
+    no(L.RH_ERR_INVALID, a5=0)
+    no(L.RH_ERR_SHAPE, a3=255)                # rows overlap
+    no(L.RH_ERR_SHAPE, a7=128)
+    no(L.RH_ERR_SHAPE, a5=257, a3=300)        # ldq is not k rounded up
+    no(L.RH_ERR_INVALID, a1=None)
+    no(L.RH_ERR_INVALID, a6=None)
+    no(L.RH_ERR_INVALID, a8=None)
+    no(L.RH_ERR_INVALID, a6=ctypes.c_void_p(4104))
+    no(L.RH_ERR_INVALID, a8=ctypes.c_void_p(4098))
+    no(L.RH_ERR_INVALID, a1=ctypes.c_void_p(4098))
+    assert L.lib.rh_fp8_scale_bytes(1, 1) == 128
+    assert L.lib.rh_fp8_scale_bytes(129, 257) == 256 * 3
+    assert L.lib.rh_fp8_scale_bytes(0, 5) == 0 == L.lib.rh_fp8_scale_bytes(5, -1)
+
+
+def test_linear_refusals_without_a_weight():
+    from rembed_amd import _lib as L
+    refused(L.RH_ERR_INVALID, "rh_matmul_fp8", None, P, 0, 16, P, 128, P, None, 1, 0)
+    refused(L.RH_ERR_INVALID, "rh_linear_fp8", None, P, 0, 16, P, 0, 16, None, 1, 0, P, 128, P)
+
+
+def test_plan_refusals():
+    from rembed_amd import _lib as L
+    Q = ctypes.c_void_p(8192)
+    ok = [None, P, P, 3, P, 5, P, 4, Q, Q, Q, Q, Q, 10, Q]
+
+    def no(code, **kw):
+        a = list(ok)
+        for i, v in kw.items():
+            a[int(i[1:])] = v
+        refused(code, "rh_cache_plan", *a)
+
+    no(L.RH_ERR_INVALID)
+    for i in ("a3", "a5", "a13"):
+        no(L.RH_ERR_INVALID, **{i: -1})
+    no(L.RH_ERR_SHAPE, a7=0)
+    for i in (1, 2, 4, 6, 8, 9, 10, 11, 12, 14):
+        no(L.RH_ERR_INVALID, **{"a%d" % i: None})
+    no(L.RH_ERR_INVALID, a10=P)               # lens is past
+    no(L.RH_ERR_INVALID, a11=ctypes.c_void_p(8196))
+
+
+def desc(pages=4, heads=2, dh=64, k=4096, v=4096, ke=4096, ve=4096):
+    from rembed_amd import _lib as L
+    return L.KVCacheDesc(pages, heads, dh, 0, k, v, ke, ve)
+
+
+def test_append_refusals():
+    from rembed_amd import _lib as L
+    ok = [None, desc(), P, 1, 256, 0, 128, P, P, P, 2, 9]
+
+    def no(code, **kw):
+        a = list(ok)
+        for i, v in kw.items():
+            a[int(i[1:])] = v
+        refused(code, "rh_cache_append", *a)
+
+    no(L.RH_ERR_INVALID)
+    no(L.RH_ERR_INVALID, a1=None)
+    for d in (32, 96, 512):
+        no(L.RH_ERR_SHAPE, a1=desc(dh=d))
+    no(L.RH_ERR_SHAPE, a1=desc(heads=0))
+    no(L.RH_ERR_SHAPE, a1=desc(pages=-1))
+    no(L.RH_ERR_INVALID, a1=desc(k=None))
+    no(L.RH_ERR_INVALID, a1=desc(ve=None))
+    no(L.RH_ERR_INVALID, a1=desc(v=4104))
+    no(L.RH_ERR_INVALID, a10=-1)
+    no(L.RH_ERR_INVALID, a11=-1)
+    for i in (2, 7, 8, 9):
+        no(L.RH_ERR_INVALID, **{"a%d" % i: None})
+    no(L.RH_ERR_SHAPE, a4=248)                # V's columns leave the row
+    no(L.RH_ERR_SHAPE, a5=4)
+    no(L.RH_ERR_SHAPE, a6=-8)
+    no(L.RH_ERR_SHAPE, a2=ctypes.c_void_p(4104))
+    no(L.RH_ERR_SHAPE, a1=desc(heads=4), a4=1024, a6=256, a10=2 ** 31 - 1, a11=2 ** 31 - 1)
+
+
+def test_attention_refusals():
+    from rembed_amd import _lib as L
+    ok = [None, P, 1, 256, 0, desc(), P, 4, P, P, 2, 5, 200, 4, 0.125, 1, 0, P, 1, 256, P, 1 << 20]
+
+    def no(code, **kw):
+        a = list(ok)
+        for i, v in kw.items():
+            a[int(i[1:])] = v
+        refused(code, "rh_cache_attention", *a)
+
+    no(L.RH_ERR_INVALID)
+    no(L.RH_ERR_SHAPE, a5=desc(dh=32))
+    for i in ("a10", "a11", "a12", "a16"):
+        no(L.RH_ERR_INVALID, **{i: -1})
+    for heads in (0, 3):
+        no(L.RH_ERR_SHAPE, a13=heads)
+    for s in (0.0, -1.0, float("inf"), float("nan")):
+        no(L.RH_ERR_INVALID, a14=s)
+    for t in (0, 2 ** 31 // 64):
+        no(L.RH_ERR_SHAPE, a7=t)
+    no(L.RH_ERR_SHAPE, a3=248)
+    no(L.RH_ERR_SHAPE, a4=8)
+    no(L.RH_ERR_SHAPE, a19=252)
+    no(L.RH_ERR_SHAPE, a19=258)
+    no(L.RH_ERR_SHAPE, a1=ctypes.c_void_p(4104))
+    no(L.RH_ERR_SHAPE, a17=ctypes.c_void_p(4100))
+    for i in (1, 6, 8, 9, 17):
+        no(L.RH_ERR_INVALID, **{"a%d" % i: None})
+    no(L.RH_ERR_SHAPE, a10=2 ** 31 - 1, a11=1 << 20)
+    assert L.lib.rh_cache_attention_scratch(1, 1, 65536, 4, 2, 64) > 0
+    no(L.RH_ERR_INVALID, a10=1, a11=1, a12=65536, a21=16)
+    no(L.RH_ERR_INVALID, a10=1, a11=1, a12=65536, a20=None)
+    for bad in ((0, 1, 1, 4, 2, 64), (1, 0, 1, 4, 2, 64), (1, 1, 1, 3, 2, 64), (1, 1, 1, 4, 0, 64)):
+        assert L.lib.rh_cache_attention_scratch(*bad) == 0
+
+
+# ---- GPU: e4m3 rows, weights, linears ---------------------------------------------------
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("m,k,lda", [(1, 1, 1), (1, 128, 128), (3, 127, 127), (2, 129, 136),
+                                     (130, 256, 260), (257, 1000, 1000), (5, 2570, 2571)])
+def test_quantize_rows(gpu_ctx, m, k, lda, dtype):
+    from rembed_amd import tensor as T
+    rng = np.random.default_rng(m * 1000 + k)
+    x = rng.standard_normal((m, lda)) * np.exp(rng.uniform(-8, 8, (m, 1)))
+    x[0, : k // 2] = 0.0                      # a block of zeros, or half of one
+    if m > 2:
+        x[1] *= 2.0 ** -130 if dtype == "f32" else 2.0 ** -120
+        x[2, 0] = 3.0e38
+    img, val = typed(x, dtype)
+    ldq = T.ldq_fp8(k)
+    d, qa = gpu_ctx.upload(img), gpu_ctx.upload(np.full((m, ldq), 0xAA, np.uint8))
+    sa = gpu_ctx.alloc(T.fp8_scale_bytes(m, k))
+    T.QuantizeRowsFP8(gpu_ctx, d, dtype == "bf16", lda, m, k, qa, ldq, sa)
+    codes, e, _ = O.quantize_rows(val[:, :k].astype(np.float64))
+    got = qa.download(np.uint8, (m, ldq))
+    kb = ldq // 128
+    assert np.array_equal(O.scale_rows(sa.download(np.uint8, (T.fp8_scale_bytes(m, k),)), m, kb), e)
+    # a zero's sign carries nothing
+    same = (got == codes) | ((got & 127 == 0) & (codes & 127 == 0))
+    assert same.all()
+
+
+@pytest.mark.gpu
+def test_quantize_rows_that_are_no_numbers(gpu_ctx):
+    from rembed_amd import tensor as T
+    x = np.random.default_rng(3).standard_normal((4, 300)).astype(np.float32)
+    x[0, 7], x[1, 130], x[2, 299] = np.nan, np.inf, -np.inf
+    qa, sa = gpu_ctx.alloc(4 * 384), gpu_ctx.alloc(T.fp8_scale_bytes(4, 300))
+    T.QuantizeRowsFP8(gpu_ctx, gpu_ctx.upload(x), False, 300, 4, 300, qa, 384, sa)
+    codes, e, _ = O.quantize_rows(x.astype(np.float64))
+    got = qa.download(np.uint8, (4, 384))
+    assert np.array_equal(np.isnan(O.CODES[got]), np.isnan(O.CODES[codes]))
+    ok = ~np.isnan(O.CODES[codes])
+    assert np.array_equal(O.CODES[got][ok], O.CODES[codes][ok])
+    assert np.array_equal(O.scale_rows(sa.download(np.uint8, (128 * 3,)), 4, 3), e)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("k,n", [(1, 16), (128, 128), (300, 272), (1000, 144)])
+def test_pack_fp8(gpu_ctx, k, n):
+    from rembed_amd import tensor as T
+    from rembed_amd import _lib
+    rng = np.random.default_rng(k + n)
+    w = (rng.standard_normal((n, k)) * np.exp(rng.uniform(-6, 6, (n, 1)))).astype(np.float32)
+    w[: n // 2, : k // 3] = 0
+    q, sc, cs = T.PackFP8(gpu_ctx, w, k, n).export()
+    codes, e, _ = O.quantize_weight(w.astype(np.float64))
+    assert cs is None and np.array_equal(sc, O.two(e).astype(np.float32))
+    assert np.array_equal(O.CODES[q.view(np.uint8)], O.CODES[codes])
+    gate = T.PackedGated(gpu_ctx, _lib.RH_MODE_FP8, w, w[::-1] * 3, k, n)
+    q, sc, _ = gate.export()
+    for half, x in enumerate((w, w[::-1] * 3)):
+        codes, e, _ = O.quantize_weight(x.astype(np.float64))
+        rows = (np.arange(n) // 4) * 8 + half * 4 + np.arange(n) % 4
+        assert np.array_equal(O.CODES[q.view(np.uint8)[rows]], O.CODES[codes])
+        assert np.array_equal(sc[rows], O.two(e).astype(np.float32))
+
+
+@pytest.mark.gpu
+def test_pack_fp8_refusals(gpu_ctx):
+    from rembed_amd import tensor as T
+    from rembed_amd import _lib as L
+    w = np.ones((32, 8), np.float32)
+    for bad, code in ((np.nan, L.RH_ERR_NONFINITE), (np.inf, L.RH_ERR_NONFINITE)):
+        x = w.copy()
+        x[31, 7] = bad
+        with pytest.raises(L.RembedError) as e:
+            T.PackFP8(gpu_ctx, x, 8, 32)
+        assert e.value.code == code
+    with pytest.raises(L.RembedError) as e:
+        T.PackFP8(gpu_ctx, w[:24], 8, 24)
+    assert e.value.code == L.RH_ERR_SHAPE
+    pb, gate = T.PackFP8(gpu_ctx, w, 8, 32), T.PackedGated(gpu_ctx, 3, w, w, 8, 32)
+    other = T.PackB8(gpu_ctx, w, 8, 32)
+    buf = gpu_ctx.alloc(1 << 16)
+    with T.Context(0) as ctx2:
+        for args, code in (((pb, 1, 0, 16, 128, 32), None), ((pb, 1, 2, 16, 128, 32), 2),
+                           ((gate, 1, 0, 16, 128, 32), 2), ((pb, -1, 0, 16, 128, 32), 2),
+                           ((pb, 1, 9, 16, 128, 32), 2), ((pb, 1, 0, 7, 128, 32), 3),
+                           ((pb, 1, 0, 16, 256, 32), 3), ((pb, 1, 0, 16, 128, 28), 3),
+                           ((pb, 1, 0, 16, 128, 34), 3), ((other, 1, 0, 16, 128, 32), 2)):
+            w_, m, act, lda, ldq, ldd = args
+            call = lambda c: T.LinearFP8(c, buf, False, ldd, buf, False, lda, w_, m, act, buf,
+                                         ldq, buf)
+            if code is None:
+                with pytest.raises(L.RembedError) as e:  # another context's weight
+                    call(ctx2)
+                assert e.value.code == L.RH_ERR_INVALID
+            else:
+                with pytest.raises(L.RembedError) as e:
+                    call(gpu_ctx)
+                assert e.value.code == code, args
+    with pytest.raises(L.RembedError):
+        T.GemmU8S8I32(gpu_ctx, buf, buf, 16, pb, 1)
+
+
+def act_of(y, act):
+    from math import erf
+    if act == 1:
+        return 0.5 * y * (1 + np.vectorize(erf)(y / 2 ** 0.5))
+    return y
+
+
+def gated(g, u, act):
+    from math import erf
+    if act == 2:
+        return g / (1 + np.exp(-g)) * u
+    if act == 3:
+        t = (2 / np.pi) ** 0.5 * (g + 0.044715 * g ** 3)
+        return 0.5 * g * (1 + np.tanh(t)) * u
+    return 0.5 * g * (1 + np.vectorize(erf)(g / 2 ** 0.5)) * u
+
+
+def run_linear(ctx, pb, img, a_bf16, m, k, n_out, act, out_bf16, ldd=None, lda=None):
+    from rembed_amd import tensor as T
+    ldd, lda = ldd or n_out, lda or k
+    ldq = T.ldq_fp8(k)
+    dst = ctx.upload(np.full((max(m, 1), ldd), 0x5A5A, np.uint16) if out_bf16
+                     else np.full((max(m, 1), ldd), 77, np.float32))
+    d = ctx.upload(img)
+    qa, sa = ctx.alloc(m * ldq), ctx.alloc(T.fp8_scale_bytes(m, k))
+    T.LinearFP8(ctx, dst, out_bf16, ldd, d, a_bf16, lda, pb, m, act, qa, ldq, sa)
+    ctx.sync()
+    if out_bf16:
+        bits = dst.download(np.uint16, (m, ldd))
+        assert (bits[:, n_out:] == 0x5A5A).all()
+        return from_bf16(bits[:, :n_out])
+    out = dst.download(np.float32, (m, ldd))
+    assert (out[:, n_out:] == 77).all()
+    return out[:, :n_out]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m,k,n", [(1, 1, 16), (1, 128, 16), (1, 1024, 272), (2, 300, 128),
+                                   (5, 96, 48), (15, 1000, 144), (16, 2048, 128), (17, 640, 256),
+                                   (33, 129, 400), (64, 512, 384), (100, 4000, 160),
+                                   (129, 384, 512), (300, 250, 272), (513, 1280, 768)])
+def test_linear_fp8(gpu_ctx, m, k, n):
+    from rembed_amd import tensor as T
+    rng = np.random.default_rng(m + k + n)
+    x = rng.standard_normal((m, k)) * np.exp(0.5 * rng.standard_normal(k))
+    w = (rng.standard_normal((n, k)) / k ** 0.5).astype(np.float32)
+    b = rng.standard_normal(n).astype(np.float32)
+    _, _, wv = O.quantize_weight(w.astype(np.float64))
+    for dtype, bias, act, out_bf16, pad in (("f32", None, 0, False, 0), ("bf16", b, 0, True, 8),
+                                            ("bf16", None, 1, False, 4), ("f32", b, 1, True, 0)):
+        img, val = typed(x, dtype)
+        _, _, xv = O.quantize_rows(val.astype(np.float64))
+        y = xv @ wv.T
+        # what the matrix cores may drop: a share of each step's largest product
+        drop = np.zeros((m, n))
+        if m * n * k <= 20_000_000:
+            for s in range(0, k, 64):
+                drop += STEP * (np.abs(xv[:, None, s:s + 64]) * np.abs(wv[None, :, s:s + 64])).max(2)
+        else:
+            for s in range(0, k, 64):
+                drop += STEP * np.outer(np.abs(xv[:, s:s + 64]).max(1), np.abs(wv[:, s:s + 64]).max(1))
+        z = y + (0 if bias is None else bias.astype(np.float64))
+        want = act_of(z, act)
+        pb = T.PackFP8(gpu_ctx, w, k, n, bias)
+        got = run_linear(gpu_ctx, pb, img, dtype == "bf16", m, k, n, act, out_bf16, n + pad)
+        # GELU's slope is at most 1.13; fp32 sums of the steps and the activation: 2^-18
+        tol = 1.13 * drop + 2.0 ** -18 * (np.abs(want) + np.abs(xv) @ np.abs(wv).T) + 1e-30
+        tol += (BF16 if out_bf16 else 0) * (np.abs(want) + 1.13 * drop)
+        assert (np.abs(got - want) <= tol).all()
+        norm = np.linalg.norm(got - want) / np.linalg.norm(want)
+        assert norm <= (BF16 if out_bf16 else 0) + 1.13 * NORM * max(
+            1.0, np.linalg.norm(y) / np.linalg.norm(want)), (dtype, act, norm)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("act", [2, 3, 4])
+@pytest.mark.parametrize("m,k,i", [(1, 256, 16), (4, 1000, 80), (31, 130, 144), (70, 512, 128),
+                                   (260, 300, 272)])
+def test_gated_linear_fp8(gpu_ctx, m, k, i, act):
+    from rembed_amd import tensor as T
+    rng = np.random.default_rng(m * 7 + k + act)
+    x = rng.standard_normal((m, k))
+    g, u = (rng.standard_normal((i, k)) / k ** 0.5).astype(np.float32), \
+        (rng.standard_normal((i, k)) * 3 / k ** 0.5).astype(np.float32)
+    pb = T.PackedGated(gpu_ctx, 3, g, u, k, i)
+    _, _, gv = O.quantize_weight(g.astype(np.float64))
+    _, _, uv = O.quantize_weight(u.astype(np.float64))
+    for dtype, out_bf16 in (("f32", False), ("bf16", True)):
+        img, val = typed(x, dtype)
+        _, _, xv = O.quantize_rows(val.astype(np.float64))
+        want = gated(xv @ gv.T, xv @ uv.T, act)
+        got = run_linear(gpu_ctx, pb, img, dtype == "bf16", m, k, i, act, out_bf16, i + 4)
+        # both factors are off by NORM of theirs (the gate through a slope of 1.13 at
+        # most), the product by the sum
+        norm = np.linalg.norm(got - want) / np.linalg.norm(want)
+        assert norm <= (BF16 if out_bf16 else 0) + 3 * NORM, (dtype, norm)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m", [1, 3, 16, 40, 130])
+def test_linear_forms_agree(gpu_ctx, m):
+    """Whole call, quantize and multiply apart, rh_linear and its form without allocation: the
+    same bits; and a row's bits do not depend on the rows beside it."""
+    from rembed_amd import tensor as T
+    k, n = 700, 272
+    rng = np.random.default_rng(m)
+    x = rng.standard_normal((m, k)).astype(np.float32)
+    pb = T.PackFP8(gpu_ctx, rng.standard_normal((n, k)).astype(np.float32), k, n,
+                   rng.standard_normal(n).astype(np.float32))
+    got = run_linear(gpu_ctx, pb, x, False, m, k, n, 1, False)
+    ldq = T.ldq_fp8(k)
+    d, dst = gpu_ctx.upload(x), gpu_ctx.alloc(m * n * 4)
+    qa, sa = gpu_ctx.alloc(m * ldq), gpu_ctx.alloc(T.fp8_scale_bytes(m, k))
+    T.QuantizeRowsFP8(gpu_ctx, d, False, k, m, k, qa, ldq, sa)
+    T.MatMulFP8(gpu_ctx, dst, False, n, qa, ldq, sa, pb, m, 1)
+    assert np.array_equal(dst.download(np.float32, (m, n)), got)
+    T.Linear(gpu_ctx, dst, d, pb, m, 1)
+    assert np.array_equal(dst.download(np.float32, (m, n)), got)
+    T.LinearNoAlloc(gpu_ctx, dst, d, pb, m, 1)
+    assert np.array_equal(dst.download(np.float32, (m, n)), got)
+    T.LinearFP8(gpu_ctx, dst, False, n, d, False, k, pb, 0, 1, qa, ldq, sa)  # no rows
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m", [1, 7, 40, 200])
+def test_linear_rows_that_are_no_numbers(gpu_ctx, m):
+    from rembed_amd import tensor as T
+    k, n = 400, 144
+    rng = np.random.default_rng(m)
+    x = rng.standard_normal((m, k)).astype(np.float32)
+    pb = T.PackFP8(gpu_ctx, rng.standard_normal((n, k)).astype(np.float32), k, n)
+    ok = run_linear(gpu_ctx, pb, x, False, m, k, n, 0, False)
+    bad = {0: np.nan, m // 2: np.inf, m - 1: -np.inf}
+    for r, v in bad.items():
+        x[r, (r * 37) % k] = v
+    got = run_linear(gpu_ctx, pb, x, False, m, k, n, 0, False)
+    for r in range(m):
+        if r in bad:
+            assert np.isnan(got[r]).all()
+        else:
+            assert np.array_equal(got[r], ok[r])
+
+
+# ---- GPU: block tables --------------------------------------------------------------
+
+def run_plan(ctx, past, fresh, free, table, rows):
+    from rembed_amd import tensor as T
+    n = len(past)
+    i32 = np.int32
+    out = [ctx.upload(np.full(s, 123456, t)) for s, t in
+           ((n + 1, i32), (n + 1, i32), (max(n, 1), i32), (max(rows, 1), np.int64),
+            (max(rows, 1), i32), (4, i32))]
+    dt = ctx.upload(table)
+    df = ctx.upload(np.array(free if len(free) else [0], i32))
+    T.CachePlan(ctx, ctx.upload(np.array(past if n else [0], i32)),
+                ctx.upload(np.array(fresh if n else [0], i32)), n, df, len(free), dt,
+                table.shape[1], *out[:5], rows, out[5])
+    ctx.sync()
+    got = [o.download(t, (s,)) for o, s, t in zip(out, (n + 1, n + 1, n, rows, rows, 4),
+                                                  (i32, i32, i32, np.int64, i32, i32))]
+    return got, dt.download(i32, table.shape)
+
+
+def check_plan(ctx, past, fresh, spare=0, ldt=None, rows=None, short=0, seed=0):
+    rng = np.random.default_rng(seed)
+    n = len(past)
+    blocks = [max(0, -(-(max(p, 0) + max(f, 0)) // 64)) for p, f in zip(past, fresh)]
+    ldt = ldt if ldt is not None else max(blocks + [1]) + 1
+    need = sum(b + -max(p, 0) // 64 for b, p in zip(blocks, past))
+    free = rng.permutation(10_000_000)[: max(0, need + spare - short)] if need + spare < 10_000_000 else []
+    table = rng.integers(0, 1 << 24, (max(n, 1), ldt)).astype(np.int32)
+    rows = rows if rows is not None else sum(max(f, 0) for f in fresh) + spare
+    want_t = table.copy()
+    want = O.plan(past, fresh, free, want_t, rows)
+    got, got_t = run_plan(ctx, past, fresh, free, table, rows)
+    for name, w, g in zip(("cu", "blocks", "lens", "slots", "pos", "status"), want, got):
+        assert np.array_equal(np.asarray(w), g), name
+    assert np.array_equal(want_t, got_t)
+    return got
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("past,fresh", [
+    ([], []), ([0], [0]), ([0], [1]), ([63], [1]), ([64], [1]), ([0], [64]), ([0], [65]),
+    ([1], [63]), ([1], [64]), ([5, 0, 128, 64, 63], [0, 0, 1, 0, 130]), ([100000], [3]),
+    ([0, 7], [5000, 1])])
+def test_plan(gpu_ctx, past, fresh):
+    check_plan(gpu_ctx, past, fresh)
+    check_plan(gpu_ctx, past, fresh, spare=37)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n,past,fresh", [(300, 5000, 1), (1024, 200, 90), (1025, 3, 3),
+                                          (2500, 130, 40), (5000, 64, 2)])
+def test_plan_of_many(gpu_ctx, n, past, fresh):
+    rng = np.random.default_rng(n)
+    check_plan(gpu_ctx, rng.integers(0, past + 1, n), rng.integers(0, fresh + 1, n), spare=11)
+
+
+@pytest.mark.gpu
+def test_plan_that_does_not_fit(gpu_ctx):
+    past, fresh = [10, 70, 0], [5, 200, 64]
+    assert check_plan(gpu_ctx, past, fresh, short=1)[5][0] == 8
+    assert check_plan(gpu_ctx, past, fresh, rows=268)[5][0] == 4
+    assert check_plan(gpu_ctx, past, fresh, ldt=4)[5][0] == 2
+    assert check_plan(gpu_ctx, [10, -1], [5, 3])[5][0] == 1
+    assert check_plan(gpu_ctx, [10, 1], [5, -2147483648])[5][0] == 1
+    assert check_plan(gpu_ctx, past, fresh, rows=3, ldt=1, short=2)[5][0] == 14
+    assert check_plan(gpu_ctx, [2147483647], [2147483647], ldt=7, rows=9)[5][0] & 2
+    assert check_plan(gpu_ctx, past, fresh, rows=269)[5][0] == 0
+
+
+@pytest.mark.gpu
+def test_plan_of_a_table_without_pages(gpu_ctx):
+    """A negative page of the past gives no slot."""
+    table = np.full((2, 3), -1, np.int32)
+    want_t = table.copy()
+    want = O.plan([10, 64], [60, 3], [8, 9, 4], want_t, 63)
+    got, got_t = run_plan(gpu_ctx, [10, 64], [60, 3], [8, 9, 4], table, 63)
+    for w, g in zip(want, got):
+        assert np.array_equal(np.asarray(w), g)
+    assert np.array_equal(got_t, want_t) and (got[3][:54] == -1).all() and got[3][54] == 8 * 64
+
+
+# ---- GPU: append ------------------------------------------------------------------------
+
+def device_cache(ctx, c):
+    from rembed_amd import tensor as T
+    return T.KVCache(ctx, c.pages, c.heads, c.dh, *[ctx.upload(x) for x in
+                                                    (c.k, c.v, c.k_exp, c.v_exp)])
+
+
+def same_cache(got, c):
+    for name in ("k", "v", "k_exp", "v_exp"):
+        want = getattr(c, name)
+        g = getattr(got, name).download(np.uint8, want.shape)
+        if name in ("k", "v"):
+            ok = (g == want) | ((g & 127 == 0) & (want & 127 == 0)) | \
+                 ((g & 127 == 127) & (want & 127 == 127))
+        else:
+            ok = g == want
+        assert ok.all(), (name, np.argwhere(~ok)[:4])
+
+
+def batch_of(rng, past, fresh, spare_pages=2):
+    """Tables of pages in no order, as a plan gives them."""
+    blocks = [-(-(p + f) // 64) for p, f in zip(past, fresh)]
+    pages = sum(blocks) + spare_pages
+    perm = rng.permutation(pages)
+    ldt = max(blocks + [1])
+    table = np.zeros((len(past), ldt), np.int32)
+    at = 0
+    for b, n in enumerate(blocks):
+        table[b, :n] = perm[at:at + n]
+        at += n
+    cu, blk, lens, slots, pos, _ = O.plan(
+        past, fresh, [table[b, j] for b in range(len(past))
+                      for j in range(-(-past[b] // 64), blocks[b])], table.copy(),
+        sum(fresh))
+    return pages, table, cu, blk, lens, slots
+
+
+def append(ctx, cache, k, v, dtype, cu, blk, slots, rows=None, front=0, back=0):
+    """k, v [rows][heads][dh] -> the values appended (as dtype holds them)."""
+    from rembed_amd import tensor as T
+    n, h, d = k.shape
+    x = np.zeros((n, front + 2 * h * d + back))
+    x[:, front:front + h * d] = v.reshape(n, -1)  # V before K: offsets count
+    x[:, front + h * d:front + 2 * h * d] = k.reshape(n, -1)
+    img, val = typed(x, dtype)
+    T.CacheAppend(ctx, cache, ctx.upload(img), dtype == "bf16", x.shape[1], front + h * d, front,
+                  ctx.upload(cu), ctx.upload(blk), ctx.upload(slots), len(cu) - 1,
+                  n if rows is None else rows)
+    ctx.sync()
+    val = val.astype(np.float64)
+    return (val[:, front + h * d:front + 2 * h * d].reshape(n, h, d),
+            val[:, front:front + h * d].reshape(n, h, d))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dh", [64, 128, 256])
+@pytest.mark.parametrize("heads,dtype", [(1, "f32"), (3, "bf16")])
+def test_append(gpu_ctx, dh, heads, dtype):
+    """Chunks of every kind behind each other: blocks opened, written on with and without
+    a larger value, a single token, nothing."""
+    rng = np.random.default_rng(dh + heads)
+    steps = [[70, 0, 1, 130], [1, 5, 63, 0], [64, 58, 1, 1], [3, 66, 200, 62], [1, 1, 1, 1]]
+    total = [sum(s[b] for s in steps) for b in range(4)]
+    pages, table, *_ = batch_of(rng, [0] * 4, total)
+    c = O.Cache(pages, heads, dh)
+    dev = device_cache(gpu_ctx, c)
+    past = [0] * 4
+    for i, fresh in enumerate(steps):
+        free = [table[b, j] for b in range(4)
+                for j in range(-(-past[b] // 64), -(-(past[b] + fresh[b]) // 64))]
+        cu, blk, lens, slots, _, _ = O.plan(past, fresh, free, table, sum(fresh))
+        n = sum(fresh)
+        size = np.exp(rng.uniform(-3, 3, (n, heads, 1)))  # some scales grow, some do not
+        k = rng.standard_normal((n, heads, dh)) * size
+        v = rng.standard_normal((n, heads, dh)) * size[::-1]
+        k, v = append(gpu_ctx, dev, k, v, dtype, cu, blk, slots, front=8 * (i % 2), back=16)
+        c.append(k, v, cu, slots)
+        same_cache(dev, c)
+        past = [p + f for p, f in zip(past, fresh)]
+
+
+@pytest.mark.gpu
+def test_append_of_extremes(gpu_ctx):
+    """Zeros, the smallest and largest magnitudes, growth by more than e4m3's range, values
+    that are no numbers."""
+    heads, dh = 2, 64
+    c = O.Cache(3, heads, dh)
+    dev = device_cache(gpu_ctx, c)
+    rng = np.random.default_rng(5)
+    slots = np.arange(64, 64 + 40, dtype=np.int64)
+    for at, n, scale in ((0, 3, 0.0), (3, 2, 2.0 ** -148), (5, 4, 1e-30), (9, 4, 1.0),
+                         (13, 1, 3e38), (14, 8, 1.0), (22, 18, 7.0)):
+        k, v = rng.uniform(-1, 1, (2, n, heads, dh)) * scale
+        if at >= 13:
+            k[0, 0, 5] = np.nan if at == 14 else k[0, 0, 5]
+            v[-1, 1, 63] = np.inf if at == 22 else v[-1, 1, 63]
+        cu, blk = np.array([0, n], np.int32), np.array([0, 1], np.int32)
+        k, v = append(gpu_ctx, dev, k, v, "f32", cu, blk, slots[at:at + n].copy())
+        c.append(k, v, cu, slots[at:at + n])
+        same_cache(dev, c)
+
+
+@pytest.mark.gpu
+def test_append_skips_what_has_no_page(gpu_ctx):
+    heads, dh = 2, 64
+    c = O.Cache(2, heads, dh)
+    dev = device_cache(gpu_ctx, c)
+    rng = np.random.default_rng(6)
+    k, v = rng.standard_normal((2, 12, heads, dh))
+    # request 0: a negative slot; 1: behind the last page; 2: page 1; none: rows behind cu
+    slots = np.array([-1, -1, 128, 129, 130, 64, 65, 66, -1, -1, -1, -1], np.int64)
+    cu, blk = np.array([0, 2, 5, 8], np.int32), np.array([0, 1, 2, 3], np.int32)
+    k, v = append(gpu_ctx, dev, k, v, "f32", cu, blk, slots)
+    c.append(k, v, cu, slots)
+    same_cache(dev, c)
+    # a plan that failed: nothing
+    append(gpu_ctx, dev, k, v, "f32", np.zeros(4, np.int32), np.zeros(4, np.int32),
+           np.full(12, -1, np.int64))
+    same_cache(dev, c)
+
+
+# ---- GPU: attention ---------------------------------------------------------------------
+
+def attend(ctx, c, q, dtype, table, cu, lens, scale, causal, window, out_bf16, rows=None,
+           max_len=None, pad=0):
+    from rembed_amd import tensor as T
+    n, heads, dh = q.shape
+    x = np.zeros((n, pad + heads * dh + 8))
+    x[:, pad:pad + heads * dh] = q.reshape(n, -1)
+    img, val = typed(x, dtype)
+    ldout = heads * dh + 4
+    total = max(n, 1) + 3  # three rows behind the last
+    out = ctx.upload(np.full((total, ldout), 0x4242, np.uint16) if out_bf16
+                     else np.full((total, ldout), 55, np.float32))
+    max_q = int(np.max(np.diff(cu))) if rows is None else rows
+    max_len = int(np.max(lens)) if max_len is None else max_len
+    need = T.cache_attention_scratch(len(lens), max_q, max_len, heads, c.heads, dh)
+    dev = c if hasattr(c, "desc") else device_cache(ctx, c)
+    T.CacheAttention(ctx, out, out_bf16, ldout, ctx.upload(img), dtype == "bf16", x.shape[1], pad,
+                     dev, ctx.upload(table), table.shape[1], ctx.upload(cu), ctx.upload(lens),
+                     len(lens), max_q, max_len, heads, scale, causal, window,
+                     ctx.alloc(need), need)
+    ctx.sync()
+    val = val[:, pad:pad + heads * dh].reshape(n, heads, dh).astype(np.float64)
+    if out_bf16:
+        bits = out.download(np.uint16, (total, ldout))
+        assert (bits[cu[-1]:] == 0x4242).all() and (bits[:, heads * dh:] == 0x4242).all()
+        return from_bf16(bits[:n, :heads * dh]).reshape(n, heads, dh), val
+    got = out.download(np.float32, (total, ldout))
+    assert (got[cu[-1]:] == 55).all() and (got[:, heads * dh:] == 55).all()
+    return got[:n, :heads * dh].reshape(n, heads, dh), val
+
+
+def check_attention(c, got, q, table, cu, lens, scale, causal, window, dtype, out_bf16):
+    for b, n in enumerate(lens):
+        qq = q[cu[b]:cu[b + 1]]
+        if not len(qq):
+            continue
+        k, v = c.rows(table[b], int(n))
+        want, mag, top = O.attention(qq, k, v, scale, causal, window)
+        g = got[cu[b]:cu[b + 1]]
+        dh = q.shape[2]
+        # a score is off by what its steps drop (both codes of q) and, for fp32 q, by its
+        # rounding to 8 bits; P and its sums by 2^-8 and what a page's step drops
+        ds = scale * top * (dh / 64 * STEP * (1 + 2.0 ** -4))
+        if dtype == "f32":
+            ds += scale * BF16 * top * dh
+        tol = (BF16 + STEP * (1 + 2.0 ** -4) + 2 * ds) * mag + 1e-6
+        if out_bf16:
+            tol = tol + BF16 * (np.abs(want) + tol)
+        assert (np.abs(g - want) <= tol).all(), (b, np.abs(g - want).max())
+        norm = np.linalg.norm(want)
+        if norm and n > 1:
+            # rounding of P and of the result, q's scores' drops on normal values
+            assert np.linalg.norm(g - want) / norm <= 2.0 ** -7 + (
+                2.0 ** -7 if dtype == "f32" else 0), b
+
+
+CASES = [  # heads, kv heads, past, fresh, causal, window
+    (1, 1, [0], [1], True, 0), (2, 1, [5], [1], True, 0), (4, 2, [0, 63, 64], [1, 1, 1], True, 0),
+    (16, 8, [700, 1, 64, 0], [1, 1, 1, 1], True, 0), (2, 2, [0, 3, 100], [64, 65, 7], True, 0),
+    (6, 2, [130, 0, 11], [33, 70, 0], True, 0), (3, 1, [200, 40], [100, 129], True, 65),
+    (8, 1, [300], [40], True, 1), (2, 1, [1000, 200], [3, 50], True, 513),
+    (4, 4, [10, 77], [20, 64], False, 0), (2, 2, [100], [90], False, 30),
+    (8, 2, [2100, 4000], [2, 1], True, 0), (10, 1, [50], [300], True, 0),
+]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dh", [64, 128, 256])
+@pytest.mark.parametrize("case", CASES, ids=lambda c: "%dx%d-%s+%s-%d-%d" % (
+    c[0], c[1], c[2], c[3], c[4], c[5]))
+def test_attention(gpu_ctx, dh, case):
+    heads, kv, past, fresh, causal, window = case
+    rng = np.random.default_rng(dh + heads * 7 + sum(past))
+    pages, table, cu, blk, lens, slots = batch_of(rng, past, fresh)
+    c = O.Cache(pages, kv, dh)  # NaN codes wherever nothing is written
+    all_cu = np.concatenate([[0], np.cumsum(lens)]).astype(np.int32)
+    all_slots = np.concatenate([table[b, np.arange(n) // 64].astype(np.int64) * 64 +
+                                np.arange(n) % 64 for b, n in enumerate(lens)])
+    k, v = rng.standard_normal((2, len(all_slots), kv, dh))
+    c.append(k * np.exp(rng.uniform(-1, 1, (len(all_slots), 1, 1))), v, all_cu, all_slots)
+    # bytes behind the last token of a block that was opened are zeros: make them NaN
+    for b, n in enumerate(lens):
+        if n % 64:
+            for at, x in ((O.k_at, c.k), (O.v_at, c.v)):
+                x[table[b, n // 64]][:, O.places(at, dh)[n % 64:]] = 0x7F
+    q = rng.standard_normal((int(cu[-1]), heads, dh)) * 2
+    for dtype, out_bf16 in (("bf16", True), ("f32", False)):
+        got, val = attend(gpu_ctx, c, q, dtype, table, cu, lens, dh ** -0.5, causal, window,
+                          out_bf16, pad=8)
+        check_attention(c, got, val, table, cu, lens, dh ** -0.5, causal, window, dtype, out_bf16)
+
+
+@pytest.mark.gpu
+def test_attention_of_other_lengths(gpu_ctx):
+    """Full attention of queries to states of another length, one of them empty, and causal
+    queries that come before every key: rows of zeros."""
+    rng = np.random.default_rng(11)
+    pages, table, _, _, lens, _ = batch_of(rng, [0, 0, 0], [90, 0, 64])
+    c = O.Cache(pages, 2, 64)
+    cu = np.concatenate([[0], np.cumsum(lens)]).astype(np.int32)
+    slots = np.concatenate([table[b, np.arange(n) // 64].astype(np.int64) * 64 + np.arange(n) % 64
+                            for b, n in enumerate(lens)])
+    k, v = rng.standard_normal((2, len(slots), 2, 64))
+    c.append(k, v, cu, slots)
+    qcu = np.array([0, 100, 103, 110], np.int32)
+    q = rng.standard_normal((110, 4, 64))
+    got, val = attend(gpu_ctx, c, q, "bf16", table, qcu, lens, 0.125, False, 0, False)
+    check_attention(c, got, val, table, qcu, lens, 0.125, False, 0, "bf16", False)
+    assert (got[100:103] == 0).all()
+    got, val = attend(gpu_ctx, c, q, "bf16", table, qcu, lens, 0.125, True, 0, False)
+    check_attention(c, got, val, table, qcu, lens, 0.125, True, 0, "bf16", False)
+    assert (got[:10] == 0).all() and (got[10] != 0).any()
+
+
+@pytest.mark.gpu
+def test_attention_skips_pages_that_are_none(gpu_ctx):
+    rng = np.random.default_rng(12)
+    pages, table, cu, blk, lens, slots = batch_of(rng, [200, 300], [5, 1])
+    c = O.Cache(pages, 1, 64)
+    acu = np.concatenate([[0], np.cumsum(lens)]).astype(np.int32)
+    asl = np.concatenate([table[b, np.arange(n) // 64].astype(np.int64) * 64 + np.arange(n) % 64
+                          for b, n in enumerate(lens)])
+    k, v = rng.standard_normal((2, len(asl), 1, 64))
+    c.append(k, v, acu, asl)
+    q = rng.standard_normal((6, 2, 64))
+    bad = table.copy()
+    bad[0, 1], bad[1, 0], bad[1, 2] = -1, pages, 2 ** 31 - 1
+    got, val = attend(gpu_ctx, c, q, "bf16", bad, cu, lens, 0.125, True, 0, False)
+    for b, gone in ((0, [1]), (1, [0, 2])):
+        kk, vv = c.rows(table[b], int(lens[b]))
+        keep = np.array([j // 64 not in gone for j in range(lens[b])])
+        for r in range(cu[b], cu[b + 1]):
+            i = lens[b] - (cu[b + 1] - r)
+            for h in range(2):
+                s = np.where(keep & (np.arange(lens[b]) <= i), kk[:, 0] @ val[r, h] * 0.125, -np.inf)
+                p = np.exp(s - s.max())
+                want = (p / p.sum()) @ vv[:, 0]
+                mag = (p / p.sum()) @ np.abs(vv[:, 0])
+                ds = 0.125 * np.abs(val[r, h]).max() * np.abs(kk).max() * STEP * 1.0625
+                assert (np.abs(got[r, h] - want) <= (BF16 + STEP * 1.0625 + 2 * ds) * mag + 1e-6).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("past", [0, 900])
+def test_attention_with_what_is_no_number(gpu_ctx, past):
+    """A token whose K or V holds none is NaN to the queries that see it, and nothing to the
+    others; a query that holds one is NaN itself."""
+    rng = np.random.default_rng(13)
+    pages, table, cu, blk, lens, slots = batch_of(rng, [past], [100])
+    c = O.Cache(pages, 1, 128)
+    n = int(lens[0])
+    k, v = rng.standard_normal((2, n, 1, 128))
+    at = table[0, np.arange(n) // 64].astype(np.int64) * 64 + np.arange(n) % 64
+    c.append(k, v, np.array([0, n], np.int32), at)
+    q = rng.standard_normal((100, 2, 128))
+    ok, _ = attend(gpu_ctx, c, q, "bf16", table, cu, lens, 0.1, True, 0, False)
+    v[past + 40, 0, 3] = np.nan
+    k[past + 70, 0, 3] = np.inf
+    c = O.Cache(pages, 1, 128)
+    c.append(k, v, np.array([0, n], np.int32), at)
+    q[5, 1, 7] = np.nan
+    got, _ = attend(gpu_ctx, c, q, "bf16", table, cu, lens, 0.1, True, 0, False)
+    assert np.isnan(got[40:]).all()
+    assert np.isnan(got[5, 1]).all()
+    got[5, 1] = ok[5, 1]
+    # the scale of the block may differ, so values need not be the same bits
+    assert np.isfinite(got[:40]).all()
+    assert np.abs(got[:40] - ok[:40]).max() < 1.0
+    # a window past the token does not see it
+    got, _ = attend(gpu_ctx, c, q, "bf16", table, cu, lens, 0.1, True, 10, False)
+    assert np.isfinite(got[50:70]).all() and np.isnan(got[40:50]).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("nq", [1, 5, 200])
+def test_attention_split_or_not(gpu_ctx, nq):
+    """What max_len promises chooses the split only: results agree to the roundings of P."""
+    rng = np.random.default_rng(14)
+    pages, table, cu, blk, lens, slots = batch_of(rng, [1900], [nq])
+    c = O.Cache(pages, 1, 128)
+    n = int(lens[0])
+    k, v = rng.standard_normal((2, n, 1, 128))
+    at = table[0, np.arange(n) // 64].astype(np.int64) * 64 + np.arange(n) % 64
+    c.append(k, v, np.array([0, n], np.int32), at)
+    q = rng.standard_normal((nq, 2, 128))
+    for max_len in (64, 1000, n, 100000):
+        got, val = attend(gpu_ctx, c, q, "bf16", table, cu, lens, 0.1, True, 0, True,
+                          max_len=max_len)
+        check_attention(c, got, val, table, cu, lens, 0.1, True, 0, "bf16", True)
+        again, _ = attend(gpu_ctx, c, q, "bf16", table, cu, lens, 0.1, True, 0, True,
+                          max_len=max_len)
+        assert np.array_equal(got, again)
