@@ -27,9 +27,12 @@ FLAGS = [
 
 # Per-file code generation: the attention kernels keep their MFMA
 # accumulators in VGPRs (no AGPR round trips for the online-softmax rescale,
-# two waves per SIMD at head dim 128).
-FILE_FLAGS = {f: ["-mllvm", "-amdgpu-mfma-vgpr-form=1"]
-              for f in ("attention.hip", "cache_attention.hip")}
+# two waves per SIMD at head dim 128). The cache's attention also keeps them
+# whole across branches: taken apart into scalars there, all of them were copied
+# to another order and back on every page (64 moves of 330 instructions).
+FILE_FLAGS = {"attention.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
+              "cache_attention.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1", "-mllvm",
+                                      "-amdgpu-codegenprepare-break-large-phis=false"]}
 
 
 def sources():

@@ -38,6 +38,18 @@ __device__ __forceinline__ void cache_key_range(const CacheAttnArgs& p, int i, i
   if (khi < klo) klo = khi = 1 << 30;
 }
 
+// The larger of a lane's value and that of lane ^ 32, in both.
+__device__ __forceinline__ float max_halves(float v) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  typedef unsigned v2u __attribute__((ext_vector_type(2)));
+  const unsigned u = __float_as_uint(v);
+  const v2u r = __builtin_bit_cast(v2u, __builtin_amdgcn_permlane32_swap(u, u, false, false));
+  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+#else
+  return v;
+#endif
+}
+
 // The columns' codes and scale bytes: lane (column, half) holds values
 // 64 s + 32 half .. + 31 of step s, as K's pieces do.
 template <int KS, bool BF16>
@@ -90,9 +102,7 @@ struct CacheTile {
 
   __device__ __forceinline__ void clear() {
 #pragma unroll
-    for (int t = 0; t < DT; t++)
-#pragma unroll
-      for (int e = 0; e < 16; e++) o[t][e] = 0.0f;
+    for (int t = 0; t < DT; t++) o[t] = v16f{};
     mref = -INFINITY;
     lrun = 0.0f;
   }
@@ -101,11 +111,7 @@ struct CacheTile {
   // key0: the page's first position; n: tokens in the cache.
   __device__ __forceinline__ void page(const v8i (&kf)[KS][2], v8i (&vf)[DT], int xk, int xv,
                                        int key0, int n, float cs, int half) {
-    v16f sc[2];
-#pragma unroll
-    for (int t = 0; t < 2; t++)
-#pragma unroll
-      for (int e = 0; e < 16; e++) sc[t][e] = 0.0f;
+    v16f sc[2] = {v16f{}, v16f{}};
 #pragma unroll
     for (int s = 0; s < KS; s++)
 #pragma unroll
@@ -139,7 +145,7 @@ struct CacheTile {
     for (int t = 0; t < 2; t++)
 #pragma unroll
       for (int e = 0; e < 16; e++) smax = fmaxf(smax, sc[t][e]);
-    smax = fmaxf(smax, __shfl_xor(smax, 32, 64));
+    smax = max_halves(smax);
     const float mloc = smax * cs;
     const bool up = mloc > mref + kHead;  // -inf + 4 = -inf: the first visible key moves it
     if (__any(up)) {
@@ -150,9 +156,7 @@ struct CacheTile {
       }
       lrun *= alpha;
 #pragma unroll
-      for (int t = 0; t < DT; t++)
-#pragma unroll
-        for (int e = 0; e < 16; e++) o[t][e] *= alpha;
+      for (int t = 0; t < DT; t++) o[t] *= alpha;
     }
     // a column with no visible key yet: every p = 2^(-inf) = 0
     const float m = mref == -INFINITY ? 0.0f : mref - kHead;
@@ -193,6 +197,31 @@ __device__ __forceinline__ void cache_fetch(const uint8_t* k, const uint8_t* v, 
   for (int t = 0; t < DH / 32; t++) vf[t] = join8(vp[t * 2 * 64], vp[(t * 2 + 1) * 64]);
 }
 
+// Page ids and scale bytes of 64 consecutive pages of a request, one a lane: read once, then
+// taken lane by lane, so that no page waits for its table entry and scales.
+struct PageWindow {
+  int page, xk, xv;  // page: -1 where the entry is no page of the cache
+  // pages g0 .. g0 + 63, none from `end` on
+  __device__ __forceinline__ void load(const CacheAttnArgs& p, int b, int h, int g0, int end,
+                                       int lane) {
+    const int g = g0 + lane;
+    page = g < end ? p.table[(size_t)b * p.ldt + g] : -1;
+    if (page < 0 || page >= p.cache.pages) page = -1;
+    const size_t unit = (size_t)max(page, 0) * p.cache.kv_heads + h;
+    xk = p.cache.k_exp[unit];
+    xv = p.cache.v_exp[unit];
+    // waited for here: at their uses, in every turn, the wait would cover younger loads
+    asm("" : "+v"(page), "+v"(xk), "+v"(xv));
+  }
+  static __device__ __forceinline__ int at(int v, int i) {
+#if defined(__HIP_DEVICE_COMPILE__)
+    return __builtin_amdgcn_readlane(v, i);
+#else
+    return v;
+#endif
+  }
+};
+
 // Workgroup -> (request, kv head, tile of columns, key range). Units of one (request,
 // kv head) read the same pages: their workgroups are dealt to one XCD (workgroup w
 // runs on XCD w % 8) and share its L2.
@@ -206,6 +235,30 @@ __device__ __forceinline__ bool cache_unit(const CacheAttnArgs& p, int tiles, in
   tile = v / splits;
   split = v % splits;
   return true;
+}
+
+// Pages [lo, hi) that columns c0 .. c1 - 1 of a request see.
+__device__ __forceinline__ void cache_page_range(const CacheAttnArgs& p, int pos0, int n, int G,
+                                                 int c0, int c1, int& lo, int& hi) {
+  lo = 0;
+  hi = (n + kPageT - 1) / kPageT;
+  const int i0 = pos0 + c0 / G, i1 = pos0 + (c1 - 1) / G;
+  if (p.causal) hi = min(hi, i1 < 0 ? 0 : i1 / kPageT + 1);
+  if (p.window > 0) {
+    lo = max(0, i0 - p.window + 1) / kPageT;
+    const long long last = (long long)i1 + p.window - 1;
+    if (last < n) hi = min(hi, last < 0 ? 0 : (int)(last / kPageT) + 1);
+  }
+}
+
+__device__ __forceinline__ void cache_store4(const CacheAttnArgs& p, size_t to, const v4f& x) {
+  if (p.out_bf16) {
+    typedef __bf16 v4bf __attribute__((ext_vector_type(4)));
+    *reinterpret_cast<v4bf*>(static_cast<__bf16*>(p.out) + to) =
+        (v4bf){(__bf16)x[0], (__bf16)x[1], (__bf16)x[2], (__bf16)x[3]};
+  } else {
+    *reinterpret_cast<v4f*>(static_cast<float*>(p.out) + to) = x;
+  }
 }
 
 template <int DH, bool BF16>
@@ -234,26 +287,23 @@ __global__ __launch_bounds__(64 * kWaves) void cache_attention_kernel(CacheAttnA
   cache_key_range(p, pos0 + c / G, n, w.klo, w.khi);
 
   // the tile's pages, this split's share of them
-  int lo = 0, hi = (n + kPageT - 1) / kPageT;
-  {
-    const int i0 = pos0 + c0 / G, i1 = pos0 + (min(c0 + kCols, cols) - 1) / G;
-    if (p.causal) hi = min(hi, i1 < 0 ? 0 : i1 / kPageT + 1);
-    if (p.window > 0) {
-      lo = max(0, i0 - p.window + 1) / kPageT;
-      const long long last = (long long)i1 + p.window - 1;
-      if (last < n) hi = min(hi, last < 0 ? 0 : (int)(last / kPageT) + 1);
-    }
-  }
+  int lo, hi;
+  cache_page_range(p, pos0, n, G, c0, min(c0 + kCols, cols), lo, hi);
   const int each = (max(0, hi - lo) + splits - 1) / splits;
   const int first = lo + split * each, end = min(hi, first + each);
-  for (int g = first + wave; g < end; g += kWaves) {
-    const int pg = p.table[(size_t)b * p.ldt + g];
-    if (pg < 0 || pg >= p.cache.pages) continue;  // no such page: no keys
-    const size_t unit = (size_t)pg * p.cache.kv_heads + h;
-    v8i kf[KS][2], vf[DT];
-    cache_fetch<DH>(p.cache.k + unit * (kPageT * DH), p.cache.v + unit * (kPageT * DH), lane, kf,
-                    vf);
-    w.page(kf, vf, p.cache.k_exp[unit], p.cache.v_exp[unit], g * kPageT, n, cs, half);
+  PageWindow win;
+  for (int g0 = first; g0 < end; g0 += 64) {
+    if (p.cache.pages < 1) break;
+    win.load(p, b, h, g0, end, lane);
+    const int last = min(end, g0 + 64);
+    for (int g = g0 + wave; g < last; g += kWaves) {
+      const int page = win.at(win.page, g - g0);
+      if (page < 0) continue;  // no such page: no keys
+      const size_t at = ((size_t)page * p.cache.kv_heads + h) * (kPageT * DH);
+      v8i kf[KS][2], vf[DT];
+      cache_fetch<DH>(p.cache.k + at, p.cache.v + at, lane, kf, vf);
+      w.page(kf, vf, win.at(win.xk, g - g0), win.at(win.xv, g - g0), g * kPageT, n, cs, half);
+    }
   }
 
   // join the waves: columns' references and sums, then O in wave order
@@ -311,14 +361,398 @@ __global__ __launch_bounds__(64 * kWaves) void cache_attention_kernel(CacheAttnA
     }
     const float inv = ll == 0.0f ? 0.0f : 1.0f / ll;
     x *= inv;
-    const size_t to = (size_t)(r0 + cc / G) * p.ldout + (h * G + cc % G) * DH + d;
-    if (p.out_bf16) {
-      typedef __bf16 v4bf __attribute__((ext_vector_type(4)));
-      *reinterpret_cast<v4bf*>(static_cast<__bf16*>(p.out) + to) =
-          (v4bf){(__bf16)x[0], (__bf16)x[1], (__bf16)x[2], (__bf16)x[3]};
-    } else {
-      *reinterpret_cast<v4f*>(static_cast<float*>(p.out) + to) = x;
+    cache_store4(p, (size_t)(r0 + cc / G) * p.ldout + (h * G + cc % G) * DH + d, x);
+  }
+}
+
+// ---- many columns --------------------------------------------------------------------
+// Four waves of 32 columns each walk the same pages. What bounds it: a page's products take
+// the matrix cores 64 cycles each (dh 128: 16 of them, 1024 cycles) and its softmax the VALU
+// 1100 to 1300, and a wave issues in order, so one after the other they cost their sum even
+// with two waves per SIMD. The loop therefore is a pipeline over pages whose body has no
+// branch: while page g's scores become P, two at a time, the products between them are
+// page g + 1's scores and page g - 1's values. K and V come to LDS by global_load_lds in
+// fragment order (1 KiB pieces, read back without bank conflicts), two turns before they are
+// used, with one barrier per turn.
+//
+// The accumulators are touched by products alone: O is kept in units of the reference a
+// column starts with (`base`), and a reference that has moved since, always by whole
+// powers of two, goes into P's scale byte. A column whose reference moves by more than
+// 2^64 (its earlier keys then weigh nothing in fp32) makes its wave go over the pages once
+// more after the loop, with CacheTile, whose rescale has no such limit: kept in the loop,
+// that branch cost the compiler a second copy of O and 20 spilled registers.
+constexpr float kFar = 64.0f;
+
+template <int DH>
+struct CachePipe {
+  static constexpr int KS = DH / 64, DT = DH / 32;
+  static constexpr int NF = 2 * KS + DT;  // fragments of a page: K's, then V's
+  v8i qh[KS], ql[KS];
+  int xh, xl;
+  v16f o[DT], sc[2];
+  v8i ph, pl;  // P of the page before,
+  int eh, el;  // its scale bytes
+  float mref, base, lrun;
+  bool far;
+  int klo, khi;
+
+  // With more than 256 registers in use (dh 256) the compiler may move a scale word to an
+  // accumulation register, which the instruction does not take: held in a VGPR here.
+  static __device__ __forceinline__ v16f mul(const v8i& a, const v8i& b, const v16f& c, int ea,
+                                             int eb) {
+    if constexpr (DH == 256) asm("" : "+v"(ea), "+v"(eb));
+    return mfma_fp8_32(a, b, c, ea, eb);
+  }
+  // fragment f of a page at its lane's place in LDS
+  static __device__ __forceinline__ v8i frag(const uint8_t* at, int f) {
+    return join8(*reinterpret_cast<const v4i*>(at + 2 * f * 1024),
+                 *reinterpret_cast<const v4i*>(at + 2 * f * 1024 + 1024));
+  }
+  __device__ __forceinline__ void scores(const uint8_t* k, int xk) {
+    v16f s[2] = {v16f{}, v16f{}};
+#pragma unroll
+    for (int f = 0; f < 2 * KS; f++) {
+      const v8i a = frag(k, f);
+      s[f & 1] = mul(a, qh[f / 2], s[f & 1], xk, xh);
+      s[f & 1] = mul(a, ql[f / 2], s[f & 1], xk, xl);
     }
+    sc[0] = s[0];
+    sc[1] = s[1];
+  }
+  __device__ __forceinline__ void values(const uint8_t* v, int xv) {
+#pragma unroll
+    for (int t = 0; t < DT; t++) {
+      const v8i a = frag(v, t);
+      o[t] = mul(a, ph, o[t], xv, eh);
+      o[t] = mul(a, pl, o[t], xv, el);
+    }
+  }
+  // Scores of page g (first position key0) to their maximum; moves the reference. `none`:
+  // the page holds no keys at all.
+  __device__ __forceinline__ void refer(int key0, bool none, float cs, int half) {
+    if (__builtin_expect(none || __any(key0 < klo || key0 + kPageT - 1 > khi), 0)) {
+      const unsigned span = (unsigned)(khi - klo);
+      const int at = key0 + half * 4 - klo;
+#pragma unroll
+      for (int t = 0; t < 2; t++)
+#pragma unroll
+        for (int e = 0; e < 16; e++) {
+          const unsigned off = (unsigned)(at + t * 32 + e / 4 * 8 + e % 4);
+          sc[t][e] = none || off > span ? -INFINITY : sc[t][e];
+        }
+    }
+    float smax = -INFINITY;
+#pragma unroll
+    for (int t = 0; t < 2; t++)
+#pragma unroll
+      for (int e = 0; e < 16; e++) smax = fmaxf(smax, sc[t][e]);
+    const float mloc = max_halves(smax) * cs;
+    const bool up = mloc > mref + kHead;  // -inf + 4 = -inf: the first visible key moves it
+    const float to = up ? __builtin_ceilf(mloc) : mref;
+    lrun *= up ? __builtin_amdgcn_exp2f(mref - to) : 1.0f;
+    mref = to;
+    base = base == -INFINITY ? to : base;
+  }
+  // P of page g, between the values of page g - 1 (v, xv) and the scores of g + 1 (k, xk).
+  __device__ __forceinline__ void turn(const uint8_t* k, int xk, const uint8_t* v, int xv,
+                                       float cs) {
+    // a column with no visible key yet: every p = 2^(-inf) = 0
+    const float m = mref == -INFINITY ? 0.0f : mref - kHead;
+    v16f s[2] = {v16f{}, v16f{}};
+    v8i nh, nl;
+    constexpr int kPairs = 16;
+    // Two scores at a time, 68 cycles of VALU beside a product's 64. Each step waits
+    // on the one before it, so three pairs are under way: the exponentials of pair j, the
+    // codes of j - 1, what those leave over of j - 2.
+    float x[3], y[3];
+    v2f rest[3];
+    auto pair = [&](int j) {
+#if defined(__HIP_DEVICE_COMPILE__)
+      if (j >= 2) {
+        const int i = j - 2, w = i / 2, q = i % 3;
+        const float u = __builtin_fmaf(x[q], 16.0f, -rest[q][0]);
+        const float t = __builtin_fmaf(y[q], 16.0f, -rest[q][1]);
+        int l = nl[w];
+        if (i % 2 == 0) {
+          asm("" : "=v"(l) : "v"(u));  // any word: both halves get written
+          l = __builtin_amdgcn_cvt_pk_fp8_f32(u, t, l, false);
+        } else {
+          l = __builtin_amdgcn_cvt_pk_fp8_f32(u, t, l, true);
+        }
+        nl[w] = l;
+      }
+      if (j >= 1 && j <= kPairs) {
+        const int i = j - 1, w = i / 2, q = i % 3;
+        lrun += x[q];
+        lrun += y[q];
+        int h = nh[w];
+        if (i % 2 == 0) {
+          asm("" : "=v"(h) : "v"(x[q]));
+          h = __builtin_amdgcn_cvt_pk_fp8_f32(x[q], y[q], h, false);
+          rest[q] = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(h, 16.0f, false);
+        } else {
+          h = __builtin_amdgcn_cvt_pk_fp8_f32(x[q], y[q], h, true);
+          rest[q] = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(h, 16.0f, true);
+        }
+        nh[w] = h;
+      }
+      if (j < kPairs) {
+        const int e = 2 * j % 16, q = j % 3;
+        x[q] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[j / 8][e], cs, -m));
+        y[q] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[j / 8][e + 1], cs, -m));
+      }
+#endif
+    };
+    // Products in fours: two fragments by hi, then by lo, so that no product waits for
+    // the one before it; values first, whose P then makes room for the scores. Three
+    // fragments at a time are in registers.
+    constexpr int NM = 2 * NF;
+    auto piece = [&](int f) { return f < DT ? frag(v, f) : frag(k, f - DT); };
+    v8i a0 = piece(0), a1 = piece(1);
+#pragma unroll
+    for (int f = 0; f < NF; f += 2) {
+      v8i b0 = a0, b1 = a1;
+#pragma unroll
+      for (int u = 0; u < 4; u++) {
+        const v8i& a = u % 2 ? a1 : a0;
+        const int g = f + u % 2, st = (f - DT) / 2;
+        if (f < DT) o[g] = mul(a, u < 2 ? ph : pl, o[g], xv, u < 2 ? eh : el);
+        else s[u % 2] = mul(a, u < 2 ? qh[st] : ql[st], s[u % 2], xk, u < 2 ? xh : xl);
+        if (u == 0 && f + 2 < NF) b0 = piece(f + 2);
+        if (u == 2 && f + 2 < NF) b1 = piece(f + 3);
+        const int at = 2 * f + u;  // of NM
+#pragma unroll
+        for (int j = at * kPairs / NM; j < (at + 1) * kPairs / NM; j++) pair(j);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      a0 = b0;
+      a1 = b1;
+    }
+    pair(kPairs);
+    pair(kPairs + 1);
+    ph = nh;
+    pl = nl;
+    const float moved = mref == -INFINITY ? 0.0f : mref - base;
+    far |= moved > kFar;
+    eh = 127 + (int)fminf(moved, kFar);
+    el = eh - 4;
+    sc[0] = s[0];
+    sc[1] = s[1];
+  }
+};
+
+template <int DH, bool BF16>
+__global__ __launch_bounds__(64 * kWaves, DH == 256 ? 1 : 2) void cache_attention_cols_kernel(
+    CacheAttnArgs p, int tiles, int splits, int part_cols) {
+  constexpr int KS = DH / 64, DT = DH / 32, kHalf = kPageT * DH;  // bytes of K or V of a page
+  constexpr int kStride = DH + 4, kLds = 6 * kHalf;  // K of three pages, V of three
+  constexpr int kPieces = kHalf / 1024 / kWaves;     // 1 KiB pieces per wave, of K and of V
+  constexpr int kBand = 8;  // output rows of a wave staged at a time
+  static_assert(kWaves * kBand * kStride * 4 <= kLds, "output staging");
+  __shared__ __attribute__((aligned(1024))) uint8_t lds[kLds];
+  const int wgs = (tiles + kWaves - 1) / kWaves;
+  int b, h, wg, split;
+  if (!cache_unit(p, wgs, splits, b, h, wg, split)) return;
+  if (p.causal) {
+    // later columns see more pages: each XCD's 32 CUs get the long ones first, then
+    // the next 32 in the other order, so that long and short ones share a CU
+    const int k = wg / 32, size = min(32, wgs - 32 * k);
+    wg = wgs - 1 - (32 * k + (k & 1 ? size - 1 - wg % 32 : wg % 32));
+  }
+  const int G = p.heads / p.cache.kv_heads;
+  const int r0 = p.cu[b], nq = p.cu[b + 1] - r0;
+  const int cols = nq * G;
+  if (wg * kWaves * kCols >= cols) return;
+  const int n = max(0, min(p.lens[b], p.ldt * kPageT));
+  const int lane = threadIdx.x & 63, col = lane & 31, half = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int tile = wg * kWaves + wave, c0 = tile * kCols;
+  const int c = min(c0 + col, cols - 1);
+  const int pos0 = n - nq;
+  const float cs = p.scale * 1.44269504088896341f;
+
+  int lo, hi;
+  cache_page_range(p, pos0, n, G, wg * kWaves * kCols, min((wg + 1) * kWaves * kCols, cols), lo, hi);
+  if (p.cache.pages < 1) hi = lo;
+  const int each = (max(0, hi - lo) + splits - 1) / splits;
+  const int first = lo + split * each, end = min(hi, first + each);
+  const bool active = c0 < cols;
+
+  // A page that is none is read as page 0 and holds no keys.
+  PageWindow win;
+  int base = first;  // the window's first page
+  auto dma = [&](const uint8_t* src, int page, uint8_t* dst) {
+    const size_t unit = (size_t)max(page, 0) * p.cache.kv_heads + h;
+    const uint8_t* at = src + unit * kHalf + wave * kPieces * 1024 + lane * 16;
+#pragma unroll
+    for (int i = 0; i < kPieces; i++)
+      lds_dma16(at + i * 1024, dst + (wave * kPieces + i) * 1024);
+  };
+  uint8_t* const ldsk = lds;
+  uint8_t* const ldsv = lds + 3 * kHalf;
+  // V behind the last token is zeroed: no NaN code may meet a zero P
+  auto clean = [&](int g, bool none, uint8_t* v) {
+    if (!none && (g + 1) * kPageT <= n) return;
+    for (int i = threadIdx.x * 4; i < kHalf; i += 64 * kWaves * 4) {
+      // four tokens of one column: 32 * part + 8 * (byte / 4) + 4 * half
+      const int t = (i / 1024 & 1) * 32 + (i % 16) / 4 * 8 + (i % 1024) / 512 * 4;
+      const int left = none ? 0 : n - (g * kPageT + t);
+      const int keep = left >= 4 ? -1 : left <= 0 ? 0 : (1 << (8 * left)) - 1;
+      *reinterpret_cast<int*>(v + i) &= keep;
+    }
+    __syncthreads();
+  };
+
+  CachePipe<DH> w;
+  if (first < end) {
+    win.load(p, b, h, first, end, lane);
+    dma(p.cache.k, win.at(win.page, 0), ldsk);
+    dma(p.cache.k, win.at(win.page, 1), ldsk + kHalf);
+    dma(p.cache.v, win.at(win.page, 0), ldsv + kHalf);
+    dma(p.cache.k, win.at(win.page, 2), ldsk + 2 * kHalf);
+  }
+  cache_load_q<KS, BF16>(p.q, (size_t)(r0 + c / G) * p.ldq + p.q_off + (h * G + c % G) * DH, half,
+                         w.qh, w.ql, w.xh, w.xl);
+#pragma unroll
+  for (int t = 0; t < DT; t++) w.o[t] = v16f{};
+  w.ph = v8i{};
+  w.pl = v8i{};
+  w.eh = w.el = 127;
+  w.mref = w.base = -INFINITY;
+  w.lrun = 0.0f;
+  w.far = false;
+  cache_key_range(p, pos0 + c / G, n, w.klo, w.khi);
+  // turn g: K of g + 1 in slot ks of ldsk, V of g - 1 in slot vs of ldsv
+  int ks = 1, vs = 0;
+  bool nonep = false, none = false;  // page g - 1, g is none
+  auto after = [](int slot) { return slot == 2 ? 0 : slot + 1; };
+  auto stage = [&](int g) {
+    wait_vmcnt<2 * kPieces>();  // all but the last turn's
+    wait_lgkmcnt0();
+    stage_barrier();
+    if (g > first) clean(g - 1, nonep, ldsv + vs * kHalf);
+    if (g + 3 >= base + 64) {
+      win.load(p, b, h, g, end, lane);
+      base = g;
+    }
+    none = win.at(win.page, g - base) < 0;
+    // V of g + 1 and K of g + 3 go where V of g - 2 and K of g were
+    dma(p.cache.v, win.at(win.page, g + 1 - base), ldsv + after(after(vs)) * kHalf);
+    dma(p.cache.k, win.at(win.page, g + 3 - base), ldsk + after(after(ks)) * kHalf);
+  };
+  auto done = [&] {
+    nonep = none;
+    ks = after(ks);
+    vs = after(vs);
+  };
+  auto last = [&] {
+    wait_vmcnt<0>();
+    wait_lgkmcnt0();
+    stage_barrier();
+    clean(end - 1, nonep, ldsv + vs * kHalf);
+  };
+  if (first < end) {
+    // V of page `first - 1` is multiplied by P = 0: any finite codes
+    for (int i = threadIdx.x * 16; i < kHalf; i += 64 * kWaves * 16)
+      *reinterpret_cast<v4i*>(ldsv + i) = v4i{0, 0, 0, 0};
+    __syncthreads();  // waits for the DMA too
+    if (!active) {  // a wave without columns stages its pieces
+      for (int g = first; g < end; g++) {
+        stage(g);
+        done();
+      }
+      last();
+    } else {
+      w.scores(ldsk + lane * 16, win.at(win.xk, 0));
+      int xvp = 127;  // scale of V of page g - 1
+      for (int g = first; g < end; g++) {
+        stage(g);
+        const uint8_t* kn = ldsk + ks * kHalf + lane * 16;
+        const uint8_t* vp = ldsv + vs * kHalf + lane * 16;
+        w.refer(g * kPageT, none, cs, half);
+        w.turn(kn, win.at(win.xk, g + 1 - base), vp, xvp, cs);
+        xvp = win.at(win.xv, g - base);
+        done();
+      }
+      last();
+      w.values(ldsv + vs * kHalf + lane * 16, xvp);
+    }
+  }
+  __syncthreads();
+  if (!active) return;
+  // O from units of the first reference to units of the last one
+  float unit = w.mref == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(w.base - w.mref);
+  if (__builtin_expect(__any(w.far), 0)) {
+    CacheTile<DH> r;
+#pragma unroll
+    for (int s = 0; s < KS; s++) {
+      r.qh[s] = w.qh[s];
+      r.ql[s] = w.ql[s];
+    }
+    r.xh = w.xh;
+    r.xl = w.xl;
+    r.klo = w.klo;
+    r.khi = w.khi;
+    r.clear();
+    for (int g = first; g < end; g++) {
+      const int page = p.table[(size_t)b * p.ldt + g];
+      if (page < 0 || page >= p.cache.pages) continue;
+      const size_t u = (size_t)page * p.cache.kv_heads + h;
+      v8i kf[KS][2], vf[DT];
+      cache_fetch<DH>(p.cache.k + u * kHalf, p.cache.v + u * kHalf, lane, kf, vf);
+      r.page(kf, vf, p.cache.k_exp[u], p.cache.v_exp[u], g * kPageT, n, cs, half);
+    }
+#pragma unroll
+    for (int t = 0; t < DT; t++) w.o[t] = r.o[t];
+    w.mref = r.mref;
+    w.lrun = r.lrun;
+    unit = 1.0f;
+  }
+
+  // O^T through this wave's LDS rows to whole output rows
+  const float l = w.lrun + __shfl_xor(w.lrun, 32, 64);
+  const float inv = splits > 1 ? unit : l == 0.0f ? 0.0f : unit / l;
+  float* st = reinterpret_cast<float*>(lds) + wave * kBand * kStride;
+  float* part = nullptr;
+  if (splits > 1) {
+    const size_t u = ((size_t)b * p.cache.kv_heads + h) * tiles + tile;
+    part = p.part + (u * splits + split) * (size_t)part_cols * (DH + 2);
+    if (half == 0 && c0 + col < cols) {
+      part[(size_t)col * (DH + 2) + DH] = w.mref;
+      part[(size_t)col * (DH + 2) + DH + 1] = l;
+    }
+  }
+  constexpr int LPR = DH / 4, RPI = 64 / LPR;  // lanes per row, rows per instruction
+  const int d = lane % LPR * 4;
+#pragma unroll
+  for (int band = 0; band < kCols; band += kBand) {
+    if (col >= band && col < band + kBand) {
+#pragma unroll
+      for (int t = 0; t < DT; t++)
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+          v4f x;
+#pragma unroll
+          for (int e = 0; e < 4; e++) x[e] = w.o[t][i * 4 + e] * inv;
+          *reinterpret_cast<v4f*>(st + (col - band) * kStride + t * 32 + i * 8 + half * 4) = x;
+        }
+    }
+    wait_lgkmcnt0();
+    __builtin_amdgcn_wave_barrier();
+    for (int rr = lane / LPR; rr < kBand; rr += RPI) {
+      const int cc = c0 + band + rr;
+      if (cc >= cols) break;
+      const v4f x = *reinterpret_cast<const v4f*>(st + rr * kStride + d);
+      if (part) {
+        typedef float v2 __attribute__((ext_vector_type(2)));
+        float* at = part + (size_t)(band + rr) * (DH + 2) + d;
+        *reinterpret_cast<v2*>(at) = (v2){x[0], x[1]};
+        *reinterpret_cast<v2*>(at + 2) = (v2){x[2], x[3]};
+      } else {
+        cache_store4(p, (size_t)(r0 + cc / G) * p.ldout + (h * G + cc % G) * DH + d, x);
+      }
+    }
+    __builtin_amdgcn_wave_barrier();
   }
 }
 
@@ -368,15 +802,24 @@ static int cache_part_cols(int max_q, int heads, int kv_heads) {
   return (int)std::min((long long)kCols, (long long)max_q * (heads / kv_heads));
 }
 
-// Key ranges: as many as give the chip's 256 CUs four workgroups each, where a range
-// still has a page for every wave.
+// Columns of one kv head that a request may have at most. Up to 32: a workgroup's waves share
+// a tile and take pages in turn; more: each wave takes a tile.
+static bool cache_by_cols(int max_q, int heads, int kv_heads) {
+  return (long long)max_q * (heads / kv_heads) > kCols;
+}
+
+// Key ranges: as many as give the chip's 256 CUs four workgroups each (by columns: one),
+// where a range still has a page for every wave (by columns: eight pages).
 void cache_attention_plan(int batch, int max_q, int max_len, int heads, int kv_heads, int dh,
                           int* splits, size_t* part_floats) {
   const long long tiles = cache_tiles(max_q, heads, kv_heads);
   const long long units = (long long)batch * kv_heads * tiles;
   const long long pages = ((long long)max_len + kPageT - 1) / kPageT;
-  long long s = units > 0 ? (1024 + units - 1) / units : 1;
-  s = std::max(1LL, std::min(s, pages / kWaves));
+  const bool cols = cache_by_cols(max_q, heads, kv_heads);
+  const long long wgs = cols ? (long long)batch * kv_heads * ((tiles + kWaves - 1) / kWaves) : units;
+  const long long want = cols ? 256 : 1024;
+  long long s = wgs > 0 ? (want + wgs - 1) / wgs : 1;
+  s = std::max(1LL, std::min(s, pages / (cols ? 8 : kWaves)));
   *splits = (int)s;
   *part_floats = s > 1 ? (size_t)units * s * cache_part_cols(max_q, heads, kv_heads) * (dh + 2) : 0;
 }
@@ -389,11 +832,18 @@ static hipError_t launch_dh(const CacheAttnArgs& a, hipStream_t s) {
   const int tiles = cache_tiles(a.max_q, a.heads, a.cache.kv_heads);
   const int pc = cache_part_cols(a.max_q, a.heads, a.cache.kv_heads);
   const int units = a.batch * a.cache.kv_heads;
-  const dim3 grid((unsigned)((units + 7) / 8 * 8 * tiles * splits)), block(64 * kWaves);
-  if (a.in_bf16)
-    hipLaunchKernelGGL((cache_attention_kernel<DH, true>), grid, block, 0, s, a, tiles, splits, pc);
-  else
-    hipLaunchKernelGGL((cache_attention_kernel<DH, false>), grid, block, 0, s, a, tiles, splits, pc);
+  const bool cols = cache_by_cols(a.max_q, a.heads, a.cache.kv_heads);
+  const int per = cols ? (tiles + kWaves - 1) / kWaves : tiles;
+  const dim3 grid((unsigned)((units + 7) / 8 * 8 * per * splits)), block(64 * kWaves);
+#define RH_ATTN(K, B) hipLaunchKernelGGL((K<DH, B>), grid, block, 0, s, a, tiles, splits, pc)
+  if (cols) {
+    if (a.in_bf16) RH_ATTN(cache_attention_cols_kernel, true);
+    else RH_ATTN(cache_attention_cols_kernel, false);
+  } else {
+    if (a.in_bf16) RH_ATTN(cache_attention_kernel, true);
+    else RH_ATTN(cache_attention_kernel, false);
+  }
+#undef RH_ATTN
   if (splits > 1)
     hipLaunchKernelGGL((cache_join_kernel<DH>), dim3(units * tiles), dim3(256), 0, s, a, tiles,
                        splits, pc);

@@ -38,12 +38,15 @@ __device__ __forceinline__ uint32_t finite_abs_bits(float v) {
 // Four values to four e4m3 codes, rounded to nearest even; |v| <= 448, and
 // infinities and NaN become NaN codes.
 __device__ __forceinline__ int fp8_pack4(float a, float b, float c, float d) {
-  int w = 0;
 #if defined(__HIP_DEVICE_COMPILE__)
-  w = __builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false);
-  w = __builtin_amdgcn_cvt_pk_fp8_f32(c, d, w, true);
+  // the first conversion keeps half of a word that the second one writes: any word
+  int w;
+  asm("" : "=v"(w) : "v"(a));
+  w = __builtin_amdgcn_cvt_pk_fp8_f32(a, b, w, false);
+  return __builtin_amdgcn_cvt_pk_fp8_f32(c, d, w, true);
+#else
+  return 0;
 #endif
-  return w;
 }
 __device__ __forceinline__ void fp8_unpack4(int w, float (&v)[4]) {
 #if defined(__HIP_DEVICE_COMPILE__)
@@ -57,12 +60,16 @@ __device__ __forceinline__ void fp8_unpack4(int w, float (&v)[4]) {
 }
 // What four values (|v| <= 448) leave over after rounding to `codes`, times 16
 // and as e4m3 again: codes + 2^-4 * rest is v to 8 bits (exactly, where v has
-// no more than bf16's 8).
+// no more than bf16's 8). 16 v - 16 code is exact, fused or not.
 __device__ __forceinline__ int fp8_rest4(int codes, float a, float b, float c, float d) {
-  float h[4] = {};
-  fp8_unpack4(codes, h);
-  return fp8_pack4((a - h[0]) * 16.0f, (b - h[1]) * 16.0f, (c - h[2]) * 16.0f,
-                   (d - h[3]) * 16.0f);
+#if defined(__HIP_DEVICE_COMPILE__)
+  const v2f lo = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(codes, 16.0f, false);
+  const v2f hi = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(codes, 16.0f, true);
+  return fp8_pack4(__builtin_fmaf(a, 16.0f, -lo[0]), __builtin_fmaf(b, 16.0f, -lo[1]),
+                   __builtin_fmaf(c, 16.0f, -hi[0]), __builtin_fmaf(d, 16.0f, -hi[1]));
+#else
+  return 0;
+#endif
 }
 
 // D += A.B over 64 (128) e4m3 k of 32 x 32 (16 x 16) rows; ea / eb: the scale

@@ -766,16 +766,28 @@ def test_attention_of_other_lengths(gpu_ctx):
 
 
 @pytest.mark.gpu
-def test_attention_skips_pages_that_are_none(gpu_ctx):
+@pytest.mark.parametrize("nq", [1, 300])
+def test_attention_without_pages(gpu_ctx, nq):
+    """A cache of no pages holds no keys."""
+    c = O.Cache(0, 1, 64)
+    q = np.ones((nq, 2, 64))
+    got, _ = attend(gpu_ctx, c, q, "bf16", np.zeros((1, 9), np.int32), np.array([0, nq], np.int32),
+                    np.array([500], np.int32), 0.125, False, 0, False)
+    assert (got == 0).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("fresh", [[5, 1], [60, 70]])
+def test_attention_skips_pages_that_are_none(gpu_ctx, fresh):
     rng = np.random.default_rng(12)
-    pages, table, cu, blk, lens, slots = batch_of(rng, [200, 300], [5, 1])
+    pages, table, cu, blk, lens, slots = batch_of(rng, [200, 300], fresh)
     c = O.Cache(pages, 1, 64)
     acu = np.concatenate([[0], np.cumsum(lens)]).astype(np.int32)
     asl = np.concatenate([table[b, np.arange(n) // 64].astype(np.int64) * 64 + np.arange(n) % 64
                           for b, n in enumerate(lens)])
     k, v = rng.standard_normal((2, len(asl), 1, 64))
     c.append(k, v, acu, asl)
-    q = rng.standard_normal((6, 2, 64))
+    q = rng.standard_normal((int(cu[-1]), 2, 64))
     bad = table.copy()
     bad[0, 1], bad[1, 0], bad[1, 2] = -1, pages, 2 ** 31 - 1
     got, val = attend(gpu_ctx, c, q, "bf16", bad, cu, lens, 0.125, True, 0, False)
@@ -822,6 +834,36 @@ def test_attention_with_what_is_no_number(gpu_ctx, past):
     # a window past the token does not see it
     got, _ = attend(gpu_ctx, c, q, "bf16", table, cu, lens, 0.1, True, 10, False)
     assert np.isfinite(got[50:70]).all() and np.isnan(got[40:50]).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dh", [64, 128, 256])
+@pytest.mark.parametrize("nq", [1, 20, 300])
+@pytest.mark.parametrize("steps", [[0, 20, 40], [0, 60, 120, 176, 240], [240, 0, 60, 288, 448],
+                                   [-448, 448, 0, 448]])
+def test_attention_of_scores_far_apart(gpu_ctx, nq, dh, steps):
+    """Blocks whose scores lie up to 896 apart, upwards and down: every score is a sum of two
+    products that the matrix cores add exactly, so only P's and the sums' roundings are left."""
+    rng = np.random.default_rng(nq + len(steps))
+    n = 64 * len(steps) + 37
+    past = max(0, n - nq)
+    pages, table, cu, blk, lens, slots = batch_of(rng, [past], [nq])
+    n = int(lens[0])
+    c = O.Cache(pages, 1, dh)
+    k = np.zeros((n, 1, dh))
+    k[:, 0, 1] = np.resize(np.repeat(steps, 64), n)
+    k[:, 0, dh - 3] = rng.integers(0, 5, n) / 4
+    v = rng.standard_normal((n, 1, dh))
+    at = table[0, np.arange(n) // 64].astype(np.int64) * 64 + np.arange(n) % 64
+    c.append(k, v, np.array([0, n], np.int32), at)
+    q = np.zeros((nq, 2, dh))
+    q[:, :, 1] = q[:, :, dh - 3] = 1.0
+    kk, vv = c.rows(table[0], n)
+    assert (kk[:, 0, 1] == k[:, 0, 1]).all() and (kk[:, 0, dh - 3] == k[:, 0, dh - 3]).all()
+    for causal in (True, False):
+        got, val = attend(gpu_ctx, c, q, "bf16", table, cu, lens, 1.0, causal, 0, False)
+        want, mag, _ = O.attention(val, kk, vv, 1.0, causal, 0)
+        assert (np.abs(got - want) <= (BF16 + STEP * (1 + 2.0 ** -4)) * mag + 1e-6).all()
 
 
 @pytest.mark.gpu
