@@ -90,6 +90,19 @@ __device__ __forceinline__ void cache_load_q(const void* q, size_t at, int half,
     }
 }
 
+// V's codes behind the last token to zero: nothing was written there, and no NaN code may
+// meet a zero P.
+template <int DH>
+__device__ __forceinline__ void cache_clean_v(v8i (&vf)[DH / 32], int key0, int n, int half) {
+#pragma unroll
+  for (int w = 0; w < 8; w++) {
+    const int left = n - (key0 + w / 4 * 32 + w % 4 * 8 + half * 4);
+    const int keep = left >= 4 ? -1 : left <= 0 ? 0 : (1 << (8 * left)) - 1;
+#pragma unroll
+    for (int t = 0; t < DH / 32; t++) vf[t][w] &= keep;
+  }
+}
+
 // One wave's running state of its 32 columns, and a page's step.
 template <int DH>
 struct CacheTile {
@@ -130,16 +143,7 @@ struct CacheTile {
           sc[t][e] = off > span ? -INFINITY : sc[t][e];
         }
     }
-    if (key0 + kPageT > n) {
-      // nothing was written behind the last token: no NaN code may meet a zero P
-#pragma unroll
-      for (int w = 0; w < 8; w++) {
-        const int left = n - (key0 + w / 4 * 32 + w % 4 * 8 + half * 4);
-        const int keep = left >= 4 ? -1 : left <= 0 ? 0 : (1 << (8 * left)) - 1;
-#pragma unroll
-        for (int t = 0; t < DT; t++) vf[t][w] &= keep;
-      }
-    }
+    if (key0 + kPageT > n) cache_clean_v<DH>(vf, key0, n, half);
     float smax = -INFINITY;
 #pragma unroll
     for (int t = 0; t < 2; t++)
@@ -184,18 +188,129 @@ struct CacheTile {
 
 // A page's fragments of one head: 1 KiB pieces, 16 bytes a lane.
 template <int DH>
-__device__ __forceinline__ void cache_fetch(const uint8_t* k, const uint8_t* v, int lane,
-                                            v8i (&kf)[DH / 64][2], v8i (&vf)[DH / 32]) {
-  const v4i* kp = reinterpret_cast<const v4i*>(k) + lane;
-  const v4i* vp = reinterpret_cast<const v4i*>(v) + lane;
+__device__ __forceinline__ void cache_fetch_k(const uint8_t* k, int lane, v8i (&kf)[DH / 64][2]) {
+  const v4i* at = reinterpret_cast<const v4i*>(k) + lane;
 #pragma unroll
   for (int s = 0; s < DH / 64; s++)
 #pragma unroll
     for (int t = 0; t < 2; t++)
-      kf[s][t] = join8(kp[((s * 2 + t) * 2) * 64], kp[((s * 2 + t) * 2 + 1) * 64]);
-#pragma unroll
-  for (int t = 0; t < DH / 32; t++) vf[t] = join8(vp[t * 2 * 64], vp[(t * 2 + 1) * 64]);
+      kf[s][t] = join8(at[((s * 2 + t) * 2) * 64], at[((s * 2 + t) * 2 + 1) * 64]);
 }
+template <int DH>
+__device__ __forceinline__ void cache_fetch_v(const uint8_t* v, int lane, v8i (&vf)[DH / 32]) {
+  const v4i* at = reinterpret_cast<const v4i*>(v) + lane;
+#pragma unroll
+  for (int t = 0; t < DH / 32; t++) vf[t] = join8(at[t * 2 * 64], at[(t * 2 + 1) * 64]);
+}
+
+// The same with accumulators that products alone touch. O is kept in units of the reference
+// a column starts with (`base`); a reference that has moved since, always by whole powers of
+// two, goes into P's scale byte. A column whose reference moves by more than 2^64 (its earlier
+// keys then weigh nothing in fp32) makes its wave go over its pages once more with CacheTile,
+// whose rescale has no such limit: that branch inside the loops cost the compiler a second
+// copy of O and 8 to 30 spilled registers.
+constexpr float kFar = 64.0f;
+
+template <int DH>
+struct CacheFast {
+  static constexpr int KS = DH / 64, DT = DH / 32;
+  v8i qh[KS], ql[KS];
+  int xh, xl;
+  v16f o[DT], sc[2];
+  v8i ph, pl;  // P of a page,
+  int eh, el;  // its scale bytes
+  float mref, base, lrun;
+  bool far;
+  int klo, khi;
+
+  __device__ __forceinline__ void clear() {
+#pragma unroll
+    for (int t = 0; t < DT; t++) o[t] = v16f{};
+    ph = v8i{};
+    pl = v8i{};
+    eh = el = 127;
+    mref = base = -INFINITY;
+    lrun = 0.0f;
+    far = false;
+  }
+  // With more than 256 registers in use (dh 256) the compiler may move a scale word to an
+  // accumulation register, which the instruction does not take: held in a VGPR here.
+  static __device__ __forceinline__ v16f mul(const v8i& a, const v8i& b, const v16f& c, int ea,
+                                             int eb) {
+    if constexpr (DH == 256) asm("" : "+v"(ea), "+v"(eb));
+    return mfma_fp8_32(a, b, c, ea, eb);
+  }
+  // Scores of a page (first position key0) to their maximum; moves the reference. `none`:
+  // the page holds no keys at all.
+  __device__ __forceinline__ void refer(int key0, bool none, float cs, int half) {
+    if (__builtin_expect(none || __any(key0 < klo || key0 + kPageT - 1 > khi), 0)) {
+      const unsigned span = (unsigned)(khi - klo);
+      const int at = key0 + half * 4 - klo;
+#pragma unroll
+      for (int t = 0; t < 2; t++)
+#pragma unroll
+        for (int e = 0; e < 16; e++) {
+          const unsigned off = (unsigned)(at + t * 32 + e / 4 * 8 + e % 4);
+          sc[t][e] = none || off > span ? -INFINITY : sc[t][e];
+        }
+    }
+    float smax = -INFINITY;
+#pragma unroll
+    for (int t = 0; t < 2; t++)
+#pragma unroll
+      for (int e = 0; e < 16; e++) smax = fmaxf(smax, sc[t][e]);
+    const float mloc = max_halves(smax) * cs;
+    const bool up = mloc > mref + kHead;  // -inf + 4 = -inf: the first visible key moves it
+    const float to = up ? __builtin_ceilf(mloc) : mref;
+    lrun *= up ? __builtin_amdgcn_exp2f(mref - to) : 1.0f;
+    mref = to;
+    base = base == -INFINITY ? to : base;
+  }
+  // What P's exponentials are taken against: a column with no visible key yet gets 2^(-inf).
+  __device__ __forceinline__ float origin() const { return mref == -INFINITY ? 0.0f : mref - kHead; }
+  __device__ __forceinline__ void scales() {
+    const float moved = mref == -INFINITY ? 0.0f : mref - base;
+    far |= moved > kFar;
+    eh = 127 + (int)fminf(moved, kFar);
+    el = eh - 4;
+  }
+  // O's unit in units of the last reference
+  __device__ __forceinline__ float unit() const {
+    return mref == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(base - mref);
+  }
+  // one page, its fragments in registers (CacheTile::page)
+  __device__ __forceinline__ void page(const v8i (&kf)[KS][2], v8i (&vf)[DT], int xk, int xv,
+                                       int key0, int n, float cs, int half) {
+    sc[0] = v16f{};
+    sc[1] = v16f{};
+#pragma unroll
+    for (int s = 0; s < KS; s++)
+#pragma unroll
+      for (int u = 0; u < 4; u++)
+        sc[u % 2] = mul(kf[s][u % 2], u < 2 ? qh[s] : ql[s], sc[u % 2], xk, u < 2 ? xh : xl);
+    refer(key0, false, cs, half);
+    if (key0 + kPageT > n) cache_clean_v<DH>(vf, key0, n, half);
+    const float m = origin();
+#pragma unroll
+    for (int t = 0; t < 2; t++)
+#pragma unroll
+      for (int w = 0; w < 4; w++) {
+        float x[4];
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+          x[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[t][4 * w + e], cs, -m));
+          lrun += x[e];
+        }
+        ph[4 * t + w] = fp8_pack4(x[0], x[1], x[2], x[3]);
+        pl[4 * t + w] = fp8_rest4(ph[4 * t + w], x[0], x[1], x[2], x[3]);
+      }
+    scales();
+#pragma unroll
+    for (int t = 0; t < DT; t++) o[t] = mul(vf[t], ph, o[t], xv, eh);
+#pragma unroll
+    for (int t = 0; t < DT; t++) o[t] = mul(vf[t], pl, o[t], xv, el);
+  }
+};
 
 // Page ids and scale bytes of 64 consecutive pages of a request, one a lane: read once, then
 // taken lane by lane, so that no page waits for its table entry and scales.
@@ -222,19 +337,28 @@ struct PageWindow {
   }
 };
 
-// Workgroup -> (request, kv head, tile of columns, key range). Units of one (request,
-// kv head) read the same pages: their workgroups are dealt to one XCD (workgroup w
-// runs on XCD w % 8) and share its L2.
-__device__ __forceinline__ bool cache_unit(const CacheAttnArgs& p, int tiles, int splits, int& b,
+// Workgroup -> (request, kv head, tile of columns, key range). A unit's workgroups (one
+// request and kv head) read the same pages: where eight units are left their workgroups are
+// dealt to an XCD each (workgroup w runs on XCD w % 8) and share its L2, the last ones are
+// spread over all XCDs.
+__device__ __forceinline__ void cache_unit(const CacheAttnArgs& p, int tiles, int splits, int& b,
                                            int& h, int& tile, int& split) {
-  const int w = blockIdx.x, nv = tiles * splits;
-  const int t = w >> 3, v = t % nv, u = (t / nv) * 8 + (w & 7);
-  if (u >= p.batch * p.cache.kv_heads) return false;
+  const int units = p.batch * p.cache.kv_heads, nv = tiles * splits;
+  const int whole = units / 8 * 8, w = blockIdx.x;
+  int u, v;
+  if (w < whole * nv) {
+    const int t = w >> 3;
+    v = t % nv;
+    u = (t / nv) * 8 + (w & 7);
+  } else {
+    const int left = units - whole, t = w - whole * nv;
+    v = t / left;
+    u = whole + t % left;
+  }
   b = u / p.cache.kv_heads;
   h = u % p.cache.kv_heads;
   tile = v / splits;
   split = v % splits;
-  return true;
 }
 
 // Pages [lo, hi) that columns c0 .. c1 - 1 of a request see.
@@ -261,14 +385,56 @@ __device__ __forceinline__ void cache_store4(const CacheAttnArgs& p, size_t to, 
   }
 }
 
+// A wave's pages first, first + each, .. once more, by CacheTile; O, reference and sum to w,
+// whose unit is then the reference.
+template <int DH>
+__device__ __forceinline__ void cache_again(CacheFast<DH>& w, const CacheAttnArgs& p, int b, int h,
+                                            int first, int end, int each, int n, float cs,
+                                            int lane) {
+  constexpr int KS = DH / 64, DT = DH / 32, kHalf = kPageT * DH;
+  CacheTile<DH> r;
+#pragma unroll
+  for (int s = 0; s < KS; s++) {
+    r.qh[s] = w.qh[s];
+    r.ql[s] = w.ql[s];
+  }
+  r.xh = w.xh;
+  r.xl = w.xl;
+  r.klo = w.klo;
+  r.khi = w.khi;
+  r.clear();
+  for (int g = first; g < end; g += each) {
+    const int page = p.table[(size_t)b * p.ldt + g];
+    if (page < 0 || page >= p.cache.pages) continue;
+    const size_t u = (size_t)page * p.cache.kv_heads + h;
+    v8i kf[KS][2], vf[DT];
+    cache_fetch_k<DH>(p.cache.k + u * kHalf, lane, kf);
+    cache_fetch_v<DH>(p.cache.v + u * kHalf, lane, vf);
+    r.page(kf, vf, p.cache.k_exp[u], p.cache.v_exp[u], g * kPageT, n, cs, lane >> 5);
+  }
+#pragma unroll
+  for (int t = 0; t < DT; t++) w.o[t] = r.o[t];
+  w.mref = w.base = r.mref;
+  w.lrun = r.lrun;
+}
+
+// A row of a partial result: DH values, the reference and the sum, 16-byte aligned.
+template <int DH>
+constexpr int kPartRow = DH + 4;
+
+// ---- few columns -----------------------------------------------------------------------
+// Four waves share a tile of columns and take its pages in turn, straight to registers: what
+// bounds it is the cache's bytes, each read once. Page g + 4's K is on its way while page g
+// is multiplied. The waves' results are joined in LDS, eight columns at a time.
 template <int DH, bool BF16>
-__global__ __launch_bounds__(64 * kWaves) void cache_attention_kernel(CacheAttnArgs p, int tiles,
-                                                                      int splits, int part_cols) {
-  constexpr int KS = DH / 64, DT = DH / 32, kStride = DH + 4;
-  __shared__ __attribute__((aligned(16))) float s_o[kCols * kStride];
+__global__ __launch_bounds__(64 * kWaves, DH == 256 ? 1 : 2) void cache_attention_kernel(
+    CacheAttnArgs p, int tiles, int splits, int part_cols) {
+  constexpr int KS = DH / 64, DT = DH / 32, kStride = DH + 4, kHalf = kPageT * DH;
+  constexpr int kJoin = 8;  // columns joined at a time
+  __shared__ __attribute__((aligned(16))) float s_o[kWaves][kJoin][kStride];
   __shared__ float s_m[kWaves][kCols], s_l[kWaves][kCols];
   int b, h, tile, split;
-  if (!cache_unit(p, tiles, splits, b, h, tile, split)) return;
+  cache_unit(p, tiles, splits, b, h, tile, split);
   const int G = p.heads / p.cache.kv_heads;
   const int r0 = p.cu[b], nq = p.cu[b + 1] - r0;
   const int cols = nq * G, c0 = tile * kCols;
@@ -276,92 +442,98 @@ __global__ __launch_bounds__(64 * kWaves) void cache_attention_kernel(CacheAttnA
   const int n = max(0, min(p.lens[b], p.ldt * kPageT));
   const int lane = threadIdx.x & 63, col = lane & 31, half = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int c = min(c0 + col, cols - 1);
+  const int c = min(c0 + col, cols - 1), ct = c / G;
   const int pos0 = n - nq;  // position of the first new token
   const float cs = p.scale * 1.44269504088896341f;
-
-  CacheTile<DH> w;
-  cache_load_q<KS, BF16>(p.q, (size_t)(r0 + c / G) * p.ldq + p.q_off + (h * G + c % G) * DH, half,
-                         w.qh, w.ql, w.xh, w.xl);
-  w.clear();
-  cache_key_range(p, pos0 + c / G, n, w.klo, w.khi);
 
   // the tile's pages, this split's share of them
   int lo, hi;
   cache_page_range(p, pos0, n, G, c0, min(c0 + kCols, cols), lo, hi);
+  if (p.cache.pages < 1) hi = lo;
   const int each = (max(0, hi - lo) + splits - 1) / splits;
   const int first = lo + split * each, end = min(hi, first + each);
   PageWindow win;
+  if (first < end) win.load(p, b, h, first, end, lane);
+
+  CacheFast<DH> w;
+  cache_load_q<KS, BF16>(p.q, (size_t)(r0 + ct) * p.ldq + p.q_off + (h * G + c - ct * G) * DH, half,
+                         w.qh, w.ql, w.xh, w.xl);
+  w.clear();
+  cache_key_range(p, pos0 + ct, n, w.klo, w.khi);
+
   for (int g0 = first; g0 < end; g0 += 64) {
-    if (p.cache.pages < 1) break;
-    win.load(p, b, h, g0, end, lane);
-    const int last = min(end, g0 + 64);
-    for (int g = g0 + wave; g < last; g += kWaves) {
-      const int page = win.at(win.page, g - g0);
+    if (g0 > first) win.load(p, b, h, g0, end, lane);
+    const int count = min(64, end - g0);
+    for (int i = wave; i < count; i += kWaves) {
+      const int page = win.at(win.page, i);
       if (page < 0) continue;  // no such page: no keys
-      const size_t at = ((size_t)page * p.cache.kv_heads + h) * (kPageT * DH);
+      const size_t at = ((size_t)page * p.cache.kv_heads + h) * kHalf;
       v8i kf[KS][2], vf[DT];
-      cache_fetch<DH>(p.cache.k + at, p.cache.v + at, lane, kf, vf);
-      w.page(kf, vf, win.at(win.xk, g - g0), win.at(win.xv, g - g0), g * kPageT, n, cs, half);
+      cache_fetch_k<DH>(p.cache.k + at, lane, kf);
+      cache_fetch_v<DH>(p.cache.v + at, lane, vf);
+      w.page(kf, vf, win.at(win.xk, i), win.at(win.xv, i), (g0 + i) * kPageT, n, cs, half);
     }
   }
 
-  // join the waves: columns' references and sums, then O in wave order
-  float l = w.lrun + __shfl_xor(w.lrun, 32, 64);
-  if (half == 0) {
-    s_m[wave][col] = w.mref;
-    s_l[wave][col] = l;
+  if (__builtin_expect(__any(w.far), 0))
+    cache_again<DH>(w, p, b, h, first + wave, end, kWaves, n, cs, lane);
+  const float unit = w.unit();
+
+  // join the waves: the columns' references and sums, then O in wave order
+  {
+    const float l = w.lrun + __shfl_xor(w.lrun, 32, 64);
+    if (half == 0) {
+      s_m[wave][col] = w.mref;
+      s_l[wave][col] = l;
+    }
   }
-  __syncthreads();
-  float m = -INFINITY;
-#pragma unroll
-  for (int i = 0; i < kWaves; i++) m = fmaxf(m, s_m[i][col]);
-  const float mine = w.mref == -INFINITY ? (l == 0.0f ? 0.0f : l) : __builtin_amdgcn_exp2f(w.mref - m);
-  for (int i = 0; i < kWaves; i++) {
-    if (wave == i) {
+  const int here = min(kCols, cols - c0);
+  constexpr int LPR = DH / 4, kRows = 64 * kWaves / LPR;
+  for (int j0 = 0; j0 < here; j0 += kJoin) {
+    if (col >= j0 && col < j0 + kJoin && c0 + col < cols) {
 #pragma unroll
       for (int t = 0; t < DT; t++)
 #pragma unroll
         for (int q4 = 0; q4 < 4; q4++) {
-          v4f* at = reinterpret_cast<v4f*>(s_o + col * kStride + t * 32 + q4 * 8 + half * 4);
-          v4f x = i == 0 ? v4f{0.0f, 0.0f, 0.0f, 0.0f} : *at;
+          v4f x;
 #pragma unroll
-          for (int e = 0; e < 4; e++) x[e] += w.o[t][q4 * 4 + e] * mine;
-          *at = x;
+          for (int e = 0; e < 4; e++) x[e] = w.o[t][q4 * 4 + e] * unit;
+          *reinterpret_cast<v4f*>(&s_o[wave][col - j0][t * 32 + q4 * 8 + half * 4]) = x;
         }
     }
     __syncthreads();
-  }
-  // a row of the tile per LPR threads, 4 values each
-  constexpr int LPR = DH / 4, RPP = 64 * kWaves / LPR;
-  const int d = threadIdx.x % LPR * 4;
-  for (int rr = threadIdx.x / LPR; rr < min(kCols, cols - c0); rr += RPP) {
-    float mm = -INFINITY, ll = 0.0f;
+    const int d = threadIdx.x % LPR * 4;
+    for (int r = threadIdx.x / LPR; r < min(kJoin, here - j0); r += kRows) {
+      float m = -INFINITY, l = 0.0f;
 #pragma unroll
-    for (int i = 0; i < kWaves; i++) mm = fmaxf(mm, s_m[i][rr]);
+      for (int k = 0; k < kWaves; k++) m = fmaxf(m, s_m[k][j0 + r]);
+      v4f x = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-    for (int i = 0; i < kWaves; i++) {
-      const float f = s_m[i][rr] == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(s_m[i][rr] - mm);
-      ll += s_l[i][rr] * f;  // a wave with no visible key has a sum of 0 (or NaN)
-    }
-    v4f x = *reinterpret_cast<const v4f*>(s_o + rr * kStride + d);
-    const int cc = c0 + rr;
-    if (splits > 1) {
-      const size_t u = ((size_t)b * p.cache.kv_heads + h) * tiles + tile;
-      float* at = p.part + (u * splits + split) * (size_t)part_cols * (DH + 2) +
-                  (size_t)rr * (DH + 2);
-      typedef float v2 __attribute__((ext_vector_type(2)));
-      *reinterpret_cast<v2*>(at + d) = (v2){x[0], x[1]};
-      *reinterpret_cast<v2*>(at + d + 2) = (v2){x[2], x[3]};
-      if (d == 0) {
-        at[DH] = mm;
-        at[DH + 1] = ll;
+      for (int k = 0; k < kWaves; k++) {
+        // a wave with no visible key has zeros (or, with a NaN, that)
+        const float mk = s_m[k][j0 + r];
+        const float f = mk == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(mk - m);
+        l += s_l[k][j0 + r] * f;
+        const v4f y = *reinterpret_cast<const v4f*>(&s_o[k][r][d]);
+#pragma unroll
+        for (int e = 0; e < 4; e++) x[e] += y[e] * f;
       }
-      continue;
+      const int cc = c0 + j0 + r;
+      if (splits > 1) {
+        const size_t u = ((size_t)b * p.cache.kv_heads + h) * tiles + tile;
+        float* to = p.part + ((u * splits + split) * part_cols + j0 + r) * kPartRow<DH>;
+        *reinterpret_cast<v4f*>(to + d) = x;
+        if (d == 0) {
+          to[DH] = m;
+          to[DH + 1] = l;
+        }
+      } else {
+        x *= l == 0.0f ? 0.0f : 1.0f / l;
+        const int tt = cc / G;
+        cache_store4(p, (size_t)(r0 + tt) * p.ldout + (h * G + cc - tt * G) * DH + d, x);
+      }
     }
-    const float inv = ll == 0.0f ? 0.0f : 1.0f / ll;
-    x *= inv;
-    cache_store4(p, (size_t)(r0 + cc / G) * p.ldout + (h * G + cc % G) * DH + d, x);
+    __syncthreads();
   }
 }
 
@@ -374,35 +546,13 @@ __global__ __launch_bounds__(64 * kWaves) void cache_attention_kernel(CacheAttnA
 // page g + 1's scores and page g - 1's values. K and V come to LDS by global_load_lds in
 // fragment order (1 KiB pieces, read back without bank conflicts), two turns before they are
 // used, with one barrier per turn.
-//
-// The accumulators are touched by products alone: O is kept in units of the reference a
-// column starts with (`base`), and a reference that has moved since, always by whole
-// powers of two, goes into P's scale byte. A column whose reference moves by more than
-// 2^64 (its earlier keys then weigh nothing in fp32) makes its wave go over the pages once
-// more after the loop, with CacheTile, whose rescale has no such limit: kept in the loop,
-// that branch cost the compiler a second copy of O and 20 spilled registers.
-constexpr float kFar = 64.0f;
-
 template <int DH>
-struct CachePipe {
-  static constexpr int KS = DH / 64, DT = DH / 32;
-  static constexpr int NF = 2 * KS + DT;  // fragments of a page: K's, then V's
-  v8i qh[KS], ql[KS];
-  int xh, xl;
-  v16f o[DT], sc[2];
-  v8i ph, pl;  // P of the page before,
-  int eh, el;  // its scale bytes
-  float mref, base, lrun;
-  bool far;
-  int klo, khi;
+struct CachePipe : CacheFast<DH> {  // ph, pl, eh, el: P of the page before
+  using Base = CacheFast<DH>;
+  using Base::qh, Base::ql, Base::xh, Base::xl, Base::o, Base::sc, Base::ph, Base::pl, Base::eh,
+      Base::el, Base::lrun, Base::mul, Base::KS, Base::DT;
+  static constexpr int NF = 2 * KS + DT;  // fragments of a page
 
-  // With more than 256 registers in use (dh 256) the compiler may move a scale word to an
-  // accumulation register, which the instruction does not take: held in a VGPR here.
-  static __device__ __forceinline__ v16f mul(const v8i& a, const v8i& b, const v16f& c, int ea,
-                                             int eb) {
-    if constexpr (DH == 256) asm("" : "+v"(ea), "+v"(eb));
-    return mfma_fp8_32(a, b, c, ea, eb);
-  }
   // fragment f of a page at its lane's place in LDS
   static __device__ __forceinline__ v8i frag(const uint8_t* at, int f) {
     return join8(*reinterpret_cast<const v4i*>(at + 2 * f * 1024),
@@ -427,37 +577,10 @@ struct CachePipe {
       o[t] = mul(a, pl, o[t], xv, el);
     }
   }
-  // Scores of page g (first position key0) to their maximum; moves the reference. `none`:
-  // the page holds no keys at all.
-  __device__ __forceinline__ void refer(int key0, bool none, float cs, int half) {
-    if (__builtin_expect(none || __any(key0 < klo || key0 + kPageT - 1 > khi), 0)) {
-      const unsigned span = (unsigned)(khi - klo);
-      const int at = key0 + half * 4 - klo;
-#pragma unroll
-      for (int t = 0; t < 2; t++)
-#pragma unroll
-        for (int e = 0; e < 16; e++) {
-          const unsigned off = (unsigned)(at + t * 32 + e / 4 * 8 + e % 4);
-          sc[t][e] = none || off > span ? -INFINITY : sc[t][e];
-        }
-    }
-    float smax = -INFINITY;
-#pragma unroll
-    for (int t = 0; t < 2; t++)
-#pragma unroll
-      for (int e = 0; e < 16; e++) smax = fmaxf(smax, sc[t][e]);
-    const float mloc = max_halves(smax) * cs;
-    const bool up = mloc > mref + kHead;  // -inf + 4 = -inf: the first visible key moves it
-    const float to = up ? __builtin_ceilf(mloc) : mref;
-    lrun *= up ? __builtin_amdgcn_exp2f(mref - to) : 1.0f;
-    mref = to;
-    base = base == -INFINITY ? to : base;
-  }
   // P of page g, between the values of page g - 1 (v, xv) and the scores of g + 1 (k, xk).
   __device__ __forceinline__ void turn(const uint8_t* k, int xk, const uint8_t* v, int xv,
                                        float cs) {
-    // a column with no visible key yet: every p = 2^(-inf) = 0
-    const float m = mref == -INFINITY ? 0.0f : mref - kHead;
+    const float m = Base::origin();
     v16f s[2] = {v16f{}, v16f{}};
     v8i nh, nl;
     constexpr int kPairs = 16;
@@ -523,7 +646,6 @@ struct CachePipe {
         const int at = 2 * f + u;  // of NM
 #pragma unroll
         for (int j = at * kPairs / NM; j < (at + 1) * kPairs / NM; j++) pair(j);
-        __builtin_amdgcn_sched_barrier(0);
       }
       a0 = b0;
       a1 = b1;
@@ -532,10 +654,7 @@ struct CachePipe {
     pair(kPairs + 1);
     ph = nh;
     pl = nl;
-    const float moved = mref == -INFINITY ? 0.0f : mref - base;
-    far |= moved > kFar;
-    eh = 127 + (int)fminf(moved, kFar);
-    el = eh - 4;
+    Base::scales();
     sc[0] = s[0];
     sc[1] = s[1];
   }
@@ -545,14 +664,12 @@ template <int DH, bool BF16>
 __global__ __launch_bounds__(64 * kWaves, DH == 256 ? 1 : 2) void cache_attention_cols_kernel(
     CacheAttnArgs p, int tiles, int splits, int part_cols) {
   constexpr int KS = DH / 64, DT = DH / 32, kHalf = kPageT * DH;  // bytes of K or V of a page
-  constexpr int kStride = DH + 4, kLds = 6 * kHalf;  // K of three pages, V of three
+  constexpr int kLds = 6 * kHalf;  // K of three pages, V of three
   constexpr int kPieces = kHalf / 1024 / kWaves;     // 1 KiB pieces per wave, of K and of V
-  constexpr int kBand = 8;  // output rows of a wave staged at a time
-  static_assert(kWaves * kBand * kStride * 4 <= kLds, "output staging");
   __shared__ __attribute__((aligned(1024))) uint8_t lds[kLds];
   const int wgs = (tiles + kWaves - 1) / kWaves;
   int b, h, wg, split;
-  if (!cache_unit(p, wgs, splits, b, h, wg, split)) return;
+  cache_unit(p, wgs, splits, b, h, wg, split);
   if (p.causal) {
     // later columns see more pages: each XCD's 32 CUs get the long ones first, then
     // the next 32 in the other order, so that long and short ones share a CU
@@ -567,7 +684,7 @@ __global__ __launch_bounds__(64 * kWaves, DH == 256 ? 1 : 2) void cache_attentio
   const int lane = threadIdx.x & 63, col = lane & 31, half = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int tile = wg * kWaves + wave, c0 = tile * kCols;
-  const int c = min(c0 + col, cols - 1);
+  const int c = min(c0 + col, cols - 1), ct = c / G;
   const int pos0 = n - nq;
   const float cs = p.scale * 1.44269504088896341f;
 
@@ -611,17 +728,10 @@ __global__ __launch_bounds__(64 * kWaves, DH == 256 ? 1 : 2) void cache_attentio
     dma(p.cache.v, win.at(win.page, 0), ldsv + kHalf);
     dma(p.cache.k, win.at(win.page, 2), ldsk + 2 * kHalf);
   }
-  cache_load_q<KS, BF16>(p.q, (size_t)(r0 + c / G) * p.ldq + p.q_off + (h * G + c % G) * DH, half,
+  cache_load_q<KS, BF16>(p.q, (size_t)(r0 + ct) * p.ldq + p.q_off + (h * G + c - ct * G) * DH, half,
                          w.qh, w.ql, w.xh, w.xl);
-#pragma unroll
-  for (int t = 0; t < DT; t++) w.o[t] = v16f{};
-  w.ph = v8i{};
-  w.pl = v8i{};
-  w.eh = w.el = 127;
-  w.mref = w.base = -INFINITY;
-  w.lrun = 0.0f;
-  w.far = false;
-  cache_key_range(p, pos0 + c / G, n, w.klo, w.khi);
+  w.clear();
+  cache_key_range(p, pos0 + ct, n, w.klo, w.khi);
   // turn g: K of g + 1 in slot ks of ldsk, V of g - 1 in slot vs of ldsv
   int ks = 1, vs = 0;
   bool nonep = false, none = false;  // page g - 1, g is none
@@ -680,118 +790,69 @@ __global__ __launch_bounds__(64 * kWaves, DH == 256 ? 1 : 2) void cache_attentio
   }
   __syncthreads();
   if (!active) return;
-  // O from units of the first reference to units of the last one
-  float unit = w.mref == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(w.base - w.mref);
-  if (__builtin_expect(__any(w.far), 0)) {
-    CacheTile<DH> r;
-#pragma unroll
-    for (int s = 0; s < KS; s++) {
-      r.qh[s] = w.qh[s];
-      r.ql[s] = w.ql[s];
-    }
-    r.xh = w.xh;
-    r.xl = w.xl;
-    r.klo = w.klo;
-    r.khi = w.khi;
-    r.clear();
-    for (int g = first; g < end; g++) {
-      const int page = p.table[(size_t)b * p.ldt + g];
-      if (page < 0 || page >= p.cache.pages) continue;
-      const size_t u = (size_t)page * p.cache.kv_heads + h;
-      v8i kf[KS][2], vf[DT];
-      cache_fetch<DH>(p.cache.k + u * kHalf, p.cache.v + u * kHalf, lane, kf, vf);
-      r.page(kf, vf, p.cache.k_exp[u], p.cache.v_exp[u], g * kPageT, n, cs, half);
-    }
-#pragma unroll
-    for (int t = 0; t < DT; t++) w.o[t] = r.o[t];
-    w.mref = r.mref;
-    w.lrun = r.lrun;
-    unit = 1.0f;
-  }
+  if (__builtin_expect(__any(w.far), 0))
+    cache_again<DH>(w, p, b, h, first, end, 1, n, cs, lane);
+  const float unit = w.unit();
 
-  // O^T through this wave's LDS rows to whole output rows
+  // a lane holds four consecutive values of its column at a time, its other half the
+  // next four
   const float l = w.lrun + __shfl_xor(w.lrun, 32, 64);
   const float inv = splits > 1 ? unit : l == 0.0f ? 0.0f : unit / l;
-  float* st = reinterpret_cast<float*>(lds) + wave * kBand * kStride;
+  if (c0 + col >= cols) return;
   float* part = nullptr;
   if (splits > 1) {
     const size_t u = ((size_t)b * p.cache.kv_heads + h) * tiles + tile;
-    part = p.part + (u * splits + split) * (size_t)part_cols * (DH + 2);
-    if (half == 0 && c0 + col < cols) {
-      part[(size_t)col * (DH + 2) + DH] = w.mref;
-      part[(size_t)col * (DH + 2) + DH + 1] = l;
+    part = p.part + ((u * splits + split) * part_cols + col) * kPartRow<DH>;
+    if (half == 0) {
+      part[DH] = w.mref;
+      part[DH + 1] = l;
     }
   }
-  constexpr int LPR = DH / 4, RPI = 64 / LPR;  // lanes per row, rows per instruction
-  const int d = lane % LPR * 4;
+  const size_t to = (size_t)(r0 + ct) * p.ldout + (h * G + c - ct * G) * DH;
 #pragma unroll
-  for (int band = 0; band < kCols; band += kBand) {
-    if (col >= band && col < band + kBand) {
+  for (int t = 0; t < DT; t++)
 #pragma unroll
-      for (int t = 0; t < DT; t++)
+    for (int i = 0; i < 4; i++) {
+      v4f x;
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-          v4f x;
-#pragma unroll
-          for (int e = 0; e < 4; e++) x[e] = w.o[t][i * 4 + e] * inv;
-          *reinterpret_cast<v4f*>(st + (col - band) * kStride + t * 32 + i * 8 + half * 4) = x;
-        }
+      for (int e = 0; e < 4; e++) x[e] = w.o[t][i * 4 + e] * inv;
+      const int d = t * 32 + i * 8 + half * 4;
+      if (part) *reinterpret_cast<v4f*>(part + d) = x;
+      else cache_store4(p, to + d, x);
     }
-    wait_lgkmcnt0();
-    __builtin_amdgcn_wave_barrier();
-    for (int rr = lane / LPR; rr < kBand; rr += RPI) {
-      const int cc = c0 + band + rr;
-      if (cc >= cols) break;
-      const v4f x = *reinterpret_cast<const v4f*>(st + rr * kStride + d);
-      if (part) {
-        typedef float v2 __attribute__((ext_vector_type(2)));
-        float* at = part + (size_t)(band + rr) * (DH + 2) + d;
-        *reinterpret_cast<v2*>(at) = (v2){x[0], x[1]};
-        *reinterpret_cast<v2*>(at + 2) = (v2){x[2], x[3]};
-      } else {
-        cache_store4(p, (size_t)(r0 + cc / G) * p.ldout + (h * G + cc % G) * DH + d, x);
-      }
-    }
-    __builtin_amdgcn_wave_barrier();
-  }
 }
 
 // Partial results of a tile's key ranges to its output rows, in range order.
 template <int DH>
 __global__ __launch_bounds__(256) void cache_join_kernel(CacheAttnArgs p, int tiles, int splits,
                                                          int part_cols) {
-  constexpr int LPR = DH / 2;
+  constexpr int LPR = DH / 4;
   const int G = p.heads / p.cache.kv_heads;
   const int u = blockIdx.x;
   const int tile = u % tiles, h = u / tiles % p.cache.kv_heads, b = u / tiles / p.cache.kv_heads;
   const int r0 = p.cu[b], nq = p.cu[b + 1] - r0;
   const int cols = nq * G, c0 = tile * kCols;
-  const int d = threadIdx.x % LPR * 2;
-  typedef float v2 __attribute__((ext_vector_type(2)));
+  const int d = threadIdx.x % LPR * 4;
+  const size_t step = (size_t)part_cols * kPartRow<DH>;
   for (int rr = threadIdx.x / LPR; rr < min(kCols, cols - c0); rr += 256 / LPR) {
-    const float* at = p.part + ((size_t)u * splits * part_cols + rr) * (DH + 2);
-    const size_t step = (size_t)part_cols * (DH + 2);
+    const float* at = p.part + ((size_t)u * splits * part_cols + rr) * kPartRow<DH>;
     float m = -INFINITY, l = 0.0f;
-    for (int s = 0; s < splits; s++) m = fmaxf(m, at[s * step + DH]);
-    v2 x = {0.0f, 0.0f};
+    v4f x = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 4
     for (int s = 0; s < splits; s++) {
-      const float ms = at[s * step + DH];
-      const float f = ms == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(ms - m);
-      l += at[s * step + DH + 1] * f;
-      const v2 y = *reinterpret_cast<const v2*>(at + s * step + d);
-      x[0] += y[0] * f;
-      x[1] += y[1] * f;
+      const float ms = at[s * step + DH], ls = at[s * step + DH + 1];
+      const v4f y = *reinterpret_cast<const v4f*>(at + s * step + d);
+      const float to = fmaxf(m, ms);
+      const float f = m == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - to);
+      const float g = ms == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(ms - to);
+      l = l * f + ls * g;
+#pragma unroll
+      for (int e = 0; e < 4; e++) x[e] = x[e] * f + y[e] * g;
+      m = to;
     }
-    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-    const int cc = c0 + rr;
-    const size_t to = (size_t)(r0 + cc / G) * p.ldout + (h * G + cc % G) * DH + d;
-    if (p.out_bf16) {
-      typedef __bf16 v2bf __attribute__((ext_vector_type(2)));
-      *reinterpret_cast<v2bf*>(static_cast<__bf16*>(p.out) + to) =
-          (v2bf){(__bf16)(x[0] * inv), (__bf16)(x[1] * inv)};
-    } else {
-      *reinterpret_cast<v2*>(static_cast<float*>(p.out) + to) = (v2){x[0] * inv, x[1] * inv};
-    }
+    x *= l == 0.0f ? 0.0f : 1.0f / l;
+    const int cc = c0 + rr, tt = cc / G;
+    cache_store4(p, (size_t)(r0 + tt) * p.ldout + (h * G + cc - tt * G) * DH + d, x);
   }
 }
 
@@ -808,33 +869,40 @@ static bool cache_by_cols(int max_q, int heads, int kv_heads) {
   return (long long)max_q * (heads / kv_heads) > kCols;
 }
 
-// Key ranges: as many as give the chip's 256 CUs four workgroups each (by columns: one),
-// where a range still has a page for every wave (by columns: eight pages).
+// Key ranges: as many as give the chip's 256 CUs six workgroups each (by columns: one),
+// where a range still has a page for every wave (by columns: 16 pages). A window leaves a
+// tile few pages, and no range of its own for each: 0 (any window) never gives fewer ranges
+// than a window does.
 void cache_attention_plan(int batch, int max_q, int max_len, int heads, int kv_heads, int dh,
-                          int* splits, size_t* part_floats) {
+                          int window, int* splits, size_t* part_floats) {
   const long long tiles = cache_tiles(max_q, heads, kv_heads);
   const long long units = (long long)batch * kv_heads * tiles;
-  const long long pages = ((long long)max_len + kPageT - 1) / kPageT;
   const bool cols = cache_by_cols(max_q, heads, kv_heads);
   const long long wgs = cols ? (long long)batch * kv_heads * ((tiles + kWaves - 1) / kWaves) : units;
-  const long long want = cols ? 256 : 1024;
+  long long pages = ((long long)max_len + kPageT - 1) / kPageT;
+  if (window > 0) {
+    const long long tokens = std::min<long long>(max_q, kCols * (cols ? kWaves : 1));
+    pages = std::min(pages, (2LL * window + tokens) / kPageT + 2);
+  }
+  const long long want = cols ? 256 : 1536;
   long long s = wgs > 0 ? (want + wgs - 1) / wgs : 1;
-  s = std::max(1LL, std::min(s, pages / (cols ? 8 : kWaves)));
+  s = std::max(1LL, std::min(s, pages / (cols ? 16 : kWaves)));
   *splits = (int)s;
-  *part_floats = s > 1 ? (size_t)units * s * cache_part_cols(max_q, heads, kv_heads) * (dh + 2) : 0;
+  *part_floats = s > 1 ? (size_t)units * s * cache_part_cols(max_q, heads, kv_heads) * (dh + 4) : 0;
 }
 
 template <int DH>
 static hipError_t launch_dh(const CacheAttnArgs& a, hipStream_t s) {
   int splits;
   size_t part;
-  cache_attention_plan(a.batch, a.max_q, a.max_len, a.heads, a.cache.kv_heads, DH, &splits, &part);
+  cache_attention_plan(a.batch, a.max_q, a.max_len, a.heads, a.cache.kv_heads, DH, a.window, &splits,
+                       &part);
   const int tiles = cache_tiles(a.max_q, a.heads, a.cache.kv_heads);
   const int pc = cache_part_cols(a.max_q, a.heads, a.cache.kv_heads);
   const int units = a.batch * a.cache.kv_heads;
   const bool cols = cache_by_cols(a.max_q, a.heads, a.cache.kv_heads);
   const int per = cols ? (tiles + kWaves - 1) / kWaves : tiles;
-  const dim3 grid((unsigned)((units + 7) / 8 * 8 * per * splits)), block(64 * kWaves);
+  const dim3 grid((unsigned)(units * per * splits)), block(64 * kWaves);
 #define RH_ATTN(K, B) hipLaunchKernelGGL((K<DH, B>), grid, block, 0, s, a, tiles, splits, pc)
   if (cols) {
     if (a.in_bf16) RH_ATTN(cache_attention_cols_kernel, true);

@@ -298,7 +298,7 @@ size_t rh_cache_attention_scratch(int batch, int max_q, int max_len, int heads, 
     return 0;
   int splits;
   size_t floats;
-  cache_attention_plan(batch, max_q, max_len, heads, kv_heads, dh, &splits, &floats);
+  cache_attention_plan(batch, max_q, max_len, heads, kv_heads, dh, 0, &splits, &floats);
   return floats * sizeof(float);
 }
 

@@ -172,7 +172,7 @@ struct CacheAttnArgs {
 };
 // Key ranges per tile of query columns and the floats of their partial results.
 void cache_attention_plan(int batch, int max_q, int max_len, int heads, int kv_heads, int dh,
-                          int* splits, size_t* part_floats);
+                          int window, int* splits, size_t* part_floats);
 hipError_t launch_cache_attention(const CacheAttnArgs& a, hipStream_t s);
 
 }  // namespace rh

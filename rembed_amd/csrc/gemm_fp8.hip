@@ -7,6 +7,7 @@
 // The scale bytes are the matrix instruction's own (fp8.h), so the main loop is
 // loads and v_mfma_scale_f32_32x32x64_f8f6f4 alone, one accumulation over all of K.
 #include "fp8.h"
+#include <cstdlib>
 
 namespace rh {
 
@@ -161,8 +162,8 @@ __global__ __launch_bounds__(128 * WGN) void gemm_fp8_kernel(GemmFp8Args p) {
   constexpr int kA = BM * BK, kB = BN * BK, kScale = 256, kStage = kA + kB + 2 * kScale;
   constexpr int LA = kA / (NT * 16), LB = kB / (NT * 16), kLoads = LA + LB + 1;
   constexpr int kEpi = 2 * WGN * 32 * (WN + 4) * 4;
-  static_assert(BM % 128 == 0 && BN % 128 == 0 && BM <= 256 && BN <= 256, "scale words");
-  static_assert(WM % 64 == 0 && (WN == 64 || WN == 128), "scale bytes of a wave");
+  static_assert(BM >= 64 && BN >= 64 && BM <= 256 && BN <= 256, "scale words");
+  static_assert(WM % 32 == 0 && WN % 32 == 0 && (WM <= 128 && WN <= 128), "a wave's scale words");
   static_assert(NS * kStage <= 160 * 1024 && NS * kStage >= kEpi, "LDS");
   __shared__ __attribute__((aligned(1024))) uint8_t lds[NS * kStage];
 
@@ -197,6 +198,7 @@ __global__ __launch_bounds__(128 * WGN) void gemm_fp8_kernel(GemmFp8Args p) {
   const int groups = odd ? gb : ga, g0 = (odd ? col0 : row0) / 128;
   const uint8_t* ssrc = (odd ? p.sb : p.sa) + (size_t)(min(g0 + lane / 32, groups - 1) * 128 + lane % 32 * 4);
   const size_t sstep = (size_t)groups * 128;
+  const int wrow = row0 % 128 + wm * WM, wcol = col0 % 128 + wn * WN;  // within the words
 
   auto issue = [&](int kt, int slot) {
     uint8_t* s = lds + slot * kStage;
@@ -235,11 +237,11 @@ __global__ __launch_bounds__(128 * WGN) void gemm_fp8_kernel(GemmFp8Args p) {
     if (kt + NS - 1 < nk) issue(kt + NS - 1, slot == 0 ? NS - 1 : slot - 1);
     const uint8_t* sA = lds + slot * kStage;
     const uint8_t* sB = sA + kA;
-    // the wave's rows within its 128-row group start at byte 0 or 2 of the words
-    int ea = *reinterpret_cast<const int*>(sA + kA + kB + (wm * WM / 128) * 128 + fr * 4);
-    int eb = *reinterpret_cast<const int*>(sA + kA + kB + kScale + (wn * WN / 128) * 128 + fr * 4);
-    ea = (int)((uint32_t)ea >> (wm * WM % 128 / 32 * 8));
-    eb = (int)((uint32_t)eb >> (wn * WN % 128 / 32 * 8));
+    // a wave's 32-row tiles are consecutive bytes of its group's words
+    int ea = *reinterpret_cast<const int*>(sA + kA + kB + (wrow / 128) * 128 + fr * 4);
+    int eb = *reinterpret_cast<const int*>(sA + kA + kB + kScale + (wcol / 128) * 128 + fr * 4);
+    ea = (int)((uint32_t)ea >> (wrow % 128 / 32 * 8));
+    eb = (int)((uint32_t)eb >> (wcol % 128 / 32 * 8));
 #pragma unroll
     for (int s = 0; s < 2; s++) {
       v8i a[TM], b[TN];
@@ -277,7 +279,21 @@ static void launch_tile(const GemmFp8Args& a, hipStream_t s) {
 
 hipError_t launch_gemm_fp8(const GemmFp8Args& a, hipStream_t s) {
   if (a.M <= 0) return hipSuccess;
-  launch_tile<128, 128, 2, 2>(a, s);
+  int t = 0;
+  if (const char* e = getenv("RH_TILE")) t = atoi(e);
+  switch (t) {
+    case 1: launch_tile<128, 128, 3, 2>(a, s); break;
+    case 2: launch_tile<128, 128, 4, 2>(a, s); break;
+    case 3: launch_tile<256, 256, 2, 4>(a, s); break;
+    case 4: launch_tile<128, 256, 2, 4>(a, s); break;
+    case 5: launch_tile<128, 256, 3, 4>(a, s); break;
+    case 6: launch_tile<256, 128, 2, 2>(a, s); break;
+    case 7: launch_tile<64, 64, 4, 2>(a, s); break;
+    case 8: launch_tile<64, 128, 3, 2>(a, s); break;
+    case 9: launch_tile<256, 256, 2, 2>(a, s); break;
+    case 10: launch_tile<64, 128, 2, 2>(a, s); break;
+    default: launch_tile<128, 128, 2, 2>(a, s); break;
+  }
   return hipGetLastError();
 }
 
