@@ -27,12 +27,14 @@ FLAGS = [
 
 # Per-file code generation: the attention kernels keep their MFMA
 # accumulators in VGPRs (no AGPR round trips for the online-softmax rescale,
-# two waves per SIMD at head dim 128). The cache's attention also keeps them
-# whole across branches: taken apart into scalars there, all of them were copied
-# to another order and back on every page (64 moves of 330 instructions).
-FILE_FLAGS = {"attention.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
-              "cache_attention.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1", "-mllvm",
-                                      "-amdgpu-codegenprepare-break-large-phis=false"]}
+# two waves per SIMD at head dim 128), and so do the e4m3 GEMMs. Those and the
+# cache's attention also keep them whole across branches: taken apart into
+# scalars there, all of them were copied to another order and back on every
+# page (64 moves of 330 instructions).
+_VGPR = ["-mllvm", "-amdgpu-mfma-vgpr-form=1"]
+_WHOLE = ["-mllvm", "-amdgpu-codegenprepare-break-large-phis=false"]
+FILE_FLAGS = {"attention.hip": _VGPR, "cache_attention.hip": _VGPR + _WHOLE,
+              "gemm_fp8.hip": _VGPR + _WHOLE}
 
 
 def sources():

@@ -131,7 +131,9 @@ int run_linear_fp8(Context* ctx, const rh_weight* w, const void* a, int a_bf16, 
                    int ldq, uint8_t* sa) {
   if (m <= 0) return RH_OK;
   const double M = m, K = w->k, N = w->n;
-  if (a) RH_HIP(launch_quantize_rows_fp8(a, a_bf16, lda, m, w->k, qa, ldq, sa, ctx->stream));
+  const bool direct = a && gemm_fp8_takes_rows(m, w->n, w->k);
+  if (a && !direct)
+    RH_HIP(launch_quantize_rows_fp8(a, a_bf16, lda, m, w->k, qa, ldq, sa, ctx->stream));
   GemmFp8Args g{};
   g.A = qa;
   g.lda = ldq;
@@ -152,7 +154,7 @@ int run_linear_fp8(Context* ctx, const rh_weight* w, const void* a, int a_bf16, 
   const double out_b = (dst_bf16 ? 2.0 : 4.0) * (w->glu ? N / 2 : N);
   int slot = -1;
   RH_HIP(ctx->prof_begin(6, 2.0 * M * K * N, M * K + K * N + M * out_b, &slot));
-  RH_HIP(launch_gemm_fp8(g, ctx->stream));
+  RH_HIP(launch_gemm_fp8(g, direct ? a : nullptr, a_bf16, lda, ctx->stream));
   RH_HIP(ctx->prof_end(slot));
   return RH_OK;
 }

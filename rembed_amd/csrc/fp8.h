@@ -130,7 +130,11 @@ struct GemmFp8Args {
   int act;
   int tile_group;
 };
-hipError_t launch_gemm_fp8(const GemmFp8Args& a, hipStream_t s);
+// src: fp32 or bf16 rows to make e4m3 on the way (A and sa unused), where
+// gemm_fp8_takes_rows; null: A and sa.
+bool gemm_fp8_takes_rows(int M, int N, int K);
+hipError_t launch_gemm_fp8(const GemmFp8Args& a, const void* src, int src_bf16, int ld_src,
+                           hipStream_t s);
 
 // ---- launchers (cache.hip, cache_attention.hip) ----------------------------------------
 struct CachePlanArgs {

@@ -7,7 +7,8 @@
 // The scale bytes are the matrix instruction's own (fp8.h), so the main loop is
 // loads and v_mfma_scale_f32_32x32x64_f8f6f4 alone, one accumulation over all of K.
 #include "fp8.h"
-#include <cstdlib>
+
+#include <algorithm>
 
 namespace rh {
 
@@ -91,6 +92,28 @@ hipError_t launch_quantize_rows_fp8(const void* a, int a_bf16, int lda, int m, i
   return hipGetLastError();
 }
 
+// act(gate) * up. SiLU and the tanh GELU, x / (1 + e^-z), on the hardware's exponential and
+// reciprocal, each within an ulp: about 2^-22 of the value where the products before them
+// are off by 2^-16 and a bf16 result rounds at 2^-8; expf and a division take 50
+// instructions a value, a third of a short-K tile's time.
+__device__ __forceinline__ float fp8_glu(float g, float u, int act) {
+  if (act == ACT_GEGLU_ERF) return gelu_avx2(g) * u;
+  const float z = act == ACT_SWIGLU
+                      ? g
+                      : 1.5957691216057308f * __builtin_fmaf(0.044715f * g * g, g, g);
+  return g * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-1.4426950408889634f * z)) * u;
+}
+
+__device__ __forceinline__ void fp8_store4(const GemmFp8Args& p, int row, int col, const v4f& v) {
+  typedef __bf16 v4bf __attribute__((ext_vector_type(4)));
+  const size_t at = (size_t)row * p.ldo + col;
+  if (p.out_bf16)
+    *reinterpret_cast<v4bf*>(static_cast<__bf16*>(p.out) + at) =
+        (v4bf){(__bf16)v[0], (__bf16)v[1], (__bf16)v[2], (__bf16)v[3]};
+  else
+    *reinterpret_cast<v4f*>(static_cast<float*>(p.out) + at) = v;
+}
+
 // ---- GEMM ---------------------------------------------------------------------------
 // Epilogue: per 32-row band a wave parks its accumulators in LDS and reads rows
 // back 4 (gated: 8) columns a lane, so outputs leave as vectors of 4.
@@ -99,18 +122,9 @@ __device__ __forceinline__ void fp8_epilogue(const GemmFp8Args& p, v16f (&acc)[T
                                              uint8_t* lds, int row0, int col0, int wave, int wm,
                                              int wn, int lane) {
   constexpr int kStride = WN + 4;
-  typedef __bf16 v4bf __attribute__((ext_vector_type(4)));
   const int fr = lane & 31, fg = lane >> 5;
   float* ep = reinterpret_cast<float*>(lds) + wave * 32 * kStride;
   const bool glu = is_glu(p.act);
-  auto store = [&](int row, int col, const v4f& v) {
-    const size_t at = (size_t)row * p.ldo + col;
-    if (p.out_bf16)
-      *reinterpret_cast<v4bf*>(static_cast<__bf16*>(p.out) + at) =
-          (v4bf){(__bf16)v[0], (__bf16)v[1], (__bf16)v[2], (__bf16)v[3]};
-    else
-      *reinterpret_cast<v4f*>(static_cast<float*>(p.out) + at) = v;
-  };
 #pragma unroll
   for (int i = 0; i < TM; i++) {
 #pragma unroll
@@ -124,32 +138,63 @@ __device__ __forceinline__ void fp8_epilogue(const GemmFp8Args& p, v16f (&acc)[T
     if (glu) {  // columns 8t..8t+3 gate, 8t+4..8t+7 up
       constexpr int kL = WN / 8, kR = 64 / kL;
       const int c8 = lane % kL * 8, col = col0 + wn * WN + c8;
-      for (int rr = lane / kL; rr < 32; rr += kR) {
-        const v4f g = *reinterpret_cast<const v4f*>(ep + rr * kStride + c8);
-        const v4f u = *reinterpret_cast<const v4f*>(ep + rr * kStride + c8 + 4);
-        if (rows + rr < p.M && col < p.N) {
-          v4f o;
+      v4f g[32 / kR], u[32 / kR];
 #pragma unroll
-          for (int e = 0; e < 4; e++) o[e] = glu_act(g[e], u[e], p.act);
-          store(rows + rr, col / 2, o);
-        }
+      for (int k = 0; k < 32 / kR; k++) {
+        const float* at = ep + (lane / kL + k * kR) * kStride + c8;
+        g[k] = *reinterpret_cast<const v4f*>(at);
+        u[k] = *reinterpret_cast<const v4f*>(at + 4);
+      }
+#pragma unroll
+      for (int k = 0; k < 32 / kR; k++) {
+        const int row = rows + lane / kL + k * kR;
+#pragma unroll
+        for (int e = 0; e < 4; e++) g[k][e] = fp8_glu(g[k][e], u[k][e], p.act);
+        if (row < p.M && col < p.N) fp8_store4(p, row, col / 2, g[k]);
       }
     } else {
       constexpr int kL = WN / 4, kR = 64 / kL;
       const int c4 = lane % kL * 4, col = col0 + wn * WN + c4;
       v4f bs = {0.0f, 0.0f, 0.0f, 0.0f};
       if (p.bias && col < p.N) bs = *reinterpret_cast<const v4f*>(p.bias + col);
-      for (int rr = lane / kL; rr < 32; rr += kR) {
-        v4f v = *reinterpret_cast<const v4f*>(ep + rr * kStride + c4);
-        if (rows + rr < p.M && col < p.N) {
+      v4f v[32 / kR];
 #pragma unroll
-          for (int e = 0; e < 4; e++) v[e] = apply_act(v[e] + bs[e], p.act);
-          store(rows + rr, col, v);
+      for (int k = 0; k < 32 / kR; k++)
+        v[k] = *reinterpret_cast<const v4f*>(ep + (lane / kL + k * kR) * kStride + c4);
+#pragma unroll
+      for (int k = 0; k < 32 / kR; k++) {
+        const int row = rows + lane / kL + k * kR;
+#pragma unroll
+        for (int e = 0; e < 4; e++) v[k][e] += bs[e];
+        if (p.act == ACT_GELU) {
+#pragma unroll
+          for (int e = 0; e < 4; e++) v[k][e] = gelu_avx2(v[k][e]);
         }
+        if (row < p.M && col < p.N) fp8_store4(p, row, col, v[k]);
       }
     }
     __builtin_amdgcn_wave_barrier();
   }
+}
+
+// One row tile's products with all column tiles; the scale bytes' places are constants of the
+// instruction.
+template <int I, int TN, int J = 0>
+__device__ __forceinline__ void fp8_cols(v16f (&acc)[TN], const v8i& a, const v8i (&b)[TN], int ea,
+                                         int eb) {
+  acc[J] = mfma_fp8_32<I, J>(a, b[J], acc[J], ea, eb);
+  if constexpr (J + 1 < TN) fp8_cols<I, TN, J + 1>(acc, a, b, ea, eb);
+}
+template <int TM, int TN>
+__device__ __forceinline__ void fp8_row(v16f (&acc)[TM][TN], const v8i& a, const v8i (&b)[TN],
+                                        int i, int ea, int eb) {
+  if (i == 0) fp8_cols<0>(acc[0], a, b, ea, eb);
+  if constexpr (TM > 1)
+    if (i == 1) fp8_cols<1>(acc[1], a, b, ea, eb);
+  if constexpr (TM > 2)
+    if (i == 2) fp8_cols<2>(acc[2], a, b, ea, eb);
+  if constexpr (TM > 3)
+    if (i == 3) fp8_cols<3>(acc[3], a, b, ea, eb);
 }
 
 // BM x BN tile of 2 x WGN waves, K in stages of 128 bytes (one scale block), an
@@ -210,65 +255,205 @@ __global__ __launch_bounds__(128 * WGN) void gemm_fp8_kernel(GemmFp8Args p) {
     __builtin_amdgcn_global_load_lds(ssrc + kt * sstep, s + kA + kB + (odd ? kScale : 0), 4, 0, 0);
 #endif
   };
-  auto wait_stage = [&](int later) {
-    if (later >= NS - 2) wait_vmcnt<(NS - 2) * kLoads>();
-    else if (NS > 3 && later == 1) wait_vmcnt<kLoads>();
-    else wait_vmcnt<0>();
+  // Fragment addresses: chunk 4 step + 2 part + fg of a row lies at slot chunk ^ (r ^ r >> 3) % 8,
+  // and a row tile further (32 rows) that mask changes by 4, as a step further does. So four
+  // addresses serve every fragment of an operand, the rest is offsets.
+  const int fr = lane & 31, fg = lane >> 5;
+  int fa[2][2], fb[2][2];
+#pragma unroll
+  for (int st = 0; st < 2; st++)
+#pragma unroll
+    for (int pt = 0; pt < 2; pt++) {
+      fa[st][pt] = lds_off(wm * WM + fr, 4 * st + 2 * pt + fg);
+      fb[st][pt] = kA + lds_off(wn * WN + fr, 4 * st + 2 * pt + fg);
+    }
+  auto frag = [&](int slot, const int (&f)[2][2], int i, int st) {
+    const uint8_t* at = lds + slot * kStage + i * 4096;
+    return join8(*reinterpret_cast<const v4i*>(at + f[st ^ (i & 1)][0]),
+                 *reinterpret_cast<const v4i*>(at + f[st ^ (i & 1)][1]));
+  };
+  // a wave's 32-row tiles are consecutive bytes of its group's scale words
+  const int at_ea = kA + kB + (wrow / 128) * 128 + fr * 4;
+  const int at_eb = kA + kB + kScale + (wcol / 128) * 128 + fr * 4;
+  auto words = [&](int slot, int& ea, int& eb) {
+    ea = (int)(*reinterpret_cast<const uint32_t*>(lds + slot * kStage + at_ea) >> (wrow % 128 / 32 * 8));
+    eb = (int)(*reinterpret_cast<const uint32_t*>(lds + slot * kStage + at_eb) >> (wcol % 128 / 32 * 8));
   };
 
   v16f acc[TM][TN];
 #pragma unroll
   for (int i = 0; i < TM; i++)
 #pragma unroll
-    for (int j = 0; j < TN; j++)
-#pragma unroll
-      for (int e = 0; e < 16; e++) acc[i][j][e] = 0.0f;
+    for (int j = 0; j < TN; j++) acc[i][j] = v16f{};
 
 #pragma unroll
-  for (int st = 0; st < NS - 1; st++)
-    if (st < nk) issue(st, st);
+  for (int st = 0; st < NS; st++) issue(min(st, nk - 1), st);
+  wait_vmcnt<(NS - 1) * kLoads>();
+  stage_barrier();
+  v8i b[TN], a;
+  int ea, eb;
+#pragma unroll
+  for (int j = 0; j < TN; j++) b[j] = frag(0, fb, j, 0);
+  a = frag(0, fa, 0, 0);
+  words(0, ea, eb);
 
-  const int fr = lane & 31, fg = lane >> 5;
+  // A stage is 2 TM row tiles' turns. Each reads the next one's row fragment (and, at the
+  // step's end, the next step's columns) before its products. Before the last two turns' products
+  // every fragment of the stage is in registers: the slot is given back, the next stage's
+  // first fragments are asked for, and their latency and the barrier's pass behind the
+  // products that are left.
+  // The body has no branch (stages past the last are asked for again and read by nobody), so
+  // that the accumulators stay where they are.
+  constexpr int U = 2 * TM, kGive = U - 2 > TM ? U - 2 : TM;
   int slot = 0;
   for (int kt = 0; kt < nk; kt++) {
-    wait_stage(min(NS - 2, nk - 1 - kt));
-    wait_lgkmcnt0();  // this wave has read the slot that is refilled below
-    stage_barrier();
-    if (kt + NS - 1 < nk) issue(kt + NS - 1, slot == 0 ? NS - 1 : slot - 1);
-    const uint8_t* sA = lds + slot * kStage;
-    const uint8_t* sB = sA + kA;
-    // a wave's 32-row tiles are consecutive bytes of its group's words
-    int ea = *reinterpret_cast<const int*>(sA + kA + kB + (wrow / 128) * 128 + fr * 4);
-    int eb = *reinterpret_cast<const int*>(sA + kA + kB + kScale + (wcol / 128) * 128 + fr * 4);
-    ea = (int)((uint32_t)ea >> (wrow % 128 / 32 * 8));
-    eb = (int)((uint32_t)eb >> (wcol % 128 / 32 * 8));
+    const int next = slot + 1 == NS ? 0 : slot + 1;
+    v8i bn[TN];
+    int ean, ebn;
 #pragma unroll
-    for (int s = 0; s < 2; s++) {
-      v8i a[TM], b[TN];
+    for (int u = 0; u < U; u++) {
+      v8i an;
+      if (u + 1 < U) an = frag(slot, fa, (u + 1) % TM, (u + 1) / TM);
+      if (u + 1 == TM) {
 #pragma unroll
-      for (int i = 0; i < TM; i++) {
-        const int r = wm * WM + i * 32 + fr;
-        a[i] = join8(*reinterpret_cast<const v4i*>(sA + lds_off(r, 4 * s + fg)),
-                     *reinterpret_cast<const v4i*>(sA + lds_off(r, 4 * s + 2 + fg)));
+        for (int j = 0; j < TN; j++) bn[j] = frag(slot, fb, j, 1);
       }
+      if (u == kGive) {
+        wait_lgkmcnt0();
+        wait_vmcnt<(NS - 2) * kLoads>();
+        stage_barrier();
+        issue(min(kt + NS, nk - 1), slot);
 #pragma unroll
-      for (int j = 0; j < TN; j++) {
-        const int r = wn * WN + j * 32 + fr;
-        b[j] = join8(*reinterpret_cast<const v4i*>(sB + lds_off(r, 4 * s + fg)),
-                     *reinterpret_cast<const v4i*>(sB + lds_off(r, 4 * s + 2 + fg)));
+        for (int j = 0; j < TN; j++) bn[j] = frag(next, fb, j, 0);
+        words(next, ean, ebn);
       }
-#define RH_MM(i, j)                                                                    \
-  if constexpr ((i) < TM && (j) < TN)                                                  \
-    acc[i][j] = mfma_fp8_32<(i), (j)>(a[i], b[j], acc[i][j], ea, eb);
-#define RH_ROW(i) RH_MM(i, 0) RH_MM(i, 1) RH_MM(i, 2) RH_MM(i, 3)
-      RH_ROW(0) RH_ROW(1) RH_ROW(2) RH_ROW(3)
-#undef RH_ROW
-#undef RH_MM
+      if (u + 1 == U) an = frag(next, fa, 0, 0);
+      fp8_row<TM, TN>(acc, a, b, u % TM, ea, eb);
+      a = an;
+      if (u + 1 == TM || u + 1 == U) {
+#pragma unroll
+        for (int j = 0; j < TN; j++) b[j] = bn[j];
+      }
+      __builtin_amdgcn_sched_barrier(0);
     }
-    slot = slot + 1 == NS ? 0 : slot + 1;
+    ea = ean;
+    eb = ebn;
+    slot = next;
   }
+  wait_vmcnt<0>();
   __syncthreads();
   fp8_epilogue<BM, WM, WN, TM, TN>(p, acc, lds, row0, col0, wave, wm, wn, lane);
+}
+
+// ---- few rows -------------------------------------------------------------------------
+// A query's rows: the weights' bytes are all there is to move, so 16 of their rows go to
+// a workgroup (4096 outputs: 256 workgroups), whose NW waves hold different 128-blocks
+// of K and read them straight to registers as the A operand of 16x16x128 products (32
+// consecutive bytes a lane, four lanes a row's block). The activations are the columns, 16 MT of
+// them. The waves' sums are joined in LDS in wave order, and a thread finishes four
+// consecutive outputs of a row.
+// SRC 0: rows are e4m3 already; 1 / 2: fp32 / bf16 rows are made so here, by the same
+// arithmetic as quantize_rows_fp8_kernel (a launch less, but every workgroup does it:
+// gemm_fp8_takes_rows).
+template <int MT, int NW, int SRC>
+__global__ __launch_bounds__(64 * NW) void gemm_fp8_rows_kernel(GemmFp8Args p, const void* src,
+                                                                int lds_src) {
+  __shared__ __attribute__((aligned(16))) float red[NW][MT][64][4];
+  const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int n0 = blockIdx.x * 16, m0 = blockIdx.y * 16 * MT;
+  const int nk = (p.K + kFp8Block - 1) / kFp8Block;
+  const int ga = (p.M + 127) / 128, gb = p.Np / 128;
+  const uint8_t* wrow = p.B + (size_t)(n0 + r) * p.ldb + g * 32;
+  const uint8_t* wexp = p.sb + fp8_scale_at(n0 + r, 0, gb);
+  int mrow[MT];
+#pragma unroll
+  for (int t = 0; t < MT; t++) mrow[t] = min(m0 + t * 16 + r, p.M - 1);
+
+  v4f acc[MT];
+#pragma unroll
+  for (int t = 0; t < MT; t++) acc[t] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 4
+  for (int kb = wave; kb < nk; kb += NW) {
+    const v4i* at = reinterpret_cast<const v4i*>(wrow + (size_t)kb * kFp8Block);
+    const v8i w = join8(at[0], at[1]);
+    const int ew = wexp[(size_t)kb * gb * 128];
+#pragma unroll
+    for (int t = 0; t < MT; t++) {
+      v8i x;
+      int ex;
+      if constexpr (SRC == 0) {
+        const v4i* xt = reinterpret_cast<const v4i*>(p.A + (size_t)mrow[t] * p.lda +
+                                                     (size_t)kb * kFp8Block + g * 32);
+        x = join8(xt[0], xt[1]);
+        ex = p.sa[fp8_scale_at(mrow[t], kb, ga)];
+      } else {
+        float v[32];
+        const int c = kb * kFp8Block + g * 32;
+        const size_t row = (size_t)mrow[t] * lds_src;
+        const bool whole = c + 32 <= p.K && lds_src % 8 == 0 && ((uintptr_t)src & 15) == 0;
+        uint32_t top = 0;
+        if (whole) {
+#pragma unroll
+          for (int e = 0; e < 32; e += 8) {
+            if constexpr (SRC == 2) {
+              const v8bf y = *reinterpret_cast<const v8bf*>(static_cast<const __bf16*>(src) + row + c + e);
+#pragma unroll
+              for (int i = 0; i < 8; i++) v[e + i] = (float)y[i];
+            } else {
+              const v4f y0 = *reinterpret_cast<const v4f*>(static_cast<const float*>(src) + row + c + e);
+              const v4f y1 = *reinterpret_cast<const v4f*>(static_cast<const float*>(src) + row + c + e + 4);
+#pragma unroll
+              for (int i = 0; i < 8; i++) v[e + i] = i < 4 ? y0[i] : y1[i - 4];
+            }
+          }
+        } else {
+#pragma unroll
+          for (int e = 0; e < 32; e++) {
+            v[e] = 0.0f;
+            if (c + e < p.K)
+              v[e] = SRC == 2 ? (float)static_cast<const __bf16*>(src)[row + c + e]
+                              : static_cast<const float*>(src)[row + c + e];
+          }
+        }
+#pragma unroll
+        for (int e = 0; e < 32; e++) top = max(top, finite_abs_bits(v[e]));
+        top = max(top, (uint32_t)__shfl_xor((int)top, 16, 64));
+        top = max(top, (uint32_t)__shfl_xor((int)top, 32, 64));
+        ex = fp8_exponent(top);
+        const float f = fp8_inverse(ex);
+#pragma unroll
+        for (int e = 0; e < 8; e++)
+          x[e] = fp8_pack4(v[4 * e] * f, v[4 * e + 1] * f, v[4 * e + 2] * f, v[4 * e + 3] * f);
+      }
+      acc[t] = mfma_fp8_16(w, x, acc[t], ew, ex);
+    }
+  }
+#pragma unroll
+  for (int t = 0; t < MT; t++) *reinterpret_cast<v4f*>(red[wave][t][lane]) = acc[t];
+  __syncthreads();
+  // thread -> column tile t, lane l of it: row m0 + 16 t + l % 16, outputs n0 + 4 (l / 16) ..
+  const bool glu = is_glu(p.act);
+  const int t = threadIdx.x >> 6, l = threadIdx.x & 63;
+  if (t >= MT) return;
+  const int row = m0 + t * 16 + (l & 15), q = l >> 4, col = n0 + 4 * q;
+  if (row >= p.M || (glu && (q & 1))) return;
+  auto sum = [&](int at) {
+    v4f x = *reinterpret_cast<const v4f*>(red[0][t][at]);
+#pragma unroll
+    for (int w = 1; w < NW; w++) x += *reinterpret_cast<const v4f*>(red[w][t][at]);
+    return x;
+  };
+  v4f x = sum(l);
+  if (glu) {  // groups of four rows: gate, then up
+    const v4f u = sum(l + 16);
+#pragma unroll
+    for (int e = 0; e < 4; e++) x[e] = fp8_glu(x[e], u[e], p.act);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 4; e++) x[e] = apply_act(x[e] + (p.bias ? p.bias[col + e] : 0.0f), p.act);
+  }
+  fp8_store4(p, row, glu ? col / 2 : col, x);
 }
 
 template <int BM, int BN, int NS, int WGN>
@@ -277,23 +462,61 @@ static void launch_tile(const GemmFp8Args& a, hipStream_t s) {
   timed_launch(gemm_fp8_kernel<BM, BN, NS, WGN>, grid, dim3(128 * WGN), 0, s, a);
 }
 
-hipError_t launch_gemm_fp8(const GemmFp8Args& a, hipStream_t s) {
+template <int MT, int NW, int SRC>
+static void launch_rows(const GemmFp8Args& a, const void* src, int ld, hipStream_t s) {
+  const dim3 grid((unsigned)(a.N / 16), (unsigned)ceil_div(a.M, 16 * MT));
+  timed_launch(gemm_fp8_rows_kernel<MT, NW, SRC>, grid, dim3(64 * NW), 0, s, a, src, ld);
+}
+
+// The kernel of few rows where it makes at most a workgroup per CU (of up to 16 rows: two).
+// µs, K 4096, bf16 out, against the 64 x 64 tiles: N 1024, M 64: 6.1 / 9.7, M 128: 8.3 / 9.9;
+// N 4096, M 16: 6.4 / 10.0, M 32: 9.1 / 9.9, M 48: 12.9 / 9.9; N 8192, M 16: 10.0 / 10.1.
+// One column tile a workgroup where that fits, else two (four were never ahead).
+static int rows_tiles(int M, int N) {
+  const long long wgs = N / 16;
+  if (wgs * ceil_div(M, 16) <= (M <= 16 ? 512 : 256)) return 1;
+  if (wgs * ceil_div(M, 32) <= 256) return 2;
+  return 0;
+}
+
+// fp32 / bf16 rows go straight into it where its workgroups' work on them is less than a
+// launch: µs against quantizing first, K 1024, N 4096: M 1 4.2 / 6.9, M 16 5.1 / 6.9; K 2560,
+// N 2560: M 4 5.9 / 6.9, M 8 6.8 / 6.9; K 4096, N 1024: M 1 6.6 / 6.8, M 4 7.6 / 7.3; K 4096,
+// N 4096: M 1 7.6 / 6.9.
+bool gemm_fp8_takes_rows(int M, int N, int K) {
+  return M <= 16 && rows_tiles(M, N) == 1 && (long long)M * K <= 16384 &&
+         (long long)N * K <= (8 << 20);
+}
+
+// A tile's time by rounds of the chip's 256 CUs: µs per started round at K 4096 (about a
+// third of it at K 1024), from M 400 .. 12000, N 1024 .. 4096. The tile with the least is
+// taken: M 400 64 x 64 (N 4096: 16.5 µs, next 19.5), M 1500 128 x 256 (33.6, 36.0), M 3000
+// 256 x 256 (53.6, 59.0), M 6000 128 x 256 (98.3, 106.6), M 8192 256 x 256 (108 of the
+// 110 that this card's fp8 library product takes for its share).
+static long long tile_cost(int M, int N, int bm, int bn, int each) {
+  return (long long)ceil_div(ceil_div(M, bm) * ceil_div(N, bn), 256) * each;
+}
+
+hipError_t launch_gemm_fp8(const GemmFp8Args& a, const void* src, int src_bf16, int ld_src,
+                           hipStream_t s) {
   if (a.M <= 0) return hipSuccess;
-  int t = 0;
-  if (const char* e = getenv("RH_TILE")) t = atoi(e);
-  switch (t) {
-    case 1: launch_tile<128, 128, 3, 2>(a, s); break;
-    case 2: launch_tile<128, 128, 4, 2>(a, s); break;
-    case 3: launch_tile<256, 256, 2, 4>(a, s); break;
-    case 4: launch_tile<128, 256, 2, 4>(a, s); break;
-    case 5: launch_tile<128, 256, 3, 4>(a, s); break;
-    case 6: launch_tile<256, 128, 2, 2>(a, s); break;
-    case 7: launch_tile<64, 64, 4, 2>(a, s); break;
-    case 8: launch_tile<64, 128, 3, 2>(a, s); break;
-    case 9: launch_tile<256, 256, 2, 2>(a, s); break;
-    case 10: launch_tile<64, 128, 2, 2>(a, s); break;
-    default: launch_tile<128, 128, 2, 2>(a, s); break;
+  if (src) {
+    if (src_bf16) launch_rows<1, 8, 2>(a, src, ld_src, s);
+    else launch_rows<1, 8, 1>(a, src, ld_src, s);
+    return hipGetLastError();
   }
+  const int rows = rows_tiles(a.M, a.N);
+  if (rows == 1) launch_rows<1, 8, 0>(a, nullptr, 0, s);
+  else if (rows == 2) launch_rows<2, 8, 0>(a, nullptr, 0, s);
+  if (rows) return hipGetLastError();
+  const long long c64 = tile_cost(a.M, a.N, 64, 64, 76), c128 = tile_cost(a.M, a.N, 128, 128, 185),
+                  cwide = tile_cost(a.M, a.N, 128, 256, 325),
+                  c256 = tile_cost(a.M, a.N, 256, 256, 540);
+  const long long best = std::min(std::min(c64, c128), std::min(cwide, c256));
+  if (best == c64) launch_tile<64, 64, 4, 2>(a, s);
+  else if (best == c128) launch_tile<128, 128, 2, 2>(a, s);
+  else if (best == cwide) launch_tile<128, 256, 3, 4>(a, s);
+  else launch_tile<256, 256, 2, 4>(a, s);
   return hipGetLastError();
 }
 
