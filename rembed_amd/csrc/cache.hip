@@ -34,59 +34,93 @@ __host__ __device__ __forceinline__ int v_at(int t, int d) {
 //   its row t lies at row cu[b] + t, position past + t, slot page * 64 + position % 64.
 // Every workgroup scans the lengths itself (they are a few KiB from L2) and then
 // fills its share of rows and table entries, so one launch serves: prefix sums in
-// a kernel of their own would cost a second launch's gap, more than the scan.
+// a kernel of their own would cost a second launch's gap, more than the scan. What bounds
+// it is latency: the lengths are loaded once (batches of up to 1024), and a thread
+// takes four consecutive rows to one search for their request.
 constexpr int kPlanThreads = 256;
 constexpr int kPlanChunk = 1024;  // requests whose prefix sums are in LDS at once
+constexpr int kPlanRows = 4;      // consecutive rows of a thread
 
-struct PlanSums {
-  long long rows, need, touched;
+// What a request adds: new tokens (high enough for any batch's sum), pages and blocks.
+struct PlanSum {
+  long long rows;
+  unsigned long long both;  // pages << 32 | blocks touched
 };
+__device__ __forceinline__ int plan_add(PlanSum& s, long long past, long long fresh, int ldt) {
+  if (past < 0 || fresh < 0) return 1;
+  const long long blk = (past + fresh + kPage - 1) / kPage;
+  const long long need = blk - (past + kPage - 1) / kPage;
+  const long long touch = fresh > 0 ? (past + fresh - 1) / kPage - past / kPage + 1 : 0;
+  s.rows += fresh;
+  s.both += (unsigned long long)need << 32 | (unsigned long long)touch;
+  return blk > ldt || past + fresh > 0x7FFFFF00 ? 2 : 0;
+}
 
 __global__ __launch_bounds__(kPlanThreads) void cache_plan_kernel(CachePlanArgs p) {
   __shared__ int s_past[kPlanChunk];
   __shared__ int s_cu[kPlanChunk + 1], s_first[kPlanChunk + 1], s_blk[kPlanChunk + 1];
-  __shared__ int s_wave[3][kPlanThreads / 64];
-  __shared__ long long s_tot[3];
-  __shared__ int s_err;
+  __shared__ PlanSum s_wave[kPlanThreads / 64];
+  __shared__ int s_err[kPlanThreads / 64];
   const int tid = threadIdx.x;
   const int lane = tid & 63, wave = tid >> 6;
   const bool writer = blockIdx.x == 0;
+  const int stride = gridDim.x * kPlanThreads, at0 = blockIdx.x * kPlanThreads + tid;
+
+  // The chunk's lengths, four consecutive requests a thread, and the sums before each
+  // thread's (`before`) and over the chunk (`all`).
+  int past[4], fresh[4], err = 0;
+  PlanSum mine, before, all;
+  auto chunk = [&](int b0, int n) {
+    mine = PlanSum{0, 0};
+    int e = 0;
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      const int b = tid * 4 + i;
+      past[i] = b < n ? p.past[b0 + b] : 0;
+      fresh[i] = b < n ? p.fresh[b0 + b] : 0;
+      e |= plan_add(mine, past[i], fresh[i], p.ldt);
+    }
+    PlanSum v = mine;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const long long r = __shfl_up(v.rows, o, 64);
+      const unsigned long long t = __shfl_up(v.both, o, 64);
+      if (lane >= o) {
+        v.rows += r;
+        v.both += t;
+      }
+    }
+    const unsigned long long any1 = __ballot(e & 1), any2 = __ballot(e & 2);
+    if (lane == 63) {
+      s_wave[wave] = v;
+      s_err[wave] = (any1 ? 1 : 0) | (any2 ? 2 : 0);
+    }
+    __syncthreads();
+    before = PlanSum{v.rows - mine.rows, v.both - mine.both};
+    all = PlanSum{0, 0};
+#pragma unroll
+    for (int w = 0; w < kPlanThreads / 64; w++) {
+      if (w < wave) {
+        before.rows += s_wave[w].rows;
+        before.both += s_wave[w].both;
+      }
+      all.rows += s_wave[w].rows;
+      all.both += s_wave[w].both;
+      err |= s_err[w];
+    }
+  };
 
   // Totals and faults first: a plan that does not fit changes nothing.
-  if (tid < 3) s_tot[tid] = 0;
-  if (tid == 0) s_err = 0;
-  __syncthreads();
-  {
-    long long rows = 0, need = 0;
-    int err = 0;
-    for (int b = tid; b < p.batch; b += kPlanThreads) {
-      const long long pa = p.past[b], fr = p.fresh[b];
-      if (pa < 0 || fr < 0) {
-        err |= 1;
-        continue;
-      }
-      const long long blk = (pa + fr + kPage - 1) / kPage;
-      if (blk > p.ldt || pa + fr > 0x7FFFFF00) err |= 2;
-      rows += fr;
-      need += blk - (pa + kPage - 1) / kPage;
-    }
-    for (int o = 32; o; o >>= 1) {
-      rows += __shfl_xor(rows, o, 64);
-      need += __shfl_xor(need, o, 64);
-      err |= __shfl_xor(err, o, 64);
-    }
-    if (lane == 0) {
-      // integer sums: the order of the atomics does not show
-      atomicAdd(reinterpret_cast<unsigned long long*>(&s_tot[0]), (unsigned long long)rows);
-      atomicAdd(reinterpret_cast<unsigned long long*>(&s_tot[1]), (unsigned long long)need);
-      atomicOr(&s_err, err);
-    }
+  const bool one = p.batch <= kPlanChunk;
+  long long rows = 0, need = 0;
+  for (int b0 = 0; b0 < p.batch; b0 += kPlanChunk) {
+    chunk(b0, min(kPlanChunk, p.batch - b0));
+    rows += all.rows;
+    need += (long long)(all.both >> 32);
+    if (!one) __syncthreads();
   }
-  __syncthreads();
-  int err = s_err;
-  if (s_tot[0] > p.rows) err |= 4;
-  if (s_tot[1] > p.n_free) err |= 8;
-  const int stride = gridDim.x * kPlanThreads, at0 = blockIdx.x * kPlanThreads + tid;
+  if (rows > p.rows) err |= 4;
+  if (need > p.n_free) err |= 8;
   if (err) {
     for (int r = at0; r < p.rows; r += stride) {
       p.slots[r] = -1;
@@ -104,41 +138,9 @@ __global__ __launch_bounds__(kPlanThreads) void cache_plan_kernel(CachePlanArgs 
   int c_rows = 0, c_need = 0, c_touch = 0;  // sums over the chunks before
   for (int b0 = 0; b0 < p.batch; b0 += kPlanChunk) {
     const int n = min(kPlanChunk, p.batch - b0);
-    // four consecutive requests per thread, then a scan over the threads
-    int past[4], fresh[4], need[4], touch[4], sum[3] = {0, 0, 0};
-#pragma unroll
-    for (int i = 0; i < 4; i++) {
-      const int b = tid * 4 + i;
-      past[i] = b < n ? p.past[b0 + b] : 0;
-      fresh[i] = b < n ? p.fresh[b0 + b] : 0;
-      need[i] = (past[i] + fresh[i] + kPage - 1) / kPage - (past[i] + kPage - 1) / kPage;
-      touch[i] = fresh[i] > 0 ? (past[i] + fresh[i] - 1) / kPage - past[i] / kPage + 1 : 0;
-      sum[0] += fresh[i];
-      sum[1] += need[i];
-      sum[2] += touch[i];
-    }
-    int before[3];
-#pragma unroll
-    for (int k = 0; k < 3; k++) {
-      int v = sum[k];
-#pragma unroll
-      for (int o = 1; o < 64; o <<= 1) {
-        const int u = __shfl_up(v, o, 64);
-        if (lane >= o) v += u;
-      }
-      before[k] = v - sum[k];
-      if (lane == 63) s_wave[k][wave] = v;
-    }
-    __syncthreads();
-    int all[3] = {0, 0, 0};
-#pragma unroll
-    for (int k = 0; k < 3; k++)
-#pragma unroll
-      for (int w = 0; w < kPlanThreads / 64; w++) {
-        if (w < wave) before[k] += s_wave[k][w];
-        all[k] += s_wave[k][w];
-      }
-    int at[3] = {c_rows + before[0], c_need + before[1], c_touch + before[2]};
+    if (!one) chunk(b0, n);
+    int at[3] = {c_rows + (int)before.rows, c_need + (int)(before.both >> 32),
+                 c_touch + (int)(uint32_t)before.both};
 #pragma unroll
     for (int i = 0; i < 4; i++) {
       const int b = tid * 4 + i;
@@ -149,14 +151,18 @@ __global__ __launch_bounds__(kPlanThreads) void cache_plan_kernel(CachePlanArgs 
         s_blk[b] = at[2];
         if (writer) p.lens[b0 + b] = past[i] + fresh[i];
       }
-      at[0] += fresh[i];
-      at[1] += need[i];
-      at[2] += touch[i];
+      PlanSum d{0, 0};
+      plan_add(d, past[i], fresh[i], p.ldt);
+      at[0] += (int)d.rows;
+      at[1] += (int)(d.both >> 32);
+      at[2] += (int)(uint32_t)d.both;
     }
+    const int end_rows = c_rows + (int)all.rows, end_need = c_need + (int)(all.both >> 32),
+              end_touch = c_touch + (int)(uint32_t)all.both;
     if (tid == 0) {
-      s_cu[n] = c_rows + all[0];
-      s_first[n] = c_need + all[1];
-      s_blk[n] = c_touch + all[2];
+      s_cu[n] = end_rows;
+      s_first[n] = end_need;
+      s_blk[n] = end_touch;
     }
     __syncthreads();
     // the last request of the chunk with start[b] <= x
@@ -176,24 +182,36 @@ __global__ __launch_bounds__(kPlanThreads) void cache_plan_kernel(CachePlanArgs 
       }
     // table entries behind the past's blocks are written here and read nowhere
     // in this launch (rows take new pages from the free list)
-    for (int e = c_need + at0; e < c_need + all[1]; e += stride) {
+    for (int e = c_need + at0; e < end_need; e += stride) {
       const int b = find(s_first, e);
       const int have = (s_past[b] + kPage - 1) / kPage;
       p.table[(size_t)(b0 + b) * p.ldt + have + e - s_first[b]] = p.free_pages[e];
     }
-    for (int r = c_rows + at0; r < c_rows + all[0]; r += stride) {
-      const int b = find(s_cu, r);
-      const int pos = s_past[b] + r - s_cu[b];
-      const int have = (s_past[b] + kPage - 1) / kPage, blk = pos / kPage;
-      const int page = blk >= have ? p.free_pages[s_first[b] + blk - have]
-                                   : p.table[(size_t)(b0 + b) * p.ldt + blk];
-      p.slots[r] = page < 0 ? -1 : (int64_t)page * kPage + pos % kPage;
-      p.pos[r] = pos;
+    for (int r0 = c_rows + at0 * kPlanRows; r0 < end_rows; r0 += stride * kPlanRows) {
+      int b = find(s_cu, r0), page = -1, page_of = -1;  // page_of: block of `page`, of request b
+#pragma unroll
+      for (int i = 0; i < kPlanRows; i++) {
+        const int r = r0 + i;
+        if (r >= end_rows) break;
+        while (r >= s_cu[b + 1]) {
+          b++;
+          page_of = -1;
+        }
+        const int pos = s_past[b] + r - s_cu[b], blk = pos / kPage;
+        if (blk != page_of) {
+          const int have = (s_past[b] + kPage - 1) / kPage;
+          page = blk >= have ? p.free_pages[s_first[b] + blk - have]
+                             : p.table[(size_t)(b0 + b) * p.ldt + blk];
+          page_of = blk;
+        }
+        p.slots[r] = page < 0 ? -1 : (int64_t)page * kPage + pos % kPage;
+        p.pos[r] = pos;
+      }
     }
-    c_rows += all[0];
-    c_need += all[1];
-    c_touch += all[2];
-    __syncthreads();
+    c_rows = end_rows;
+    c_need = end_need;
+    c_touch = end_touch;
+    if (!one) __syncthreads();
   }
   for (int r = c_rows + at0; r < p.rows; r += stride) {  // rows behind the last request
     p.slots[r] = -1;
@@ -210,7 +228,7 @@ __global__ __launch_bounds__(kPlanThreads) void cache_plan_kernel(CachePlanArgs 
 }
 
 hipError_t launch_cache_plan(const CachePlanArgs& a, hipStream_t s) {
-  const int wgs = std::max(1, std::min(512, ceil_div(a.rows, 2 * kPlanThreads)));
+  const int wgs = std::max(1, std::min(512, ceil_div(a.rows, kPlanRows * kPlanThreads)));
   hipLaunchKernelGGL(cache_plan_kernel, dim3(wgs), dim3(kPlanThreads), 0, s, a);
   return hipGetLastError();
 }
@@ -220,30 +238,43 @@ hipError_t launch_cache_plan(const CachePlanArgs& a, hipStream_t s) {
 // token: the new rows stay in registers, the block's codes are put together in
 // LDS and written whole. With e the byte of the new tokens' largest magnitude:
 //   x' = max(e, x of the codes kept),  kept codes * 2^(x - x'),  new value * 2^(127 - x').
-// A block whose first token is new keeps nothing: zeros behind the new tokens.
+// A block whose first token is new keeps nothing: zeros behind the new tokens. One
+// whose scale stays (most single tokens) is not read at all: only the new codes are written.
 // A token whose K or V has an infinity or NaN in a head is stored as K = NaN,
 // V = 0: whoever sees the token gets NaN, and nobody else does (0 * NaN would
 // reach queries that must not see it through V). It sets no scale.
+// Single tokens are bound by latency, so a request is found by a 64-way search (one load of
+// a wave per level; a binary search took 3 µs of 7.6 for 48 requests) and its rows are
+// asked for before their slots are known.
 constexpr int kAppendThreads = 256;
+
+// The last request b with blocks[b] <= seg: every level looks at 64 evenly spaced ones.
+__device__ __forceinline__ int append_request(const int32_t* blocks, int batch, int seg, int lane) {
+  int lo = 0, n = batch;  // it is among lo .. lo + n - 1
+  while (n > 1) {
+    const int step = (n + 63) / 64;
+    const int at = lo + lane * step;
+    const bool le = lane * step < n && blocks[at] <= seg;
+    const int k = __popcll(__ballot(le)) - 1;  // blocks do not fall: the first k + 1 of them
+    lo += max(k, 0) * step;
+    n = min(step, n - max(k, 0) * step);
+  }
+  return lo;
+}
 
 template <int DH, bool BF16>
 __global__ __launch_bounds__(kAppendThreads) void cache_append_kernel(CacheAppendArgs p) {
   constexpr int kBytes = kPage * DH, E = DH / 4;  // a head's block; values per thread
   __shared__ __attribute__((aligned(16))) uint8_t s_k[kBytes], s_v[kBytes];
-  __shared__ uint32_t s_max[2];
+  __shared__ uint32_t s_max[kAppendThreads / 64][2];
   const int tid = threadIdx.x;
   const int heads = p.cache.kv_heads;
   const int seg = blockIdx.x / heads, h = blockIdx.x % heads;
+  const int b = append_request(p.blocks, p.batch, seg, tid & 63);
   if (seg >= p.blocks[p.batch]) return;
-  int lo = 0, hi = p.batch - 1;  // the last request with blocks[b] <= seg
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) >> 1;
-    if (p.blocks[mid] <= seg) lo = mid;
-    else hi = mid - 1;
-  }
-  const int j = seg - p.blocks[lo];
-  const int r0 = p.cu[lo], fresh = p.cu[lo + 1] - r0;
-  if (r0 < 0 || fresh <= 0 || r0 + fresh > p.rows) return;
+  const int j = seg - p.blocks[b];
+  const int r0 = p.cu[b], fresh = p.cu[b + 1] - r0;
+  if (r0 < 0 || fresh <= 0 || r0 + (long long)fresh > p.rows) return;
   const int64_t slot0 = p.slots[r0];
   if (slot0 < 0) return;
   const int off0 = (int)(slot0 % kPage);
@@ -251,93 +282,130 @@ __global__ __launch_bounds__(kAppendThreads) void cache_append_kernel(CacheAppen
   const int off = j == 0 ? off0 : 0;
   const int cnt = min(kPage - off, fresh - first);
   if (cnt <= 0) return;
-  const int64_t slot = p.slots[r0 + first];
-  if (slot < 0 || slot / kPage >= p.cache.pages) return;
-  const size_t unit = (size_t)(slot / kPage) * heads + h;
-  uint8_t* gk = p.cache.k + unit * kBytes;
-  uint8_t* gv = p.cache.v + unit * kBytes;
 
-  if (tid < 2) s_max[tid] = 0;
   // this thread's quarter of its token's K and V
   const int tok = tid >> 2, quarter = tid & 3;
   float k[E], v[E];
   uint32_t mk = 0, mv = 0;
-  bool bad = false;
   if (tok < cnt) {
     const size_t at = (size_t)(r0 + first + tok) * p.ldkv + h * DH + quarter * E;
+    constexpr int kStep = BF16 ? 8 : 4;
 #pragma unroll
-    for (int e = 0; e < E; e++) {
+    for (int e = 0; e < E; e += kStep) {
       if constexpr (BF16) {
-        k[e] = (float)(static_cast<const __bf16*>(p.kv) + p.k_off)[at + e];
-        v[e] = (float)(static_cast<const __bf16*>(p.kv) + p.v_off)[at + e];
+        const __bf16* row = static_cast<const __bf16*>(p.kv) + at + e;
+        const v8bf x = *reinterpret_cast<const v8bf*>(row + p.k_off);
+        const v8bf y = *reinterpret_cast<const v8bf*>(row + p.v_off);
+#pragma unroll
+        for (int i = 0; i < kStep; i++) {
+          k[e + i] = (float)x[i];
+          v[e + i] = (float)y[i];
+        }
       } else {
-        k[e] = (static_cast<const float*>(p.kv) + p.k_off)[at + e];
-        v[e] = (static_cast<const float*>(p.kv) + p.v_off)[at + e];
+        const float* row = static_cast<const float*>(p.kv) + at + e;
+        const v4f x = *reinterpret_cast<const v4f*>(row + p.k_off);
+        const v4f y = *reinterpret_cast<const v4f*>(row + p.v_off);
+#pragma unroll
+        for (int i = 0; i < kStep; i++) {
+          k[e + i] = x[i];
+          v[e + i] = y[i];
+        }
       }
-      const uint32_t uk = __float_as_uint(k[e]) & 0x7FFFFFFFu;
-      const uint32_t uv = __float_as_uint(v[e]) & 0x7FFFFFFFu;
-      bad |= uk >= 0x7F800000u || uv >= 0x7F800000u;
-      mk = max(mk, uk);
-      mv = max(mv, uv);
     }
   }
-  int any = bad;
-  any |= __shfl_xor(any, 1, 64);
-  any |= __shfl_xor(any, 2, 64);
-  if (any) mk = mv = 0;
-  for (int o = 32; o; o >>= 1) {
+  const int64_t slot = p.slots[r0 + first];
+  const bool here = slot >= 0 && slot / kPage < p.cache.pages;
+  const size_t unit = here ? (size_t)(slot / kPage) * heads + h : 0;
+  uint8_t* gk = p.cache.k + unit * kBytes;
+  uint8_t* gv = p.cache.v + unit * kBytes;
+  const int ok = p.cache.k_exp[unit], ov = p.cache.v_exp[unit];
+  if (tok < cnt) {
+#pragma unroll
+    for (int e = 0; e < E; e++) {
+      mk = max(mk, __float_as_uint(k[e]) & 0x7FFFFFFFu);
+      mv = max(mv, __float_as_uint(v[e]) & 0x7FFFFFFFu);
+    }
+  }
+  int bad = mk >= 0x7F800000u || mv >= 0x7F800000u;
+  bad |= __shfl_xor(bad, 1, 64);
+  bad |= __shfl_xor(bad, 2, 64);
+  if (bad) mk = mv = 0;
+  for (int o = 32; o >= 4; o >>= 1) {
     mk = max(mk, (uint32_t)__shfl_xor((int)mk, o, 64));
     mv = max(mv, (uint32_t)__shfl_xor((int)mv, o, 64));
   }
-  __syncthreads();
+  mk = max(mk, (uint32_t)__shfl_xor((int)mk, 1, 64));
+  mv = max(mv, (uint32_t)__shfl_xor((int)mv, 1, 64));
+  mk = max(mk, (uint32_t)__shfl_xor((int)mk, 2, 64));
+  mv = max(mv, (uint32_t)__shfl_xor((int)mv, 2, 64));
   if ((tid & 63) == 0) {
-    atomicMax(&s_max[0], mk);
-    atomicMax(&s_max[1], mv);
+    s_max[tid >> 6][0] = mk;
+    s_max[tid >> 6][1] = mv;
   }
+  if (!here) return;  // the whole workgroup
   __syncthreads();
-  int xk = fp8_exponent(s_max[0]), xv = fp8_exponent(s_max[1]);
-  // the codes kept, four at a time
+#pragma unroll
+  for (int w = 0; w < kAppendThreads / 64; w++) {
+    mk = max(mk, s_max[w][0]);
+    mv = max(mv, s_max[w][1]);
+  }
+  int xk = fp8_exponent(mk), xv = fp8_exponent(mv);
+  bool whole_k = true, whole_v = true;  // the block's bytes are all written
+  auto scaled = [](int w, int down) {
+    const float f = __uint_as_float((uint32_t)(127 - min(down, 126)) << 23);
+    float c[4] = {};
+    fp8_unpack4(w, c);
+    return fp8_pack4(c[0] * f, c[1] * f, c[2] * f, c[3] * f);
+  };
   if (off == 0) {
-    for (int i = tid * 4; i < kBytes; i += kAppendThreads * 4) {
-      *reinterpret_cast<int*>(s_k + i) = 0;
-      *reinterpret_cast<int*>(s_v + i) = 0;
+    if (cnt < kPage) {
+      for (int i = tid * 16; i < kBytes; i += kAppendThreads * 16) {
+        *reinterpret_cast<v4i*>(s_k + i) = v4i{0, 0, 0, 0};
+        *reinterpret_cast<v4i*>(s_v + i) = v4i{0, 0, 0, 0};
+      }
+      __syncthreads();
     }
   } else {
-    const int ok = p.cache.k_exp[unit], ov = p.cache.v_exp[unit];
+    whole_k = xk > ok;
+    whole_v = xv > ov;
     xk = max(xk, ok);
     xv = max(xv, ov);
-    auto scaled = [](int w, int down) {
-      if (down == 0) return w;
-      const float f = __uint_as_float((uint32_t)(127 - min(down, 126)) << 23);
-      float c[4] = {};
-      fp8_unpack4(w, c);
-      return fp8_pack4(c[0] * f, c[1] * f, c[2] * f, c[3] * f);
-    };
-    for (int i = tid * 4; i < kBytes; i += kAppendThreads * 4) {
-      *reinterpret_cast<int*>(s_k + i) = scaled(*reinterpret_cast<const int*>(gk + i), xk - ok);
-      *reinterpret_cast<int*>(s_v + i) = scaled(*reinterpret_cast<const int*>(gv + i), xv - ov);
+    for (int i = tid * 16; i < kBytes && (whole_k || whole_v); i += kAppendThreads * 16) {
+      v4i a, c;
+      if (whole_k) a = *reinterpret_cast<const v4i*>(gk + i);
+      if (whole_v) c = *reinterpret_cast<const v4i*>(gv + i);
+#pragma unroll
+      for (int e = 0; e < 4; e++) {
+        if (whole_k) a[e] = scaled(a[e], xk - ok);
+        if (whole_v) c[e] = scaled(c[e], xv - ov);
+      }
+      if (whole_k) *reinterpret_cast<v4i*>(s_k + i) = a;
+      if (whole_v) *reinterpret_cast<v4i*>(s_v + i) = c;
     }
+    if (whole_k || whole_v) __syncthreads();
   }
-  __syncthreads();
   if (tok < cnt) {
     const float fk = fp8_inverse(xk), fv = fp8_inverse(xv);
+    uint8_t* to_k = whole_k ? s_k : gk;
+    uint8_t* to_v = whole_v ? s_v : gv;
 #pragma unroll
     for (int e = 0; e < E; e += 4) {
       int wk = 0x7F7F7F7F, wv = 0;
-      if (!any) {
+      if (!bad) {
         wk = fp8_pack4(k[e] * fk, k[e + 1] * fk, k[e + 2] * fk, k[e + 3] * fk);
         wv = fp8_pack4(v[e] * fv, v[e + 1] * fv, v[e + 2] * fv, v[e + 3] * fv);
       }
       const int d = quarter * E + e;
-      *reinterpret_cast<int*>(s_k + k_at(off + tok, d)) = wk;
+      *reinterpret_cast<int*>(to_k + k_at(off + tok, d)) = wk;
 #pragma unroll
-      for (int i = 0; i < 4; i++) s_v[v_at(off + tok, d + i)] = (uint8_t)(wv >> (8 * i));
+      for (int i = 0; i < 4; i++) to_v[v_at(off + tok, d + i)] = (uint8_t)(wv >> (8 * i));
     }
   }
+  if (!whole_k && !whole_v) return;  // the scales stay as well
   __syncthreads();
   for (int i = tid * 16; i < kBytes; i += kAppendThreads * 16) {
-    *reinterpret_cast<v4i*>(gk + i) = *reinterpret_cast<const v4i*>(s_k + i);
-    *reinterpret_cast<v4i*>(gv + i) = *reinterpret_cast<const v4i*>(s_v + i);
+    if (whole_k) *reinterpret_cast<v4i*>(gk + i) = *reinterpret_cast<const v4i*>(s_k + i);
+    if (whole_v) *reinterpret_cast<v4i*>(gv + i) = *reinterpret_cast<const v4i*>(s_v + i);
   }
   if (tid == 0) {
     p.cache.k_exp[unit] = (uint8_t)xk;
