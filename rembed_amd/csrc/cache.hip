@@ -14,6 +14,7 @@
 #include "fp8.h"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace rh {
 
@@ -262,6 +263,12 @@ __device__ __forceinline__ int append_request(const int32_t* blocks, int batch, 
   return lo;
 }
 
+// Where a byte of V lies in LDS: 16-byte pieces change places within their 512 bytes, so
+// that the words a wave writes at once (tokens 4 apart, values DH/4 apart) meet different banks.
+__device__ __forceinline__ int spread(int at) {
+  return at ^ ((at >> 9 & 1) << 6 | (at >> 11 & 1) << 7);
+}
+
 template <int DH, bool BF16>
 __global__ __launch_bounds__(kAppendThreads) void cache_append_kernel(CacheAppendArgs p) {
   constexpr int kBytes = kPage * DH, E = DH / 4;  // a head's block; values per thread
@@ -283,34 +290,22 @@ __global__ __launch_bounds__(kAppendThreads) void cache_append_kernel(CacheAppen
   const int cnt = min(kPage - off, fresh - first);
   if (cnt <= 0) return;
 
-  // this thread's quarter of its token's K and V
-  const int tok = tid >> 2, quarter = tid & 3;
-  float k[E], v[E];
+  // this thread's quarter of its token's K and V; four lanes beside each other have the
+  // four tokens of one word of V
+  const int tok = tid / 16 * 4 + tid % 4, quarter = tid / 4 % 4;
+  const bool mine = tok >= off && tok < off + cnt;
+  using T = std::conditional_t<BF16, v8bf, v4f>;  // 16 bytes of a row, widened when used
+  constexpr int kStep = BF16 ? 8 : 4;
+  T k[E / kStep], v[E / kStep];
   uint32_t mk = 0, mv = 0;
-  if (tok < cnt) {
-    const size_t at = (size_t)(r0 + first + tok) * p.ldkv + h * DH + quarter * E;
-    constexpr int kStep = BF16 ? 8 : 4;
+  if (mine) {
+    const size_t at = (size_t)(r0 + first + tok - off) * p.ldkv + h * DH + quarter * E;
+    using S = std::conditional_t<BF16, __bf16, float>;
+    const S* row = static_cast<const S*>(p.kv) + at;
 #pragma unroll
-    for (int e = 0; e < E; e += kStep) {
-      if constexpr (BF16) {
-        const __bf16* row = static_cast<const __bf16*>(p.kv) + at + e;
-        const v8bf x = *reinterpret_cast<const v8bf*>(row + p.k_off);
-        const v8bf y = *reinterpret_cast<const v8bf*>(row + p.v_off);
-#pragma unroll
-        for (int i = 0; i < kStep; i++) {
-          k[e + i] = (float)x[i];
-          v[e + i] = (float)y[i];
-        }
-      } else {
-        const float* row = static_cast<const float*>(p.kv) + at + e;
-        const v4f x = *reinterpret_cast<const v4f*>(row + p.k_off);
-        const v4f y = *reinterpret_cast<const v4f*>(row + p.v_off);
-#pragma unroll
-        for (int i = 0; i < kStep; i++) {
-          k[e + i] = x[i];
-          v[e + i] = y[i];
-        }
-      }
+    for (int e = 0; e < E / kStep; e++) {
+      k[e] = *reinterpret_cast<const T*>(row + p.k_off + e * kStep);
+      v[e] = *reinterpret_cast<const T*>(row + p.v_off + e * kStep);
     }
   }
   const int64_t slot = p.slots[r0 + first];
@@ -319,25 +314,22 @@ __global__ __launch_bounds__(kAppendThreads) void cache_append_kernel(CacheAppen
   uint8_t* gk = p.cache.k + unit * kBytes;
   uint8_t* gv = p.cache.v + unit * kBytes;
   const int ok = p.cache.k_exp[unit], ov = p.cache.v_exp[unit];
-  if (tok < cnt) {
+  if (mine) {
 #pragma unroll
     for (int e = 0; e < E; e++) {
-      mk = max(mk, __float_as_uint(k[e]) & 0x7FFFFFFFu);
-      mv = max(mv, __float_as_uint(v[e]) & 0x7FFFFFFFu);
+      mk = max(mk, __float_as_uint((float)k[e / kStep][e % kStep]) & 0x7FFFFFFFu);
+      mv = max(mv, __float_as_uint((float)v[e / kStep][e % kStep]) & 0x7FFFFFFFu);
     }
   }
   int bad = mk >= 0x7F800000u || mv >= 0x7F800000u;
-  bad |= __shfl_xor(bad, 1, 64);
-  bad |= __shfl_xor(bad, 2, 64);
+  bad |= __shfl_xor(bad, 4, 64);
+  bad |= __shfl_xor(bad, 8, 64);
   if (bad) mk = mv = 0;
-  for (int o = 32; o >= 4; o >>= 1) {
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) {
     mk = max(mk, (uint32_t)__shfl_xor((int)mk, o, 64));
     mv = max(mv, (uint32_t)__shfl_xor((int)mv, o, 64));
   }
-  mk = max(mk, (uint32_t)__shfl_xor((int)mk, 1, 64));
-  mv = max(mv, (uint32_t)__shfl_xor((int)mv, 1, 64));
-  mk = max(mk, (uint32_t)__shfl_xor((int)mk, 2, 64));
-  mv = max(mv, (uint32_t)__shfl_xor((int)mv, 2, 64));
   if ((tid & 63) == 0) {
     s_max[tid >> 6][0] = mk;
     s_max[tid >> 6][1] = mv;
@@ -380,32 +372,63 @@ __global__ __launch_bounds__(kAppendThreads) void cache_append_kernel(CacheAppen
         if (whole_v) c[e] = scaled(c[e], xv - ov);
       }
       if (whole_k) *reinterpret_cast<v4i*>(s_k + i) = a;
-      if (whole_v) *reinterpret_cast<v4i*>(s_v + i) = c;
+      if (whole_v) *reinterpret_cast<v4i*>(s_v + spread(i)) = c;
     }
     if (whole_k || whole_v) __syncthreads();
   }
-  if (tok < cnt) {
+  if (mine) {
     const float fk = fp8_inverse(xk), fv = fp8_inverse(xv);
-    uint8_t* to_k = whole_k ? s_k : gk;
-    uint8_t* to_v = whole_v ? s_v : gv;
+    int wk[E / 4], wv[E / 4];
 #pragma unroll
     for (int e = 0; e < E; e += 4) {
-      int wk = 0x7F7F7F7F, wv = 0;
-      if (!bad) {
-        wk = fp8_pack4(k[e] * fk, k[e + 1] * fk, k[e + 2] * fk, k[e + 3] * fk);
-        wv = fp8_pack4(v[e] * fv, v[e + 1] * fv, v[e + 2] * fv, v[e + 3] * fv);
+      const T x = k[e / kStep], y = v[e / kStep];
+      const int i = e % kStep;
+      wk[e / 4] = fp8_pack4((float)x[i] * fk, (float)x[i + 1] * fk, (float)x[i + 2] * fk,
+                            (float)x[i + 3] * fk);
+      wv[e / 4] = fp8_pack4((float)y[i] * fv, (float)y[i + 1] * fv, (float)y[i + 2] * fv,
+                            (float)y[i + 3] * fv);
+      if (bad) {
+        wk[e / 4] = 0x7F7F7F7F;
+        wv[e / 4] = 0;
       }
-      const int d = quarter * E + e;
-      *reinterpret_cast<int*>(to_k + k_at(off + tok, d)) = wk;
+    }
 #pragma unroll
-      for (int i = 0; i < 4; i++) to_v[v_at(off + tok, d + i)] = (uint8_t)(wv >> (8 * i));
+    for (int e = 0; e < E; e += 16) {
+      const int at = k_at(tok, quarter * E + e);
+      const v4i w = {wk[e / 4], wk[e / 4 + 1], wk[e / 4 + 2], wk[e / 4 + 3]};
+      if (whole_k) *reinterpret_cast<v4i*>(s_k + at) = w;
+      else *reinterpret_cast<v4i*>(gk + at) = w;
+    }
+    if (tok - tid % 4 >= off && tok - tid % 4 + 3 < off + cnt) {
+      // all four tokens are new: four values of one token each become four tokens'
+      // value d + tid % 4 (bytes change places with the neighbour's, pairs with the pair's)
+      const int odd = tid & 1, high = tid & 2;
+#pragma unroll
+      for (int e = 0; e < E; e += 4) {
+        int w = wv[e / 4];
+        int o = __builtin_amdgcn_mov_dpp(w, 0xB1, 0xF, 0xF, true);  // lanes 1 0 3 2
+        w = __builtin_amdgcn_perm(o, w, odd ? 0x03070105 : 0x06020400);
+        o = __builtin_amdgcn_mov_dpp(w, 0x4E, 0xF, 0xF, true);  // lanes 2 3 0 1
+        w = __builtin_amdgcn_perm(o, w, high ? 0x03020706 : 0x05040100);
+        const int at = v_at(tok - tid % 4, quarter * E + e + tid % 4);
+        if (whole_v) *reinterpret_cast<int*>(s_v + spread(at)) = w;
+        else *reinterpret_cast<int*>(gv + at) = w;
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < E; e++) {
+        const int at = v_at(tok, quarter * E + e);
+        const uint8_t c = (uint8_t)(wv[e / 4] >> (e % 4 * 8));
+        if (whole_v) s_v[spread(at)] = c;
+        else gv[at] = c;
+      }
     }
   }
   if (!whole_k && !whole_v) return;  // the scales stay as well
   __syncthreads();
   for (int i = tid * 16; i < kBytes; i += kAppendThreads * 16) {
     if (whole_k) *reinterpret_cast<v4i*>(gk + i) = *reinterpret_cast<const v4i*>(s_k + i);
-    if (whole_v) *reinterpret_cast<v4i*>(gv + i) = *reinterpret_cast<const v4i*>(s_v + i);
+    if (whole_v) *reinterpret_cast<v4i*>(gv + i) = *reinterpret_cast<const v4i*>(s_v + spread(i));
   }
   if (tid == 0) {
     p.cache.k_exp[unit] = (uint8_t)xk;
