@@ -15,6 +15,7 @@
 #include "fp8.h"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace rh {
 
@@ -51,43 +52,91 @@ __device__ __forceinline__ float max_halves(float v) {
 }
 
 // The columns' codes and scale bytes: lane (column, half) holds values
-// 64 s + 32 half .. + 31 of step s, as K's pieces do.
+// 64 s + 32 half .. + 31 of step s, as K's pieces do. A wave does this once, in line, so its
+// instructions count (9 a value took 4.9 µs of dh 256's 29 at 8 pages): conversions that
+// scale by themselves, 4.5 a value. Columns with infinities or NaN, and those below 2^-103,
+// whose unit's reciprocal conversions take other ways, go by the plain one.
 template <int KS, bool BF16>
 __device__ __forceinline__ void cache_load_q(const void* q, size_t at, int half, v8i (&hi)[KS],
                                              v8i (&lo)[KS], int& xh, int& xl) {
-  float v[KS][32];
+#if defined(__HIP_DEVICE_COMPILE__)
+  using S = std::conditional_t<BF16, __bf16, float>;
+  using T = std::conditional_t<BF16, v8bf, v4f>;
+  constexpr int E = BF16 ? 8 : 4;
+  T v[KS][32 / E];
   uint32_t m = 0;
 #pragma unroll
   for (int s = 0; s < KS; s++)
 #pragma unroll
-    for (int e = 0; e < 32; e += 8) {
-      const size_t o = at + s * 64 + half * 32 + e;
-      if constexpr (BF16) {
-        const v8bf x = *reinterpret_cast<const v8bf*>(static_cast<const __bf16*>(q) + o);
+    for (int i = 0; i < 32 / E; i++)
+      v[s][i] =
+          *reinterpret_cast<const T*>(static_cast<const S*>(q) + at + s * 64 + half * 32 + i * E);
+  if constexpr (BF16) {
+    typedef uint16_t v2u16 __attribute__((ext_vector_type(2)));
+    v2u16 top = {0, 0};
 #pragma unroll
-        for (int i = 0; i < 8; i++) v[s][e + i] = (float)x[i];
-      } else {
-        const v4f a = *reinterpret_cast<const v4f*>(static_cast<const float*>(q) + o);
-        const v4f b = *reinterpret_cast<const v4f*>(static_cast<const float*>(q) + o + 4);
+    for (int s = 0; s < KS; s++)
 #pragma unroll
-        for (int i = 0; i < 8; i++) v[s][e + i] = i < 4 ? a[i] : b[i - 4];
+      for (int i = 0; i < 32 / E; i++) {
+        const v4i w = __builtin_bit_cast(v4i, v[s][i]);
+#pragma unroll
+        for (int e = 0; e < 4; e++)
+          top = __builtin_elementwise_max(top, __builtin_bit_cast(v2u16, w[e] & 0x7FFF7FFF));
       }
+    m = (uint32_t)max(top[0], top[1]) << 16;
+  } else {
 #pragma unroll
-      for (int i = 0; i < 8; i++) m = max(m, finite_abs_bits(v[s][e + i]));
-    }
+    for (int s = 0; s < KS; s++)
+#pragma unroll
+      for (int i = 0; i < 32 / E; i++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) m = max(m, __float_as_uint(v[s][i][e]) & 0x7FFFFFFFu);
+  }
   m = max(m, (uint32_t)__shfl_xor((int)m, 32, 64));
   xh = fp8_exponent(m);
-  xl = max(xh - 4, 0);
-  const float f = fp8_inverse(xh);
+  auto value = [&](int s, int i) { return (float)v[s][i / E][i % E]; };
+  if (__builtin_expect(__any(m >= 0x7F800000u || xh < 16), 0)) {
+    m = 0;
+    for (int s = 0; s < KS; s++)
+      for (int i = 0; i < 32; i++) m = max(m, finite_abs_bits(value(s, i)));
+    m = max(m, (uint32_t)__shfl_xor((int)m, 32, 64));
+    xh = fp8_exponent(m);
+    xl = max(xh - 4, 0);
+    const float f = fp8_inverse(xh);
+#pragma unroll
+    for (int s = 0; s < KS; s++)
+#pragma unroll
+      for (int w = 0; w < 8; w++) {
+        const float a = value(s, 4 * w) * f, b = value(s, 4 * w + 1) * f,
+                    c = value(s, 4 * w + 2) * f, d = value(s, 4 * w + 3) * f;
+        hi[s][w] = fp8_pack4(a, b, c, d);
+        lo[s][w] = xh >= 4 ? fp8_rest4(hi[s][w], a, b, c, d) : 0;
+      }
+    return;
+  }
+  xl = xh - 4;
+  const float unit = __uint_as_float((uint32_t)xh << 23), rest = unit * 0.0625f;
+  typedef short v2s __attribute__((ext_vector_type(2)));
 #pragma unroll
   for (int s = 0; s < KS; s++)
 #pragma unroll
     for (int w = 0; w < 8; w++) {
-      const float a = v[s][4 * w] * f, b = v[s][4 * w + 1] * f, c = v[s][4 * w + 2] * f,
-                  d = v[s][4 * w + 3] * f;
-      hi[s][w] = fp8_pack4(a, b, c, d);
-      lo[s][w] = xh >= 4 ? fp8_rest4(hi[s][w], a, b, c, d) : 0;
+      const float a = value(s, 4 * w), b = value(s, 4 * w + 1), c = value(s, 4 * w + 2),
+                  d = value(s, 4 * w + 3);
+      v2s h, l;
+      asm("" : "=v"(h) : "v"(a));  // any word: both halves get written
+      h = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(h, a, b, unit, false);
+      h = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(h, c, d, unit, true);
+      const int codes = __builtin_bit_cast(int, h);
+      const v2f x = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(codes, unit, false);
+      const v2f y = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(codes, unit, true);
+      asm("" : "=v"(l) : "v"(a));
+      l = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(l, a - x[0], b - x[1], rest, false);
+      l = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(l, c - y[0], d - y[1], rest, true);
+      hi[s][w] = codes;
+      lo[s][w] = __builtin_bit_cast(int, l);
     }
+#endif
 }
 
 // V's codes behind the last token to zero: nothing was written there, and no NaN code may
@@ -538,14 +587,16 @@ __global__ __launch_bounds__(64 * kWaves, DH == 256 ? 1 : 2) void cache_attentio
 }
 
 // ---- many columns --------------------------------------------------------------------
-// Four waves of 32 columns each walk the same pages. What bounds it: a page's products take
+// CW waves of 32 columns each walk the same pages, PG such groups a part of them each. What bounds it: a page's products take
 // the matrix cores 64 cycles each (dh 128: 16 of them, 1024 cycles) and its softmax the VALU
 // 1100 to 1300, and a wave issues in order, so one after the other they cost their sum even
 // with two waves per SIMD. The loop therefore is a pipeline over pages whose body has no
 // branch: while page g's scores become P, two at a time, the products between them are
 // page g + 1's scores and page g - 1's values. K and V come to LDS by global_load_lds in
 // fragment order (1 KiB pieces, read back without bank conflicts), two turns before they are
-// used, with one barrier per turn.
+// used (one turn where LDS has room for two pages only), with one barrier per turn. Where few
+// workgroups come together, a CU has one of them and a wave's own chain bounds a turn: then
+// two waves take two tiles, and two more the second half of the pages, joined in LDS.
 template <int DH>
 struct CachePipe : CacheFast<DH> {  // ph, pl, eh, el: P of the page before
   using Base = CacheFast<DH>;
@@ -660,14 +711,16 @@ struct CachePipe : CacheFast<DH> {  // ph, pl, eh, el: P of the page before
   }
 };
 
-template <int DH, bool BF16>
-__global__ __launch_bounds__(64 * kWaves, DH == 256 ? 1 : 2) void cache_attention_cols_kernel(
+template <int DH, bool BF16, int CW, int PG, int SLOTS>
+__global__ __launch_bounds__(64 * CW * PG, DH == 256 ? 1 : 2) void cache_attention_cols_kernel(
     CacheAttnArgs p, int tiles, int splits, int part_cols) {
   constexpr int KS = DH / 64, DT = DH / 32, kHalf = kPageT * DH;  // bytes of K or V of a page
-  constexpr int kLds = 6 * kHalf;  // K of three pages, V of three
-  constexpr int kPieces = kHalf / 1024 / kWaves;     // 1 KiB pieces per wave, of K and of V
+  constexpr int kRing = 2 * SLOTS * kHalf;  // a group's K pages, then its V pages
+  constexpr int kJoin = PG > 1 ? CW * kCols * (DH + 2) * 4 : 0;
+  constexpr int kLds = PG * kRing > kJoin ? PG * kRing : kJoin;
+  constexpr int kPieces = kHalf / 1024 / CW;  // 1 KiB pieces per wave, of K and of V
   __shared__ __attribute__((aligned(1024))) uint8_t lds[kLds];
-  const int wgs = (tiles + kWaves - 1) / kWaves;
+  const int wgs = (tiles + CW - 1) / CW;
   int b, h, wg, split;
   cache_unit(p, wgs, splits, b, h, wg, split);
   if (p.causal) {
@@ -679,20 +732,24 @@ __global__ __launch_bounds__(64 * kWaves, DH == 256 ? 1 : 2) void cache_attentio
   const int G = p.heads / p.cache.kv_heads;
   const int r0 = p.cu[b], nq = p.cu[b + 1] - r0;
   const int cols = nq * G;
-  if (wg * kWaves * kCols >= cols) return;
+  if (wg * CW * kCols >= cols) return;
   const int n = max(0, min(p.lens[b], p.ldt * kPageT));
   const int lane = threadIdx.x & 63, col = lane & 31, half = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int tile = wg * kWaves + wave, c0 = tile * kCols;
+  const int group = PG > 1 ? wave / CW : 0, part_of = PG > 1 ? wave % CW : wave;
+  const int tile = wg * CW + part_of, c0 = tile * kCols;
   const int c = min(c0 + col, cols - 1), ct = c / G;
   const int pos0 = n - nq;
   const float cs = p.scale * 1.44269504088896341f;
 
   int lo, hi;
-  cache_page_range(p, pos0, n, G, wg * kWaves * kCols, min((wg + 1) * kWaves * kCols, cols), lo, hi);
+  cache_page_range(p, pos0, n, G, wg * CW * kCols, min((wg + 1) * CW * kCols, cols), lo, hi);
   if (p.cache.pages < 1) hi = lo;
   const int each = (max(0, hi - lo) + splits - 1) / splits;
-  const int first = lo + split * each, end = min(hi, first + each);
+  // the group's pages; the last group's may end behind the range, with pages that are none
+  const int limit = min(hi, lo + (split + 1) * each);
+  const int turns = (max(0, limit - lo - split * each) + PG - 1) / PG;
+  const int first = lo + split * each + group * turns, end = first + turns;
   const bool active = c0 < cols;
 
   // A page that is none is read as page 0 and holds no keys.
@@ -700,33 +757,33 @@ __global__ __launch_bounds__(64 * kWaves, DH == 256 ? 1 : 2) void cache_attentio
   int base = first;  // the window's first page
   auto dma = [&](const uint8_t* src, int page, uint8_t* dst) {
     const size_t unit = (size_t)max(page, 0) * p.cache.kv_heads + h;
-    const uint8_t* at = src + unit * kHalf + wave * kPieces * 1024 + lane * 16;
+    const uint8_t* at = src + unit * kHalf + part_of * kPieces * 1024 + lane * 16;
 #pragma unroll
     for (int i = 0; i < kPieces; i++)
-      lds_dma16(at + i * 1024, dst + (wave * kPieces + i) * 1024);
+      lds_dma16(at + i * 1024, dst + (part_of * kPieces + i) * 1024);
   };
-  uint8_t* const ldsk = lds;
-  uint8_t* const ldsv = lds + 3 * kHalf;
-  // V behind the last token is zeroed: no NaN code may meet a zero P
+  uint8_t* const ldsk = lds + group * kRing;
+  uint8_t* const ldsv = ldsk + SLOTS * kHalf;
+  // V behind the last token is zeroed: no NaN code may meet a zero P. A wave does it to the
+  // pieces it fetched, before the barrier that gives them to the others.
   auto clean = [&](int g, bool none, uint8_t* v) {
     if (!none && (g + 1) * kPageT <= n) return;
-    for (int i = threadIdx.x * 4; i < kHalf; i += 64 * kWaves * 4) {
+    for (int i = part_of * kPieces * 1024 + lane * 4; i < (part_of + 1) * kPieces * 1024; i += 256) {
       // four tokens of one column: 32 * part + 8 * (byte / 4) + 4 * half
       const int t = (i / 1024 & 1) * 32 + (i % 16) / 4 * 8 + (i % 1024) / 512 * 4;
       const int left = none ? 0 : n - (g * kPageT + t);
       const int keep = left >= 4 ? -1 : left <= 0 ? 0 : (1 << (8 * left)) - 1;
       *reinterpret_cast<int*>(v + i) &= keep;
     }
-    __syncthreads();
   };
 
   CachePipe<DH> w;
-  if (first < end) {
-    win.load(p, b, h, first, end, lane);
+  if (turns > 0) {
+    win.load(p, b, h, first, limit, lane);
     dma(p.cache.k, win.at(win.page, 0), ldsk);
     dma(p.cache.k, win.at(win.page, 1), ldsk + kHalf);
     dma(p.cache.v, win.at(win.page, 0), ldsv + kHalf);
-    dma(p.cache.k, win.at(win.page, 2), ldsk + 2 * kHalf);
+    if (SLOTS > 2) dma(p.cache.k, win.at(win.page, 2), ldsk + 2 * kHalf);
   }
   cache_load_q<KS, BF16>(p.q, (size_t)(r0 + ct) * p.ldq + p.q_off + (h * G + c - ct * G) * DH, half,
                          w.qh, w.ql, w.xh, w.xl);
@@ -735,20 +792,26 @@ __global__ __launch_bounds__(64 * kWaves, DH == 256 ? 1 : 2) void cache_attentio
   // turn g: K of g + 1 in slot ks of ldsk, V of g - 1 in slot vs of ldsv
   int ks = 1, vs = 0;
   bool nonep = false, none = false;  // page g - 1, g is none
-  auto after = [](int slot) { return slot == 2 ? 0 : slot + 1; };
+  auto after = [](int slot) { return slot == SLOTS - 1 ? 0 : slot + 1; };
+  constexpr int kAhead = SLOTS;  // K of g + kAhead, V of g + kAhead - 2 are asked for in turn g
   auto stage = [&](int g) {
-    wait_vmcnt<2 * kPieces>();  // all but the last turn's
+    if (SLOTS > 2) wait_vmcnt<2 * kPieces>();  // all but the last turn's
+    else wait_vmcnt<0>();
+    if (g > first) clean(g - 1, nonep, ldsv + vs * kHalf);
     wait_lgkmcnt0();
     stage_barrier();
-    if (g > first) clean(g - 1, nonep, ldsv + vs * kHalf);
-    if (g + 3 >= base + 64) {
-      win.load(p, b, h, g, end, lane);
+    if (g + kAhead >= base + 64) {
+      win.load(p, b, h, g, limit, lane);
       base = g;
     }
     none = win.at(win.page, g - base) < 0;
-    // V of g + 1 and K of g + 3 go where V of g - 2 and K of g were
-    dma(p.cache.v, win.at(win.page, g + 1 - base), ldsv + after(after(vs)) * kHalf);
-    dma(p.cache.k, win.at(win.page, g + 3 - base), ldsk + after(after(ks)) * kHalf);
+    // Three slots: V of g + 1 and K of g + 3 go where V of g - 2 and K of g were.
+    // Two: V of g (the first is there) and K of g + 2.
+    const int vto = SLOTS > 2 ? after(after(vs)) : after(vs);
+    const int kto = SLOTS > 2 ? after(after(ks)) : after(ks);
+    if (SLOTS > 2 || g > first)
+      dma(p.cache.v, win.at(win.page, g + kAhead - 2 - base), ldsv + vto * kHalf);
+    dma(p.cache.k, win.at(win.page, g + kAhead - base), ldsk + kto * kHalf);
   };
   auto done = [&] {
     nonep = none;
@@ -757,13 +820,13 @@ __global__ __launch_bounds__(64 * kWaves, DH == 256 ? 1 : 2) void cache_attentio
   };
   auto last = [&] {
     wait_vmcnt<0>();
+    clean(end - 1, nonep, ldsv + vs * kHalf);
     wait_lgkmcnt0();
     stage_barrier();
-    clean(end - 1, nonep, ldsv + vs * kHalf);
   };
-  if (first < end) {
+  if (turns > 0) {
     // V of page `first - 1` is multiplied by P = 0: any finite codes
-    for (int i = threadIdx.x * 16; i < kHalf; i += 64 * kWaves * 16)
+    for (int i = part_of * 1024 + lane * 16; i < kHalf; i += CW * 1024)
       *reinterpret_cast<v4i*>(ldsv + i) = v4i{0, 0, 0, 0};
     __syncthreads();  // waits for the DMA too
     if (!active) {  // a wave without columns stages its pieces
@@ -789,15 +852,86 @@ __global__ __launch_bounds__(64 * kWaves, DH == 256 ? 1 : 2) void cache_attentio
     }
   }
   __syncthreads();
+  if (__builtin_expect(active && __any(w.far), 0))
+    cache_again<DH>(w, p, b, h, first, min(end, limit), 1, n, cs, lane);
+  float unit = w.unit();
+  float l = w.lrun + __shfl_xor(w.lrun, 32, 64);
+  if constexpr (PG > 1) {
+    // the second group's results to the first, lane by lane
+    float* at = reinterpret_cast<float*>(lds) + part_of * kCols * (DH + 2);
+    float* mine = at + lane * 4;
+    float* top = at + kCols * DH;
+    if (group == 1 && active) {
+#pragma unroll
+      for (int t = 0; t < DT; t++)
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+          v4f x;
+#pragma unroll
+          for (int e = 0; e < 4; e++) x[e] = w.o[t][i * 4 + e] * unit;
+          *reinterpret_cast<v4f*>(mine + (t * 4 + i) * 256) = x;
+        }
+      top[col] = w.mref;
+      top[kCols + col] = l;
+    }
+    __syncthreads();
+    if (group == 1) return;
+    if (active) {
+      const float m2 = top[col], l2 = top[kCols + col], to = fmaxf(w.mref, m2);
+      const float f = w.mref == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(w.mref - to);
+      const float f2 = m2 == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m2 - to);
+      unit *= f;
+      l = l * f + l2 * f2;
+#pragma unroll
+      for (int t = 0; t < DT; t++)
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+          const v4f x = *reinterpret_cast<const v4f*>(mine + (t * 4 + i) * 256);
+#pragma unroll
+          for (int e = 0; e < 4; e++)
+            w.o[t][i * 4 + e] = w.o[t][i * 4 + e] * unit + x[e] * f2;
+        }
+      unit = 1.0f;
+      w.mref = to;
+    }
+  }
   if (!active) return;
-  if (__builtin_expect(__any(w.far), 0))
-    cache_again<DH>(w, p, b, h, first, end, 1, n, cs, lane);
-  const float unit = w.unit();
 
-  // a lane holds four consecutive values of its column at a time, its other half the
-  // next four
-  const float l = w.lrun + __shfl_xor(w.lrun, 32, 64);
   const float inv = splits > 1 ? unit : l == 0.0f ? 0.0f : unit / l;
+  const size_t to = (size_t)(r0 + ct) * p.ldout + (h * G + c - ct * G) * DH;
+  if (splits == 1 && p.out_bf16) {
+    // A lane holds four consecutive values of its column at a time, its other half the next
+    // four: written as they are, 64 pieces of 8 bytes a store. Whole rows instead, through LDS
+    // (16-byte pieces at places that the row turns, so that a column of them meets all banks).
+    uint8_t* own = lds + part_of * (PG > 1 ? kCols * (DH + 2) * 4 : kCols * (DH * 2 + 8));
+    int64_t* dest = reinterpret_cast<int64_t*>(own + kCols * DH * 2);
+    auto place = [&](int row, int piece) {
+      return own + row * (DH * 2) + (piece ^ (DH == 64 ? row / 2 % 8 : row % 16)) * 16;
+    };
+    if (half == 0) dest[col] = c0 + col < cols ? (int64_t)to : -1;
+#pragma unroll
+    for (int t = 0; t < DT; t++)
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        typedef __bf16 v4bf __attribute__((ext_vector_type(4)));
+        const v4bf x = {(__bf16)(w.o[t][i * 4] * inv), (__bf16)(w.o[t][i * 4 + 1] * inv),
+                        (__bf16)(w.o[t][i * 4 + 2] * inv), (__bf16)(w.o[t][i * 4 + 3] * inv)};
+        *reinterpret_cast<v4bf*>(place(col, t * 4 + i) + half * 8) = x;
+      }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    constexpr int kLanes = DH / 8;  // of a row
+    typedef v8bf Out __attribute__((aligned(8)));
+#pragma unroll
+    for (int r = 0; r < kCols; r += 64 / kLanes) {
+      const int row = r + lane / kLanes;
+      const v8bf x = *reinterpret_cast<const v8bf*>(place(row, lane % kLanes));
+      const int64_t at = dest[row];
+      if (at >= 0)
+        *reinterpret_cast<Out*>(static_cast<__bf16*>(p.out) + at + lane % kLanes * 8) = x;
+    }
+    return;
+  }
   if (c0 + col >= cols) return;
   float* part = nullptr;
   if (splits > 1) {
@@ -807,8 +941,9 @@ __global__ __launch_bounds__(64 * kWaves, DH == 256 ? 1 : 2) void cache_attentio
       part[DH] = w.mref;
       part[DH + 1] = l;
     }
+  } else {
+    part = static_cast<float*>(p.out) + to;
   }
-  const size_t to = (size_t)(r0 + ct) * p.ldout + (h * G + c - ct * G) * DH;
 #pragma unroll
   for (int t = 0; t < DT; t++)
 #pragma unroll
@@ -816,9 +951,7 @@ __global__ __launch_bounds__(64 * kWaves, DH == 256 ? 1 : 2) void cache_attentio
       v4f x;
 #pragma unroll
       for (int e = 0; e < 4; e++) x[e] = w.o[t][i * 4 + e] * inv;
-      const int d = t * 32 + i * 8 + half * 4;
-      if (part) *reinterpret_cast<v4f*>(part + d) = x;
-      else cache_store4(p, to + d, x);
+      *reinterpret_cast<v4f*>(part + t * 32 + i * 8 + half * 4) = x;
     }
 }
 
@@ -869,47 +1002,80 @@ static bool cache_by_cols(int max_q, int heads, int kv_heads) {
   return (long long)max_q * (heads / kv_heads) > kCols;
 }
 
-// Key ranges: as many as give the chip's 256 CUs six workgroups each (by columns: one),
-// where a range still has a page for every wave (by columns: 16 pages). A window leaves a
-// tile few pages, and no range of its own for each: 0 (any window) never gives fewer ranges
-// than a window does.
-void cache_attention_plan(int batch, int max_q, int max_len, int heads, int kv_heads, int dh,
-                          int window, int* splits, size_t* part_floats) {
-  const long long tiles = cache_tiles(max_q, heads, kv_heads);
-  const long long units = (long long)batch * kv_heads * tiles;
+static long long cache_pages(int max_q, int max_len, int window, int cols) {
+  const long long pages = ((long long)max_len + kPageT - 1) / kPageT;
+  if (window <= 0) return pages;
+  return std::min(pages, (2LL * window + std::min(max_q, cols)) / kPageT + 2);
+}
+
+// Many columns: two tiles or four per workgroup. A page then takes a CU with one workgroup
+// 0.62 µs (two tiles) or 1.1 (four), with two of them 1.11 or 2.05 (dh 128), so two tiles are
+// faster while they fill the chip at most one and a half times (32 requests of 9 to 70
+// rows: 24.9 µs against 28.3), four are by 8% behind that (4096 rows). dh 256 has room for
+// one workgroup per CU, 1.0 or 1.6 µs a page, and where enough key ranges of four tiles can be
+// made, they fill the chip (2000 rows over 4000: 56 µs against 69).
+static bool cache_two_tiles(int batch, int max_q, int heads, int kv_heads, int dh,
+                            long long pages) {
+  const long long tiles = cache_tiles(max_q, heads, kv_heads), units = (long long)batch * kv_heads;
+  if (dh == 256) return units * ((tiles + 3) / 4) * std::max(1LL, pages / 8) <= 128;
+  return units * ((tiles + 1) / 2) <= 768;
+}
+
+// Key ranges: as many as give the chip's 256 CUs six workgroups each (many columns: one),
+// where a range still has a page for every wave (many columns: 16 pages, dh 256: 8). A window
+// leaves a tile few pages, and no range of its own for each.
+static int cache_ranges(int batch, int max_q, int heads, int kv_heads, int dh, int per_wg,
+                        long long pages) {
   const bool cols = cache_by_cols(max_q, heads, kv_heads);
-  const long long wgs = cols ? (long long)batch * kv_heads * ((tiles + kWaves - 1) / kWaves) : units;
-  long long pages = ((long long)max_len + kPageT - 1) / kPageT;
-  if (window > 0) {
-    const long long tokens = std::min<long long>(max_q, kCols * (cols ? kWaves : 1));
-    pages = std::min(pages, (2LL * window + tokens) / kPageT + 2);
-  }
+  const long long tiles = cache_tiles(max_q, heads, kv_heads);
+  const long long wgs = (long long)batch * kv_heads * ((tiles + per_wg - 1) / per_wg);
   const long long want = cols ? 256 : 1536;
-  long long s = wgs > 0 ? (want + wgs - 1) / wgs : 1;
-  s = std::max(1LL, std::min(s, pages / (cols ? 16 : kWaves)));
-  *splits = (int)s;
-  *part_floats = s > 1 ? (size_t)units * s * cache_part_cols(max_q, heads, kv_heads) * (dh + 4) : 0;
+  const bool one = cols && dh == 256;  // a CU has room for one: no second round
+  const long long s = wgs > 0 ? (one ? want : want + wgs - 1) / wgs : 1;
+  return (int)std::max(1LL, std::min(s, pages / (!cols ? kWaves : one ? 8 : 16)));
+}
+
+// Tiles per workgroup and key ranges per tile.
+static void cache_split(int batch, int max_q, int max_len, int heads, int kv_heads, int dh,
+                        int window, int* per_wg, int* splits) {
+  const bool cols = cache_by_cols(max_q, heads, kv_heads);
+  const long long pages = cache_pages(max_q, max_len, window, cols ? 4 * kCols : kCols);
+  *per_wg = !cols ? 1 : cache_two_tiles(batch, max_q, heads, kv_heads, dh, pages) ? 2 : 4;
+  *splits = cache_ranges(batch, max_q, heads, kv_heads, dh, *per_wg, pages);
+}
+
+// For any window: all pages, and four tiles, which never make fewer ranges than two.
+size_t cache_attention_floats(int batch, int max_q, int max_len, int heads, int kv_heads, int dh) {
+  const int per_wg = cache_by_cols(max_q, heads, kv_heads) ? 4 : 1;
+  const int splits = cache_ranges(batch, max_q, heads, kv_heads, dh, per_wg,
+                                  cache_pages(max_q, max_len, 0, 0));
+  if (splits < 2) return 0;
+  return (size_t)batch * kv_heads * cache_tiles(max_q, heads, kv_heads) * splits *
+         cache_part_cols(max_q, heads, kv_heads) * (dh + 4);
 }
 
 template <int DH>
 static hipError_t launch_dh(const CacheAttnArgs& a, hipStream_t s) {
-  int splits;
-  size_t part;
-  cache_attention_plan(a.batch, a.max_q, a.max_len, a.heads, a.cache.kv_heads, DH, a.window, &splits,
-                       &part);
+  int per_wg, splits;
+  cache_split(a.batch, a.max_q, a.max_len, a.heads, a.cache.kv_heads, DH, a.window, &per_wg,
+              &splits);
   const int tiles = cache_tiles(a.max_q, a.heads, a.cache.kv_heads);
   const int pc = cache_part_cols(a.max_q, a.heads, a.cache.kv_heads);
   const int units = a.batch * a.cache.kv_heads;
-  const bool cols = cache_by_cols(a.max_q, a.heads, a.cache.kv_heads);
-  const int per = cols ? (tiles + kWaves - 1) / kWaves : tiles;
-  const dim3 grid((unsigned)(units * per * splits)), block(64 * kWaves);
-#define RH_ATTN(K, B) hipLaunchKernelGGL((K<DH, B>), grid, block, 0, s, a, tiles, splits, pc)
-  if (cols) {
-    if (a.in_bf16) RH_ATTN(cache_attention_cols_kernel, true);
-    else RH_ATTN(cache_attention_cols_kernel, false);
+  const dim3 grid((unsigned)(units * ((tiles + per_wg - 1) / per_wg) * splits)), block(64 * kWaves);
+#define RH_ATTN(B)                                                                             \
+  if (per_wg == 4)                                                                             \
+    hipLaunchKernelGGL((cache_attention_cols_kernel<DH, B, 4, 1, 3>), grid, block, 0, s, a,    \
+                       tiles, splits, pc);                                                     \
+  else if (per_wg == 2)                                                                        \
+    hipLaunchKernelGGL((cache_attention_cols_kernel<DH, B, 2, 2, DH == 64 ? 3 : 2>), grid,     \
+                       block, 0, s, a, tiles, splits, pc);                                     \
+  else                                                                                         \
+    hipLaunchKernelGGL((cache_attention_kernel<DH, B>), grid, block, 0, s, a, tiles, splits, pc)
+  if (a.in_bf16) {
+    RH_ATTN(true);
   } else {
-    if (a.in_bf16) RH_ATTN(cache_attention_kernel, true);
-    else RH_ATTN(cache_attention_kernel, false);
+    RH_ATTN(false);
   }
 #undef RH_ATTN
   if (splits > 1)

@@ -298,10 +298,7 @@ size_t rh_cache_attention_scratch(int batch, int max_q, int max_len, int heads, 
   if (batch <= 0 || max_q <= 0 || max_len < 0 || kv_heads < 1 || heads < kv_heads ||
       heads % kv_heads || dh < 1)
     return 0;
-  int splits;
-  size_t floats;
-  cache_attention_plan(batch, max_q, max_len, heads, kv_heads, dh, 0, &splits, &floats);
-  return floats * sizeof(float);
+  return cache_attention_floats(batch, max_q, max_len, heads, kv_heads, dh) * sizeof(float);
 }
 
 int rh_cache_attention(rh_context* ctx, const void* q, int q_bf16, int ldq, int q_off,

@@ -172,11 +172,10 @@ struct CacheAttnArgs {
   int causal, window;
   void* out;
   int out_bf16, ldout;
-  float* part;  // partial results of split key ranges (cache_attention_plan)
+  float* part;  // partial results of split key ranges (cache_attention_floats)
 };
-// Key ranges per tile of query columns and the floats of their partial results.
-void cache_attention_plan(int batch, int max_q, int max_len, int heads, int kv_heads, int dh,
-                          int window, int* splits, size_t* part_floats);
+// Floats that the partial results of split key ranges take.
+size_t cache_attention_floats(int batch, int max_q, int max_len, int heads, int kv_heads, int dh);
 hipError_t launch_cache_attention(const CacheAttnArgs& a, hipStream_t s);
 
 }  // namespace rh
