@@ -26,17 +26,18 @@ constexpr int kWaves = 4;    // per workgroup
 // by more than 2^4, so codes stay within 2^8 < 448.
 constexpr float kHead = 4.0f;
 
-// Visible keys [klo, khi] of a query at position i of n; none: klo = khi = 2^30.
+// Visible keys [klo, khi] of a query at position i of n; none: klo = khi = 2^31 - 1, behind
+// any. A window may be as long as an int, a query lie before every key.
 __device__ __forceinline__ void cache_key_range(const CacheAttnArgs& p, int i, int n, int& klo,
                                                 int& khi) {
   khi = n - 1;
   klo = 0;
   if (p.causal) khi = min(khi, i);
   if (p.window > 0) {
-    khi = min(khi, i + p.window - 1);
-    klo = max(klo, i - p.window + 1);
+    khi = (int)min((long long)khi, (long long)i + p.window - 1);
+    klo = (int)max((long long)klo, (long long)i - p.window + 1);
   }
-  if (khi < klo) klo = khi = 1 << 30;
+  if (khi < klo) klo = khi = 0x7FFFFFFF;
 }
 
 // The larger of a lane's value and that of lane ^ 32, in both.
@@ -418,7 +419,7 @@ __device__ __forceinline__ void cache_page_range(const CacheAttnArgs& p, int pos
   const int i0 = pos0 + c0 / G, i1 = pos0 + (c1 - 1) / G;
   if (p.causal) hi = min(hi, i1 < 0 ? 0 : i1 / kPageT + 1);
   if (p.window > 0) {
-    lo = max(0, i0 - p.window + 1) / kPageT;
+    lo = (int)(max(0LL, (long long)i0 - p.window + 1) / kPageT);
     const long long last = (long long)i1 + p.window - 1;
     if (last < n) hi = min(hi, last < 0 ? 0 : (int)(last / kPageT) + 1);
   }

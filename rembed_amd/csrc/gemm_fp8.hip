@@ -19,11 +19,13 @@ namespace rh {
 template <bool BF16, bool VEC>
 __global__ __launch_bounds__(256) void quantize_rows_fp8_kernel(const void* a, int lda, int m,
                                                                 int k, uint8_t* qa, int ldq,
-                                                                uint8_t* sa, int per_row) {
+                                                                uint8_t* sa, int per_row,
+                                                                int r0) {
   const int wave = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
-  const int r = wave / per_row;
-  if (r >= m) return;
-  const int c = (wave - r * per_row) * 512 + lane * 8;
+  const int row = wave / per_row;
+  if (row >= m - r0) return;
+  const int r = r0 + row;
+  const int c = (wave - row * per_row) * 512 + lane * 8;
   float v[8];
   const size_t at = (size_t)r * lda + c;
   if constexpr (VEC) {  // k % 8 == 0, rows 16-byte aligned
@@ -76,17 +78,22 @@ hipError_t launch_quantize_rows_fp8(const void* a, int a_bf16, int lda, int m, i
                                     int ldq, uint8_t* sa, hipStream_t s) {
   if (m <= 0) return hipSuccess;
   const int per_row = ceil_div(ldq, 512);
-  const dim3 grid((unsigned)(((long long)m * per_row + 3) / 4)), block(256);
   const bool vec = k % 8 == 0 && lda % 8 == 0 && ((uintptr_t)a & 15) == 0;
+  // a launch holds fewer than 2^32 threads
+  const int each = std::max(1, (1 << 25) / per_row);
+  for (int r0 = 0; r0 < m; r0 += std::min(each, m - r0)) {
+    const int rows = std::min(each, m - r0);
+    const dim3 grid((unsigned)(((long long)rows * per_row + 3) / 4)), block(256);
 #define RH_Q(B, V)                                                                              \
   hipLaunchKernelGGL((quantize_rows_fp8_kernel<B, V>), grid, block, 0, s, a, lda, m, k, qa, ldq, \
-                     sa, per_row)
-  if (a_bf16) {
-    if (vec) RH_Q(true, true);
-    else RH_Q(true, false);
-  } else {
-    if (vec) RH_Q(false, true);
-    else RH_Q(false, false);
+                     sa, per_row, r0)
+    if (a_bf16) {
+      if (vec) RH_Q(true, true);
+      else RH_Q(true, false);
+    } else {
+      if (vec) RH_Q(false, true);
+      else RH_Q(false, false);
+    }
   }
 #undef RH_Q
   return hipGetLastError();

@@ -303,9 +303,10 @@ def test_gated_linears_of_many_rows(gpu_ctx, m, k, i):
 
 
 def test_linear_of_rows_past_32_bits(gpu_ctx):
-    """2^24 + 300 rows of one value: codes of more than 2^31 bytes."""
+    """2^25 + 300 rows of one value: codes of more than 2^32 bytes, more rows than a launch
+    of the quantizer takes."""
     from rembed_amd import tensor as T
-    m, n = (1 << 24) + 300, 16
+    m, n = (1 << 25) + 300, 16
     x = np.random.default_rng(1).standard_normal((m, 1)).astype(np.float32)
     w = np.arange(1, 17, dtype=np.float32)[:, None]
     _, _, wv = O.quantize_weight(w.astype(np.float64))
@@ -313,14 +314,16 @@ def test_linear_of_rows_past_32_bits(gpu_ctx):
     d, dst = gpu_ctx.upload(x), gpu_ctx.alloc(m * n * 2)
     qa, sa = gpu_ctx.alloc(m * 128), gpu_ctx.alloc(T.fp8_scale_bytes(m, 1))
     T.LinearFP8(gpu_ctx, dst, True, n, d, False, 1, pb, m, 0, qa, 128, sa)
-    got = F.from_bf16(dst.download(np.uint16, (m, n)))
-    codes, e, xv = O.quantize_rows(x[-3000:].astype(np.float64))
+    bits = dst.download(np.uint16, (m, n))
+    at = np.concatenate([np.arange(0, m, 997), np.arange(1 << 24, (1 << 24) + 500),
+                         np.arange((1 << 25) - 500, m)])
+    _, _, xv = O.quantize_rows(x[at].astype(np.float64))
     want = xv @ wv.T
-    assert (np.abs(got[-3000:] - want) <= F.BF16 * 1.01 * np.abs(want) + 1e-30).all()
-    assert (np.abs(got - x * w.T) <= (2.0 ** -4 + 2.0 ** -7) * np.abs(x * w.T) + 1e-30).all()
+    assert (np.abs(F.from_bf16(bits[at]) - want) <= F.BF16 * 1.01 * np.abs(want) + 1e-30).all()
 
 
-WIDE = [  # heads, kv heads, dh, past, fresh, causal, window: four tiles per workgroup
+# heads, kv heads, dh, past, fresh, causal, window: four tiles per workgroup
+WIDE = [
     (32, 16, 64, [100], [1600], True, 0), (32, 16, 64, [100] * 5, [300, 7, 290, 0, 299], True, 200),
     (16, 8, 128, [0, 65, 300], [1050, 1060, 1], True, 0), (8, 4, 128, [500], [6300], True, 300),
     (8, 2, 256, [1800, 3], [300, 299], True, 0), (8, 2, 256, [1000] * 4, [600, 1, 65, 610], False, 100),
@@ -419,3 +422,24 @@ def cache_view(cache):
     """What attend takes in place of an oracle's cache."""
     cache.heads = cache.kv_heads
     return cache
+
+
+@pytest.mark.parametrize("nq,past", [(1, 300), (20, 300), (300, 70)])
+@pytest.mark.parametrize("causal", [True, False])
+def test_attention_of_the_longest_windows(gpu_ctx, nq, past, causal):
+    """A window of 2^31 - 1 is none, also for queries that lie before every key."""
+    rng = np.random.default_rng(nq)
+    pages, table, cu, blk, lens, slots = F.batch_of(rng, [past, 0], [nq, 40])
+    c = O.Cache(pages, 2, 64)
+    acu = np.concatenate([[0], np.cumsum(lens)]).astype(I32)
+    asl = np.concatenate([table[b, np.arange(n) // 64].astype(np.int64) * 64 + np.arange(n) % 64
+                          for b, n in enumerate(lens)])
+    k, v = rng.standard_normal((2, len(asl), 2, 64))
+    c.append(k, v, acu, asl)
+    qcu = np.array([0, nq, nq + 90], I32)  # 50 queries of the second before its keys
+    q = rng.standard_normal((nq + 90, 4, 64))
+    for window in (2 ** 31 - 1, 2 ** 31 - 60, 2 ** 30):
+        got, val = F.attend(gpu_ctx, c, q, "bf16", table, qcu, lens, 0.125, causal, window, True)
+        F.check_attention(c, got, val, table, qcu, lens, 0.125, causal, 0, "bf16", True)
+        if causal:
+            assert (got[nq:nq + 50] == 0).all()
