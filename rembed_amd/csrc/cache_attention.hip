@@ -474,8 +474,10 @@ constexpr int kPartRow = DH + 4;
 
 // ---- few columns -----------------------------------------------------------------------
 // Four waves share a tile of columns and take its pages in turn, straight to registers: what
-// bounds it is the cache's bytes, each read once. Page g + 4's K is on its way while page g
-// is multiplied. The waves' results are joined in LDS, eight columns at a time.
+// bounds it is the cache's bytes, each read once: 48 single tokens over 500 to 8191 (463 MB,
+// 16 heads over 8 of dh 128) take 94 µs, 4.9 TB/s, what a large copy reaches. Two workgroups
+// to a CU hide each other's waits; the next page's K asked for a page ahead did not gain and
+// cost registers. The waves' results are joined in LDS, eight columns at a time.
 template <int DH, bool BF16>
 __global__ __launch_bounds__(64 * kWaves, DH == 256 ? 1 : 2) void cache_attention_kernel(
     CacheAttnArgs p, int tiles, int splits, int part_cols) {
@@ -630,8 +632,11 @@ struct CachePipe : CacheFast<DH> {  // ph, pl, eh, el: P of the page before
     }
   }
   // P of page g, between the values of page g - 1 (v, xv) and the scores of g + 1 (k, xk).
+  // `fetch` asks for the next pages, a 1 KiB piece of kFetch at a time: all at once they hold
+  // the wave up while their addresses go out (32 queries of 9 to 70 rows: 24.8 µs, so 23.6).
+  template <int kFetch, typename Fetch>
   __device__ __forceinline__ void turn(const uint8_t* k, int xk, const uint8_t* v, int xv,
-                                       float cs) {
+                                       float cs, Fetch&& fetch) {
     const float m = Base::origin();
     v16f s[2] = {v16f{}, v16f{}};
     v8i nh, nl;
@@ -697,6 +702,8 @@ struct CachePipe : CacheFast<DH> {  // ph, pl, eh, el: P of the page before
         if (u == 2 && f + 2 < NF) b1 = piece(f + 3);
         const int at = 2 * f + u;  // of NM
 #pragma unroll
+        for (int j = at * kFetch / NM; j < (at + 1) * kFetch / NM; j++) fetch(j);
+#pragma unroll
         for (int j = at * kPairs / NM; j < (at + 1) * kPairs / NM; j++) pair(j);
       }
       a0 = b0;
@@ -756,9 +763,12 @@ __global__ __launch_bounds__(64 * CW * PG, DH == 256 ? 1 : 2) void cache_attenti
   // A page that is none is read as page 0 and holds no keys.
   PageWindow win;
   int base = first;  // the window's first page
-  auto dma = [&](const uint8_t* src, int page, uint8_t* dst) {
+  auto source = [&](const uint8_t* src, int page) {
     const size_t unit = (size_t)max(page, 0) * p.cache.kv_heads + h;
-    const uint8_t* at = src + unit * kHalf + part_of * kPieces * 1024 + lane * 16;
+    return src + unit * kHalf + part_of * kPieces * 1024 + lane * 16;
+  };
+  auto dma = [&](const uint8_t* src, int page, uint8_t* dst) {
+    const uint8_t* at = source(src, page);
 #pragma unroll
     for (int i = 0; i < kPieces; i++)
       lds_dma16(at + i * 1024, dst + (part_of * kPieces + i) * 1024);
@@ -783,8 +793,10 @@ __global__ __launch_bounds__(64 * CW * PG, DH == 256 ? 1 : 2) void cache_attenti
     win.load(p, b, h, first, limit, lane);
     dma(p.cache.k, win.at(win.page, 0), ldsk);
     dma(p.cache.k, win.at(win.page, 1), ldsk + kHalf);
-    dma(p.cache.v, win.at(win.page, 0), ldsv + kHalf);
-    if (SLOTS > 2) dma(p.cache.k, win.at(win.page, 2), ldsk + 2 * kHalf);
+    if (SLOTS > 2) {
+      dma(p.cache.v, win.at(win.page, 0), ldsv + kHalf);
+      dma(p.cache.k, win.at(win.page, 2), ldsk + 2 * kHalf);
+    }
   }
   cache_load_q<KS, BF16>(p.q, (size_t)(r0 + ct) * p.ldq + p.q_off + (h * G + c - ct * G) * DH, half,
                          w.qh, w.ql, w.xh, w.xl);
@@ -794,6 +806,8 @@ __global__ __launch_bounds__(64 * CW * PG, DH == 256 ? 1 : 2) void cache_attenti
   int ks = 1, vs = 0;
   bool nonep = false, none = false;  // page g - 1, g is none
   auto after = [](int slot) { return slot == SLOTS - 1 ? 0 : slot + 1; };
+  const uint8_t *vfrom = nullptr, *kfrom = nullptr;
+  uint8_t *vplace = nullptr, *kplace = nullptr;
   constexpr int kAhead = SLOTS;  // K of g + kAhead, V of g + kAhead - 2 are asked for in turn g
   auto stage = [&](int g) {
     if (SLOTS > 2) wait_vmcnt<2 * kPieces>();  // all but the last turn's
@@ -807,12 +821,17 @@ __global__ __launch_bounds__(64 * CW * PG, DH == 256 ? 1 : 2) void cache_attenti
     }
     none = win.at(win.page, g - base) < 0;
     // Three slots: V of g + 1 and K of g + 3 go where V of g - 2 and K of g were.
-    // Two: V of g (the first is there) and K of g + 2.
+    // Two: V of g and K of g + 2.
     const int vto = SLOTS > 2 ? after(after(vs)) : after(vs);
     const int kto = SLOTS > 2 ? after(after(ks)) : after(ks);
-    if (SLOTS > 2 || g > first)
-      dma(p.cache.v, win.at(win.page, g + kAhead - 2 - base), ldsv + vto * kHalf);
-    dma(p.cache.k, win.at(win.page, g + kAhead - base), ldsk + kto * kHalf);
+    vfrom = source(p.cache.v, win.at(win.page, g + kAhead - 2 - base));
+    kfrom = source(p.cache.k, win.at(win.page, g + kAhead - base));
+    vplace = ldsv + vto * kHalf + part_of * kPieces * 1024;
+    kplace = ldsk + kto * kHalf + part_of * kPieces * 1024;
+  };
+  auto fetch = [&](int i) {
+    if (i < kPieces) lds_dma16(vfrom + i * 1024, vplace + i * 1024);
+    else lds_dma16(kfrom + (i - kPieces) * 1024, kplace + (i - kPieces) * 1024);
   };
   auto done = [&] {
     nonep = none;
@@ -833,6 +852,8 @@ __global__ __launch_bounds__(64 * CW * PG, DH == 256 ? 1 : 2) void cache_attenti
     if (!active) {  // a wave without columns stages its pieces
       for (int g = first; g < end; g++) {
         stage(g);
+#pragma unroll
+        for (int i = 0; i < 2 * kPieces; i++) fetch(i);
         done();
       }
       last();
@@ -844,7 +865,7 @@ __global__ __launch_bounds__(64 * CW * PG, DH == 256 ? 1 : 2) void cache_attenti
         const uint8_t* kn = ldsk + ks * kHalf + lane * 16;
         const uint8_t* vp = ldsv + vs * kHalf + lane * 16;
         w.refer(g * kPageT, none, cs, half);
-        w.turn(kn, win.at(win.xk, g + 1 - base), vp, xvp, cs);
+        w.template turn<2 * kPieces>(kn, win.at(win.xk, g + 1 - base), vp, xvp, cs, fetch);
         xvp = win.at(win.xv, g - base);
         done();
       }
