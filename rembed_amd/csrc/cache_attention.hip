@@ -705,6 +705,8 @@ struct CachePipe : CacheFast<DH> {  // ph, pl, eh, el: P of the page before
         for (int j = at * kFetch / NM; j < (at + 1) * kFetch / NM; j++) fetch(j);
 #pragma unroll
         for (int j = at * kPairs / NM; j < (at + 1) * kPairs / NM; j++) pair(j);
+        // one wave per SIMD: every two products keep the scores' work written beside them
+        if (DH == 256 && u % 2 == 1) __builtin_amdgcn_sched_barrier(0);
       }
       a0 = b0;
       a1 = b1;
@@ -865,7 +867,10 @@ __global__ __launch_bounds__(64 * CW * PG, DH == 256 ? 1 : 2) void cache_attenti
         const uint8_t* kn = ldsk + ks * kHalf + lane * 16;
         const uint8_t* vp = ldsv + vs * kHalf + lane * 16;
         w.refer(g * kPageT, none, cs, half);
+        // of a SIMD's two waves the one that has products to feed goes first (3%)
+        if (DH < 256) __builtin_amdgcn_s_setprio(2);
         w.template turn<2 * kPieces>(kn, win.at(win.xk, g + 1 - base), vp, xvp, cs, fetch);
+        if (DH < 256) __builtin_amdgcn_s_setprio(0);
         xvp = win.at(win.xv, g - base);
         done();
       }
