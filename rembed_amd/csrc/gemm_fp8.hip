@@ -122,65 +122,87 @@ __device__ __forceinline__ void fp8_store4(const GemmFp8Args& p, int row, int co
 }
 
 // ---- GEMM ---------------------------------------------------------------------------
-// Epilogue: per 32-row band a wave parks its accumulators in LDS and reads rows
-// back 4 (gated: 8) columns a lane, so outputs leave as vectors of 4.
-template <int BM, int WM, int WN, int TM, int TN>
-__device__ __forceinline__ void fp8_epilogue(const GemmFp8Args& p, v16f (&acc)[TM][TN],
-                                             uint8_t* lds, int row0, int col0, int wave, int wm,
-                                             int wn, int lane) {
-  constexpr int kStride = WN + 4;
+// The weights are the products' rows and the activations their columns, so a lane holds four
+// consecutive outputs of one row at a time (gated: gates in lanes 0..31, their ups in
+// 32..63, which one exchange of halves brings together). Per 32 rows a wave finishes them in
+// registers, parks them in LDS as they will be stored and writes whole rows, 16 bytes a lane.
+template <int WM, int WN, int TM, int TN, bool GLU, bool BF16>
+__device__ __forceinline__ void fp8_rows_out(const GemmFp8Args& p, v16f (&acc)[TM][TN],
+                                             uint8_t* own, int row0, int col0, int lane) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  constexpr int kCols = GLU ? WN / 2 : WN, kEach = BF16 ? 2 : 4;
+  constexpr int kRow = kCols * kEach + 16;  // bytes; 16 rows apart by 4 mod 64 banks
+  typedef __bf16 v4bf __attribute__((ext_vector_type(4)));
   const int fr = lane & 31, fg = lane >> 5;
-  float* ep = reinterpret_cast<float*>(lds) + wave * 32 * kStride;
-  const bool glu = is_glu(p.act);
 #pragma unroll
   for (int i = 0; i < TM; i++) {
+    uint8_t* mine = own + fr * kRow;
+    auto park = [&](int at, const v4f& v) {
+      if constexpr (BF16)
+        *reinterpret_cast<v4bf*>(mine + at * 2) =
+            (v4bf){(__bf16)v[0], (__bf16)v[1], (__bf16)v[2], (__bf16)v[3]};
+      else
+        *reinterpret_cast<v4f*>(mine + at * 4) = v;
+    };
 #pragma unroll
     for (int j = 0; j < TN; j++)
 #pragma unroll
-      for (int r = 0; r < 16; r++)
-        ep[((r >> 2) * 8 + fg * 4 + (r & 3)) * kStride + j * 32 + fr] = acc[i][j][r];
+      for (int q = 0; q < 4; q += GLU ? 2 : 1) {
+        v4f v;
+        if constexpr (GLU) {
+          typedef unsigned v2u __attribute__((ext_vector_type(2)));
+#pragma unroll
+          for (int e = 0; e < 4; e++) {
+            const v2u x = __builtin_bit_cast(
+                v2u, __builtin_amdgcn_permlane32_swap(__float_as_uint(acc[i][j][q * 4 + e]),
+                                                      __float_as_uint(acc[i][j][q * 4 + 4 + e]),
+                                                      false, false));
+            v[e] = fp8_glu(__uint_as_float(x[0]), __uint_as_float(x[1]), p.act);
+          }
+          park(j * 16 + q * 4 + fg * 4, v);
+        } else {
+          const int col = j * 32 + q * 8 + fg * 4;
+          v4f bs = {0.0f, 0.0f, 0.0f, 0.0f};
+          if (p.bias && col0 + col < p.N) bs = *reinterpret_cast<const v4f*>(p.bias + col0 + col);
+#pragma unroll
+          for (int e = 0; e < 4; e++) v[e] = acc[i][j][q * 4 + e] + bs[e];
+          if (p.act == ACT_GELU) {
+#pragma unroll
+            for (int e = 0; e < 4; e++) v[e] = gelu_avx2(v[e]);
+          }
+          park(col, v);
+        }
+      }
     wait_lgkmcnt0();
     __builtin_amdgcn_wave_barrier();
-    const int rows = row0 + wm * WM + i * 32;
-    if (glu) {  // columns 8t..8t+3 gate, 8t+4..8t+7 up
-      constexpr int kL = WN / 8, kR = 64 / kL;
-      const int c8 = lane % kL * 8, col = col0 + wn * WN + c8;
-      v4f g[32 / kR], u[32 / kR];
+    constexpr int kL = kCols * kEach / 16, kR = 64 / kL;  // lanes of a row, rows at once
+    const int l = lane % kL, to = (GLU ? col0 / 2 : col0) + l * (16 / kEach);
 #pragma unroll
-      for (int k = 0; k < 32 / kR; k++) {
-        const float* at = ep + (lane / kL + k * kR) * kStride + c8;
-        g[k] = *reinterpret_cast<const v4f*>(at);
-        u[k] = *reinterpret_cast<const v4f*>(at + 4);
-      }
-#pragma unroll
-      for (int k = 0; k < 32 / kR; k++) {
-        const int row = rows + lane / kL + k * kR;
-#pragma unroll
-        for (int e = 0; e < 4; e++) g[k][e] = fp8_glu(g[k][e], u[k][e], p.act);
-        if (row < p.M && col < p.N) fp8_store4(p, row, col / 2, g[k]);
-      }
-    } else {
-      constexpr int kL = WN / 4, kR = 64 / kL;
-      const int c4 = lane % kL * 4, col = col0 + wn * WN + c4;
-      v4f bs = {0.0f, 0.0f, 0.0f, 0.0f};
-      if (p.bias && col < p.N) bs = *reinterpret_cast<const v4f*>(p.bias + col);
-      v4f v[32 / kR];
-#pragma unroll
-      for (int k = 0; k < 32 / kR; k++)
-        v[k] = *reinterpret_cast<const v4f*>(ep + (lane / kL + k * kR) * kStride + c4);
-#pragma unroll
-      for (int k = 0; k < 32 / kR; k++) {
-        const int row = rows + lane / kL + k * kR;
-#pragma unroll
-        for (int e = 0; e < 4; e++) v[k][e] += bs[e];
-        if (p.act == ACT_GELU) {
-#pragma unroll
-          for (int e = 0; e < 4; e++) v[k][e] = gelu_avx2(v[k][e]);
-        }
-        if (row < p.M && col < p.N) fp8_store4(p, row, col, v[k]);
-      }
+    for (int k = 0; k < 32; k += kR) {
+      const int r = k + lane / kL, row = row0 + i * 32 + r;
+      const v4i x = *reinterpret_cast<const v4i*>(own + r * kRow + l * 16);
+      typedef v4i Out __attribute__((aligned(8)));
+      if (row < p.M && to < (GLU ? p.N / 2 : p.N))
+        *reinterpret_cast<Out*>(static_cast<uint8_t*>(p.out) +
+                                ((size_t)row * p.ldo + to) * kEach) = x;
     }
     __builtin_amdgcn_wave_barrier();
+  }
+#endif
+}
+
+template <int WM, int WN, int TM, int TN>
+__device__ __forceinline__ void fp8_epilogue(const GemmFp8Args& p, v16f (&acc)[TM][TN],
+                                             uint8_t* lds, int row0, int col0, int wave, int wm,
+                                             int wn, int lane) {
+  uint8_t* own = lds + wave * 32 * (WN + 4) * 4;
+  const int r = row0 + wm * WM, c = col0 + wn * WN;
+  if (is_glu(p.act)) {
+    if (p.out_bf16) fp8_rows_out<WM, WN, TM, TN, true, true>(p, acc, own, r, c, lane);
+    else fp8_rows_out<WM, WN, TM, TN, true, false>(p, acc, own, r, c, lane);
+  } else {
+    if (p.out_bf16) fp8_rows_out<WM, WN, TM, TN, false, true>(p, acc, own, r, c, lane);
+    else fp8_rows_out<WM, WN, TM, TN, false, false>(p, acc, own, r, c, lane);
   }
 }
 
@@ -189,7 +211,7 @@ __device__ __forceinline__ void fp8_epilogue(const GemmFp8Args& p, v16f (&acc)[T
 template <int I, int TN, int J = 0>
 __device__ __forceinline__ void fp8_cols(v16f (&acc)[TN], const v8i& a, const v8i (&b)[TN], int ea,
                                          int eb) {
-  acc[J] = mfma_fp8_32<I, J>(a, b[J], acc[J], ea, eb);
+  acc[J] = mfma_fp8_32<J, I>(b[J], a, acc[J], eb, ea);
   if constexpr (J + 1 < TN) fp8_cols<I, TN, J + 1>(acc, a, b, ea, eb);
 }
 template <int TM, int TN>
@@ -349,7 +371,7 @@ __global__ __launch_bounds__(128 * WGN) void gemm_fp8_kernel(GemmFp8Args p) {
   }
   wait_vmcnt<0>();
   __syncthreads();
-  fp8_epilogue<BM, WM, WN, TM, TN>(p, acc, lds, row0, col0, wave, wm, wn, lane);
+  fp8_epilogue<WM, WN, TM, TN>(p, acc, lds, row0, col0, wave, wm, wn, lane);
 }
 
 // ---- few rows -------------------------------------------------------------------------
