@@ -443,3 +443,53 @@ def test_attention_of_the_longest_windows(gpu_ctx, nq, past, causal):
         F.check_attention(c, got, val, table, qcu, lens, 0.125, causal, 0, "bf16", True)
         if causal:
             assert (got[nq:nq + 50] == 0).all()
+
+
+class Part:
+    """Elements of a device buffer from `first` on."""
+
+    def __init__(self, ctx, ptr, size):
+        self.ctx, self.ptr, self.size = ctx, ptr, size
+
+    def read(self, first, dtype, n):
+        from rembed_amd import _lib
+        out = np.empty(n, dtype)
+        _lib.check(_lib.lib.rh_memcpy_d2h(self.ctx.h, out.ctypes.data,
+                                          self.ptr + first * out.itemsize, out.nbytes))
+        return out
+
+
+@pytest.mark.parametrize("fits", [True, False])
+def test_plan_of_the_most_rows(gpu_ctx, fits):
+    """2^31 - 1 rows, whose last loops pass 2^31; one text of most of them, or too long for its
+    table."""
+    from rembed_amd import tensor as T
+    ctx, rows = gpu_ctx, 2 ** 31 - 1
+    n = [70, 2 ** 31 - 300, 100]
+    blocks = -(-n[1] // 64)
+    need = 2 + blocks + 2
+    free = np.arange(5, need + 5, dtype=I32)
+    ldt = blocks if fits else blocks - 1
+    table = ctx.alloc(3 * ldt * 4)
+    slots, pos = ctx.alloc(rows * 8), ctx.alloc(rows * 4)
+    cu, blk, lens, status = (ctx.alloc(x) for x in (16, 16, 12, 16))
+    T.CachePlan(ctx, ctx.upload(np.zeros(3, I32)), ctx.upload(np.array(n, I32)), 3, ctx.upload(free),
+                need, table, ldt, cu, blk, lens, slots, pos, rows, status)
+    ctx.sync()
+    S, P = Part(ctx, slots.ptr, rows), Part(ctx, pos.ptr, rows)
+    got = status.download(I32, (4,)).tolist()
+    if not fits:
+        assert got == [2, 0, 0, 0]
+        for at in (0, 2 ** 30, rows - 5000):
+            assert (S.read(at, np.int64, 5000) == -1).all() and (P.read(at, I32, 5000) == 0).all()
+        return
+    total = sum(n)
+    assert got == [0, total, need, need] and cu.download(I32, (4,)).tolist() == [0, 70, n[1] + 70, total]
+    for at in (70, 2 ** 30 + 1, total - 100 - 5000):
+        i = np.arange(at - 70, at - 70 + 5000, dtype=np.int64)
+        assert np.array_equal(P.read(at, I32, 5000), i)
+        assert np.array_equal(S.read(at, np.int64, 5000), (2 + i // 64 + 5) * 64 + i % 64)
+    i = np.arange(100)
+    assert np.array_equal(S.read(total - 100, np.int64, 100), (2 + blocks + i // 64 + 5) * 64 + i % 64)
+    tail = rows - total
+    assert (S.read(total, np.int64, tail) == -1).all() and (P.read(total, I32, tail) == 0).all()
