@@ -387,6 +387,11 @@ struct PageWindow {
   }
 };
 
+// Many columns, up to so many workgroups of a unit (one request and kv head): the grid is
+// units x workgroups x key ranges, so that those that short requests leave empty come last and
+// not between the others (32 queries of 9 to 70 rows: 22.9 µs, so 22.3).
+constexpr int kFewTiles = 4;
+
 // Workgroup -> (request, kv head, tile of columns, key range). A unit's workgroups (one
 // request and kv head) read the same pages: where eight units are left their workgroups are
 // dealt to an XCD each (workgroup w runs on XCD w % 8) and share its L2, the last ones are
@@ -732,8 +737,15 @@ __global__ __launch_bounds__(64 * CW * PG, DH == 256 ? 1 : 2) void cache_attenti
   __shared__ __attribute__((aligned(1024))) uint8_t lds[kLds];
   const int wgs = (tiles + CW - 1) / CW;
   int b, h, wg, split;
-  cache_unit(p, wgs, splits, b, h, wg, split);
-  if (p.causal) {
+  if (wgs <= kFewTiles) {
+    b = blockIdx.x / p.cache.kv_heads;
+    h = blockIdx.x % p.cache.kv_heads;
+    wg = blockIdx.y;
+    split = blockIdx.z;
+  } else {
+    cache_unit(p, wgs, splits, b, h, wg, split);
+  }
+  if (p.causal && wgs > kFewTiles) {
     // later columns see more pages: each XCD's 32 CUs get the long ones first, then
     // the next 32 in the other order, so that long and short ones share a CU
     const int k = wg / 32, size = min(32, wgs - 32 * k);
@@ -1089,7 +1101,11 @@ static hipError_t launch_dh(const CacheAttnArgs& a, hipStream_t s) {
   const int tiles = cache_tiles(a.max_q, a.heads, a.cache.kv_heads);
   const int pc = cache_part_cols(a.max_q, a.heads, a.cache.kv_heads);
   const int units = a.batch * a.cache.kv_heads;
-  const dim3 grid((unsigned)(units * ((tiles + per_wg - 1) / per_wg) * splits)), block(64 * kWaves);
+  const int wgs = (tiles + per_wg - 1) / per_wg;  // of a unit and key range
+  const bool few = per_wg > 1 && wgs <= kFewTiles;
+  const dim3 grid = few ? dim3((unsigned)units, (unsigned)wgs, (unsigned)splits)
+                        : dim3((unsigned)(units * wgs * splits));
+  const dim3 block(64 * kWaves);
 #define RH_ATTN(B)                                                                             \
   if (per_wg == 4)                                                                             \
     hipLaunchKernelGGL((cache_attention_cols_kernel<DH, B, 4, 1, 3>), grid, block, 0, s, a,    \
