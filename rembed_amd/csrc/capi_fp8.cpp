@@ -131,7 +131,7 @@ int run_linear_fp8(Context* ctx, const rh_weight* w, const void* a, int a_bf16, 
                    int ldq, uint8_t* sa) {
   if (m <= 0) return RH_OK;
   const double M = m, K = w->k, N = w->n;
-  const bool direct = a && gemm_fp8_takes_rows(m, w->n, w->k);
+  const bool direct = a && gemm_fp8_takes_rows(m, w->n, w->k, a, a_bf16, lda);
   if (a && !direct)
     RH_HIP(launch_quantize_rows_fp8(a, a_bf16, lda, m, w->k, qa, ldq, sa, ctx->stream));
   GemmFp8Args g{};

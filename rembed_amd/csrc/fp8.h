@@ -132,7 +132,7 @@ struct GemmFp8Args {
 };
 // src: fp32 or bf16 rows to make e4m3 on the way (A and sa unused), where
 // gemm_fp8_takes_rows; null: A and sa.
-bool gemm_fp8_takes_rows(int M, int N, int K);
+bool gemm_fp8_takes_rows(int M, int N, int K, const void* a, int a_bf16, int lda);
 hipError_t launch_gemm_fp8(const GemmFp8Args& a, const void* src, int src_bf16, int ld_src,
                            hipStream_t s);
 

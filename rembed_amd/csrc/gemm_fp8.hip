@@ -508,13 +508,18 @@ static int rows_tiles(int M, int N) {
   return 0;
 }
 
-// fp32 / bf16 rows go straight into it where its workgroups' work on them is less than a
-// launch: µs against quantizing first, K 1024, N 4096: M 1 4.2 / 6.9, M 16 5.1 / 6.9; K 2560,
-// N 2560: M 4 5.9 / 6.9, M 8 6.8 / 6.9; K 4096, N 1024: M 1 6.6 / 6.8, M 4 7.6 / 7.3; K 4096,
-// N 4096: M 1 7.6 / 6.9.
-bool gemm_fp8_takes_rows(int M, int N, int K) {
-  return M <= 16 && rows_tiles(M, N) == 1 && (long long)M * K <= 16384 &&
-         (long long)N * K <= (8 << 20);
+// fp32 / bf16 rows go straight into it where its workgroups' work on them, up to 16 rows of K
+// each, is less than a launch. µs against quantizing first, rows in 16-byte pieces: bf16, N 1024:
+// M 16 K 1024 4.5 / 7.1, M 64 K 2560 6.6 / 7.6, M 16 K 4096 8.3 / 8.7; fp32, N 1024: M 64 K 1024
+// 5.3 / 7.2, M 5 K 3584 7.2 / 7.2, M 16 K 2560 8.4 / 7.3; M 1 K 4096 6.9 / 6.9, K 8192 10.8 / 9.4;
+// two workgroups to a CU, N 8192 K 1024 M 16: bf16 5.9 / 6.9, fp32 7.7 / 6.8. Rows read value by
+// value: M 16 K 301 5.7 / 6.8, K 516 5.8 / 7.1, K 1001 8.2 / 7.1, K 3500 22 / 8.7.
+bool gemm_fp8_takes_rows(int M, int N, int K, const void* a, int a_bf16, int lda) {
+  if (rows_tiles(M, N) != 1) return false;
+  const bool two = (long long)(N / 16) * ceil_div(M, 16) > 256;
+  if (lda % 8 || ((uintptr_t)a & 15)) return !two && K <= 512;
+  const long long bytes = (long long)std::min(M, 16) * K * (a_bf16 ? 2 : 4);
+  return K <= 3584 && bytes * (two ? 2 : 1) <= 80 * 1024;
 }
 
 // A tile's time by rounds of the chip's 256 CUs: µs per started round at K 4096 (about a

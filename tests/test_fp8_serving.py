@@ -268,6 +268,39 @@ def test_two_contexts_at_once():
                     assert np.array_equal(x[name].view(np.uint32), y[name].view(np.uint32)), name
 
 
+@pytest.mark.parametrize("m,k,n,dtype", [
+    (1, 512, 272, "f32"), (16, 1280, 144, "f32"), (17, 640, 272, "bf16"), (40, 2560, 400, "bf16"),
+    (130, 1024, 144, "f32"), (250, 250, 256, "bf16"), (64, 301, 144, "f32"), (5, 3584, 144, "f32"),
+    (16, 1000, 8192, "bf16")])
+def test_linear_of_rows_made_on_the_way(gpu_ctx, m, k, n, dtype):
+    """Few rows are made e4m3 inside the product: the bits of quantizing them first, whatever
+    the stride and alignment by which they are read."""
+    from rembed_amd import tensor as T
+    rng = np.random.default_rng(m + k)
+    x = rng.standard_normal((m, k)) * np.exp(rng.uniform(-9, 9, (m, 1)))
+    x[0, : k // 2] = 0.0
+    img, val = F.typed(x, dtype)
+    b = rng.standard_normal(n).astype(np.float32)
+    w = (rng.standard_normal((n, k)) / k ** 0.5).astype(np.float32)
+    pb = T.PackFP8(gpu_ctx, w, k, n, b)
+    ldq, bf = T.ldq_fp8(k), dtype == "bf16"
+    qa, sa = gpu_ctx.alloc(m * ldq), gpu_ctx.alloc(T.fp8_scale_bytes(m, k))
+    dst = gpu_ctx.alloc(m * n * 4)
+    T.QuantizeRowsFP8(gpu_ctx, gpu_ctx.upload(img), bf, k, m, k, qa, ldq, sa)
+    T.MatMulFP8(gpu_ctx, dst, False, n, qa, ldq, sa, pb, m, 1)
+    want = dst.download(np.float32, (m, n))
+    close_linear(want, val, O.quantize_weight(w.astype(np.float64))[2], b, 1, False)
+    for lda, front in ((k, 0), (k + 3, 0), ((k + 15) // 8 * 8, 0), ((k + 15) // 8 * 8, 1)):
+        rows = np.full((m, lda), 0x7FC0 if bf else np.nan, img.dtype)  # NaN beside the rows
+        rows[:, :k] = img
+        d = gpu_ctx.upload(np.concatenate([np.zeros(front, img.dtype), rows.ravel(),
+                                           np.zeros(8, img.dtype)]))
+        at = Part(gpu_ctx, d.ptr + front * img.itemsize, 0)
+        T.LinearFP8(gpu_ctx, dst, False, n, at, bf, lda, pb, m, 1, qa, ldq, sa)
+        assert np.array_equal(dst.download(np.float32, (m, n)).view(np.uint32),
+                              want.view(np.uint32)), (lda, front)
+
+
 # sizes by which tiles of 64 x 64, 128 x 128, 128 x 256 and 256 x 256 are chosen
 @pytest.mark.parametrize("m,k,n", [(1100, 200, 1008), (1500, 384, 2000), (2050, 256, 3008),
                                    (4097, 320, 2064), (4000, 136, 4000)])
