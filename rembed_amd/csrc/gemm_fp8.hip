@@ -9,6 +9,7 @@
 #include "fp8.h"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace rh {
 
@@ -375,15 +376,90 @@ __global__ __launch_bounds__(128 * WGN) void gemm_fp8_kernel(GemmFp8Args p) {
 }
 
 // ---- few rows -------------------------------------------------------------------------
+template <bool BF16>
+struct Fp8RowBlock {
+  using S = std::conditional_t<BF16, __bf16, float>;
+  using T = std::conditional_t<BF16, v8bf, v4f>;
+  static constexpr int E = BF16 ? 8 : 4;
+  T v[32 / E];  // 32 values of a row's block, the others 16, 32 and 48 lanes further
+
+  __device__ __forceinline__ void load(const void* src, size_t row, int c, int K, bool vec) {
+    const S* at = static_cast<const S*>(src) + row + c;
+    if (vec && c + 32 <= K) {
+#pragma unroll
+      for (int i = 0; i < 32 / E; i++) v[i] = *reinterpret_cast<const T*>(at + i * E);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 32; e++) v[e / E][e % E] = c + e < K ? at[e] : (S)0.0f;
+    }
+  }
+  // Its codes; ex: the block's byte. Conversions that scale by themselves, 2.5 instructions a
+  // value of bf16 for 6.5; blocks with infinities or NaN, and below 2^-103, go the quantizer's
+  // way.
+  __device__ __forceinline__ v8i codes(int& ex) const {
+    v8i x = {};
+#if defined(__HIP_DEVICE_COMPILE__)
+    auto value = [&](int e) { return (float)v[e / E][e % E]; };
+    auto block = [](uint32_t top) {
+      top = max(top, (uint32_t)__shfl_xor((int)top, 16, 64));
+      return max(top, (uint32_t)__shfl_xor((int)top, 32, 64));
+    };
+    uint32_t top = 0;
+    if constexpr (BF16) {
+      typedef uint16_t v2u16 __attribute__((ext_vector_type(2)));
+      v2u16 m = {0, 0};
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        const v4i w = __builtin_bit_cast(v4i, v[i]);
+#pragma unroll
+        for (int e = 0; e < 4; e++)
+          m = __builtin_elementwise_max(m, __builtin_bit_cast(v2u16, w[e] & 0x7FFF7FFF));
+      }
+      top = (uint32_t)max(m[0], m[1]) << 16;
+    } else {
+#pragma unroll
+      for (int e = 0; e < 32; e++) top = max(top, __float_as_uint(value(e)) & 0x7FFFFFFFu);
+    }
+    top = block(top);
+    ex = fp8_exponent(top);
+    if (__builtin_expect(__any(top >= 0x7F800000u || ex < 16), 0)) {
+      top = 0;
+#pragma unroll
+      for (int e = 0; e < 32; e++) top = max(top, finite_abs_bits(value(e)));
+      ex = fp8_exponent(block(top));
+      const float f = fp8_inverse(ex);
+#pragma unroll
+      for (int e = 0; e < 8; e++)
+        x[e] = fp8_pack4(value(4 * e) * f, value(4 * e + 1) * f, value(4 * e + 2) * f,
+                         value(4 * e + 3) * f);
+      return x;
+    }
+    const float unit = __uint_as_float((uint32_t)ex << 23);
+#pragma unroll
+    for (int e = 0; e < 8; e++) {
+      typedef short v2s __attribute__((ext_vector_type(2)));
+      v2s h;
+      asm("" : "=v"(h) : "v"(unit));  // any word: both halves get written
+      h = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(h, value(4 * e), value(4 * e + 1), unit, false);
+      h = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(h, value(4 * e + 2), value(4 * e + 3), unit,
+                                                   true);
+      x[e] = __builtin_bit_cast(int, h);
+    }
+#endif
+    return x;
+  }
+};
+
 // A query's rows: the weights' bytes are all there is to move, so 16 of their rows go to
 // a workgroup (4096 outputs: 256 workgroups), whose NW waves hold different 128-blocks
 // of K and read them straight to registers as the A operand of 16x16x128 products (32
 // consecutive bytes a lane, four lanes a row's block). The activations are the columns, 16 MT of
 // them. The waves' sums are joined in LDS in wave order, and a thread finishes four
 // consecutive outputs of a row.
-// SRC 0: rows are e4m3 already; 1 / 2: fp32 / bf16 rows are made so here, by the same
-// arithmetic as quantize_rows_fp8_kernel (a launch less, but every workgroup does it:
-// gemm_fp8_takes_rows).
+// SRC 0: rows are e4m3 already; 1 / 2: fp32 / bf16 rows are made so here, to the same codes as
+// quantize_rows_fp8_kernel's (a launch less, but every workgroup does it: gemm_fp8_takes_rows).
+// 37 rows of bf16 by 2560 x 1024 take 6.2 µs, 2.2 over a launch; the next block's rows asked for a
+// block ahead did not gain (6.5).
 template <int MT, int NW, int SRC>
 __global__ __launch_bounds__(64 * NW) void gemm_fp8_rows_kernel(GemmFp8Args p, const void* src,
                                                                 int lds_src) {
@@ -402,60 +478,33 @@ __global__ __launch_bounds__(64 * NW) void gemm_fp8_rows_kernel(GemmFp8Args p, c
   v4f acc[MT];
 #pragma unroll
   for (int t = 0; t < MT; t++) acc[t] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+  if constexpr (SRC == 0) {
 #pragma unroll 4
-  for (int kb = wave; kb < nk; kb += NW) {
-    const v4i* at = reinterpret_cast<const v4i*>(wrow + (size_t)kb * kFp8Block);
-    const v8i w = join8(at[0], at[1]);
-    const int ew = wexp[(size_t)kb * gb * 128];
+    for (int kb = wave; kb < nk; kb += NW) {
+      const v4i* at = reinterpret_cast<const v4i*>(wrow + (size_t)kb * kFp8Block);
+      const v8i w = join8(at[0], at[1]);
+      const int ew = wexp[(size_t)kb * gb * 128];
 #pragma unroll
-    for (int t = 0; t < MT; t++) {
-      v8i x;
-      int ex;
-      if constexpr (SRC == 0) {
+      for (int t = 0; t < MT; t++) {
         const v4i* xt = reinterpret_cast<const v4i*>(p.A + (size_t)mrow[t] * p.lda +
                                                      (size_t)kb * kFp8Block + g * 32);
-        x = join8(xt[0], xt[1]);
-        ex = p.sa[fp8_scale_at(mrow[t], kb, ga)];
-      } else {
-        float v[32];
-        const int c = kb * kFp8Block + g * 32;
-        const size_t row = (size_t)mrow[t] * lds_src;
-        const bool whole = c + 32 <= p.K && lds_src % 8 == 0 && ((uintptr_t)src & 15) == 0;
-        uint32_t top = 0;
-        if (whole) {
-#pragma unroll
-          for (int e = 0; e < 32; e += 8) {
-            if constexpr (SRC == 2) {
-              const v8bf y = *reinterpret_cast<const v8bf*>(static_cast<const __bf16*>(src) + row + c + e);
-#pragma unroll
-              for (int i = 0; i < 8; i++) v[e + i] = (float)y[i];
-            } else {
-              const v4f y0 = *reinterpret_cast<const v4f*>(static_cast<const float*>(src) + row + c + e);
-              const v4f y1 = *reinterpret_cast<const v4f*>(static_cast<const float*>(src) + row + c + e + 4);
-#pragma unroll
-              for (int i = 0; i < 8; i++) v[e + i] = i < 4 ? y0[i] : y1[i - 4];
-            }
-          }
-        } else {
-#pragma unroll
-          for (int e = 0; e < 32; e++) {
-            v[e] = 0.0f;
-            if (c + e < p.K)
-              v[e] = SRC == 2 ? (float)static_cast<const __bf16*>(src)[row + c + e]
-                              : static_cast<const float*>(src)[row + c + e];
-          }
-        }
-#pragma unroll
-        for (int e = 0; e < 32; e++) top = max(top, finite_abs_bits(v[e]));
-        top = max(top, (uint32_t)__shfl_xor((int)top, 16, 64));
-        top = max(top, (uint32_t)__shfl_xor((int)top, 32, 64));
-        ex = fp8_exponent(top);
-        const float f = fp8_inverse(ex);
-#pragma unroll
-        for (int e = 0; e < 8; e++)
-          x[e] = fp8_pack4(v[4 * e] * f, v[4 * e + 1] * f, v[4 * e + 2] * f, v[4 * e + 3] * f);
+        const int ex = p.sa[fp8_scale_at(mrow[t], kb, ga)];
+        acc[t] = mfma_fp8_16(w, join8(xt[0], xt[1]), acc[t], ew, ex);
       }
-      acc[t] = mfma_fp8_16(w, x, acc[t], ew, ex);
+    }
+  } else {
+    static_assert(MT == 1, "one column tile");
+    const bool vec = lds_src % 8 == 0 && ((uintptr_t)src & 15) == 0;
+#pragma unroll 4
+    for (int kb = wave; kb < nk; kb += NW) {
+      const v4i* at = reinterpret_cast<const v4i*>(wrow + (size_t)kb * kFp8Block);
+      const v8i w = join8(at[0], at[1]);
+      const int ew = wexp[(size_t)kb * gb * 128];
+      Fp8RowBlock<SRC == 2> rows;
+      rows.load(src, (size_t)mrow[0] * lds_src, kb * kFp8Block + g * 32, p.K, vec);
+      int ex;
+      const v8i x = rows.codes(ex);
+      acc[0] = mfma_fp8_16(w, x, acc[0], ew, ex);
     }
   }
 #pragma unroll
