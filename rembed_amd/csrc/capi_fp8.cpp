@@ -6,7 +6,7 @@
 // (rh_linear's workspace apart) or waits, so they can be captured into a HIP graph.
 #include <algorithm>
 #include <cmath>
-#include <cstring>
+#include <cstdio>
 #include <memory>
 #include <vector>
 
@@ -14,73 +14,55 @@
 
 namespace rh {
 
-// The e4m3 code nearest to |x| <= 448, ties to even.
-static uint8_t e4m3_rne(float x) {
-  uint32_t u;
-  memcpy(&u, &x, 4);
-  const uint8_t sign = (uint8_t)(u >> 24 & 0x80);
-  u &= 0x7FFFFFFFu;
-  float a;
-  memcpy(&a, &u, 4);
-  if (a < 0.015625f) return sign | (uint8_t)(int)nearbyintf(a * 512.0f);  // steps of 2^-9
-  u += 0x7FFFFu + (u >> 20 & 1);
-  return sign | (uint8_t)((u >> 20) - (120u << 3));  // exponent bias 127 -> 7
-}
+// Device memory of one call.
+struct Staging {
+  void* p = nullptr;
+  ~Staging() {
+    if (p) (void)hipFree(p);
+  }
+};
 
-// One matrix bT [n][k]: codes [n][k] and the scale byte of each row and 128 columns, the
-// same for the rows of a 128 x 128 block.
-static void quantize_fp8(const float* bT, int k, int n, std::vector<uint8_t>& q,
-                         std::vector<uint8_t>& x) {
-  const int kb = ceil_div(k, kFp8Block);
-  q.resize((size_t)n * k);
-  x.resize((size_t)n * kb);
-  for (int j0 = 0; j0 < n; j0 += kFp8Block)
-    for (int b = 0; b < kb; b++) {
-      const int j1 = std::min(n, j0 + kFp8Block), c0 = b * kFp8Block,
-                c1 = std::min(k, c0 + kFp8Block);
-      uint32_t top = 0;
-      for (int j = j0; j < j1; j++)
-        for (int c = c0; c < c1; c++) {
-          uint32_t u;
-          memcpy(&u, bT + (size_t)j * k + c, 4);
-          top = std::max(top, u & 0x7FFFFFFFu);
-        }
-      const int e = fp8_exponent(top);
-      const float f = ldexpf(1.0f, 127 - e);
-      for (int j = j0; j < j1; j++) {
-        x[(size_t)j * kb + b] = (uint8_t)e;
-        for (int c = c0; c < c1; c++)
-          q[(size_t)j * k + c] = e4m3_rne(bT[(size_t)j * k + c] * f);
-      }
-    }
-}
-
-static int upload_fp8(Context* ctx, const std::vector<uint8_t>& q, const std::vector<uint8_t>& x,
-                      const float* bias, int k, int n, bool glu, rh_weight** out) {
+// The matrices [n][k] of a weight (gate and up, or one alone) to codes and scale bytes, on the
+// device: a 4096 x 4096 matrix took the host 42 ms.
+static int pack_fp8(Context* ctx, const float* const* mats, int count, const float* bias, int k,
+                    int n, rh_weight** out) {
   std::unique_ptr<rh_weight, void (*)(rh_weight*)> w(new rh_weight(), destroy_weight);
   w->ctx = ctx;
   w->mode = RH_MODE_FP8;
   w->k = k;
-  w->n = n;
-  w->glu = glu;
+  w->n = n * count;
+  w->glu = count == 2;
   w->kp = (int)round_up(k, kWeightKPad);
-  w->np = (int)round_up(n, kWeightRowPad);
-  const int kb = w->kp / kFp8Block, groups = w->np / kFp8Block;
-  std::vector<uint8_t> img((size_t)w->np * w->kp, 0), exps((size_t)w->np * kb, 0);
-  for (int j = 0; j < n; j++) {
-    memcpy(&img[(size_t)j * w->kp], &q[(size_t)j * k], k);
-    for (int b = 0; b < kb; b++) exps[fp8_scale_at(j, b, groups)] = x[(size_t)j * kb + b];
+  w->np = (int)round_up(w->n, kWeightRowPad);
+  const int groups = w->np / kFp8Block;
+  const size_t codes = (size_t)w->np * w->kp, exps = (size_t)w->np * (w->kp / kFp8Block);
+  const size_t bytes = (size_t)n * k * sizeof(float), flag = round_up(bytes, 8);
+  Staging stage;
+  RH_HIP(hipMalloc(&stage.p, flag + 8));
+  RH_HIP(hipMalloc(&w->d_data, codes));
+  RH_HIP(hipMalloc((void**)&w->d_exp, exps));
+  RH_HIP(hipMemsetAsync(w->d_data, 0, codes, ctx->stream));
+  RH_HIP(hipMemsetAsync(w->d_exp, 0, exps, ctx->stream));
+  auto* bad = reinterpret_cast<unsigned long long*>(static_cast<uint8_t*>(stage.p) + flag);
+  for (int h = 0; h < count; h++) {
+    unsigned long long at = ~0ull;
+    RH_HIP(hipMemcpyAsync(bad, &at, 8, hipMemcpyHostToDevice, ctx->stream));
+    RH_HIP(hipMemcpyAsync(stage.p, mats[h], bytes, hipMemcpyHostToDevice, ctx->stream));
+    RH_HIP(launch_pack_fp8(static_cast<const float*>(stage.p), k, n,
+                           static_cast<uint8_t*>(w->d_data), w->kp, w->d_exp, groups,
+                           count == 2 ? h : -1, bad, ctx->stream));
+    RH_HIP(hipMemcpyAsync(&at, bad, 8, hipMemcpyDeviceToHost, ctx->stream));
+    RH_HIP(hipStreamSynchronize(ctx->stream));
+    if (at != ~0ull) {
+      char buf[160];
+      snprintf(buf, sizeof buf, "PackFP8: weight [%llu,%llu] is not finite", at / k, at % k);
+      return fail(RH_ERR_NONFINITE, buf);
+    }
   }
-  hipError_t e = hipMalloc(&w->d_data, img.size());
-  if (e == hipSuccess) e = hipMemcpy(w->d_data, img.data(), img.size(), hipMemcpyHostToDevice);
-  if (e == hipSuccess) e = hipMalloc((void**)&w->d_exp, exps.size());
-  if (e == hipSuccess) e = hipMemcpy(w->d_exp, exps.data(), exps.size(), hipMemcpyHostToDevice);
-  if (e == hipSuccess && bias) {
-    e = hipMalloc((void**)&w->d_bias, n * sizeof(float));
-    if (e == hipSuccess)
-      e = hipMemcpy(w->d_bias, bias, n * sizeof(float), hipMemcpyHostToDevice);
+  if (bias) {
+    RH_HIP(hipMalloc((void**)&w->d_bias, n * sizeof(float)));
+    RH_HIP(hipMemcpy(w->d_bias, bias, n * sizeof(float), hipMemcpyHostToDevice));
   }
-  if (e != hipSuccess) return hip_fail(e, "weight upload", __FILE__, __LINE__);
   ctx_retain(ctx);
   *out = w.release();
   return RH_OK;
@@ -88,31 +70,14 @@ static int upload_fp8(Context* ctx, const std::vector<uint8_t>& q, const std::ve
 
 int pack_weight_fp8(Context* ctx, const float* bT, const float* bias, int k, int n,
                     rh_weight** out) {
-  int st = pack_check(RH_MODE_FP8, bT, k, n);
-  if (st != RH_OK) return st;
-  std::vector<uint8_t> q, x;
-  quantize_fp8(bT, k, n, q, x);
-  return upload_fp8(ctx, q, x, bias, k, n, false, out);
+  return pack_fp8(ctx, &bT, 1, bias, k, n, out);
 }
 
 // gate and up keep blocks of their own; rows interleave in groups of kGluGroup.
 int pack_weight_fp8_gated(Context* ctx, const float* gate, const float* up, int k, int i,
                           rh_weight** out) {
-  const int kb = ceil_div(k, kFp8Block);
-  std::vector<uint8_t> q((size_t)2 * i * k), x((size_t)2 * i * kb);
-  for (int half = 0; half < 2; half++) {
-    const float* src = half ? up : gate;
-    int st = pack_check(RH_MODE_FP8, src, k, i);
-    if (st != RH_OK) return st;
-    std::vector<uint8_t> q1, x1;
-    quantize_fp8(src, k, i, q1, x1);
-    for (int r = 0; r < i; r++) {
-      const size_t to = (size_t)(r / kGluGroup) * 2 * kGluGroup + half * kGluGroup + r % kGluGroup;
-      memcpy(&q[to * k], &q1[(size_t)r * k], k);
-      memcpy(&x[to * kb], &x1[(size_t)r * kb], kb);
-    }
-  }
-  return upload_fp8(ctx, q, x, nullptr, k, 2 * i, true, out);
+  const float* mats[2] = {gate, up};
+  return pack_fp8(ctx, mats, 2, nullptr, k, i, out);
 }
 
 int export_fp8_scales(const rh_weight* w, float* scales, int32_t* colsum) {

@@ -143,7 +143,7 @@ int run_gemm_i8(Context* ctx, const rh_weight* w, const uint8_t* qa, int ldq,
 // run_gemm_i8 with the residual + LayerNorm finish (launch_gemm_i8_ln).
 int run_gemm_i8_ln(Context* ctx, const rh_weight* w, const uint8_t* qa, int ldq,
                    const float* rs, int m, const I8LnArgs& f, double ops);
-// The FP8 mode (capi_fp8.cpp). The packers' shapes and values are checked by the
+// The FP8 mode (capi_fp8.cpp). The packers' shapes are checked by the
 // caller (pack_weight, pack_weight_gated).
 constexpr int kFp8Block = 128;
 int pack_weight_fp8(Context* ctx, const float* bT, const float* bias, int k, int n,

@@ -115,6 +115,11 @@ __host__ __device__ __forceinline__ size_t fp8_scale_at(int r, int kb, int group
 // zeros past k) and their scale bytes (fp8_scale_at)
 hipError_t launch_quantize_rows_fp8(const void* a, int a_bf16, int lda, int m, int k, uint8_t* qa,
                                     int ldq, uint8_t* sa, hipStream_t s);
+// w [n][k] on the device -> codes [..][kp] and scale bytes of blocks of 128 x 128; half: -1, or
+// 0 / 1 for the gate / up rows of an interleaved pair. *bad becomes the place of the first value
+// that is not finite (its block is then left out); the caller sets it to all ones.
+hipError_t launch_pack_fp8(const float* w, int k, int n, uint8_t* img, int kp, uint8_t* exps,
+                           int groups, int half, unsigned long long* bad, hipStream_t s);
 struct GemmFp8Args {
   const uint8_t* A;   // codes [M][lda]
   int lda;            // bytes, round_up(K, 128)

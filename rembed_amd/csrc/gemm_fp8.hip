@@ -100,6 +100,58 @@ hipError_t launch_quantize_rows_fp8(const void* a, int a_bf16, int lda, int m, i
   return hipGetLastError();
 }
 
+// ---- weights to e4m3 ----------------------------------------------------------------
+// A workgroup takes one 128 x 128 block, 16 words of four consecutive values a thread. half: -1,
+// or which of a gated pair's matrices this is, whose rows interleave in groups of kGluGroup.
+// bad: the first value that is not finite, by its place in the matrix.
+__global__ __launch_bounds__(256) void pack_fp8_kernel(const float* w, int k, int n, uint8_t* img,
+                                                       int kp, uint8_t* exps, int groups, int half,
+                                                       unsigned long long* bad) {
+  constexpr int kWords = kFp8Block * kFp8Block / 4 / 256;
+  __shared__ uint32_t s_top[4];
+  const int tid = threadIdx.x, kb = blockIdx.x;
+  const int c = kb * kFp8Block + tid % 32 * 4, r0 = blockIdx.y * kFp8Block + tid / 32;
+  float v[kWords][4];
+  uint32_t top = 0;
+#pragma unroll
+  for (int i = 0; i < kWords; i++) {
+    const int r = r0 + i * 8;
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+      const size_t at = (size_t)r * k + c + e;
+      v[i][e] = r < n && c + e < k ? w[at] : 0.0f;
+      const uint32_t u = __float_as_uint(v[i][e]) & 0x7FFFFFFFu;
+      if (u >= 0x7F800000u) atomicMin(bad, (unsigned long long)at);
+      top = max(top, u);
+    }
+  }
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) top = max(top, (uint32_t)__shfl_xor((int)top, o, 64));
+  if (tid % 64 == 0) s_top[tid / 64] = top;
+  __syncthreads();
+  top = max(max(s_top[0], s_top[1]), max(s_top[2], s_top[3]));
+  if (top >= 0x7F800000u) return;  // refused
+  const int x = fp8_exponent(top);
+  const float f = fp8_inverse(x);
+#pragma unroll
+  for (int i = 0; i < kWords; i++) {
+    const int r = r0 + i * 8;
+    if (r >= n) break;
+    const int to = half < 0 ? r : (r / kGluGroup * 2 + half) * kGluGroup + r % kGluGroup;
+    *reinterpret_cast<int*>(img + (size_t)to * kp + c) =
+        fp8_pack4(v[i][0] * f, v[i][1] * f, v[i][2] * f, v[i][3] * f);
+    if (tid % 32 == 0) exps[fp8_scale_at(to, kb, groups)] = (uint8_t)x;
+  }
+}
+
+hipError_t launch_pack_fp8(const float* w, int k, int n, uint8_t* img, int kp, uint8_t* exps,
+                           int groups, int half, unsigned long long* bad, hipStream_t s) {
+  hipLaunchKernelGGL(pack_fp8_kernel,
+                     dim3((unsigned)ceil_div(k, kFp8Block), (unsigned)ceil_div(n, kFp8Block)),
+                     dim3(256), 0, s, w, k, n, img, kp, exps, groups, half, bad);
+  return hipGetLastError();
+}
+
 // act(gate) * up. SiLU and the tanh GELU, x / (1 + e^-z), on the hardware's exponential and
 // reciprocal, each within an ulp: about 2^-22 of the value where the products before them
 // are off by 2^-16 and a bf16 result rounds at 2^-8; expf and a division take 50
