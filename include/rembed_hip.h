@@ -378,7 +378,9 @@ int rh_cache_append(rh_context *ctx, const rh_kv_cache *cache, const void *kv, i
  * are left as they are. Table entries that are no page of the cache hold no keys. max_q
  * must be >= every request's rows; max_len should be >= every lens (it only chooses how the
  * work is split). ldq and q_off multiples of 8, ldout of 4, q 16-byte, out 16-byte (bf16:
- * 8-byte) aligned; scratch: rh_cache_attention_scratch bytes, 16-byte aligned. */
+ * 8-byte) aligned; scratch: rh_cache_attention_scratch bytes, 16-byte aligned. Fewer rows may
+ * take more of it (their key ranges are split further): a buffer for calls of several sizes
+ * holds the largest of theirs. */
 size_t rh_cache_attention_scratch(int batch, int max_q, int max_len, int heads, int kv_heads,
                                   int dh);
 int rh_cache_attention(rh_context *ctx, const void *q, int q_bf16, int ldq, int q_off,
