@@ -595,10 +595,10 @@ __global__ __launch_bounds__(64 * kWaves, DH == 256 ? 1 : 2) void cache_attentio
 }
 
 // ---- many columns --------------------------------------------------------------------
-// CW waves of 32 columns each walk the same pages, PG such groups a part of them each. What bounds it: a page's products take
-// the matrix cores 64 cycles each (dh 128: 16 of them, 1024 cycles) and its softmax the VALU
-// 1100 to 1300, and a wave issues in order, so one after the other they cost their sum even
-// with two waves per SIMD. The loop therefore is a pipeline over pages whose body has no
+// CW waves of 32 columns each walk the same pages, PG such groups a part of them each. What
+// bounds it: a page's products take the matrix cores 64 cycles each (dh 128: 16 of them, 1024
+// cycles) and its softmax the VALU 1450, and a wave issues in order, so one after the other they
+// cost their sum even with two waves per SIMD. The loop is a pipeline over pages whose body has no
 // branch: while page g's scores become P, two at a time, the products between them are
 // page g + 1's scores and page g - 1's values. K and V come to LDS by global_load_lds in
 // fragment order (1 KiB pieces, read back without bank conflicts), two turns before they are
