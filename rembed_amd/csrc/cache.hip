@@ -251,8 +251,9 @@ hipError_t launch_cache_plan(const CachePlanArgs& a, hipStream_t s) {
 // Single tokens are bound by latency, so a request is found by a 64-way search (one load of
 // a wave per level; a binary search took 3 µs of 7.6 for 48 requests) and its rows are
 // asked for before their slots are known: 48 single tokens of 8 heads of 128 take 5.5 µs. Many
-// tokens are bound by their bytes: 22k tokens, 140 MB, take 36 µs, 3.9 TB/s of a copy's
-// 4.9 (values written to LDS byte by byte, and 90 registers for 62: 37.3).
+// tokens are bound by their bytes: 22k tokens, 140 MB, take 30.6 µs, 4.6 TB/s of a copy's 4.9
+// (36.2 with stores that stay in the L2; before that values written to LDS byte by byte, and 90
+// registers for 62: 37.3).
 constexpr int kAppendThreads = 256;
 
 // The last request b with blocks[b] <= seg: every level looks at 64 evenly spaced ones.
@@ -433,8 +434,13 @@ __global__ __launch_bounds__(kAppendThreads) void cache_append_kernel(CacheAppen
   if (!whole_k && !whole_v) return;  // the scales stay as well
   __syncthreads();
   for (int i = tid * 16; i < kBytes; i += kAppendThreads * 16) {
-    if (whole_k) *reinterpret_cast<v4i*>(gk + i) = *reinterpret_cast<const v4i*>(s_k + i);
-    if (whole_v) *reinterpret_cast<v4i*>(gv + i) = *reinterpret_cast<const v4i*>(s_v + spread(i));
+    // whole lines, past the L2, whose own would be written back at the kernel's end
+    if (whole_k)
+      __builtin_nontemporal_store(*reinterpret_cast<const v4i*>(s_k + i),
+                                  reinterpret_cast<v4i*>(gk + i));
+    if (whole_v)
+      __builtin_nontemporal_store(*reinterpret_cast<const v4i*>(s_v + spread(i)),
+                                  reinterpret_cast<v4i*>(gv + i));
   }
   if (tid == 0) {
     p.cache.k_exp[unit] = (uint8_t)xk;

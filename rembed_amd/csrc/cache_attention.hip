@@ -968,8 +968,11 @@ __global__ __launch_bounds__(64 * CW * PG, DH == 256 ? 1 : 2) void cache_attenti
       const int row = r + lane / kLanes;
       const v8bf x = *reinterpret_cast<const v8bf*>(place(row, lane % kLanes));
       const int64_t at = dest[row];
+      // past the L2, whose lines would be written back at the kernel's end (dh 256, windowed:
+      // 30.1 -> 29.2 µs)
       if (at >= 0)
-        *reinterpret_cast<Out*>(static_cast<__bf16*>(p.out) + at + lane % kLanes * 8) = x;
+        __builtin_nontemporal_store(
+            (Out)x, reinterpret_cast<Out*>(static_cast<__bf16*>(p.out) + at + lane % kLanes * 8));
     }
     return;
   }

@@ -236,9 +236,14 @@ __device__ __forceinline__ void fp8_rows_out(const GemmFp8Args& p, v16f (&acc)[T
       const int r = k + lane / kL, row = row0 + i * 32 + r;
       const v4i x = *reinterpret_cast<const v4i*>(own + r * kRow + l * 16);
       typedef v4i Out __attribute__((aligned(8)));
-      if (row < p.M && to < (GLU ? p.N / 2 : p.N))
-        *reinterpret_cast<Out*>(static_cast<uint8_t*>(p.out) +
-                                ((size_t)row * p.ldo + to) * kEach) = x;
+      if (row >= p.M || to >= (GLU ? p.N / 2 : p.N)) continue;
+      Out* at = reinterpret_cast<Out*>(static_cast<uint8_t*>(p.out) +
+                                       ((size_t)row * p.ldo + to) * kEach);
+      // past the L2, whose lines would be written back at the kernel's end (8192 x 4096 x 4096
+      // with its quantizer 136.8 -> 132.7 µs); the small tile's pieces of lines stay in it
+      // (300 x 640 x 640 6.5 µs, past it 7.0)
+      if constexpr (WN >= 64) __builtin_nontemporal_store((Out)x, at);
+      else *at = x;
     }
     __builtin_amdgcn_wave_barrier();
   }
@@ -284,9 +289,9 @@ __device__ __forceinline__ void fp8_row(v16f (&acc)[TM][TN], const v8i& a, const
 // NS-slot ring filled by global_load_lds; the stage's scale words come the same
 // way, behind its codes. What bounds it are LDS and the matrix cores alike: a stage of 256 x 256
 // reads 192 KB of fragments and takes in 64 KB, 2048 cycles at 128 bytes each, as its products
-// do (128 x 256: 1400 and 1024). 8192 x 4096 x 4096 takes 116 µs, 2.37 PFLOP/s, where the card's
-// library product takes 110; four waves of 128 x 128, which read a third less, 135, because one
-// wave a SIMD hides less than two.
+// do (128 x 256: 1400 and 1024). 8192 x 4096 x 4096 takes 112 µs, 2.45 PFLOP/s, where the card's
+// library product takes 110; four waves of 128 x 128, which read a third less, 19 more than this,
+// because one wave a SIMD hides less than two.
 template <int BM, int BN, int NS, int WGN>
 __global__ __launch_bounds__(128 * WGN) void gemm_fp8_kernel(GemmFp8Args p) {
   constexpr int NT = 128 * WGN, BK = 128, CPR = BK / 16;
