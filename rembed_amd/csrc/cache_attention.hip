@@ -236,21 +236,27 @@ struct CacheTile {
   }
 };
 
-// A page's fragments of one head: 1 KiB pieces, 16 bytes a lane.
-template <int DH>
+// A page's fragments of one head: 1 KiB pieces, 16 bytes a lane. STREAM: read by nobody else,
+// so they need not stay in the L2.
+template <bool STREAM>
+__device__ __forceinline__ v8i cache_fetch(const v4i* at) {
+  if constexpr (STREAM)
+    return join8(__builtin_nontemporal_load(at), __builtin_nontemporal_load(at + 64));
+  return join8(at[0], at[64]);
+}
+template <int DH, bool STREAM>
 __device__ __forceinline__ void cache_fetch_k(const uint8_t* k, int lane, v8i (&kf)[DH / 64][2]) {
   const v4i* at = reinterpret_cast<const v4i*>(k) + lane;
 #pragma unroll
   for (int s = 0; s < DH / 64; s++)
 #pragma unroll
-    for (int t = 0; t < 2; t++)
-      kf[s][t] = join8(at[((s * 2 + t) * 2) * 64], at[((s * 2 + t) * 2 + 1) * 64]);
+    for (int t = 0; t < 2; t++) kf[s][t] = cache_fetch<STREAM>(at + (s * 2 + t) * 128);
 }
-template <int DH>
+template <int DH, bool STREAM>
 __device__ __forceinline__ void cache_fetch_v(const uint8_t* v, int lane, v8i (&vf)[DH / 32]) {
   const v4i* at = reinterpret_cast<const v4i*>(v) + lane;
 #pragma unroll
-  for (int t = 0; t < DH / 32; t++) vf[t] = join8(at[t * 2 * 64], at[(t * 2 + 1) * 64]);
+  for (int t = 0; t < DH / 32; t++) vf[t] = cache_fetch<STREAM>(at + t * 128);
 }
 
 // The same with accumulators that products alone touch. O is kept in units of the reference
@@ -463,8 +469,8 @@ __device__ __forceinline__ void cache_again(CacheFast<DH>& w, const CacheAttnArg
     if (page < 0 || page >= p.cache.pages) continue;
     const size_t u = (size_t)page * p.cache.kv_heads + h;
     v8i kf[KS][2], vf[DT];
-    cache_fetch_k<DH>(p.cache.k + u * kHalf, lane, kf);
-    cache_fetch_v<DH>(p.cache.v + u * kHalf, lane, vf);
+    cache_fetch_k<DH, false>(p.cache.k + u * kHalf, lane, kf);
+    cache_fetch_v<DH, false>(p.cache.v + u * kHalf, lane, vf);
     r.page(kf, vf, p.cache.k_exp[u], p.cache.v_exp[u], g * kPageT, n, cs, lane >> 5);
   }
 #pragma unroll
@@ -480,10 +486,11 @@ constexpr int kPartRow = DH + 4;
 // ---- few columns -----------------------------------------------------------------------
 // Four waves share a tile of columns and take its pages in turn, straight to registers: what
 // bounds it is the cache's bytes, each read once: 48 single tokens over 500 to 8191 (463 MB,
-// 16 heads over 8 of dh 128) take 94 µs, 4.9 TB/s, what a large copy reaches. Two workgroups
+// 16 heads over 8 of dh 128) take 80 µs, 5.8 TB/s, where a large copy reaches 4.9 and pages kept in
+// the L2 94 µs (cache_streams). Two workgroups
 // to a CU hide each other's waits; the next page's K asked for a page ahead did not gain and
 // cost registers. The waves' results are joined in LDS, eight columns at a time.
-template <int DH, bool BF16>
+template <int DH, bool BF16, bool STREAM>
 __global__ __launch_bounds__(64 * kWaves, DH == 256 ? 1 : 2) void cache_attention_kernel(
     CacheAttnArgs p, int tiles, int splits, int part_cols) {
   constexpr int KS = DH / 64, DT = DH / 32, kStride = DH + 4, kHalf = kPageT * DH;
@@ -526,8 +533,8 @@ __global__ __launch_bounds__(64 * kWaves, DH == 256 ? 1 : 2) void cache_attentio
       if (page < 0) continue;  // no such page: no keys
       const size_t at = ((size_t)page * p.cache.kv_heads + h) * kHalf;
       v8i kf[KS][2], vf[DT];
-      cache_fetch_k<DH>(p.cache.k + at, lane, kf);
-      cache_fetch_v<DH>(p.cache.v + at, lane, vf);
+      cache_fetch_k<DH, STREAM>(p.cache.k + at, lane, kf);
+      cache_fetch_v<DH, STREAM>(p.cache.v + at, lane, vf);
       w.page(kf, vf, win.at(win.xk, i), win.at(win.xv, i), (g0 + i) * kPageT, n, cs, half);
     }
   }
@@ -1088,6 +1095,13 @@ static void cache_split(int batch, int max_q, int max_len, int heads, int kv_hea
   *splits = cache_ranges(batch, max_q, heads, kv_heads, dh, *per_wg, pages);
 }
 
+// Few columns: pages past the L2 where all requests' could not stay in the memory's own 256 MiB
+// cache, so that each comes from memory. Below, texts that share pages find them (48 tokens over
+// 700 of which 640 are shared: 16.2 µs, past the L2 17.6).
+static bool cache_streams(const CacheAttnArgs& a, long long pages) {
+  return pages * kPageT * a.batch * a.cache.kv_heads * a.cache.dh * 2 > 256LL << 20;
+}
+
 // For any window: all pages, and four tiles, which never make fewer ranges than two.
 size_t cache_attention_floats(int batch, int max_q, int max_len, int heads, int kv_heads, int dh) {
   const int per_wg = cache_by_cols(max_q, heads, kv_heads) ? 4 : 1;
@@ -1118,8 +1132,12 @@ static hipError_t launch_dh(const CacheAttnArgs& a, hipStream_t s) {
   else if (per_wg == 2)                                                                        \
     hipLaunchKernelGGL((cache_attention_cols_kernel<DH, B, 2, 2, DH == 64 ? 3 : 2>), grid,     \
                        block, 0, s, a, tiles, splits, pc);                                     \
+  else if (cache_streams(a, cache_pages(a.max_q, a.max_len, a.window, kCols)))                 \
+    hipLaunchKernelGGL((cache_attention_kernel<DH, B, true>), grid, block, 0, s, a, tiles,     \
+                       splits, pc);                                                            \
   else                                                                                         \
-    hipLaunchKernelGGL((cache_attention_kernel<DH, B>), grid, block, 0, s, a, tiles, splits, pc)
+    hipLaunchKernelGGL((cache_attention_kernel<DH, B, false>), grid, block, 0, s, a, tiles,    \
+                       splits, pc)
   if (a.in_bf16) {
     RH_ATTN(true);
   } else {

@@ -400,6 +400,28 @@ def test_attention_of_many_columns(gpu_ctx, case):
                 assert np.linalg.norm(g - want[0]) <= 2.0 ** -7 * np.linalg.norm(want[0]), (b, r)
 
 
+@pytest.mark.parametrize("dh", [64, 128, 256])
+@pytest.mark.parametrize("nq,window", [(1, 0), (5, 0), (16, 300)])
+def test_attention_over_a_cache_said_to_be_large(gpu_ctx, dh, nq, window):
+    """Few columns over more pages than the memory's cache holds, by what max_len says, read
+    past the L2: the results of the same pages read through it, but for the ranges' joins."""
+    rng = np.random.default_rng(dh + nq)
+    past, fresh = [700, 64, 0, 1300], [nq, 1, nq, nq]
+    pages, table, cu, blk, lens, slots = F.batch_of(rng, past, fresh)
+    c = O.Cache(pages, 2, dh)
+    acu = np.concatenate([[0], np.cumsum(lens)]).astype(I32)
+    asl = np.concatenate([table[b, np.arange(n) // 64].astype(np.int64) * 64 + np.arange(n) % 64
+                          for b, n in enumerate(lens)])
+    k, v = rng.standard_normal((2, len(asl), 2, dh))
+    c.append(k, v, acu, asl)
+    q = rng.standard_normal((int(cu[-1]), 4, dh))
+    for max_len in (int(max(lens)), 3_000_000):
+        for dtype, out_bf16 in (("bf16", True), ("f32", False)):
+            got, val = F.attend(gpu_ctx, c, q, dtype, table, cu, lens, dh ** -0.5, True, window,
+                                out_bf16, max_len=max_len)
+            F.check_attention(c, got, val, table, cu, lens, dh ** -0.5, True, window, dtype, out_bf16)
+
+
 @pytest.mark.parametrize("dh,kv,nq", [(64, 16, 300), (128, 8, 300), (256, 2, 300)])
 def test_wide_attention_of_scores_far_apart(gpu_ctx, dh, kv, nq):
     """Blocks whose scores lie up to 896 apart, in the form of four tiles per workgroup."""
