@@ -270,10 +270,10 @@ __device__ __forceinline__ int append_request(const int32_t* blocks, int batch, 
   return lo;
 }
 
-// Where a byte of V lies in LDS: 16-byte pieces change places within their 512 bytes, so
-// that the words a wave writes at once (tokens 4 apart, values DH/4 apart) meet different banks.
+// Where a byte of V lies in LDS: 16-byte pieces change places within their 256 bytes, so
+// that the words a wave writes at once (tokens 4 apart among them) meet all banks.
 __device__ __forceinline__ int spread(int at) {
-  return at ^ ((at >> 9 & 1) << 6 | (at >> 11 & 1) << 7);
+  return at ^ (at >> 9 & 1) << 6;
 }
 
 template <int DH, bool BF16>
@@ -297,8 +297,8 @@ __global__ __launch_bounds__(kAppendThreads) void cache_append_kernel(CacheAppen
   const int cnt = min(kPage - off, fresh - first);
   if (cnt <= 0) return;
 
-  // this thread's quarter of its token's K and V; four lanes beside each other have the
-  // four tokens of one word of V
+  // every fourth 16 bytes of its token's K and V to a thread (so a load of a token's four takes 64
+  // bytes at a time); four lanes beside each other have the four tokens of one word of V
   const int tok = tid / 16 * 4 + tid % 4, quarter = tid / 4 % 4;
   const bool mine = tok >= off && tok < off + cnt;
   using T = std::conditional_t<BF16, v8bf, v4f>;  // 16 bytes of a row, widened when used
@@ -306,13 +306,13 @@ __global__ __launch_bounds__(kAppendThreads) void cache_append_kernel(CacheAppen
   T k[E / kStep], v[E / kStep];
   uint32_t mk = 0, mv = 0;
   if (mine) {
-    const size_t at = (size_t)(r0 + first + tok - off) * p.ldkv + h * DH + quarter * E;
+    const size_t at = (size_t)(r0 + first + tok - off) * p.ldkv + h * DH + quarter * kStep;
     using S = std::conditional_t<BF16, __bf16, float>;
     const S* row = static_cast<const S*>(p.kv) + at;
 #pragma unroll
     for (int e = 0; e < E / kStep; e++) {
-      k[e] = *reinterpret_cast<const T*>(row + p.k_off + e * kStep);
-      v[e] = *reinterpret_cast<const T*>(row + p.v_off + e * kStep);
+      k[e] = *reinterpret_cast<const T*>(row + p.k_off + e * 4 * kStep);
+      v[e] = *reinterpret_cast<const T*>(row + p.v_off + e * 4 * kStep);
     }
   }
   const int64_t slot = p.slots[r0 + first];
@@ -399,12 +399,15 @@ __global__ __launch_bounds__(kAppendThreads) void cache_append_kernel(CacheAppen
         wv[e / 4] = 0;
       }
     }
+    // value e of the thread lies at this one of the row
+    auto place = [&](int e) { return (e / kStep * 4 + quarter) * kStep + e % kStep; };
+    typedef int W __attribute__((ext_vector_type(kStep / 4)));
 #pragma unroll
-    for (int e = 0; e < E; e += 16) {
-      const int at = k_at(tok, quarter * E + e);
-      const v4i w = {wk[e / 4], wk[e / 4 + 1], wk[e / 4 + 2], wk[e / 4 + 3]};
-      if (whole_k) *reinterpret_cast<v4i*>(s_k + at) = w;
-      else *reinterpret_cast<v4i*>(gk + at) = w;
+    for (int e = 0; e < E; e += kStep) {
+      W w;
+#pragma unroll
+      for (int i = 0; i < kStep / 4; i++) w[i] = wk[e / 4 + i];
+      *reinterpret_cast<W*>((whole_k ? s_k : gk) + k_at(tok, place(e))) = w;
     }
     if (tok - tid % 4 >= off && tok - tid % 4 + 3 < off + cnt) {
       // all four tokens are new: four values of one token each become four tokens'
@@ -417,14 +420,14 @@ __global__ __launch_bounds__(kAppendThreads) void cache_append_kernel(CacheAppen
         w = __builtin_amdgcn_perm(o, w, odd ? 0x03070105 : 0x06020400);
         o = __builtin_amdgcn_mov_dpp(w, 0x4E, 0xF, 0xF, true);  // lanes 2 3 0 1
         w = __builtin_amdgcn_perm(o, w, high ? 0x03020706 : 0x05040100);
-        const int at = v_at(tok - tid % 4, quarter * E + e + tid % 4);
+        const int at = v_at(tok - tid % 4, place(e) + tid % 4);
         if (whole_v) *reinterpret_cast<int*>(s_v + spread(at)) = w;
         else *reinterpret_cast<int*>(gv + at) = w;
       }
     } else {
 #pragma unroll
       for (int e = 0; e < E; e++) {
-        const int at = v_at(tok, quarter * E + e);
+        const int at = v_at(tok, place(e));
         const uint8_t c = (uint8_t)(wv[e / 4] >> (e % 4 * 8));
         if (whole_v) s_v[spread(at)] = c;
         else gv[at] = c;
