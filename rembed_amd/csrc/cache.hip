@@ -251,9 +251,9 @@ hipError_t launch_cache_plan(const CachePlanArgs& a, hipStream_t s) {
 // Single tokens are bound by latency, so a request is found by a 64-way search (one load of
 // a wave per level; a binary search took 3 µs of 7.6 for 48 requests) and its rows are
 // asked for before their slots are known: 48 single tokens of 8 heads of 128 take 5.5 µs. Many
-// tokens are bound by their bytes: 22k tokens, 140 MB, take 30.6 µs, 4.6 TB/s of a copy's 4.9
-// (36.2 with stores that stay in the L2; before that values written to LDS byte by byte, and 90
-// registers for 62: 37.3).
+// tokens are bound by their bytes: 22k tokens, 140 MB, take 28.6 µs, 4.9 TB/s, what a large copy
+// reaches (a thread's loads one after the other in a row instead of 64 bytes by four threads:
+// 30.7; stores that stay in the L2: 36.2).
 constexpr int kAppendThreads = 256;
 
 // The last request b with blocks[b] <= seg: every level looks at 64 evenly spaced ones.
@@ -383,6 +383,8 @@ __global__ __launch_bounds__(kAppendThreads) void cache_append_kernel(CacheAppen
     }
     if (whole_k || whole_v) __syncthreads();
   }
+  // single tokens' values of V, a byte to a place, from all threads by way of LDS
+  const bool few = !whole_v && cnt < 4;
   if (mine) {
     const float fk = fp8_inverse(xk), fv = fp8_inverse(xv);
     int wk[E / 4], wv[E / 4];
@@ -409,7 +411,11 @@ __global__ __launch_bounds__(kAppendThreads) void cache_append_kernel(CacheAppen
       for (int i = 0; i < kStep / 4; i++) w[i] = wk[e / 4 + i];
       *reinterpret_cast<W*>((whole_k ? s_k : gk) + k_at(tok, place(e))) = w;
     }
-    if (tok - tid % 4 >= off && tok - tid % 4 + 3 < off + cnt) {
+    if (few) {
+#pragma unroll
+      for (int e = 0; e < E; e += 4)
+        *reinterpret_cast<int*>(s_v + (tok - off) * DH + place(e)) = wv[e / 4];
+    } else if (tok - tid % 4 >= off && tok - tid % 4 + 3 < off + cnt) {
       // all four tokens are new: four values of one token each become four tokens'
       // value d + tid % 4 (bytes change places with the neighbour's, pairs with the pair's)
       const int odd = tid & 1, high = tid & 2;
@@ -433,6 +439,10 @@ __global__ __launch_bounds__(kAppendThreads) void cache_append_kernel(CacheAppen
         else gv[at] = c;
       }
     }
+  }
+  if (few) {
+    __syncthreads();
+    for (int i = tid; i < cnt * DH; i += kAppendThreads) gv[v_at(off + i / DH, i % DH)] = s_v[i];
   }
   if (!whole_k && !whole_v) return;  // the scales stay as well
   __syncthreads();
