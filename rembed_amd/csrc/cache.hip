@@ -250,7 +250,7 @@ hipError_t launch_cache_plan(const CachePlanArgs& a, hipStream_t s) {
 // reach queries that must not see it through V). It sets no scale.
 // Single tokens are bound by latency, so a request is found by a 64-way search (one load of
 // a wave per level; a binary search took 3 µs of 7.6 for 48 requests) and its rows are
-// asked for before their slots are known: 48 single tokens of 8 heads of 128 take 5.5 µs. Many
+// asked for before their page is known: 48 single tokens of 8 heads of 128 take 5.5 µs. Many
 // tokens are bound by their bytes: 22k tokens, 140 MB, take 28.6 µs, 4.9 TB/s, what a large copy
 // reaches (a thread's loads one after the other in a row instead of 64 bytes by four threads:
 // 30.7; stores that stay in the L2: 36.2).
