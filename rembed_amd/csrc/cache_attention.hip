@@ -371,7 +371,7 @@ struct CacheFast {
 // Page ids and scale bytes of 64 consecutive pages of a request, one a lane: read once, then
 // taken lane by lane, so that no page waits for its table entry and scales.
 struct PageWindow {
-  int page, xk, xv;  // page: -1 where the entry is no page of the cache
+  int page, xk, xv;  // page: -1, scales 1, where the entry is no page of the cache
   // pages g0 .. g0 + 63, none from `end` on
   __device__ __forceinline__ void load(const CacheAttnArgs& p, int b, int h, int g0, int end,
                                        int lane) {
@@ -379,8 +379,10 @@ struct PageWindow {
     page = g < end ? p.table[(size_t)b * p.ldt + g] : -1;
     if (page < 0 || page >= p.cache.pages) page = -1;
     const size_t unit = (size_t)max(page, 0) * p.cache.kv_heads + h;
-    xk = p.cache.k_exp[unit];
-    xv = p.cache.v_exp[unit];
+    // no scale of page 0 for what is none: nobody may have written it, 255 is NaN there, and a
+    // product of zeros under it NaN too
+    xk = page < 0 ? 127 : p.cache.k_exp[unit];
+    xv = page < 0 ? 127 : p.cache.v_exp[unit];
     // waited for here: at their uses, in every turn, the wait would cover younger loads
     asm("" : "+v"(page), "+v"(xk), "+v"(xv));
   }
