@@ -372,8 +372,10 @@ int rh_cache_append(rh_context *ctx, const rh_kv_cache *cache, const void *kv, i
  * the lens[b] that request b has there (positions lens[b] - count ..), or, without causal
  * and window, queries of any kind (attention to an encoder's states of another length).
  * q head h starts at column q_off + h*dh of q [rows][ldq], fp32 (rounded to 8 significant
- * bits here) or bf16, its kv head is h / (heads/kv_heads); causal and window as in
- * rh_attention; scale > 0. P is held to 8 significant bits and the sums in fp32. out is fp32
+ * bits here) or bf16, values under 2^-13 of a head's largest being off by up to 2^-21 of it;
+ * its kv head is h / (heads/kv_heads); causal and window as in rh_attention; scale > 0. A
+ * weight of the softmax is off by at most 2^-9 of itself or, if more, 2^-21 of the largest
+ * that its query has in the same page; the sums are fp32. out is fp32
  * or bf16 [rows][ldout], head h at h*dh. A row that sees no key is 0; rows behind cu[batch]
  * are left as they are. Table entries that are no page of the cache hold no keys. max_q
  * must be >= every request's rows; max_len should be >= every lens (it only chooses how the

@@ -8,13 +8,18 @@
 // they are: codes as operands, the block's scale byte as the instruction's scale.
 // A query row (bf16, or fp32 rounded to 8 bits) is the sum of two e4m3 codes,
 //   q = 2^x (hi + lo / 16),
-// exactly: the residue of rounding 8 significant bits to 4 has at most 4. P is
-// split the same way (off by 2^-8 of itself, as bf16 is), so two products of the
-// double-rate fp8 instruction take the place of one bf16 product and no key or
-// value is ever converted.
+// the residue of rounding 8 significant bits to 4 having at most 4: exactly, down to
+// 2^-13 of the row's largest value, and off by at most 2^-21 of that below. P is split the
+// same way, so two products of the double-rate fp8 instruction take the place of one
+// bf16 product and no key or value is ever converted. A column's weights of a page are
+// taken against the page's own largest, what that lies above or below other pages' being
+// left to the instruction's scale: each is off by at most 2^-9 of itself or 2^-21 of the
+// page's largest. (One reference for all pages made weights 12 nats under a single key's, as a
+// text's first token draws them, wrong by their own size.)
 #include "fp8.h"
 
 #include <algorithm>
+#include <cfloat>
 #include <type_traits>
 
 namespace rh {
@@ -22,9 +27,11 @@ namespace rh {
 constexpr int kPageT = RH_CACHE_BLOCK;
 constexpr int kCols = 32;    // query columns per tile
 constexpr int kWaves = 4;    // per workgroup
-// P^T is 2^4 * exp(score - reference): the reference moves when a score passes it
-// by more than 2^4, so codes stay within 2^8 < 448.
-constexpr float kHead = 4.0f;
+// P^T is taken against a reference of its page: the first whole number that no score of it,
+// times cs, passes, less kHead, so that codes are about 2^8 at most, of 448.
+constexpr float kHead = 8.0f;
+// Powers of two that a page's reference may lie from the running one.
+constexpr float kFar = 64.0f;
 
 // Visible keys [klo, khi] of a query at position i of n; none: klo = khi = 2^31 - 1, behind
 // any. A window may be as long as an int, a query lie before every key.
@@ -153,7 +160,8 @@ __device__ __forceinline__ void cache_clean_v(v8i (&vf)[DH / 32], int key0, int 
   }
 }
 
-// One wave's running state of its 32 columns, and a page's step.
+// One wave's running state of its 32 columns, and a page's step, for scores of any size: O and
+// the sum in units of the largest reference so far (mref).
 template <int DH>
 struct CacheTile {
   static constexpr int KS = DH / 64, DT = DH / 32;
@@ -200,20 +208,24 @@ struct CacheTile {
 #pragma unroll
       for (int e = 0; e < 16; e++) smax = fmaxf(smax, sc[t][e]);
     smax = max_halves(smax);
-    const float mloc = smax * cs;
-    const bool up = mloc > mref + kHead;  // -inf + 4 = -inf: the first visible key moves it
+    const float mloc = smax * cs, to = __builtin_ceilf(mloc) - kHead;
+    const bool up = to > mref;
     if (__any(up)) {
       float alpha = 1.0f;
       if (up) {
-        alpha = __builtin_amdgcn_exp2f(mref - mloc);
-        mref = mloc;
+        alpha = __builtin_amdgcn_exp2f(mref - to);
+        mref = to;
       }
       lrun *= alpha;
 #pragma unroll
       for (int t = 0; t < DT; t++) o[t] *= alpha;
     }
-    // a column with no visible key yet: every p = 2^(-inf) = 0
-    const float m = mref == -INFINITY ? 0.0f : mref - kHead;
+    // the page's reference in units of the running one; against its largest score first, as a
+    // difference of large products is no number near 0. No visible key: every p = 2^(-inf) = 0
+    const float near = smax == -INFINITY ? 0.0f : smax;
+    const float head = smax == -INFINITY ? 0.0f : kHead - (__builtin_ceilf(mloc) - mloc);
+    const int unit = 127 + (smax == -INFINITY ? 0 : (int)fmaxf(to - mref, -kFar));
+    float sum = 0.0f;
     v8i ph, pl;
 #pragma unroll
     for (int t = 0; t < 2; t++)
@@ -222,16 +234,17 @@ struct CacheTile {
         float x[4];
 #pragma unroll
         for (int e = 0; e < 4; e++) {
-          x[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[t][4 * w + e], cs, -m));
-          lrun += x[e];
+          x[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[t][4 * w + e] - near, cs, head));
+          sum += x[e];
         }
         ph[4 * t + w] = fp8_pack4(x[0], x[1], x[2], x[3]);
         pl[4 * t + w] = fp8_rest4(ph[4 * t + w], x[0], x[1], x[2], x[3]);
       }
+    lrun = __builtin_fmaf(sum, __uint_as_float((uint32_t)unit << 23), lrun);
 #pragma unroll
     for (int t = 0; t < DT; t++) {
-      o[t] = mfma_fp8_32(vf[t], ph, o[t], xv, 127);
-      o[t] = mfma_fp8_32(vf[t], pl, o[t], xv, 123);
+      o[t] = mfma_fp8_32(vf[t], ph, o[t], xv, unit);
+      o[t] = mfma_fp8_32(vf[t], pl, o[t], xv, unit - 4);
     }
   }
 };
@@ -259,14 +272,12 @@ __device__ __forceinline__ void cache_fetch_v(const uint8_t* v, int lane, v8i (&
   for (int t = 0; t < DH / 32; t++) vf[t] = cache_fetch<STREAM>(at + t * 128);
 }
 
-// The same with accumulators that products alone touch. O is kept in units of the reference
-// a column starts with (`base`); a reference that has moved since, always by whole powers of
-// two, goes into P's scale byte. A column whose reference moves by more than 2^64 (its earlier
-// keys then weigh nothing in fp32) makes its wave go over its pages once more with CacheTile,
-// whose rescale has no such limit: that branch inside the loops cost the compiler a second
-// copy of O and 8 to 30 spilled registers.
-constexpr float kFar = 64.0f;
-
+// The same with accumulators that products alone touch. O and the sum are kept in units of
+// the first page's reference (`base`); what a page's lies above or below it, always a whole
+// power of two, goes into P's scale byte. Pages more than 2^64 below weigh nothing in fp32 and
+// count from there. A column with one more than 2^64 above, or with scores of 2^24 and more, whose
+// rounding reaches the references, makes its wave go over its pages once more with CacheTile:
+// its rescale inside the loops cost the compiler a second copy of O and 8 to 30 spilled registers.
 template <int DH>
 struct CacheFast {
   static constexpr int KS = DH / 64, DT = DH / 32;
@@ -275,8 +286,8 @@ struct CacheFast {
   v16f o[DT], sc[2];
   v8i ph, pl;  // P of a page,
   int eh, el;  // its scale bytes
-  float mref, base, lrun;
-  bool far;
+  float ref, base, lrun;  // the page's reference, the first one's (-inf: none), the sum of P
+  unsigned long long far;  // lanes whose column is
   int klo, khi;
 
   __device__ __forceinline__ void clear() {
@@ -285,9 +296,10 @@ struct CacheFast {
     ph = v8i{};
     pl = v8i{};
     eh = el = 127;
-    mref = base = -INFINITY;
+    ref = 0.0f;
+    base = -INFINITY;
     lrun = 0.0f;
-    far = false;
+    far = 0;
   }
   // With more than 256 registers in use (dh 256) the compiler may move a scale word to an
   // accumulation register, which the instruction does not take: held in a VGPR here.
@@ -296,8 +308,8 @@ struct CacheFast {
     if constexpr (DH == 256) asm("" : "+v"(ea), "+v"(eb));
     return mfma_fp8_32(a, b, c, ea, eb);
   }
-  // Scores of a page (first position key0) to their maximum; moves the reference. `none`:
-  // the page holds no keys at all.
+  // Scores of a page (first position key0) to its reference. `none`: the page holds no keys
+  // at all.
   __device__ __forceinline__ void refer(int key0, bool none, float cs, int half) {
     if (__builtin_expect(none || __any(key0 < klo || key0 + kPageT - 1 > khi), 0)) {
       const unsigned span = (unsigned)(khi - klo);
@@ -315,24 +327,19 @@ struct CacheFast {
     for (int t = 0; t < 2; t++)
 #pragma unroll
       for (int e = 0; e < 16; e++) smax = fmaxf(smax, sc[t][e]);
-    const float mloc = max_halves(smax) * cs;
-    const bool up = mloc > mref + kHead;  // -inf + 4 = -inf: the first visible key moves it
-    const float to = up ? __builtin_ceilf(mloc) : mref;
-    lrun *= up ? __builtin_amdgcn_exp2f(mref - to) : 1.0f;
-    mref = to;
+    const float to = __builtin_ceilf(max_halves(smax) * cs) - kHead;
+    // a column with no visible key yet: any finite number, every p = 2^(-inf) = 0
+    ref = fmaxf(fmaxf(to, base - kFar), -FLT_MAX);
     base = base == -INFINITY ? to : base;
   }
-  // What P's exponentials are taken against: a column with no visible key yet gets 2^(-inf).
-  __device__ __forceinline__ float origin() const { return mref == -INFINITY ? 0.0f : mref - kHead; }
-  __device__ __forceinline__ void scales() {
-    const float moved = mref == -INFINITY ? 0.0f : mref - base;
-    far |= moved > kFar;
+  // P's scale bytes; the page's weights into the sum
+  __device__ __forceinline__ void scales(float sum) {
+    const float moved = base == -INFINITY ? 0.0f : ref - base;
+    far |= __ballot(moved > kFar) |
+           __ballot((base > -INFINITY) & (__builtin_fabsf(ref) >= 0x1p24f));
     eh = 127 + (int)fminf(moved, kFar);
     el = eh - 4;
-  }
-  // O's unit in units of the last reference
-  __device__ __forceinline__ float unit() const {
-    return mref == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(base - mref);
+    lrun = __builtin_fmaf(sum, __uint_as_float((uint32_t)eh << 23), lrun);
   }
   // one page, its fragments in registers (CacheTile::page)
   __device__ __forceinline__ void page(const v8i (&kf)[KS][2], v8i (&vf)[DT], int xk, int xv,
@@ -346,7 +353,7 @@ struct CacheFast {
         sc[u % 2] = mul(kf[s][u % 2], u < 2 ? qh[s] : ql[s], sc[u % 2], xk, u < 2 ? xh : xl);
     refer(key0, false, cs, half);
     if (key0 + kPageT > n) cache_clean_v<DH>(vf, key0, n, half);
-    const float m = origin();
+    float sum = 0.0f;
 #pragma unroll
     for (int t = 0; t < 2; t++)
 #pragma unroll
@@ -354,13 +361,13 @@ struct CacheFast {
         float x[4];
 #pragma unroll
         for (int e = 0; e < 4; e++) {
-          x[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[t][4 * w + e], cs, -m));
-          lrun += x[e];
+          x[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[t][4 * w + e], cs, -ref));
+          sum += x[e];
         }
         ph[4 * t + w] = fp8_pack4(x[0], x[1], x[2], x[3]);
         pl[4 * t + w] = fp8_rest4(ph[4 * t + w], x[0], x[1], x[2], x[3]);
       }
-    scales();
+    scales(sum);
 #pragma unroll
     for (int t = 0; t < DT; t++) o[t] = mul(vf[t], ph, o[t], xv, eh);
 #pragma unroll
@@ -448,8 +455,7 @@ __device__ __forceinline__ void cache_store4(const CacheAttnArgs& p, size_t to, 
   }
 }
 
-// A wave's pages first, first + each, .. once more, by CacheTile; O, reference and sum to w,
-// whose unit is then the reference.
+// A wave's pages first, first + each, .. once more, by CacheTile; O, reference and sum to w.
 template <int DH>
 __device__ __forceinline__ void cache_again(CacheFast<DH>& w, const CacheAttnArgs& p, int b, int h,
                                             int first, int end, int each, int n, float cs,
@@ -477,7 +483,7 @@ __device__ __forceinline__ void cache_again(CacheFast<DH>& w, const CacheAttnArg
   }
 #pragma unroll
   for (int t = 0; t < DT; t++) w.o[t] = r.o[t];
-  w.mref = w.base = r.mref;
+  w.base = r.mref;
   w.lrun = r.lrun;
 }
 
@@ -541,15 +547,14 @@ __global__ __launch_bounds__(64 * kWaves, DH == 256 ? 1 : 2) void cache_attentio
     }
   }
 
-  if (__builtin_expect(__any(w.far), 0))
+  if (__builtin_expect(w.far != 0, 0))
     cache_again<DH>(w, p, b, h, first + wave, end, kWaves, n, cs, lane);
-  const float unit = w.unit();
 
   // join the waves: the columns' references and sums, then O in wave order
   {
     const float l = w.lrun + __shfl_xor(w.lrun, 32, 64);
     if (half == 0) {
-      s_m[wave][col] = w.mref;
+      s_m[wave][col] = w.base;
       s_l[wave][col] = l;
     }
   }
@@ -563,7 +568,7 @@ __global__ __launch_bounds__(64 * kWaves, DH == 256 ? 1 : 2) void cache_attentio
         for (int q4 = 0; q4 < 4; q4++) {
           v4f x;
 #pragma unroll
-          for (int e = 0; e < 4; e++) x[e] = w.o[t][q4 * 4 + e] * unit;
+          for (int e = 0; e < 4; e++) x[e] = w.o[t][q4 * 4 + e];
           *reinterpret_cast<v4f*>(&s_o[wave][col - j0][t * 32 + q4 * 8 + half * 4]) = x;
         }
     }
@@ -620,7 +625,7 @@ template <int DH>
 struct CachePipe : CacheFast<DH> {  // ph, pl, eh, el: P of the page before
   using Base = CacheFast<DH>;
   using Base::qh, Base::ql, Base::xh, Base::xl, Base::o, Base::sc, Base::ph, Base::pl, Base::eh,
-      Base::el, Base::lrun, Base::mul, Base::KS, Base::DT;
+      Base::el, Base::ref, Base::mul, Base::KS, Base::DT;
   static constexpr int NF = 2 * KS + DT;  // fragments of a page
 
   // fragment f of a page at its lane's place in LDS
@@ -653,9 +658,9 @@ struct CachePipe : CacheFast<DH> {  // ph, pl, eh, el: P of the page before
   template <int kFetch, typename Fetch>
   __device__ __forceinline__ void turn(const uint8_t* k, int xk, const uint8_t* v, int xv,
                                        float cs, Fetch&& fetch) {
-    const float m = Base::origin();
     v16f s[2] = {v16f{}, v16f{}};
     v8i nh, nl;
+    float sum = 0.0f;
     constexpr int kPairs = 16;
     // Two scores at a time, 68 cycles of VALU beside a product's 64. Each step waits
     // on the one before it, so three pairs are under way: the exponentials of pair j, the
@@ -679,8 +684,8 @@ struct CachePipe : CacheFast<DH> {  // ph, pl, eh, el: P of the page before
       }
       if (j >= 1 && j <= kPairs) {
         const int i = j - 1, w = i / 2, q = i % 3;
-        lrun += x[q];
-        lrun += y[q];
+        sum += x[q];
+        sum += y[q];
         int h = nh[w];
         if (i % 2 == 0) {
           asm("" : "=v"(h) : "v"(x[q]));
@@ -694,8 +699,8 @@ struct CachePipe : CacheFast<DH> {  // ph, pl, eh, el: P of the page before
       }
       if (j < kPairs) {
         const int e = 2 * j % 16, q = j % 3;
-        x[q] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[j / 8][e], cs, -m));
-        y[q] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[j / 8][e + 1], cs, -m));
+        x[q] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[j / 8][e], cs, -ref));
+        y[q] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[j / 8][e + 1], cs, -ref));
       }
 #endif
     };
@@ -721,8 +726,6 @@ struct CachePipe : CacheFast<DH> {  // ph, pl, eh, el: P of the page before
         for (int j = at * kFetch / NM; j < (at + 1) * kFetch / NM; j++) fetch(j);
 #pragma unroll
         for (int j = at * kPairs / NM; j < (at + 1) * kPairs / NM; j++) pair(j);
-        // one wave per SIMD: every two products keep the scores' work written beside them
-        if (DH == 256 && u % 2 == 1) __builtin_amdgcn_sched_barrier(0);
       }
       a0 = b0;
       a1 = b1;
@@ -731,7 +734,7 @@ struct CachePipe : CacheFast<DH> {  // ph, pl, eh, el: P of the page before
     pair(kPairs + 1);
     ph = nh;
     pl = nl;
-    Base::scales();
+    Base::scales(sum);
     sc[0] = s[0];
     sc[1] = s[1];
   }
@@ -902,9 +905,8 @@ __global__ __launch_bounds__(64 * CW * PG, DH == 256 ? 1 : 2) void cache_attenti
     }
   }
   __syncthreads();
-  if (__builtin_expect(active && __any(w.far), 0))
+  if (__builtin_expect(active && w.far != 0, 0))
     cache_again<DH>(w, p, b, h, first, min(end, limit), 1, n, cs, lane);
-  float unit = w.unit();
   float l = w.lrun + __shfl_xor(w.lrun, 32, 64);
   if constexpr (PG > 1) {
     // the second group's results to the first, lane by lane
@@ -918,19 +920,18 @@ __global__ __launch_bounds__(64 * CW * PG, DH == 256 ? 1 : 2) void cache_attenti
         for (int i = 0; i < 4; i++) {
           v4f x;
 #pragma unroll
-          for (int e = 0; e < 4; e++) x[e] = w.o[t][i * 4 + e] * unit;
+          for (int e = 0; e < 4; e++) x[e] = w.o[t][i * 4 + e];
           *reinterpret_cast<v4f*>(mine + (t * 4 + i) * 256) = x;
         }
-      top[col] = w.mref;
+      top[col] = w.base;
       top[kCols + col] = l;
     }
     __syncthreads();
     if (group == 1) return;
     if (active) {
-      const float m2 = top[col], l2 = top[kCols + col], to = fmaxf(w.mref, m2);
-      const float f = w.mref == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(w.mref - to);
+      const float m2 = top[col], l2 = top[kCols + col], to = fmaxf(w.base, m2);
+      const float f = w.base == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(w.base - to);
       const float f2 = m2 == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m2 - to);
-      unit *= f;
       l = l * f + l2 * f2;
 #pragma unroll
       for (int t = 0; t < DT; t++)
@@ -939,15 +940,14 @@ __global__ __launch_bounds__(64 * CW * PG, DH == 256 ? 1 : 2) void cache_attenti
           const v4f x = *reinterpret_cast<const v4f*>(mine + (t * 4 + i) * 256);
 #pragma unroll
           for (int e = 0; e < 4; e++)
-            w.o[t][i * 4 + e] = w.o[t][i * 4 + e] * unit + x[e] * f2;
+            w.o[t][i * 4 + e] = w.o[t][i * 4 + e] * f + x[e] * f2;
         }
-      unit = 1.0f;
-      w.mref = to;
+      w.base = to;
     }
   }
   if (!active) return;
 
-  const float inv = splits > 1 ? unit : l == 0.0f ? 0.0f : unit / l;
+  const float inv = splits > 1 ? 1.0f : l == 0.0f ? 0.0f : 1.0f / l;
   const size_t to = (size_t)(r0 + ct) * p.ldout + (h * G + c - ct * G) * DH;
   if (splits == 1 && p.out_bf16) {
     // A lane holds four consecutive values of its column at a time, its other half the next
@@ -991,7 +991,7 @@ __global__ __launch_bounds__(64 * CW * PG, DH == 256 ? 1 : 2) void cache_attenti
     const size_t u = ((size_t)b * p.cache.kv_heads + h) * tiles + tile;
     part = p.part + ((u * splits + split) * part_cols + col) * kPartRow<DH>;
     if (half == 0) {
-      part[DH] = w.mref;
+      part[DH] = w.base;
       part[DH + 1] = l;
     }
   } else {

@@ -48,3 +48,81 @@ def test_attention_beside_bytes_never_written(gpu_ctx, dh, batch, kv, nq, n, gon
         assert np.array_equal(got[:-nq], want[:-nq])
         F.check_attention(c, got[-nq:], val[-nq:], table[-1:, 1:], np.array([0, nq], I32),
                           lens[-1:] - 64, scale, False, 0, "bf16", False)
+
+
+# ---- GPU: weights far below a row's largest -----------------------------------------------
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dh,nq", [(64, 1), (128, 1), (256, 1), (64, 17), (128, 17), (256, 17),
+                                   (128, 200)])
+@pytest.mark.parametrize("below", [7.0, 10.0, 12.0, 14.0])
+@pytest.mark.parametrize("sinks,low,split", [([0], False, False), ([0, 2000], False, True),
+                                             ([4095], False, False), ([100], True, False),
+                                             ([100], True, True)])
+def test_attention_of_weights_that_are_small(gpu_ctx, dh, nq, below, sinks, low, split):
+    """A few keys hold nearly all of the weight and no value; thousands lie `below` nats under
+    them, with values of one sign, and are all of the result. low: 64 keys before them 96 nats
+    further down, so that the reference moves by more than 2^64.
+
+    Every score is a sum of two products that the matrix cores add exactly. A weight p is off by
+    half a step of its two codes: 2^-9 of itself, or 2^-21 of the largest weight that its column
+    has in its page. A page's products lose STEP of the largest (both codes of P: 1 + 2^-4). The
+    fp32 exponents, sums and rescales stay under 2^-15.
+    """
+    rng = np.random.default_rng(int(below) + nq + dh)
+    n = 4133 if split else 4096
+    heads = 2
+    pages, table, cu, blk, lens, slots = F.batch_of(rng, [n - nq], [nq])
+    c = O.Cache(pages, 1, dh)
+    k = np.zeros((n, 1, dh))
+    k[:, 0, dh - 3] = rng.integers(0, 5, n) / 4
+    v = rng.uniform(0.5, 1.5, (n, 1, dh))
+    if low:
+        k[:64, 0, 1] = -96.0
+    for s in sinks:
+        k[s, 0, 1], k[s, 0, dh - 3], v[s] = below, 0.0, 0.0
+    at = table[0, np.arange(n) // 64].astype(np.int64) * 64 + np.arange(n) % 64
+    c.append(k, v, np.array([0, n], I32), at)
+    kk, vv = c.rows(table[0], n)
+    assert (kk[:, 0, 1] == k[:, 0, 1]).all() and (kk[:, 0, dh - 3] == k[:, 0, dh - 3]).all()
+    q = np.zeros((nq, heads, dh))
+    q[:, :, 1] = q[:, :, dh - 3] = 1.0
+    got, _ = F.attend(gpu_ctx, c, q, "bf16", table, cu, lens, 1.0, False, 0, False,
+                      max_len=n if split else 64)
+    s = kk[:, 0, 1] + kk[:, 0, dh - 3]
+    p = np.exp(s - s.max())
+    p /= p.sum()
+    top = np.repeat(np.maximum.reduceat(p, np.arange(0, n, 64)), 64)[:n]
+    want = p @ vv[:, 0]
+    off = np.maximum(2.0 ** -9 * p, 2.0 ** -21 * top) @ np.abs(vv[:, 0])
+    drop = np.maximum.reduceat(p[:, None] * np.abs(vv[:, 0]), np.arange(0, n, 64), 0).sum(0)
+    tol = off + F.STEP * (1 + 2.0 ** -4) * drop + 2.0 ** -15 * want
+    assert (tol <= 2.0 ** -5 * want).all()  # it says something about the small weights
+    assert (np.abs(got - want) <= tol).all(), np.abs(got / want - 1).max()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dh,nq", [(64, 1), (128, 20), (256, 200)])
+@pytest.mark.parametrize("size", [20, 23, 24, 25, 26, 27, 28, 29, 60, 100])
+def test_attention_of_scores_of_any_size(gpu_ctx, dh, nq, size):
+    """Scores of 2^size and half of it, up and down from page to page: the keys of the larger
+    ones share the weight, each p the same number within 2^-9 of 1 / their count."""
+    rng = np.random.default_rng(size)
+    n = 64 * 9 + 11
+    pages, table, cu, blk, lens, slots = F.batch_of(rng, [max(0, n - nq)], [nq])
+    c = O.Cache(pages, 1, dh)
+    k = np.zeros((n, 1, dh))
+    one = rng.integers(0, 3, n) == 0
+    one[:64] = False  # the first page is far below the others
+    k[:, 0, 1] = np.where(one, 2.0, 1.0) * 2.0 ** (size // 2 - 1)
+    v = rng.standard_normal((n, 1, dh))
+    at = table[0, np.arange(n) // 64].astype(np.int64) * 64 + np.arange(n) % 64
+    c.append(k, v, np.array([0, n], I32), at)
+    kk, vv = c.rows(table[0], n)
+    assert (kk == k).all()
+    q = np.zeros((nq, 2, dh))
+    q[:, :, 1] = 2.0 ** (size - size // 2)
+    got, _ = F.attend(gpu_ctx, c, q, "bf16", table, cu, lens, 1.0, False, 0, False)
+    want, mag = vv[one, 0].mean(0), np.abs(vv[one, 0]).mean(0)
+    tol = (2.0 ** -9 + F.STEP * (1 + 2.0 ** -4)) * mag + 2.0 ** -20
+    assert (np.abs(got - want) <= tol).all()
