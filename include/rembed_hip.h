@@ -363,8 +363,8 @@ int rh_cache_plan(rh_context *ctx, const int32_t *past, const int32_t *fresh, in
  * becomes the larger of its own and the new tokens', and the codes kept are rescaled
  * (exact but for values that fall below e4m3's normal range). A token with an infinity
  * or NaN in a head's K or V is kept as K = NaN, V = 0 there: queries that see it get NaN,
- * others are not touched. Rows whose slot is negative or behind the last page are
- * skipped. */
+ * others are not touched. Blocks whose slots are negative or behind the last page are
+ * skipped, a request's others written. */
 int rh_cache_append(rh_context *ctx, const rh_kv_cache *cache, const void *kv, int kv_bf16,
                     int ldkv, int k_off, int v_off, const int32_t *cu, const int32_t *blocks,
                     const int64_t *slots, int batch, int rows);

@@ -289,9 +289,12 @@ __global__ __launch_bounds__(kAppendThreads) void cache_append_kernel(CacheAppen
   const int j = seg - p.blocks[b];
   const int r0 = p.cu[b], fresh = p.cu[b + 1] - r0;
   if (r0 < 0 || fresh <= 0 || r0 + (long long)fresh > p.rows) return;
-  const int64_t slot0 = p.slots[r0];
-  if (slot0 < 0) return;
-  const int off0 = (int)(slot0 % kPage);
+  // a row of this block, wherever in its first block the request starts
+  const int probe = j > (fresh - 1) / kPage ? fresh - 1 : j * kPage;
+  int64_t start = p.slots[r0];
+  const int64_t slot = p.slots[r0 + probe];
+  if (__builtin_expect(start < 0, 0)) start = slot - probe;  // the first block has no page
+  const int off0 = (int)(start & (kPage - 1));
   const int first = j == 0 ? 0 : j * kPage - off0;  // first new token of this block
   const int off = j == 0 ? off0 : 0;
   const int cnt = min(kPage - off, fresh - first);
@@ -315,7 +318,6 @@ __global__ __launch_bounds__(kAppendThreads) void cache_append_kernel(CacheAppen
       v[e] = *reinterpret_cast<const T*>(row + p.v_off + e * 4 * kStep);
     }
   }
-  const int64_t slot = p.slots[r0 + first];
   const bool here = slot >= 0 && slot / kPage < p.cache.pages;
   const size_t unit = here ? (size_t)(slot / kPage) * heads + h : 0;
   uint8_t* gk = p.cache.k + unit * kBytes;

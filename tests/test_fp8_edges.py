@@ -126,3 +126,32 @@ def test_attention_of_scores_of_any_size(gpu_ctx, dh, nq, size):
     want, mag = vv[one, 0].mean(0), np.abs(vv[one, 0]).mean(0)
     tol = (2.0 ** -9 + F.STEP * (1 + 2.0 ** -4)) * mag + 2.0 ** -20
     assert (np.abs(got - want) <= tol).all()
+
+
+# ---- GPU: rows without a page ---------------------------------------------------------------
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dh", [64, 256])
+@pytest.mark.parametrize("none", [-1, 1 << 20])
+def test_append_behind_a_page_that_is_none(gpu_ctx, dh, none):
+    """A block whose page is negative or behind the cache's last is skipped; the request's
+    other blocks are written, from its first row of theirs on."""
+    past, fresh = [10, 70, 63, 5, 0, 127], [54 + 64 + 9, 3, 1, 60, 130, 66]
+    rng = np.random.default_rng(dh)
+    heads, pages = 2, 16
+    table = np.full((6, 4), none, I32)
+    table[1, :2] = [0, 1]
+    free = rng.permutation(np.arange(2, pages)).astype(I32)
+    n = sum(fresh)
+    cu, blk, lens, slots, _, status = O.plan(past, fresh, free, table, n)
+    assert status[0] == 0
+    table[4, 1] = none  # a middle block of request 4 as well
+    first = int(cu[4])
+    slots[first + 64:first + 128] = -1 if none < 0 else none * 64 + np.arange(64)
+    c = O.Cache(pages, heads, dh)
+    dev = F.device_cache(gpu_ctx, c)
+    k, v = rng.standard_normal((2, n, heads, dh))
+    k, v = F.append(gpu_ctx, dev, k, v, "bf16", cu, blk, slots)
+    c.append(k, v, cu, slots)
+    assert (c.k_exp[table[0, 1]] != 200).all()  # the second block of request 0 was written
+    F.same_cache(dev, c)
