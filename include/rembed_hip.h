@@ -378,8 +378,8 @@ int rh_cache_append(rh_context *ctx, const rh_kv_cache *cache, const void *kv, i
  * that its query has in the same page; the sums are fp32. out is fp32
  * or bf16 [rows][ldout], head h at h*dh. A row that sees no key is 0; rows behind cu[batch]
  * are left as they are. Table entries that are no page of the cache hold no keys. max_q
- * must be >= every request's rows; max_len should be >= every lens (it only chooses how the
- * work is split). ldq and q_off multiples of 8, ldout of 4, q 16-byte, out 16-byte (bf16:
+ * should be >= every request's rows: those behind a request's first max_q are left as they
+ * are. max_len should be >= every lens (it only chooses how the work is split). ldq and q_off multiples of 8, ldout of 4, q 16-byte, out 16-byte (bf16:
  * 8-byte) aligned; scratch: rh_cache_attention_scratch bytes, 16-byte aligned. Fewer rows may
  * take more of it (their key ranges are split further): a buffer for calls of several sizes
  * holds the largest of theirs. */

@@ -500,7 +500,7 @@ constexpr int kPartRow = DH + 4;
 // cost registers. The waves' results are joined in LDS, eight columns at a time.
 template <int DH, bool BF16, bool STREAM>
 __global__ __launch_bounds__(64 * kWaves, DH == 256 ? 1 : 2) void cache_attention_kernel(
-    CacheAttnArgs p, int tiles, int splits, int part_cols) {
+    CacheAttnArgs p, int tiles, int splits, int max_cols) {
   constexpr int KS = DH / 64, DT = DH / 32, kStride = DH + 4, kHalf = kPageT * DH;
   constexpr int kJoin = 8;  // columns joined at a time
   __shared__ __attribute__((aligned(16))) float s_o[kWaves][kJoin][kStride];
@@ -509,7 +509,7 @@ __global__ __launch_bounds__(64 * kWaves, DH == 256 ? 1 : 2) void cache_attentio
   cache_unit(p, tiles, splits, b, h, tile, split);
   const int G = p.heads / p.cache.kv_heads;
   const int r0 = p.cu[b], nq = p.cu[b + 1] - r0;
-  const int cols = nq * G, c0 = tile * kCols;
+  const int cols = min(nq * G, max_cols), c0 = tile * kCols;
   if (c0 >= cols) return;
   const int n = max(0, min(p.lens[b], p.ldt * kPageT));
   const int lane = threadIdx.x & 63, col = lane & 31, half = lane >> 5;
@@ -592,7 +592,8 @@ __global__ __launch_bounds__(64 * kWaves, DH == 256 ? 1 : 2) void cache_attentio
       const int cc = c0 + j0 + r;
       if (splits > 1) {
         const size_t u = ((size_t)b * p.cache.kv_heads + h) * tiles + tile;
-        float* to = p.part + ((u * splits + split) * part_cols + j0 + r) * kPartRow<DH>;
+        float* to =
+            p.part + ((u * splits + split) * min(kCols, max_cols) + j0 + r) * kPartRow<DH>;
         *reinterpret_cast<v4f*>(to + d) = x;
         if (d == 0) {
           to[DH] = m;
@@ -742,7 +743,7 @@ struct CachePipe : CacheFast<DH> {  // ph, pl, eh, el: P of the page before
 
 template <int DH, bool BF16, int CW, int PG, int SLOTS>
 __global__ __launch_bounds__(64 * CW * PG, DH == 256 ? 1 : 2) void cache_attention_cols_kernel(
-    CacheAttnArgs p, int tiles, int splits, int part_cols) {
+    CacheAttnArgs p, int tiles, int splits, int max_cols) {
   constexpr int KS = DH / 64, DT = DH / 32, kHalf = kPageT * DH;  // bytes of K or V of a page
   constexpr int kRing = 2 * SLOTS * kHalf;  // a group's K pages, then its V pages
   constexpr int kJoin = PG > 1 ? CW * kCols * (DH + 2) * 4 : 0;
@@ -767,7 +768,7 @@ __global__ __launch_bounds__(64 * CW * PG, DH == 256 ? 1 : 2) void cache_attenti
   }
   const int G = p.heads / p.cache.kv_heads;
   const int r0 = p.cu[b], nq = p.cu[b + 1] - r0;
-  const int cols = nq * G;
+  const int cols = min(nq * G, max_cols);
   if (wg * CW * kCols >= cols) return;
   const int n = max(0, min(p.lens[b], p.ldt * kPageT));
   const int lane = threadIdx.x & 63, col = lane & 31, half = lane >> 5;
@@ -989,7 +990,7 @@ __global__ __launch_bounds__(64 * CW * PG, DH == 256 ? 1 : 2) void cache_attenti
   float* part = nullptr;
   if (splits > 1) {
     const size_t u = ((size_t)b * p.cache.kv_heads + h) * tiles + tile;
-    part = p.part + ((u * splits + split) * part_cols + col) * kPartRow<DH>;
+    part = p.part + ((u * splits + split) * kCols + col) * kPartRow<DH>;
     if (half == 0) {
       part[DH] = w.base;
       part[DH + 1] = l;
@@ -1011,14 +1012,15 @@ __global__ __launch_bounds__(64 * CW * PG, DH == 256 ? 1 : 2) void cache_attenti
 // Partial results of a tile's key ranges to its output rows, in range order.
 template <int DH>
 __global__ __launch_bounds__(256) void cache_join_kernel(CacheAttnArgs p, int tiles, int splits,
-                                                         int part_cols) {
+                                                         int max_cols) {
   constexpr int LPR = DH / 4;
   const int G = p.heads / p.cache.kv_heads;
   const int u = blockIdx.x;
   const int tile = u % tiles, h = u / tiles % p.cache.kv_heads, b = u / tiles / p.cache.kv_heads;
   const int r0 = p.cu[b], nq = p.cu[b + 1] - r0;
-  const int cols = nq * G, c0 = tile * kCols;
+  const int cols = min(nq * G, max_cols), c0 = tile * kCols;
   const int d = threadIdx.x % LPR * 4;
+  const int part_cols = min(kCols, max_cols);
   const size_t step = (size_t)part_cols * kPartRow<DH>;
   for (int rr = threadIdx.x / LPR; rr < min(kCols, cols - c0); rr += 256 / LPR) {
     const float* at = p.part + ((size_t)u * splits * part_cols + rr) * kPartRow<DH>;
@@ -1120,7 +1122,8 @@ static hipError_t launch_dh(const CacheAttnArgs& a, hipStream_t s) {
   cache_split(a.batch, a.max_q, a.max_len, a.heads, a.cache.kv_heads, DH, a.window, &per_wg,
               &splits);
   const int tiles = cache_tiles(a.max_q, a.heads, a.cache.kv_heads);
-  const int pc = cache_part_cols(a.max_q, a.heads, a.cache.kv_heads);
+  const int max_cols =
+      (int)std::min(0x7FFFFFFFLL, (long long)a.max_q * (a.heads / a.cache.kv_heads));
   const int units = a.batch * a.cache.kv_heads;
   const int wgs = (tiles + per_wg - 1) / per_wg;  // of a unit and key range
   const bool few = per_wg > 1 && wgs <= kFewTiles;
@@ -1130,16 +1133,16 @@ static hipError_t launch_dh(const CacheAttnArgs& a, hipStream_t s) {
 #define RH_ATTN(B)                                                                             \
   if (per_wg == 4)                                                                             \
     hipLaunchKernelGGL((cache_attention_cols_kernel<DH, B, 4, 1, 3>), grid, block, 0, s, a,    \
-                       tiles, splits, pc);                                                     \
+                       tiles, splits, max_cols);                                               \
   else if (per_wg == 2)                                                                        \
     hipLaunchKernelGGL((cache_attention_cols_kernel<DH, B, 2, 2, DH == 64 ? 3 : 2>), grid,     \
-                       block, 0, s, a, tiles, splits, pc);                                     \
+                       block, 0, s, a, tiles, splits, max_cols);                               \
   else if (cache_streams(a, cache_pages(a.max_q, a.max_len, a.window, kCols)))                 \
     hipLaunchKernelGGL((cache_attention_kernel<DH, B, true>), grid, block, 0, s, a, tiles,     \
-                       splits, pc);                                                            \
+                       splits, max_cols);                                                      \
   else                                                                                         \
     hipLaunchKernelGGL((cache_attention_kernel<DH, B, false>), grid, block, 0, s, a, tiles,    \
-                       splits, pc)
+                       splits, max_cols)
   if (a.in_bf16) {
     RH_ATTN(true);
   } else {
@@ -1148,7 +1151,7 @@ static hipError_t launch_dh(const CacheAttnArgs& a, hipStream_t s) {
 #undef RH_ATTN
   if (splits > 1)
     hipLaunchKernelGGL((cache_join_kernel<DH>), dim3(units * tiles), dim3(256), 0, s, a, tiles,
-                       splits, pc);
+                       splits, max_cols);
   return hipGetLastError();
 }
 

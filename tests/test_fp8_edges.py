@@ -155,3 +155,47 @@ def test_append_behind_a_page_that_is_none(gpu_ctx, dh, none):
     c.append(k, v, cu, slots)
     assert (c.k_exp[table[0, 1]] != 200).all()  # the second block of request 0 was written
     F.same_cache(dev, c)
+
+
+# ---- GPU: more rows than a call was told of -------------------------------------------------
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dh,heads,max_q,past", [
+    (64, 2, 2, 4000), (128, 4, 1, 4000), (256, 2, 3, 2000),  # few columns, key ranges split
+    (64, 2, 7, 200), (128, 2, 40, 4000), (256, 2, 70, 300)])
+def test_attention_of_more_rows_than_max_q(gpu_ctx, dh, heads, max_q, past):
+    """A request's first max_q rows are what they are in a call of that many rows' room; the
+    others, and the bytes behind the scratch, are left as they were."""
+    from rembed_amd import tensor as T
+    rng = np.random.default_rng(dh + max_q)
+    fresh = [max_q + 9, max_q, max_q + 90, 1]
+    pages, table, cu, blk, lens, slots = F.batch_of(rng, [past] * 4, fresh)
+    c = O.Cache(pages, 1, dh)
+    acu = np.concatenate([[0], np.cumsum(lens)]).astype(I32)
+    at = np.concatenate([table[b, np.arange(n) // 64].astype(np.int64) * 64 + np.arange(n) % 64
+                         for b, n in enumerate(lens)])
+    k, v = rng.standard_normal((2, len(at), 1, dh))
+    c.append(k, v, acu, at)
+    dev, scale = F.device_cache(gpu_ctx, c), dh ** -0.5
+    img, val = F.typed(rng.standard_normal((int(cu[-1]), heads * dh)), "bf16")
+    q = val.astype(np.float64).reshape(-1, heads, dh)
+    need = T.cache_attention_scratch(4, max_q, int(max(lens)), heads, 1, dh)
+    assert (need > 0) == (past > 1000)
+    scratch = gpu_ctx.upload(np.full(need + (1 << 20), 0x5A, np.uint8))
+    out = gpu_ctx.upload(np.full((int(cu[-1]), heads * dh), 55, np.float32))
+    T.CacheAttention(gpu_ctx, out, False, heads * dh, gpu_ctx.upload(img), True, heads * dh, 0, dev,
+                     gpu_ctx.upload(table), table.shape[1], gpu_ctx.upload(cu),
+                     gpu_ctx.upload(lens), 4, max_q, int(max(lens)), heads, scale, True, 0,
+                     scratch, need)
+    gpu_ctx.sync()
+    assert (scratch.download(np.uint8, (need + (1 << 20),))[need:] == 0x5A).all()
+    got = out.download(np.float32, (int(cu[-1]), heads * dh))
+    for b, n in enumerate(fresh):
+        first = slice(cu[b], cu[b] + min(n, max_q))
+        assert (got[first.stop:cu[b + 1]] == 55).all()
+        kk, vv = c.rows(table[b], int(lens[b]))
+        want, mag, top = O.attention(q[cu[b]:cu[b + 1]], kk, vv, scale, True, 0)
+        rows = first.stop - first.start
+        ds = scale * top * (dh / 64 * F.STEP * (1 + 2.0 ** -4))
+        tol = (F.BF16 + F.STEP * (1 + 2.0 ** -4) + 2 * ds) * mag[:rows] + 1e-6
+        assert (np.abs(got[first].reshape(rows, heads, dh) - want[:rows]) <= tol).all()
