@@ -306,8 +306,8 @@ int rh_quantize_rows_fp8(rh_context *ctx, const void *a, int a_bf16, int lda, in
 int rh_matmul_fp8(rh_context *ctx, void *dst, int dst_bf16, int ldd, const uint8_t *qa, int ldq,
                   const uint8_t *sa, const rh_weight *w, int m, int act);
 /* Both: a's rows become e4m3 in the scratch qa [m][ldq] and sa (whose contents
- * afterwards are unspecified), then rh_matmul_fp8. rh_linear does the same for fp32
- * rows through the context's workspace. */
+ * afterwards are unspecified), then rh_matmul_fp8; dst may lie on a. rh_linear does the
+ * same for fp32 rows through the context's workspace. */
 int rh_linear_fp8(rh_context *ctx, void *dst, int dst_bf16, int ldd, const void *a, int a_bf16,
                   int lda, const rh_weight *w, int m, int act, uint8_t *qa, int ldq, uint8_t *sa);
 

@@ -91,12 +91,27 @@ int export_fp8_scales(const rh_weight* w, float* scales, int32_t* colsum) {
   return RH_OK;
 }
 
+// Whether m rows of `wa` bytes, `sa` apart, share bytes with m rows of `wb`, `sb` apart. Rows of
+// one stride beside each other (columns of one buffer) do not; other strides go by their ranges.
+bool rows_overlap(const void* a, size_t wa, size_t sa, const void* b, size_t wb, size_t sb, int m) {
+  const uintptr_t x = (uintptr_t)a, y = (uintptr_t)b;
+  const size_t above = (size_t)(m - 1);
+  if (m <= 0 || x + above * sa + wa <= y || y + above * sb + wb <= x) return false;
+  if (sa != sb) return true;
+  const size_t off = y >= x ? (y - x) % sa : (sa - (x - y) % sa) % sa;  // b's rows in a's
+  return off < wa || off + wb > sa;
+}
+
 int run_linear_fp8(Context* ctx, const rh_weight* w, const void* a, int a_bf16, int lda, int m,
                    void* dst, int dst_bf16, int ldd, int act, const float* bias, uint8_t* qa,
                    int ldq, uint8_t* sa) {
   if (m <= 0) return RH_OK;
   const double M = m, K = w->k, N = w->n;
-  const bool direct = a && gemm_fp8_takes_rows(m, w->n, w->k, a, a_bf16, lda);
+  // Rows made e4m3 by the product's own workgroups are read while others of them store theirs:
+  // not where dst lies on them.
+  const size_t ea = a_bf16 ? 2 : 4, ed = dst_bf16 ? 2 : 4, cols = w->glu ? w->n / 2 : w->n;
+  const bool direct = a && gemm_fp8_takes_rows(m, w->n, w->k, a, a_bf16, lda) &&
+                      !rows_overlap(a, w->k * ea, lda * ea, dst, cols * ed, ldd * ed, m);
   if (a && !direct)
     RH_HIP(launch_quantize_rows_fp8(a, a_bf16, lda, m, w->k, qa, ldq, sa, ctx->stream));
   GemmFp8Args g{};

@@ -199,3 +199,55 @@ def test_attention_of_more_rows_than_max_q(gpu_ctx, dh, heads, max_q, past):
         ds = scale * top * (dh / 64 * F.STEP * (1 + 2.0 ** -4))
         tol = (F.BF16 + F.STEP * (1 + 2.0 ** -4) + 2 * ds) * mag[:rows] + 1e-6
         assert (np.abs(got[first].reshape(rows, heads, dh) - want[:rows]) <= tol).all()
+
+
+# ---- linears whose output lies on their rows ----------------------------------------------
+
+def test_rows_that_share_bytes():
+    import ctypes
+
+    from rembed_amd import _lib
+    f = ctypes.CDLL(_lib.LIB_PATH)._ZN2rh12rows_overlapEPKvmmS1_mmi
+    P, S = ctypes.c_void_p, ctypes.c_size_t
+    f.argtypes, f.restype = [P, S, S, P, S, S, ctypes.c_int], ctypes.c_bool
+
+    def brute(a, wa, sa, b, wb, sb, m):
+        rows = lambda x, w, s: {x + r * s + i for r in range(m) for i in range(w)}
+        return bool(rows(a, wa, sa) & rows(b, wb, sb))
+
+    rng = np.random.default_rng(0)
+    for _ in range(3000):
+        m, wa, wb = rng.integers(1, 5), rng.integers(1, 9), rng.integers(1, 9)
+        sa = sb = max(wa, wb) + int(rng.integers(0, 9))
+        a, b = (4096 + int(x) for x in rng.integers(0, 60, 2))
+        if rng.random() < 0.5:
+            sa, sb = wa + int(rng.integers(0, 9)), wb + int(rng.integers(0, 9))
+        want, got = brute(a, wa, sa, b, wb, sb, m), f(a, wa, sa, b, wb, sb, int(m))
+        # rows side by side exactly, others never too few
+        assert got == want if sa == sb and abs(b - a) < sa else got >= want
+    assert not f(4096, 8, 24, 4096 + 8, 16, 24, 9) and f(4096, 8, 24, 4096 + 7, 16, 24, 9)
+    assert not f(4096 + 16, 8, 24, 4096, 16, 24, 9) and f(4096, 8, 8, 4096, 8, 8, 9)
+    assert not f(4096, 8, 8, 4096, 8, 8, 0)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m,k,n", [(1, 4096, 4096), (16, 1024, 1024), (5, 3584, 3584), (40, 640, 640),
+                                   (64, 512, 512), (300, 768, 768)])
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_linear_over_its_own_rows(gpu_ctx, m, k, n, dtype):
+    """dst is a: the same bits as into a buffer of its own."""
+    from rembed_amd import tensor as T
+    rng = np.random.default_rng(m + k)
+    img, _ = F.typed(rng.standard_normal((m, k)), dtype)
+    pb = T.PackFP8(gpu_ctx, rng.standard_normal((n, k)).astype(np.float32), k, n)
+    bf, ldq = dtype == "bf16", T.ldq_fp8(k)
+    qa, sa = gpu_ctx.alloc(m * ldq), gpu_ctx.alloc(T.fp8_scale_bytes(m, k))
+    a, out = gpu_ctx.upload(img), gpu_ctx.alloc(img.nbytes)
+    T.LinearFP8(gpu_ctx, out, bf, n, a, bf, k, pb, m, 0, qa, ldq, sa)
+    want = out.download(img.dtype, (m, n))
+    T.LinearFP8(gpu_ctx, a, bf, n, a, bf, k, pb, m, 0, qa, ldq, sa)
+    assert np.array_equal(a.download(img.dtype, (m, n)), want)
+    if dtype == "f32":
+        a = gpu_ctx.upload(img)
+        T.Linear(gpu_ctx, a, a, pb, m)
+        assert np.array_equal(a.download(img.dtype, (m, n)), want)
