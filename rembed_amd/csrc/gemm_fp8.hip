@@ -79,7 +79,7 @@ __global__ __launch_bounds__(256) void quantize_rows_fp8_kernel(const void* a, i
 hipError_t launch_quantize_rows_fp8(const void* a, int a_bf16, int lda, int m, int k, uint8_t* qa,
                                     int ldq, uint8_t* sa, hipStream_t s) {
   if (m <= 0) return hipSuccess;
-  const int per_row = ceil_div(ldq, 512);
+  const int per_row = (ldq - 1) / 512 + 1;  // ldq may be the last multiple of 128 below 2^31
   const bool vec = k % 8 == 0 && lda % 8 == 0 && ((uintptr_t)a & 15) == 0;
   // a launch holds fewer than 2^32 threads
   const int each = std::max(1, (1 << 25) / per_row);

@@ -251,3 +251,28 @@ def test_linear_over_its_own_rows(gpu_ctx, m, k, n, dtype):
         a = gpu_ctx.upload(img)
         T.Linear(gpu_ctx, a, a, pb, m)
         assert np.array_equal(a.download(img.dtype, (m, n)), want)
+
+
+# ---- GPU: rows of nearly 2^31 values ---------------------------------------------------------
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("k", [0x7FFFFF00, 0x7FFFFF00 - 3, 0x7FFFFE00])
+def test_quantize_the_longest_rows(gpu_ctx, k):
+    """One bf16 row of up to the most values that a call takes: its last blocks."""
+    from rembed_amd import _lib
+    from rembed_amd import tensor as T
+    ldq, tail = T.ldq_fp8(k), 1000
+    rng = np.random.default_rng(1)
+    val, bits = F.bf16(rng.standard_normal(tail) * np.exp(rng.uniform(-4, 4, tail)))
+    a, qa = gpu_ctx.alloc(k * 2), gpu_ctx.alloc(ldq)
+    sa = gpu_ctx.alloc(T.fp8_scale_bytes(1, k))
+    _lib.check(_lib.lib.rh_memcpy_h2d(gpu_ctx.h, a.ptr + (k - tail) * 2, bits.ctypes.data, tail * 2))
+    T.QuantizeRowsFP8(gpu_ctx, a, True, k, 1, k, qa, ldq, sa)
+    codes, exps = np.empty(512, np.uint8), np.empty(4 * 128, np.uint8)
+    _lib.check(_lib.lib.rh_memcpy_d2h(gpu_ctx.h, codes.ctypes.data, qa.ptr + ldq - 512, 512))
+    _lib.check(_lib.lib.rh_memcpy_d2h(gpu_ctx.h, exps.ctypes.data, sa.ptr + ldq - 512, 512))
+    last = np.zeros(512)
+    last[:512 - (ldq - k)] = val[tail - (512 - (ldq - k)):]
+    want, e, _ = O.quantize_rows(last[None])
+    assert np.array_equal(exps.reshape(4, 128)[:, 0], e[0])
+    assert np.array_equal(O.CODES[codes], O.CODES[want[0]])
