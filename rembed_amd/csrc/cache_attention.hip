@@ -1099,11 +1099,12 @@ static void cache_split(int batch, int max_q, int max_len, int heads, int kv_hea
   *splits = cache_ranges(batch, max_q, heads, kv_heads, dh, *per_wg, pages);
 }
 
-// Few columns: pages past the L2 where all requests' could not stay in the memory's own 256 MiB
-// cache, so that each comes from memory. Below, texts that share pages find them (48 tokens over
-// 700 of which 640 are shared: 16.2 µs, past the L2 17.6).
-static bool cache_streams(const CacheAttnArgs& a, long long pages) {
-  return pages * kPageT * a.batch * a.cache.kv_heads * a.cache.dh * 2 > 256LL << 20;
+// Few columns: pages past the L2 where those of all requests, of which a cache of `pool` pages
+// has no more, could not stay in the memory's own 256 MiB cache. Below, texts that share pages
+// find them (512 queries of 4 tokens behind a shared 640: 71 µs, past the L2 80). An upper
+// estimate: texts that share, or are shorter than the longest, may read less from a large pool.
+bool cache_streams(long long pages, int batch, int pool, int kv_heads, int dh) {
+  return std::min(pages * batch, (long long)pool) * kPageT * kv_heads * dh * 2 > 256LL << 20;
 }
 
 // For any window: all pages, and four tiles, which never make fewer ranges than two.
@@ -1130,6 +1131,7 @@ static hipError_t launch_dh(const CacheAttnArgs& a, hipStream_t s) {
   const dim3 grid = few ? dim3((unsigned)units, (unsigned)wgs, (unsigned)splits)
                         : dim3((unsigned)(units * wgs * splits));
   const dim3 block(64 * kWaves);
+  const long long pages = cache_pages(a.max_q, a.max_len, a.window, kCols);
 #define RH_ATTN(B)                                                                             \
   if (per_wg == 4)                                                                             \
     hipLaunchKernelGGL((cache_attention_cols_kernel<DH, B, 4, 1, 3>), grid, block, 0, s, a,    \
@@ -1137,7 +1139,7 @@ static hipError_t launch_dh(const CacheAttnArgs& a, hipStream_t s) {
   else if (per_wg == 2)                                                                        \
     hipLaunchKernelGGL((cache_attention_cols_kernel<DH, B, 2, 2, DH == 64 ? 3 : 2>), grid,     \
                        block, 0, s, a, tiles, splits, max_cols);                               \
-  else if (cache_streams(a, cache_pages(a.max_q, a.max_len, a.window, kCols)))                 \
+  else if (cache_streams(pages, a.batch, a.cache.pages, a.cache.kv_heads, DH))                 \
     hipLaunchKernelGGL((cache_attention_kernel<DH, B, true>), grid, block, 0, s, a, tiles,     \
                        splits, max_cols);                                                      \
   else                                                                                         \

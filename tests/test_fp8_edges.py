@@ -276,3 +276,21 @@ def test_quantize_the_longest_rows(gpu_ctx, k):
     want, e, _ = O.quantize_rows(last[None])
     assert np.array_equal(exps.reshape(4, 128)[:, 0], e[0])
     assert np.array_equal(O.CODES[codes], O.CODES[want[0]])
+
+
+# ---- the rule that reads pages past the L2 --------------------------------------------------
+
+def test_pages_read_past_the_l2():
+    """Only where pages that exist, of at most all requests, exceed 256 MiB: texts behind a
+    shared beginning do not make them more than the cache holds."""
+    import ctypes
+
+    from rembed_amd import _lib
+    f = ctypes.CDLL(_lib.LIB_PATH)._ZN2rh13cache_streamsExiiii
+    f.argtypes, f.restype = [ctypes.c_longlong] + [ctypes.c_int] * 4, ctypes.c_bool
+    assert f(128, 48, 4000, 8, 128)            # 48 texts of up to 8192: 524 MB of pages
+    assert not f(11, 256, 266, 8, 128)         # 256 queries behind one prefix of ten pages
+    assert f(11, 256, 2816, 8, 128)            # each with ten of its own
+    page = 64 * 8 * 128 * 2
+    assert not f(1, 2 ** 28 // page, 1 << 20, 8, 128) and f(1, 2 ** 28 // page + 1, 1 << 20, 8, 128)
+    assert not f(2 ** 25, 2 ** 20, 0, 8, 128) and f(2 ** 25, 2 ** 20, 2 ** 31 - 1, 64, 256)
