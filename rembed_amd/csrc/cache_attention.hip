@@ -612,7 +612,7 @@ __global__ __launch_bounds__(64 * kWaves, DH == 256 ? 1 : 2) void cache_attentio
 // ---- many columns --------------------------------------------------------------------
 // CW waves of 32 columns each walk the same pages, PG such groups a part of them each. What
 // bounds it: a page's products take the matrix cores 64 cycles each (dh 128: 16 of them, 1024
-// cycles) and its softmax the VALU 1450, and a wave issues in order, so one after the other they
+// cycles) and its softmax the VALU 1390, and a wave issues in order, so one after the other they
 // cost their sum even with two waves per SIMD. The loop is a pipeline over pages whose body has no
 // branch: while page g's scores become P, two at a time, the products between them are
 // page g + 1's scores and page g - 1's values. K and V come to LDS by global_load_lds in
@@ -620,7 +620,7 @@ __global__ __launch_bounds__(64 * kWaves, DH == 256 ? 1 : 2) void cache_attentio
 // used (one turn where LDS has room for two pages only), with one barrier per turn. Where few
 // workgroups come together, a CU has one of them and a wave's own chain bounds a turn: then
 // two waves take two tiles, and two more the second half of the pages, joined in LDS.
-// 4096 rows over 8192 of 16 heads over 8 of dh 128 take 314 µs, 1.09 PFLOP/s of attention and
+// 4096 rows over 8192 of 16 heads over 8 of dh 128 take 305 µs, 1.13 PFLOP/s of attention and
 // twice that of e4m3 products, with the VALU busy 70% of the time and the matrix cores 50%.
 template <int DH>
 struct CachePipe : CacheFast<DH> {  // ph, pl, eh, el: P of the page before

@@ -7,7 +7,7 @@
 // e4m3's largest. Multiplying by a power of two is exact, so every code is the
 // e4m3 value nearest to its input and no scale is ever rounded; against a scale
 // of max / 448 a power of two costs nothing but up to one bit of the range below
-// the block's maximum (2^-15 of it is still a normal number). CDNA4's
+// the block's maximum (2^-13 of it is still a normal number). CDNA4's
 // v_mfma_scale_* takes these bytes as they are (E8M0), one for each row and 32 k.
 #pragma once
 
@@ -60,7 +60,7 @@ __device__ __forceinline__ void fp8_unpack4(int w, float (&v)[4]) {
 }
 // What four values (|v| <= 448) leave over after rounding to `codes`, times 16
 // and as e4m3 again: codes + 2^-4 * rest is v to 8 bits (exactly, where v has
-// no more than bf16's 8). 16 v - 16 code is exact, fused or not.
+// no more than bf16's 8) from 2^-6 on, off by up to 2^-14 below. 16 v - 16 code is exact, fused or not.
 __device__ __forceinline__ int fp8_rest4(int codes, float a, float b, float c, float d) {
 #if defined(__HIP_DEVICE_COMPILE__)
   const v2f lo = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(codes, 16.0f, false);
