@@ -294,3 +294,34 @@ def test_pages_read_past_the_l2():
     page = 64 * 8 * 128 * 2
     assert not f(1, 2 ** 28 // page, 1 << 20, 8, 128) and f(1, 2 ** 28 // page + 1, 1 << 20, 8, 128)
     assert not f(2 ** 25, 2 ** 20, 0, 8, 128) and f(2 ** 25, 2 ** 20, 2 ** 31 - 1, 64, 256)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dh", [64, 128, 256])
+@pytest.mark.parametrize("nq", [1, 5])
+def test_attention_over_a_cache_that_is_large(gpu_ctx, dh, nq):
+    """Few columns over a cache of more than 256 MiB, pages read past the L2, some of them shared,
+    from all over it; bytes that were never written lie between."""
+    from rembed_amd import tensor as T
+    rng = np.random.default_rng(dh + nq)
+    past, fresh, heads = [700, 64, 0, 1300], [nq, 1, nq, nq], 2
+    pages, table, cu, blk, lens, slots = F.batch_of(rng, past, fresh)
+    many = 2 ** 28 // (heads * 64 * dh * 2) + 100
+    where = rng.choice(many, pages, replace=False).astype(I32)
+    c, dev = O.Cache(pages, heads, dh), T.KVCache(gpu_ctx, many, heads, dh)
+    acu = np.concatenate([[0], np.cumsum(lens)]).astype(I32)
+    ablk = np.concatenate([[0], np.cumsum(-(-np.asarray(lens) // 64))]).astype(I32)
+    at = np.concatenate([table[b, np.arange(n) // 64].astype(np.int64) * 64 + np.arange(n) % 64
+                         for b, n in enumerate(lens)])
+    k, v = rng.standard_normal((2, len(at), heads, dh))
+    k, v = F.append(gpu_ctx, dev, k, v, "bf16", acu, ablk,
+                    where[at // 64].astype(np.int64) * 64 + at % 64)
+    c.append(k, v, acu, at)
+    table[1, 0] = table[0, 0]  # a shared page
+    dev.heads = heads
+    q = rng.standard_normal((int(cu[-1]), 4, dh))
+    for max_len in (int(max(lens)), 3_000_000):
+        for dtype, out_bf16 in (("bf16", True), ("f32", False)):
+            got, val = F.attend(gpu_ctx, dev, q, dtype, where[table], cu, lens, dh ** -0.5, True, 0,
+                                out_bf16, max_len=max_len)
+            F.check_attention(c, got, val, table, cu, lens, dh ** -0.5, True, 0, dtype, out_bf16)
