@@ -391,6 +391,119 @@ int rh_cache_attention(rh_context *ctx, const void *q, int q_bf16, int ldq, int 
                        float scale, int causal, int window, void *out, int out_bf16, int ldout,
                        void *scratch, size_t scratch_bytes);
 
+/* ---- rows between a layer's products ---------------------------------------------------
+ * What a decoder layer on the operators above runs around its linears and its attention.
+ * Like them, none of these calls allocates or waits (rh_rope_create apart), and each may be
+ * captured into a HIP graph. Arithmetic is fp32 on unrounded values, with one rounding where a
+ * value is stored; sums of squares are fp32, so values from 2^63 on overflow them. `used` may
+ * name a device integer (a plan's cu + batch, status + 1): rows from it on are left as they
+ * are; NULL: all rows are taken. An output may lie exactly on an input of its own type and
+ * stride, as said; other overlaps are refused. Rows and columns have no alignment beyond
+ * their type's unless said; 16-byte aligned rows of whole 16-byte groups are read faster. */
+
+/* A norm of rows or heads: v * weight / sqrt(mean(v^2) + eps) (RMSNorm, tensor.go:459-471), or
+ * (v - mean) * weight / sqrt(var + eps) + bias with the biased variance (LayerNorm,
+ * tensor.go:433-452). */
+#define RH_NORM_NONE 0
+#define RH_NORM_RMS 1
+#define RH_NORM_LAYER 2
+typedef struct {
+  int kind;
+  float eps;           /* >= 0 */
+  const float *weight; /* dev [n]; NULL: ones */
+  const float *bias;   /* dev [n], RH_NORM_LAYER only; NULL: zeros */
+} rh_norm;
+
+/* A block's end and the next one's beginning (Add and the norms around it, tensor.go:383-389;
+ * Gemma's norm sandwich, gemma3.go:357,376):
+ *   sum = x_scale * x + y_scale * gate * post(y),   out = pre(sum). */
+typedef struct {
+  rh_norm post;      /* of the block's output y; RH_NORM_NONE: as it is */
+  rh_norm pre;       /* of the sum; RH_NORM_NONE: out is the sum */
+  const float *gate; /* dev [n] (ldg 0) or [m][ldg]; NULL: ones */
+  int ldg;
+  float x_scale, y_scale; /* finite */
+} rh_residual;
+/* x [m][ldx], fp32 or bf16: the residual stream. y [m][ldy]: the block's output; NULL: sum =
+ * x_scale * x (post and gate then not given). sum (x's type, [m][ldsum]), out (fp32 or bf16,
+ * [m][ldout]) and qa / sa (out's e4m3 codes [m][ldq] and scale bytes as rh_quantize_rows_fp8
+ * makes them, from the fp32 values; qa 16-byte, sa 4-byte aligned) may each be NULL, not all;
+ * sum and out may lie on x or y. n <= 16384. */
+int rh_residual_norm(rh_context *ctx, const rh_residual *r, const void *x, int x_bf16, int ldx,
+                     const void *y, int y_bf16, int ldy, void *sum, int ldsum, void *out,
+                     int out_bf16, int ldout, uint8_t *qa, int ldq, uint8_t *sa, int m, int n,
+                     const int32_t *used);
+
+/* Rotary positions (the RoPE table and applyRoPE, modernbert.go:111-143). The leading `rot`
+ * values of a head are pairs, (i, i + rot/2) or (2i, 2i + 1), that turn by pos * f_i:
+ *   a' = amp * (a cos - b sin),  b' = amp * (b cos + a sin);  the rest of the head passes.
+ * f_i = theta^(-2i/rot) radians a position, scaled for texts longer than trained on:
+ *   LINEAR     f_i / factor
+ *   NTK        theta * factor^(rot / (rot - 2)) in theta's place
+ *   YARN       pairs that turn more than `fast` times (0: 32) in `original` positions stay, under
+ *              `slow` (0: 1) are / factor, between them a mean that is linear in i between the
+ *              whole i around those; amp = 0.1 ln(factor) + 1
+ *   WAVELENGTH the same with a mean linear in the turns themselves; fast 0: 4, slow 0: 1; amp 1
+ *   GIVEN      f_i = freq[i]
+ * Angles are exact to 2^-33 of a turn at every 32-bit position, negative ones turn back. */
+#define RH_ROPE_HALVES 0
+#define RH_ROPE_PAIRS 1
+#define RH_ROPE_PLAIN 0
+#define RH_ROPE_LINEAR 1
+#define RH_ROPE_NTK 2
+#define RH_ROPE_YARN 3
+#define RH_ROPE_WAVELENGTH 4
+#define RH_ROPE_GIVEN 5
+typedef struct {
+  int layout;
+  int rot;            /* even, 2..256 */
+  int scaling;
+  int original;       /* YARN, WAVELENGTH: positions trained on */
+  double theta;       /* > 1 (GIVEN: unused) */
+  double factor;      /* >= 1 */
+  double fast, slow;
+  double amp;         /* 0: the method's own */
+  const double *freq; /* GIVEN: host [rot/2], finite */
+} rh_rope_config;
+/* f_i [rot/2] and amp, on the host (either may be NULL). */
+int rh_rope_frequencies(const rh_rope_config *cfg, double *freq, double *amp);
+/* A turn's frequencies in HBM, used with the context that made it. */
+typedef struct rh_rope rh_rope;
+int rh_rope_create(rh_context *ctx, const rh_rope_config *cfg, rh_rope **out);
+void rh_rope_destroy(rh_rope *rope);
+
+/* q and k heads of fused rows [rows][ldx], fp32 or bf16, normed (RH_NORM_RMS without a bias;
+ * NULL: not) and turned at pos[row], to the same columns of out [rows][ldout] (fp32 or bf16; may
+ * be x itself). q head h starts at column q_off + h*dh, k head h at k_off + h*dh; heads or
+ * kv_heads may be 0. v_off >= 0: the kv_heads heads from there are copied as well (converted;
+ * with out on x they are left); -1: not. dh even, 2..256, rot <= dh. Replaces the QK-norm and
+ * RoPE loops of qwen3.go:483-505, gemma3.go:293-316. */
+int rh_rope_rows(rh_context *ctx, const rh_rope *rope, const void *x, int x_bf16, int ldx,
+                 void *out, int out_bf16, int ldout, int q_off, int k_off, int v_off, int heads,
+                 int kv_heads, int dh, const int32_t *pos, int rows, const rh_norm *q_norm,
+                 const rh_norm *k_norm, const int32_t *used);
+/* rh_rope_rows of fused q|k|v rows whose K and V go into the cache instead, as rh_cache_append
+ * puts them there (K's codes are those of the turned fp32 values; a token is kept as K = NaN, V =
+ * 0 where those or V are no numbers), q's heads to q [rows][ldq], head h at h*dh (fp32 or bf16;
+ * may be x + q_off with x's type and stride). heads may be 0. pos, cu, blocks and slots are a
+ * plan's; rows of q behind cu[batch] are left as they are. rot a multiple of 16; x and q 16-byte
+ * aligned, ldx, ldq and the offsets multiples of 8. */
+int rh_rope_append(rh_context *ctx, const rh_rope *rope, const rh_kv_cache *cache, const void *x,
+                   int x_bf16, int ldx, int q_off, int k_off, int v_off, void *q, int q_bf16,
+                   int ldq, int heads, const int32_t *pos, const int32_t *cu,
+                   const int32_t *blocks, const int64_t *slots, int batch, int rows,
+                   const rh_norm *q_norm, const rh_norm *k_norm);
+/* Tokens of the cache back as rows: those at positions first[b] .. of request b (first NULL: from
+ * 0) to rows cu[b] .. cu[b+1]-1 of out [rows][ldout], fp32 or bf16, kv head h of K at column k_off
+ * + h*dh, of V at v_off + h*dh: what rh_cache_append and rh_attention take. To move a beginning
+ * to other positions: read it, turn K by the difference, append it elsewhere. Values are what the
+ * codes stand for, exactly (bf16: below 2^-126 rounded). Positions without a page of the cache
+ * are zeros; rows behind cu[batch] are left as they are. out 16-byte aligned, ldout and the
+ * offsets multiples of 8. */
+int rh_cache_read(rh_context *ctx, const rh_kv_cache *cache, const int32_t *table, int ldt,
+                  const int32_t *cu, const int32_t *first, int batch, int rows, void *out,
+                  int out_bf16, int ldout, int k_off, int v_off);
+
 /* ---- encoder model ------------------------------------------------------------
  * Replaces model.Load + Model.Forward/ForwardTokens + the Embed batch loop
  * (internal/model/bert.go:307-524,649-731; rembed.go:287-411) with one

@@ -42,6 +42,10 @@ RH_CTX_F32_ALGO, RH_CTX_W8_TERMS, RH_CTX_I8_TILE, RH_CTX_BF_ALGO, RH_CTX_BF_TILE
 RH_CTX_TILE_GROUP = 6
 RH_NOALLOC_SCRATCH_BYTES = 64 * 1024 * 1024
 RH_CACHE_BLOCK = 64
+RH_NORM_NONE, RH_NORM_RMS, RH_NORM_LAYER = 0, 1, 2
+RH_ROPE_HALVES, RH_ROPE_PAIRS = 0, 1
+RH_ROPE_PLAIN, RH_ROPE_LINEAR, RH_ROPE_NTK, RH_ROPE_YARN, RH_ROPE_WAVELENGTH = 0, 1, 2, 3, 4
+RH_ROPE_GIVEN = 5
 
 # Symbols the header declares (checked by the CPU test suite).
 EXPORTS = [
@@ -56,7 +60,8 @@ EXPORTS = [
     "rh_linear_noalloc", "rh_gelu",
     "rh_layernorm", "rh_fp8_scale_bytes", "rh_quantize_rows_fp8", "rh_matmul_fp8",
     "rh_linear_fp8", "rh_cache_plan", "rh_cache_append", "rh_cache_attention_scratch",
-    "rh_cache_attention", "rh_model_create", "rh_model_set_tensor",
+    "rh_cache_attention", "rh_residual_norm", "rh_rope_frequencies", "rh_rope_create",
+    "rh_rope_destroy", "rh_rope_rows", "rh_rope_append", "rh_cache_read", "rh_model_create", "rh_model_set_tensor",
     "rh_model_finalize", "rh_model_share", "rh_model_destroy", "rh_model_set_option",
     "rh_model_quantized", "rh_model_quantized_activations", "rh_model_embed",
     "rh_model_embed_tokens", "rh_model_embed_device", "rh_model_check",
@@ -95,6 +100,27 @@ class KVCacheDesc(ctypes.Structure):
     _fields_ = [("pages", ctypes.c_int), ("kv_heads", ctypes.c_int), ("dh", ctypes.c_int),
                 ("reserved", ctypes.c_int), ("k", ctypes.c_void_p), ("v", ctypes.c_void_p),
                 ("k_exp", ctypes.c_void_p), ("v_exp", ctypes.c_void_p)]
+
+
+class NormDesc(ctypes.Structure):
+    """rh_norm."""
+    _fields_ = [("kind", ctypes.c_int), ("eps", ctypes.c_float), ("weight", ctypes.c_void_p),
+                ("bias", ctypes.c_void_p)]
+
+
+class ResidualDesc(ctypes.Structure):
+    """rh_residual."""
+    _fields_ = [("post", NormDesc), ("pre", NormDesc), ("gate", ctypes.c_void_p),
+                ("ldg", ctypes.c_int), ("x_scale", ctypes.c_float), ("y_scale", ctypes.c_float)]
+
+
+class RopeConfig(ctypes.Structure):
+    """rh_rope_config."""
+    _fields_ = [("layout", ctypes.c_int), ("rot", ctypes.c_int), ("scaling", ctypes.c_int),
+                ("original", ctypes.c_int), ("theta", ctypes.c_double),
+                ("factor", ctypes.c_double), ("fast", ctypes.c_double),
+                ("slow", ctypes.c_double), ("amp", ctypes.c_double),
+                ("freq", ctypes.c_void_p)]
 
 
 class ProfileStat(ctypes.Structure):
@@ -157,6 +183,17 @@ def _load():
         "rh_cache_attention_scratch": (S, [I, I, I, I, I, I]),
         "rh_cache_attention": (I, [P, P, I, I, I, ctypes.POINTER(KVCacheDesc), P, I, P, P, I, I,
                                    I, I, F, I, I, P, I, I, P, S]),
+        "rh_residual_norm": (I, [P, ctypes.POINTER(ResidualDesc), P, I, I, P, I, I, P, I, P, I, I,
+                                 P, I, P, I, I, P]),
+        "rh_rope_frequencies": (I, [ctypes.POINTER(RopeConfig), P, P]),
+        "rh_rope_create": (I, [P, ctypes.POINTER(RopeConfig), ctypes.POINTER(P)]),
+        "rh_rope_destroy": (None, [P]),
+        "rh_rope_rows": (I, [P, P, P, I, I, P, I, I, I, I, I, I, I, I, P, I,
+                             ctypes.POINTER(NormDesc), ctypes.POINTER(NormDesc), P]),
+        "rh_rope_append": (I, [P, P, ctypes.POINTER(KVCacheDesc), P, I, I, I, I, I, P, I, I, I, P,
+                               P, P, P, I, I, ctypes.POINTER(NormDesc),
+                               ctypes.POINTER(NormDesc)]),
+        "rh_cache_read": (I, [P, ctypes.POINTER(KVCacheDesc), P, I, P, P, I, I, P, I, I, I, I]),
         "rh_model_create": (I, [P, ctypes.POINTER(ModelConfig), I, ctypes.POINTER(P)]),
         "rh_model_set_tensor": (I, [P, ctypes.c_char_p, P, P, I]),
         "rh_model_finalize": (I, [P]),

@@ -11,7 +11,7 @@
 //      + (t%8/4 * 32 + d%32) * 16 + t%32/8 * 4 + t%4
 // so a wave's fragment load is 1 KiB of consecutive bytes, and V's tokens come in
 // the order in which the score tiles leave the matrix cores.
-#include "fp8.h"
+#include "rope_rows.h"
 
 #include <algorithm>
 #include <type_traits>
@@ -276,14 +276,16 @@ __device__ __forceinline__ int spread(int at) {
   return at ^ (at >> 9 & 1) << 6;
 }
 
-template <int DH, bool BF16>
-__global__ __launch_bounds__(kAppendThreads) void cache_append_kernel(CacheAppendArgs p) {
+// TURN: K's heads are normed and turned (rope.h) on the way, in fp32. Four lanes have a token
+// here too, each every fourth chunk of eight pairs.
+template <int DH, bool BF16, bool TURN>
+__device__ __forceinline__ void append_block(const CacheAppendArgs& p, const RopeArgs& rope,
+                                             unsigned block, uint8_t* s_k, uint8_t* s_v,
+                                             uint32_t (*s_max)[2]) {
   constexpr int kBytes = kPage * DH, E = DH / 4;  // a head's block; values per thread
-  __shared__ __attribute__((aligned(16))) uint8_t s_k[kBytes], s_v[kBytes];
-  __shared__ uint32_t s_max[kAppendThreads / 64][2];
   const int tid = threadIdx.x;
   const int heads = p.cache.kv_heads;
-  const int seg = blockIdx.x / heads, h = blockIdx.x % heads;
+  const int seg = block / heads, h = block % heads;
   const int b = append_request(p.blocks, p.batch, seg, tid & 63);
   if (seg >= p.blocks[p.batch]) return;
   const int j = seg - p.blocks[b];
@@ -307,15 +309,32 @@ __global__ __launch_bounds__(kAppendThreads) void cache_append_kernel(CacheAppen
   using T = std::conditional_t<BF16, v8bf, v4f>;  // 16 bytes of a row, widened when used
   constexpr int kStep = BF16 ? 8 : 4;
   T k[E / kStep], v[E / kStep];
+  float turned[TURN ? E / 16 : 1][2][8];
   uint32_t mk = 0, mv = 0;
+  const int row_at = r0 + first + tok - off;
+  int pos = 0;
   if (mine) {
-    const size_t at = (size_t)(r0 + first + tok - off) * p.ldkv + h * DH + quarter * kStep;
+    const size_t at = (size_t)row_at * p.ldkv + h * DH + quarter * kStep;
     using S = std::conditional_t<BF16, __bf16, float>;
     const S* row = static_cast<const S*>(p.kv) + at;
+    if constexpr (TURN) pos = rope.pos[row_at];
 #pragma unroll
     for (int e = 0; e < E / kStep; e++) {
-      k[e] = *reinterpret_cast<const T*>(row + p.k_off + e * 4 * kStep);
+      if constexpr (!TURN) k[e] = *reinterpret_cast<const T*>(row + p.k_off + e * 4 * kStep);
       v[e] = *reinterpret_cast<const T*>(row + p.v_off + e * 4 * kStep);
+    }
+  }
+  if constexpr (TURN) {
+#pragma unroll
+    for (int j = 0; j < E / 16; j++) {
+      const RopePlace<8> to(rope.turn, quarter + 4 * j);
+#pragma unroll
+      for (int i = 0; i < 8; i++) turned[j][0][i] = turned[j][1][i] = 0.0f;
+      if (mine) {
+        const size_t at = (size_t)row_at * p.ldkv + p.k_off + h * DH;
+        load_values<8, BF16>(p.kv, at + to.a, turned[j][0]);
+        load_values<8, BF16>(p.kv, at + to.b, turned[j][1]);
+      }
     }
   }
   const bool here = slot >= 0 && slot / kPage < p.cache.pages;
@@ -323,10 +342,58 @@ __global__ __launch_bounds__(kAppendThreads) void cache_append_kernel(CacheAppen
   uint8_t* gk = p.cache.k + unit * kBytes;
   uint8_t* gv = p.cache.v + unit * kBytes;
   const int ok = p.cache.k_exp[unit], ov = p.cache.v_exp[unit];
+  if constexpr (TURN) {
+    float inv = 0.0f;
+    if (rope.k_norm.on) {
+      float ss = 0.0f;
+#pragma unroll
+      for (int j = 0; j < E / 16; j++)
+#pragma unroll
+        for (int i = 0; i < 16; i++) ss += turned[j][i / 8][i % 8] * turned[j][i / 8][i % 8];
+#if defined(__HIP_DEVICE_COMPILE__)
+#define RH_ROR(n)                                                                                 \
+  ss += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(ss), 0x120 + n, 0xF, 0xF, true))
+      RH_ROR(4);  // the token's four lanes
+      RH_ROR(8);
+#undef RH_ROR
+#endif
+      inv = 1.0f / sqrtf(ss / (float)DH + rope.k_norm.eps);
+    }
+    if (mine) {
+#pragma unroll
+      for (int j = 0; j < E / 16; j++) {
+        const int chunk = quarter + 4 * j;
+        const RopePlace<8> to(rope.turn, chunk);
+        if (rope.k_norm.on) {
+#pragma unroll
+          for (int half = 0; half < 2; half++) {
+            const int d = half ? to.b : to.a;
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+              turned[j][half][i] *= inv;
+              if (rope.k_norm.weight) turned[j][half][i] *= rope.k_norm.weight[d + i];
+            }
+          }
+        }
+        if (to.turns) {
+          float c[8], sn[8];
+#pragma unroll
+          for (int i = 0; i < 8; i++)
+            turn_cos_sin(turn_at(rope.turn.freq[chunk * 8 + i], pos), rope.turn.amp, c[i], sn[i]);
+          rope_turn<8>(turned[j][0], turned[j][1], c, sn, rope.turn.halves);
+        }
+      }
+    }
+  }
+  // value e of the thread's of K
+  auto key = [&](int e) -> float {
+    if constexpr (TURN) return turned[e / 16][e / 8 % 2][e % 8];
+    else return (float)k[e / kStep][e % kStep];
+  };
   if (mine) {
 #pragma unroll
     for (int e = 0; e < E; e++) {
-      mk = max(mk, __float_as_uint((float)k[e / kStep][e % kStep]) & 0x7FFFFFFFu);
+      mk = max(mk, __float_as_uint(key(e)) & 0x7FFFFFFFu);
       mv = max(mv, __float_as_uint((float)v[e / kStep][e % kStep]) & 0x7FFFFFFFu);
     }
   }
@@ -392,10 +459,9 @@ __global__ __launch_bounds__(kAppendThreads) void cache_append_kernel(CacheAppen
     int wk[E / 4], wv[E / 4];
 #pragma unroll
     for (int e = 0; e < E; e += 4) {
-      const T x = k[e / kStep], y = v[e / kStep];
+      const T y = v[e / kStep];
       const int i = e % kStep;
-      wk[e / 4] = fp8_pack4((float)x[i] * fk, (float)x[i + 1] * fk, (float)x[i + 2] * fk,
-                            (float)x[i + 3] * fk);
+      wk[e / 4] = fp8_pack4(key(e) * fk, key(e + 1) * fk, key(e + 2) * fk, key(e + 3) * fk);
       wv[e / 4] = fp8_pack4((float)y[i] * fv, (float)y[i + 1] * fv, (float)y[i + 2] * fv,
                             (float)y[i + 3] * fv);
       if (bad) {
@@ -405,13 +471,19 @@ __global__ __launch_bounds__(kAppendThreads) void cache_append_kernel(CacheAppen
     }
     // value e of the thread lies at this one of the row
     auto place = [&](int e) { return (e / kStep * 4 + quarter) * kStep + e % kStep; };
-    typedef int W __attribute__((ext_vector_type(kStep / 4)));
+    constexpr int kRun = TURN ? 8 : kStep;  // values of K beside each other
+    typedef int W __attribute__((ext_vector_type(kRun / 4)));
 #pragma unroll
-    for (int e = 0; e < E; e += kStep) {
+    for (int e = 0; e < E; e += kRun) {
       W w;
 #pragma unroll
-      for (int i = 0; i < kStep / 4; i++) w[i] = wk[e / 4 + i];
-      *reinterpret_cast<W*>((whole_k ? s_k : gk) + k_at(tok, place(e))) = w;
+      for (int i = 0; i < kRun / 4; i++) w[i] = wk[e / 4 + i];
+      int d = place(e);
+      if constexpr (TURN) {
+        const RopePlace<8> to(rope.turn, quarter + e / 16 * 4);
+        d = e / 8 % 2 ? to.b : to.a;
+      }
+      *reinterpret_cast<W*>((whole_k ? s_k : gk) + k_at(tok, d)) = w;
     }
     if (few) {
 #pragma unroll
@@ -463,11 +535,65 @@ __global__ __launch_bounds__(kAppendThreads) void cache_append_kernel(CacheAppen
   }
 }
 
-hipError_t launch_cache_append(const CacheAppendArgs& a, hipStream_t s) {
-  // every touched block holds a new row, and each request has at most two
-  // partly new blocks
+template <int DH, bool BF16>
+__global__ __launch_bounds__(kAppendThreads) void cache_append_kernel(CacheAppendArgs p) {
+  __shared__ __attribute__((aligned(16))) uint8_t s_k[kPage * DH], s_v[kPage * DH];
+  __shared__ uint32_t s_max[kAppendThreads / 64][2];
+  append_block<DH, BF16, false>(p, RopeArgs{}, blockIdx.x, s_k, s_v, s_max);
+}
+
+// Workgroups for blocks of K and V, then ones for rows of q, which are shorter: one launch for
+// both, and K never as rows.
+template <int DH, bool BF16, bool OB>
+__global__ __launch_bounds__(kAppendThreads) void rope_append_kernel(CacheAppendArgs p,
+                                                                     RopeArgs rope,
+                                                                     unsigned blocks, int group) {
+  constexpr int P = BF16 ? 8 : 4;
+  __shared__ __attribute__((aligned(16))) uint8_t s_two[2 * kPage * DH];
+  __shared__ uint32_t s_max[kAppendThreads / 64][2];
+  static_assert((2 * kRopePairs + 2 * DH) * sizeof(float) <= sizeof s_two, "the turns' LDS");
+  static_assert(kAppendThreads == kRopeThreads, "workgroups of one size");
+  if (blockIdx.x < blocks)
+    append_block<DH, BF16, true>(p, rope, blockIdx.x, s_two, s_two + kPage * DH, s_max);
+  else
+    rope_rows<DH / 2 / P, P, BF16, OB>(rope, group, blockIdx.x - blocks, gridDim.x - blocks,
+                                       reinterpret_cast<float*>(s_two));
+}
+
+// Every touched block holds a new row, and each request has at most two partly new blocks.
+static long long append_blocks(const CacheAppendArgs& a) {
   const long long segs = std::min((long long)a.rows, (long long)a.rows / kPage + 2LL * a.batch);
-  const dim3 grid((unsigned)(segs * a.cache.kv_heads)), block(kAppendThreads);
+  return segs * a.cache.kv_heads;
+}
+
+hipError_t launch_rope_append(const CacheAppendArgs& a, const RopeArgs& rope, hipStream_t s) {
+  const unsigned blocks = (unsigned)append_blocks(a);
+  const int group = rope_group(rope, a.cache.dh / (a.in_bf16 ? 16 : 8));
+  const unsigned more = rope.heads ? ((unsigned)rope.rows + group - 1) / group : 0;
+  const dim3 grid(blocks + std::min(more, 1u << 20)), block(kAppendThreads);
+  if (grid.x == 0) return hipSuccess;
+#define RH_APPEND(D, X, O) \
+  hipLaunchKernelGGL((rope_append_kernel<D, X, O>), grid, block, 0, s, a, rope, blocks, group)
+#define RH_DIM(D)                             \
+  if (a.cache.dh == D) {                      \
+    if (a.in_bf16) {                          \
+      if (rope.out_bf16) RH_APPEND(D, true, true); \
+      else RH_APPEND(D, true, false);         \
+    } else {                                  \
+      if (rope.out_bf16) RH_APPEND(D, false, true); \
+      else RH_APPEND(D, false, false);        \
+    }                                         \
+  }
+  RH_DIM(64)
+  RH_DIM(128)
+  RH_DIM(256)
+#undef RH_DIM
+#undef RH_APPEND
+  return hipGetLastError();
+}
+
+hipError_t launch_cache_append(const CacheAppendArgs& a, hipStream_t s) {
+  const dim3 grid((unsigned)append_blocks(a)), block(kAppendThreads);
 #define RH_APPEND(D)                                                                          \
   if (a.cache.dh == D) {                                                                      \
     if (a.in_bf16) hipLaunchKernelGGL((cache_append_kernel<D, true>), grid, block, 0, s, a);  \
@@ -477,6 +603,129 @@ hipError_t launch_cache_append(const CacheAppendArgs& a, hipStream_t s) {
   RH_APPEND(128)
   RH_APPEND(256)
 #undef RH_APPEND
+  return hipGetLastError();
+}
+
+// ---- read back --------------------------------------------------------------------------
+// A workgroup takes one block of a request and one kv head: the block's tokens among
+// first[b] .. first[b] + count - 1 go to rows cu[b] + position - first[b]. K's 16-byte pieces are
+// runs of a token's values; V's are 16 tokens of one column, so its block goes through LDS
+// (16 more bytes behind every 128: a wave's words then meet all banks) and a thread takes
+// eight columns of four tokens. A code times its power of two is exact in fp32, and in bf16 from
+// its smallest normal value on.
+// Requests are found without a table of their blocks: request b starts at unit
+// cu[b] / 64 + 2 b, which leaves room for the blocks that its count can touch.
+__device__ __forceinline__ int read_unit(const int32_t* cu, int b) {
+  return (cu[b] >> 6) + 2 * b;
+}
+__device__ __forceinline__ int read_request(const int32_t* cu, int batch, int unit, int lane) {
+  int lo = 0, n = batch;  // as append_request
+  while (n > 1) {
+    const int step = (n + 63) / 64;
+    const int at = lo + lane * step;
+    const bool le = lane * step < n && read_unit(cu, at) <= unit;
+    const int k = __popcll(__ballot(le)) - 1;
+    lo += max(k, 0) * step;
+    n = min(step, n - max(k, 0) * step);
+  }
+  return lo;
+}
+__device__ __forceinline__ float fp8_power(int x) {  // 2^(x - 127)
+  return __uint_as_float(x ? (uint32_t)x << 23 : 0x400000u);
+}
+
+template <int DH, bool OB>
+__global__ __launch_bounds__(256) void cache_read_kernel(CacheReadArgs p) {
+  constexpr int kBytes = kPage * DH;
+  __shared__ __attribute__((aligned(16))) uint8_t s_v[kBytes / 8 * 9];
+  const int tid = threadIdx.x, heads = p.cache.kv_heads;
+  const int unit = blockIdx.x / heads, h = blockIdx.x % heads;
+  const int b = read_request(p.cu, p.batch, unit, tid & 63);
+  const int j = unit - read_unit(p.cu, b);
+  const int r0 = p.cu[b], count = p.cu[b + 1] - r0;
+  if (j < 0 || r0 < 0 || count <= 0 || (long long)r0 + count > p.rows) return;
+  const int first = p.first ? p.first[b] : 0;
+  const long long blk = (long long)(first >> 6) + j, last = (long long)first + count - 1;
+  if (blk > last >> 6) return;
+  const int lo = (int)max((long long)first - blk * kPage, 0LL);
+  const int hi = (int)min(last - blk * kPage, (long long)kPage - 1);
+  const size_t row0 = (size_t)((long long)r0 + blk * kPage - first);  // of the block's token 0
+  const int page = blk >= 0 && blk < p.ldt ? p.table[(size_t)b * p.ldt + blk] : -1;
+  const bool here = page >= 0 && page < p.cache.pages;
+  const size_t at = here ? (size_t)page * heads + h : 0;
+
+  constexpr int kChunks = DH / 8, kPieces = kBytes / 16 / 256;
+  constexpr int kLoads = kPage * kChunks / 256;  // eight values of K each
+  typedef int v2i __attribute__((ext_vector_type(2)));
+  v2i k[kLoads];
+  v4i v[kPieces];
+  float fk = 0.0f, fv = 0.0f;
+  if (here) {
+    const uint8_t* gk = p.cache.k + at * kBytes;
+    const uint8_t* gv = p.cache.v + at * kBytes;
+#pragma unroll
+    for (int i = 0; i < kPieces; i++)
+      v[i] = *reinterpret_cast<const v4i*>(gv + (tid + i * 256) * 16);
+#pragma unroll
+    for (int i = 0; i < kLoads; i++)
+      k[i] = *reinterpret_cast<const v2i*>(
+          gk + k_at(tid / kChunks + i * (256 / kChunks), tid % kChunks * 8));
+    fk = fp8_power(p.cache.k_exp[at]);
+    fv = fp8_power(p.cache.v_exp[at]);
+#pragma unroll
+    for (int i = 0; i < kPieces; i++) {
+      const int piece = tid + i * 256;
+      *reinterpret_cast<v4i*>(s_v + (piece + piece / 8) * 16) = v[i];
+    }
+  }
+  __syncthreads();
+  auto store = [&](int t, int col, const float (&x)[8]) {
+    if (t >= lo && t <= hi) store_values<8, OB>(p.out, (row0 + t) * p.ldout + col, x);
+  };
+#pragma unroll
+  for (int i = 0; i < kLoads; i++) {
+    const int t = tid / kChunks + i * (256 / kChunks), d = tid % kChunks * 8;
+    float x[8] = {};
+    if (here) {
+      float y[4];
+#pragma unroll
+      for (int w = 0; w < 2; w++) {
+        fp8_unpack4(k[i][w], y);
+#pragma unroll
+        for (int e = 0; e < 4; e++) x[4 * w + e] = y[e] * fk;
+      }
+    }
+    store(t, p.k_off + h * DH + d, x);
+  }
+  for (int task = tid; task < kChunks * (kPage / 4); task += 256) {
+    const int d = task % kChunks * 8, t0 = task / kChunks * 4;
+    float x[4][8] = {};
+    if (here) {
+#pragma unroll
+      for (int i = 0; i < 8; i++) {
+        const int byte = v_at(t0, d + i);
+        float y[4];
+        fp8_unpack4(*reinterpret_cast<const int*>(s_v + byte + byte / 128 * 16), y);
+#pragma unroll
+        for (int e = 0; e < 4; e++) x[e][i] = y[e] * fv;
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < 4; e++) store(t0 + e, p.v_off + h * DH + d, x[e]);
+  }
+}
+
+hipError_t launch_cache_read(const CacheReadArgs& a, hipStream_t s) {
+  const dim3 grid((unsigned)(((long long)a.rows / kPage + 2LL * a.batch) * a.cache.kv_heads));
+#define RH_READ(D)                                                                              \
+  if (a.cache.dh == D) {                                                                        \
+    if (a.out_bf16) hipLaunchKernelGGL((cache_read_kernel<D, true>), grid, dim3(256), 0, s, a); \
+    else hipLaunchKernelGGL((cache_read_kernel<D, false>), grid, dim3(256), 0, s, a);           \
+  }
+  RH_READ(64)
+  RH_READ(128)
+  RH_READ(256)
+#undef RH_READ
   return hipGetLastError();
 }
 

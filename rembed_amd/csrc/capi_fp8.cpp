@@ -162,7 +162,7 @@ static int check_fp8(const rh_context* ctx, const rh_weight* w, const void* dst,
   return RH_OK;
 }
 
-static int check_cache(const rh_kv_cache* c) {
+int check_cache(const rh_kv_cache* c) {
   if (!c) return fail(RH_ERR_INVALID, "null cache");
   if (c->dh != 64 && c->dh != 128 && c->dh != 256)
     return fail(RH_ERR_SHAPE, "cache head dim must be 64, 128 or 256");

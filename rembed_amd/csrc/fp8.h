@@ -141,6 +141,11 @@ bool gemm_fp8_takes_rows(int M, int N, int K, const void* a, int a_bf16, int lda
 hipError_t launch_gemm_fp8(const GemmFp8Args& a, const void* src, int src_bf16, int ld_src,
                            hipStream_t s);
 
+// ---- shared checks (capi_fp8.cpp) ------------------------------------------------------
+int check_cache(const rh_kv_cache* c);
+// Whether m rows of `wa` bytes, `sa` apart, share bytes with m rows of `wb`, `sb` apart.
+bool rows_overlap(const void* a, size_t wa, size_t sa, const void* b, size_t wb, size_t sb, int m);
+
 // ---- launchers (cache.hip, cache_attention.hip) ----------------------------------------
 struct CachePlanArgs {
   const int32_t *past, *fresh;

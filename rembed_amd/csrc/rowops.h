@@ -1,0 +1,204 @@
+// rowops.h — the row operators between a layer's products: residual norms, rotary turns of
+// heads, the paged cache read back; and what the kernels that turn heads share.
+//
+// A pair (a, b) of a head's values at position t turns by t times its frequency f:
+//   a' = m (a cos(t f) - b sin(t f)),   b' = m (b cos(t f) + a sin(t f)).
+// Positions are whole numbers, so whole turns of f drop out: f is kept as a 64-bit fraction of a
+// turn, t f mod 1 is a product mod 2^64, exact but for f's own rounding (2^-65 of a turn a
+// position; 2^-34 at 2^31), and no table limits how long a text is. fp32 angles would be off
+// by 2^-24 of the angle itself: 0.004 rad at position 65536.
+#pragma once
+
+#include "fp8.h"
+
+namespace rh {
+
+// Sums over groups of L consecutive lanes, every lane of a group getting its sum. All lanes of
+// the wave have to be active.
+template <int L>
+__device__ __forceinline__ float group_sum(float v) {
+#if defined(__HIP_DEVICE_COMPILE__)
+#define RH_DPP(ctrl) \
+  v += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), ctrl, 0xF, 0xF, true))
+  if constexpr (L >= 2) RH_DPP(0xB1);   // quad_perm [1, 0, 3, 2]
+  if constexpr (L >= 4) RH_DPP(0x4E);   // quad_perm [2, 3, 0, 1]
+  if constexpr (L >= 8) RH_DPP(0x141);  // row_half_mirror: the other quad, whose lanes are equal
+  if constexpr (L >= 16) RH_DPP(0x128);  // row_ror:8
+#undef RH_DPP
+  typedef unsigned v2u __attribute__((ext_vector_type(2)));
+  if constexpr (L >= 32) {
+    const unsigned u = __float_as_uint(v);
+    const v2u r = __builtin_bit_cast(v2u, __builtin_amdgcn_permlane16_swap(u, u, false, false));
+    v = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+  }
+  if constexpr (L >= 64) {
+    const unsigned u = __float_as_uint(v);
+    const v2u r = __builtin_bit_cast(v2u, __builtin_amdgcn_permlane32_swap(u, u, false, false));
+    v = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+  }
+#endif
+  return v;
+}
+
+// Eight (N) consecutive values of fp32 or bf16 rows, 16-byte aligned, and back.
+template <int N, bool BF16>
+__device__ __forceinline__ void load_values(const void* base, size_t at, float (&v)[N]) {
+  static_assert(BF16 ? N % 8 == 0 : N % 4 == 0, "whole 16-byte loads");
+  if constexpr (BF16) {
+#pragma unroll
+    for (int j = 0; j < N; j += 8) {
+      const v8bf x = *reinterpret_cast<const v8bf*>(static_cast<const __bf16*>(base) + at + j);
+#pragma unroll
+      for (int e = 0; e < 8; e++) v[j + e] = (float)x[e];
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < N; j += 4) {
+      const v4f x = *reinterpret_cast<const v4f*>(static_cast<const float*>(base) + at + j);
+#pragma unroll
+      for (int e = 0; e < 4; e++) v[j + e] = x[e];
+    }
+  }
+}
+template <int N, bool BF16>
+__device__ __forceinline__ void store_values(void* base, size_t at, const float (&v)[N]) {
+  if constexpr (BF16) {
+    constexpr int W = N < 8 ? N : 8;
+    typedef __bf16 T __attribute__((ext_vector_type(W)));
+#pragma unroll
+    for (int j = 0; j < N; j += W) {
+      T x;
+#pragma unroll
+      for (int e = 0; e < W; e++) x[e] = (__bf16)v[j + e];
+      *reinterpret_cast<T*>(static_cast<__bf16*>(base) + at + j) = x;
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < N; j += 4)
+      *reinterpret_cast<v4f*>(static_cast<float*>(base) + at + j) =
+          (v4f){v[j], v[j + 1], v[j + 2], v[j + 3]};
+  }
+}
+
+// ---- the turn ---------------------------------------------------------------------------
+struct RopeTurn {
+  const uint64_t* freq;  // [pairs] 2^64 times the turns a position
+  int pairs;             // rot / 2: the head's leading 2 * pairs values turn
+  int halves;            // pair i is (i, i + pairs); else (2i, 2i + 1)
+  float amp;             // cos and sin are multiplied by it
+};
+// The 32-bit fraction of a turn at position t.
+__device__ __forceinline__ uint32_t turn_at(uint64_t freq, int t) {
+  const uint32_t lo = (uint32_t)freq, hi = (uint32_t)(freq >> 32), u = (uint32_t)t;
+  return __umulhi(u, lo) + u * hi - (t < 0 ? lo : 0u);
+}
+// cos and sin of a fraction of a turn: its distance from the nearest quarter (at most pi / 4) by
+// Taylor's polynomials (rests under 2e-9 and 2e-10), off by at most 1.5e-7 with the roundings.
+__device__ __forceinline__ void turn_cos_sin(uint32_t turn, float amp, float& c, float& s) {
+  const uint32_t q = (turn + 0x20000000u) >> 30;
+  const float x = (float)(int)(turn - (q << 30)) * 1.46291807926715968e-9f;  // 2 pi / 2^32
+  const float x2 = x * x;
+  float u = __builtin_fmaf(x2, 1.0f / 362880, -1.0f / 5040);
+  u = __builtin_fmaf(x2, u, 1.0f / 120);
+  u = __builtin_fmaf(x2, u, -1.0f / 6);
+  const float sn = __builtin_fmaf(x * x2, u, x);
+  float w = __builtin_fmaf(x2, -1.0f / 3628800, 1.0f / 40320);
+  w = __builtin_fmaf(x2, w, -1.0f / 720);
+  w = __builtin_fmaf(x2, w, 1.0f / 24);
+  w = __builtin_fmaf(x2, w, -0.5f);
+  const float cs = __builtin_fmaf(x2, w, 1.0f);
+  // quarters 0..3: (c, s), (-s, c), (-c, -s), (s, -c)
+  const float a = q & 1 ? sn : cs, b = q & 1 ? cs : sn;
+  c = ((q + 1) & 2 ? -a : a) * amp;
+  s = (q & 2 ? -b : b) * amp;
+}
+
+// Where chunk l of P pairs of a head lies: its two runs of P values. Behind the pairs that turn
+// a chunk is 2 P consecutive values, of either layout.
+template <int P>
+struct RopePlace {
+  int a, b;
+  bool turns;
+  __device__ __forceinline__ RopePlace(const RopeTurn& t, int l) {
+    turns = l * P < t.pairs;
+    const bool apart = turns && t.halves;
+    a = apart ? l * P : 2 * l * P;
+    b = apart ? l * P + t.pairs : 2 * l * P + P;
+  }
+};
+// The chunk's pairs turned by c and s.
+template <int P>
+__device__ __forceinline__ void rope_turn(float (&a)[P], float (&b)[P], const float (&c)[P],
+                                          const float (&s)[P], bool halves) {
+  if (halves) {
+#pragma unroll
+    for (int i = 0; i < P; i++) {
+      const float x = a[i], y = b[i];
+      a[i] = __builtin_fmaf(x, c[i], -(y * s[i]));
+      b[i] = __builtin_fmaf(y, c[i], x * s[i]);
+    }
+  } else {
+    auto at = [&](int e) -> float& { return e < P ? a[e] : b[e - P]; };
+#pragma unroll
+    for (int i = 0; i < P; i++) {
+      const float x = at(2 * i), y = at(2 * i + 1);
+      at(2 * i) = __builtin_fmaf(x, c[i], -(y * s[i]));
+      at(2 * i + 1) = __builtin_fmaf(y, c[i], x * s[i]);
+    }
+  }
+}
+
+// ---- launchers ----------------------------------------------------------------------------
+struct HeadNorm {  // RMS norm of a head's values
+  int on;
+  float eps;
+  const float* weight;  // [dh] or null: ones
+};
+struct RopeArgs {
+  RopeTurn turn;
+  const void* x;
+  void* out;
+  int x_bf16, ldx, out_bf16, ldout;
+  int q_off, k_off, v_off;     // columns in x
+  int q_out, k_out, v_out;     // and in out
+  int heads, kv_heads, v_heads, dh;  // v_heads: kv heads that are copied, or 0
+  HeadNorm q_norm, k_norm;
+  const int32_t* pos;
+  const int32_t* used;  // null: all rows
+  int rows;
+};
+hipError_t launch_rope_rows(const RopeArgs& a, hipStream_t s);
+// The append with K's heads normed and turned on the way (append.kv: the q|k|v rows), and q's heads
+// as rows (rope: x, q_off, heads; rows behind cu[batch] are left as they are).
+hipError_t launch_rope_append(const CacheAppendArgs& append, const RopeArgs& rope, hipStream_t s);
+
+struct CacheReadArgs {
+  rh_kv_cache cache;
+  const int32_t* table;
+  int ldt;
+  const int32_t *cu, *first;  // first may be null: zeros
+  int batch, rows;
+  void* out;
+  int out_bf16, ldout, k_off, v_off;
+};
+hipError_t launch_cache_read(const CacheReadArgs& a, hipStream_t s);
+
+struct ResidualArgs {
+  const void* x;
+  const void* y;    // null: x alone
+  void* sum;        // x's type; null: not stored
+  void* out;        // null: not stored
+  int x_bf16, ldx, y_bf16, ldy, ldsum, out_bf16, ldout;
+  uint8_t* qa;      // e4m3 codes of out; null: none
+  uint8_t* sa;
+  int ldq;
+  rh_norm post, pre;
+  const float* gate;  // null: ones
+  int ldg;            // 0: one row for all
+  float x_scale, y_scale;
+  const int32_t* used;
+  int m, n;
+};
+hipError_t launch_residual_norm(const ResidualArgs& a, hipStream_t s);
+
+}  // namespace rh

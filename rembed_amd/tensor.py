@@ -339,6 +339,112 @@ def CacheAttention(ctx, out, out_bf16, ldout, q, q_bf16, ldq, q_off, cache, tabl
                                  _ptr(scratch), scratch_bytes))
 
 
+# ---- rows between a layer's products --------------------------------------------
+
+class Norm:
+    """A norm of rows or heads (rh_norm): RMS, or with layer=True a layer norm. weight and
+    bias: device buffers of fp32, None for ones and zeros."""
+
+    def __init__(self, weight=None, eps=1e-6, bias=None, layer=False):
+        self.weight, self.bias = weight, bias  # kept alive
+        self.desc = _lib.NormDesc(_lib.RH_NORM_LAYER if layer else _lib.RH_NORM_RMS, eps,
+                                  _ptr(weight), _ptr(bias))
+
+
+def _norm_desc(norm):
+    return None if norm is None else norm.desc
+
+
+class Residual:
+    """A block's end and the next one's beginning (rh_residual): sum = x_scale * x +
+    y_scale * gate * post(y), out = pre(sum). gate: fp32 [n], or [m][ldg] with ldg > 0."""
+
+    def __init__(self, post=None, pre=None, gate=None, ldg=0, x_scale=1.0, y_scale=1.0):
+        self.post, self.pre, self.gate = post, pre, gate  # kept alive
+        none = _lib.NormDesc()
+        self.desc = _lib.ResidualDesc(_norm_desc(post) or none, _norm_desc(pre) or none,
+                                      _ptr(gate), ldg, x_scale, y_scale)
+
+
+def ResidualNorm(ctx, res, x, x_bf16, ldx, y, y_bf16, ldy, total, ldsum, out, out_bf16, ldout, qa,
+                 ldq, sa, m, n, used=None):
+    """Residual sum and norms of rows, to rows and / or e4m3 codes (rh_residual_norm); y, total,
+    out, qa with sa, and used may be None."""
+    check(lib.rh_residual_norm(ctx.h, res.desc, x.ptr, x_bf16, ldx, _ptr(y), y_bf16, ldy,
+                               _ptr(total), ldsum, _ptr(out), out_bf16, ldout, _ptr(qa), ldq,
+                               _ptr(sa), m, n, _ptr(used)))
+
+
+def _rope_config(rot, theta, layout, scaling, factor, original, fast, slow, amp, freq):
+    f = None if freq is None else np.ascontiguousarray(freq, dtype=np.float64)
+    if f is not None and f.size != rot // 2:
+        raise _lib.RembedError(_lib.RH_ERR_SHAPE, f"freq has {f.size} values, want {rot // 2}")
+    cfg = _lib.RopeConfig(layout, rot, scaling, original, theta, factor, fast, slow, amp,
+                          None if f is None else f.ctypes.data)
+    return cfg, f
+
+
+def rope_frequencies(rot, theta=10000.0, scaling=_lib.RH_ROPE_PLAIN, factor=1.0, original=0,
+                     fast=0.0, slow=0.0, amp=0.0, freq=None):
+    """Radians a position of each pair, and what cosines and sines are multiplied by, on the
+    host (rh_rope_frequencies)."""
+    cfg, held = _rope_config(rot, theta, 0, scaling, factor, original, fast, slow, amp, freq)
+    f, a = np.empty(max(rot, 0) // 2), ctypes.c_double()
+    check(lib.rh_rope_frequencies(cfg, f.ctypes.data, ctypes.addressof(a)))
+    return f, a.value
+
+
+class Rope:
+    """Rotary positions of a head's leading `rot` values (rh_rope): pairs of halves
+    (RH_ROPE_HALVES) or of neighbours (RH_ROPE_PAIRS), frequencies plain or scaled."""
+
+    def __init__(self, ctx, rot, theta=10000.0, layout=_lib.RH_ROPE_HALVES,
+                 scaling=_lib.RH_ROPE_PLAIN, factor=1.0, original=0, fast=0.0, slow=0.0, amp=0.0,
+                 freq=None):
+        cfg, held = _rope_config(rot, theta, layout, scaling, factor, original, fast, slow, amp,
+                                 freq)
+        h = ctypes.c_void_p()
+        check(lib.rh_rope_create(ctx.h, cfg, ctypes.byref(h)))
+        self.ctx, self.h, self.rot = ctx, h, rot
+
+    def close(self):
+        if self.h:
+            lib.rh_rope_destroy(self.h)
+            self.h = None
+
+    def __del__(self):
+        if sys.is_finalizing():
+            return  # the HIP runtime may already be torn down
+        try:
+            self.close()
+        except Exception:
+            pass
+
+
+def RopeRows(ctx, rope, x, x_bf16, ldx, out, out_bf16, ldout, q_off, k_off, v_off, heads,
+             kv_heads, dh, pos, rows, q_norm=None, k_norm=None, used=None):
+    """q and k heads of fused rows normed and turned (rh_rope_rows); v_off >= 0: v's heads
+    copied too."""
+    check(lib.rh_rope_rows(ctx.h, rope.h, x.ptr, x_bf16, ldx, out.ptr, out_bf16, ldout, q_off,
+                           k_off, v_off, heads, kv_heads, dh, pos.ptr, rows, _norm_desc(q_norm),
+                           _norm_desc(k_norm), _ptr(used)))
+
+
+def RopeAppend(ctx, rope, cache, x, x_bf16, ldx, q_off, k_off, v_off, q, q_bf16, ldq, heads, pos,
+               cu, blocks, slots, batch, rows, q_norm=None, k_norm=None):
+    """q heads normed and turned to rows, K and V of the same rows into the cache
+    (rh_rope_append)."""
+    check(lib.rh_rope_append(ctx.h, rope.h, cache.desc, x.ptr, x_bf16, ldx, q_off, k_off, v_off,
+                             _ptr(q), q_bf16, ldq, heads, pos.ptr, cu.ptr, blocks.ptr, slots.ptr,
+                             batch, rows, _norm_desc(q_norm), _norm_desc(k_norm)))
+
+
+def CacheRead(ctx, cache, table, ldt, cu, first, batch, rows, out, out_bf16, ldout, k_off, v_off):
+    """Tokens of the cache back as rows of K and V (rh_cache_read); first None: from 0."""
+    check(lib.rh_cache_read(ctx.h, cache.desc, table.ptr, ldt, cu.ptr, _ptr(first), batch, rows,
+                            out.ptr, out_bf16, ldout, k_off, v_off))
+
+
 # ---- host-array conveniences used by tests and the bench -----------------------
 
 def matmul_host(ctx, a, pb, act=None):
