@@ -276,12 +276,19 @@ __device__ __forceinline__ int spread(int at) {
   return at ^ (at >> 9 & 1) << 6;
 }
 
+// What a turning workgroup holds of K's norm and, of few tokens, their cosines and sines: those
+// are then made by all threads rather than by the tokens' own four.
+struct AppendTurn {
+  static constexpr int kPairs = 256;
+  float w[256], c[kPairs], s[kPairs];
+};
+
 // TURN: K's heads are normed and turned (rope.h) on the way, in fp32. Four lanes have a token
 // here too, each every fourth chunk of eight pairs.
 template <int DH, bool BF16, bool TURN>
 __device__ __forceinline__ void append_block(const CacheAppendArgs& p, const RopeArgs& rope,
                                              unsigned block, uint8_t* s_k, uint8_t* s_v,
-                                             uint32_t (*s_max)[2]) {
+                                             uint32_t (*s_max)[2], AppendTurn* s_turn) {
   constexpr int kBytes = kPage * DH, E = DH / 4;  // a head's block; values per thread
   const int tid = threadIdx.x;
   const int heads = p.cache.kv_heads;
@@ -324,18 +331,31 @@ __device__ __forceinline__ void append_block(const CacheAppendArgs& p, const Rop
       v[e] = *reinterpret_cast<const T*>(row + p.v_off + e * 4 * kStep);
     }
   }
+  constexpr int kRaw = BF16 ? 1 : 2;  // 16 bytes each, of eight values
+  v4i raw[TURN ? E / 16 : 1][2][kRaw];
+  bool few_turns = false;
   if constexpr (TURN) {
+    if (mine) {
+      using S = std::conditional_t<BF16, __bf16, float>;
+      const S* x = static_cast<const S*>(p.kv) + (size_t)row_at * p.ldkv + p.k_off + h * DH;
 #pragma unroll
-    for (int j = 0; j < E / 16; j++) {
-      const RopePlace<8> to(rope.turn, quarter + 4 * j);
+      for (int j = 0; j < E / 16; j++) {
+        const RopePlace<8> to(rope.turn, quarter + 4 * j);
 #pragma unroll
-      for (int i = 0; i < 8; i++) turned[j][0][i] = turned[j][1][i] = 0.0f;
-      if (mine) {
-        const size_t at = (size_t)row_at * p.ldkv + p.k_off + h * DH;
-        load_values<8, BF16>(p.kv, at + to.a, turned[j][0]);
-        load_values<8, BF16>(p.kv, at + to.b, turned[j][1]);
+        for (int i = 0; i < kRaw; i++) {
+          raw[j][0][i] = *reinterpret_cast<const v4i*>(x + to.a + i * kStep);
+          raw[j][1][i] = *reinterpret_cast<const v4i*>(x + to.b + i * kStep);
+        }
       }
     }
+    if (rope.k_norm.on && tid < DH) s_turn->w[tid] = rope.k_norm.weight ? rope.k_norm.weight[tid] : 1.0f;
+    few_turns = cnt * rope.turn.pairs <= AppendTurn::kPairs;
+    if (few_turns && tid < cnt * rope.turn.pairs) {
+      const int t = tid / rope.turn.pairs;
+      turn_cos_sin(turn_at(rope.turn.freq[tid - t * rope.turn.pairs], rope.pos[r0 + first + t]),
+                   rope.turn.amp, s_turn->c[tid], s_turn->s[tid]);
+    }
+    __syncthreads();
   }
   const bool here = slot >= 0 && slot / kPage < p.cache.pages;
   const size_t unit = here ? (size_t)(slot / kPage) * heads + h : 0;
@@ -343,23 +363,28 @@ __device__ __forceinline__ void append_block(const CacheAppendArgs& p, const Rop
   uint8_t* gv = p.cache.v + unit * kBytes;
   const int ok = p.cache.k_exp[unit], ov = p.cache.v_exp[unit];
   if constexpr (TURN) {
-    float inv = 0.0f;
-    if (rope.k_norm.on) {
-      float ss = 0.0f;
+    float ss = 0.0f;
 #pragma unroll
-      for (int j = 0; j < E / 16; j++)
+    for (int j = 0; j < E / 16; j++)
 #pragma unroll
-        for (int i = 0; i < 16; i++) ss += turned[j][i / 8][i % 8] * turned[j][i / 8][i % 8];
+      for (int half = 0; half < 2; half++) {
+#pragma unroll
+        for (int i = 0; i < kRaw; i++) widen<BF16>(raw[j][half][i], turned[j][half], i * kStep);
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+          if (!mine) turned[j][half][i] = 0.0f;
+          ss += turned[j][half][i] * turned[j][half][i];
+        }
+      }
 #if defined(__HIP_DEVICE_COMPILE__)
 #define RH_ROR(n)                                                                                 \
   ss += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(ss), 0x120 + n, 0xF, 0xF, true))
-      RH_ROR(4);  // the token's four lanes
-      RH_ROR(8);
+    RH_ROR(4);  // the token's four lanes
+    RH_ROR(8);
 #undef RH_ROR
 #endif
-      inv = 1.0f / sqrtf(ss / (float)DH + rope.k_norm.eps);
-    }
     if (mine) {
+      const float inv = inverse_root(ss / (float)DH + rope.k_norm.eps);
 #pragma unroll
       for (int j = 0; j < E / 16; j++) {
         const int chunk = quarter + 4 * j;
@@ -367,19 +392,22 @@ __device__ __forceinline__ void append_block(const CacheAppendArgs& p, const Rop
         if (rope.k_norm.on) {
 #pragma unroll
           for (int half = 0; half < 2; half++) {
-            const int d = half ? to.b : to.a;
+            float w[8];
+            load_floats(s_turn->w + (half ? to.b : to.a), w);
 #pragma unroll
-            for (int i = 0; i < 8; i++) {
-              turned[j][half][i] *= inv;
-              if (rope.k_norm.weight) turned[j][half][i] *= rope.k_norm.weight[d + i];
-            }
+            for (int i = 0; i < 8; i++) turned[j][half][i] = turned[j][half][i] * inv * w[i];
           }
         }
         if (to.turns) {
           float c[8], sn[8];
+          if (few_turns) {
+            load_floats(s_turn->c + (tok - off) * rope.turn.pairs + chunk * 8, c);
+            load_floats(s_turn->s + (tok - off) * rope.turn.pairs + chunk * 8, sn);
+          } else {
 #pragma unroll
-          for (int i = 0; i < 8; i++)
-            turn_cos_sin(turn_at(rope.turn.freq[chunk * 8 + i], pos), rope.turn.amp, c[i], sn[i]);
+            for (int i = 0; i < 8; i++)
+              turn_cos_sin(turn_at(rope.turn.freq[chunk * 8 + i], pos), rope.turn.amp, c[i], sn[i]);
+          }
           rope_turn<8>(turned[j][0], turned[j][1], c, sn, rope.turn.halves);
         }
       }
@@ -539,25 +567,27 @@ template <int DH, bool BF16>
 __global__ __launch_bounds__(kAppendThreads) void cache_append_kernel(CacheAppendArgs p) {
   __shared__ __attribute__((aligned(16))) uint8_t s_k[kPage * DH], s_v[kPage * DH];
   __shared__ uint32_t s_max[kAppendThreads / 64][2];
-  append_block<DH, BF16, false>(p, RopeArgs{}, blockIdx.x, s_k, s_v, s_max);
+  append_block<DH, BF16, false>(p, RopeArgs{}, blockIdx.x, s_k, s_v, s_max, nullptr);
 }
 
 // Workgroups for blocks of K and V, then ones for rows of q, which are shorter: one launch for
 // both, and K never as rows.
-template <int DH, bool BF16, bool OB>
+template <int DH, bool BF16, bool OB, int ITEMS>
 __global__ __launch_bounds__(kAppendThreads) void rope_append_kernel(CacheAppendArgs p,
                                                                      RopeArgs rope,
-                                                                     unsigned blocks, int group) {
+                                                                     unsigned blocks, RopeShare share) {
   constexpr int P = BF16 ? 8 : 4;
   __shared__ __attribute__((aligned(16))) uint8_t s_two[2 * kPage * DH];
   __shared__ uint32_t s_max[kAppendThreads / 64][2];
+  __shared__ __attribute__((aligned(16))) AppendTurn s_turn;
   static_assert((2 * kRopePairs + 2 * DH) * sizeof(float) <= sizeof s_two, "the turns' LDS");
   static_assert(kAppendThreads == kRopeThreads, "workgroups of one size");
   if (blockIdx.x < blocks)
-    append_block<DH, BF16, true>(p, rope, blockIdx.x, s_two, s_two + kPage * DH, s_max);
+    append_block<DH, BF16, true>(p, rope, blockIdx.x, s_two, s_two + kPage * DH, s_max,
+                                   &s_turn);
   else
-    rope_rows<DH / 2 / P, P, BF16, OB>(rope, group, blockIdx.x - blocks, gridDim.x - blocks,
-                                       reinterpret_cast<float*>(s_two));
+    rope_rows<DH / 2 / P, P, BF16, OB, ITEMS>(rope, share, blockIdx.x - blocks,
+                                              reinterpret_cast<float*>(s_two));
 }
 
 // Every touched block holds a new row, and each request has at most two partly new blocks.
@@ -568,26 +598,32 @@ static long long append_blocks(const CacheAppendArgs& a) {
 
 hipError_t launch_rope_append(const CacheAppendArgs& a, const RopeArgs& rope, hipStream_t s) {
   const unsigned blocks = (unsigned)append_blocks(a);
-  const int group = rope_group(rope, a.cache.dh / (a.in_bf16 ? 16 : 8));
-  const unsigned more = rope.heads ? ((unsigned)rope.rows + group - 1) / group : 0;
-  const dim3 grid(blocks + std::min(more, 1u << 20)), block(kAppendThreads);
+  const RopeShare share = rope_share(rope, a.cache.dh / (a.in_bf16 ? 16 : 8));
+  const unsigned more = rope.heads ? (unsigned)share.blocks(rope.rows) : 0;
+  const dim3 grid(blocks + more), block(kAppendThreads);
   if (grid.x == 0) return hipSuccess;
-#define RH_APPEND(D, X, O) \
-  hipLaunchKernelGGL((rope_append_kernel<D, X, O>), grid, block, 0, s, a, rope, blocks, group)
-#define RH_DIM(D)                             \
-  if (a.cache.dh == D) {                      \
-    if (a.in_bf16) {                          \
-      if (rope.out_bf16) RH_APPEND(D, true, true); \
-      else RH_APPEND(D, true, false);         \
-    } else {                                  \
-      if (rope.out_bf16) RH_APPEND(D, false, true); \
-      else RH_APPEND(D, false, false);        \
-    }                                         \
+#define RH_APPEND(D, X, O, I) \
+  hipLaunchKernelGGL((rope_append_kernel<D, X, O, I>), grid, block, 0, s, a, rope, blocks, share)
+#define RH_MANY(D, X, O)                              \
+  {                                                   \
+    if (share.many) RH_APPEND(D, X, O, kRopeItems);   \
+    else RH_APPEND(D, X, O, 1);                       \
+  }
+#define RH_DIM(D)                               \
+  if (a.cache.dh == D) {                        \
+    if (a.in_bf16) {                            \
+      if (rope.out_bf16) RH_MANY(D, true, true) \
+      else RH_MANY(D, true, false)              \
+    } else {                                    \
+      if (rope.out_bf16) RH_MANY(D, false, true) \
+      else RH_MANY(D, false, false)             \
+    }                                           \
   }
   RH_DIM(64)
   RH_DIM(128)
   RH_DIM(256)
 #undef RH_DIM
+#undef RH_MANY
 #undef RH_APPEND
   return hipGetLastError();
 }

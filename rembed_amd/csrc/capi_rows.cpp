@@ -355,7 +355,9 @@ int rh_rope_append(rh_context* ctx, const rh_rope* rope, const rh_kv_cache* cach
              : share(out, rows_of(x, x_bf16, end, ldx), rows))
       return fail(RH_ERR_INVALID, "q overlaps x without being its own columns");
     const long long segs = std::min((long long)rows, (long long)rows / RH_CACHE_BLOCK + 2LL * batch);
-    if (segs * cache->kv_heads > 1 << 23) return fail(RH_ERR_SHAPE, "too many blocks for one call");
+    // workgroups for blocks, and (eight heads of a row each, or more) for rows of q
+    if (segs * cache->kv_heads > 1 << 23 || rows * (heads / 8 + 1LL) > 1 << 23)
+      return fail(RH_ERR_SHAPE, "too many rows for one call");
     CTX_GUARD(ctx);
     if (batch == 0 || rows == 0) return RH_OK;
     CacheAppendArgs c{*cache, x, x_bf16 ? 1 : 0, ldx, k_off, v_off, cu, blocks, slots, batch,

@@ -80,7 +80,7 @@ __device__ __forceinline__ void norm_row(float (&v)[V][8], const rh_norm& norm, 
       const bool in = VEC ? (t + T * e) * 8 < n : (t + T * e) * 8 + i < n;
       ss += in ? v[e][i] * v[e][i] : 0.0f;
     }
-  const float inv = 1.0f / sqrtf(sum(ss) / (float)n + norm.eps);
+  const float inv = inverse_root(sum(ss) / (float)n + norm.eps);
 #pragma unroll
   for (int e = 0; e < V; e++) {
     const int c = (t + T * e) * 8;

@@ -10,10 +10,10 @@
 
 namespace rh {
 
-template <int LPH, int P, bool XB, bool OB>
-__global__ __launch_bounds__(kRopeThreads) void rope_rows_kernel(RopeArgs p, int group) {
+template <int LPH, int P, bool XB, bool OB, int ITEMS>
+__global__ __launch_bounds__(kRopeThreads) void rope_rows_kernel(RopeArgs p, RopeShare share) {
   __shared__ __attribute__((aligned(16))) float lds[2 * kRopePairs + 4 * LPH * P];
-  rope_rows<LPH, P, XB, OB>(p, group, blockIdx.x, gridDim.x, lds);
+  rope_rows<LPH, P, XB, OB, ITEMS>(p, share, blockIdx.x, lds);
 }
 
 // Heads of any even size, rows of any alignment: a wave takes a head at a time, a lane the pairs
@@ -49,7 +49,7 @@ __global__ __launch_bounds__(256) void rope_any_kernel(RopeArgs p) {
     }
     const HeadNorm norm = at.part == 0 ? p.q_norm : p.k_norm;
     const bool normed = at.part < 2 && norm.on;
-    const float inv = 1.0f / sqrtf(group_sum<64>(ss) / (float)p.dh + norm.eps);
+    const float inv = inverse_root(group_sum<64>(ss) / (float)p.dh + norm.eps);
     const int t = p.pos[row];
 #pragma unroll
     for (int e = 0; e < 2; e++) {
@@ -107,26 +107,36 @@ hipError_t launch_rope_rows(const RopeArgs& a, hipStream_t s) {
     return hipGetLastError();
   }
   const int lanes = a.dh / (a.x_bf16 ? 16 : 8);
-  const int group = rope_group(a, lanes);
-  const unsigned wgs = (unsigned)std::min(((long long)a.rows + group - 1) / group, 1LL << 20);
-#define RH_ROPE(L, P, X, O) \
-  hipLaunchKernelGGL((rope_rows_kernel<L, P, X, O>), dim3(wgs), dim3(kRopeThreads), 0, s, a, group)
-#define RH_LANES(D)                                  \
-  if (a.dh == D) {                                   \
-    if (a.x_bf16) {                                  \
-      if (a.out_bf16) RH_ROPE(D / 16, 8, true, true); \
-      else RH_ROPE(D / 16, 8, true, false);          \
-    } else {                                         \
-      if (a.out_bf16) RH_ROPE(D / 8, 4, false, true); \
-      else RH_ROPE(D / 8, 4, false, false);          \
-    }                                                \
+  RopeShare share = rope_share(a, lanes);
+  // a launch holds fewer than 2^32 threads
+  const int most = std::max(1, (1 << 23) / share.slices) * share.group;
+  for (; share.first < a.rows; share.first += std::min(most, a.rows - share.first)) {
+    const dim3 grid((unsigned)share.blocks(std::min(most, a.rows - share.first)));
+#define RH_ROPE(L, P, X, O, I) \
+  hipLaunchKernelGGL((rope_rows_kernel<L, P, X, O, I>), grid, dim3(kRopeThreads), 0, s, a, share)
+#define RH_MANY(L, P, X, O)                              \
+  {                                                      \
+    if (share.many) RH_ROPE(L, P, X, O, kRopeItems);     \
+    else RH_ROPE(L, P, X, O, 1);                         \
   }
-  RH_LANES(32)
-  RH_LANES(64)
-  RH_LANES(128)
-  RH_LANES(256)
+#define RH_LANES(D)                                       \
+  if (a.dh == D) {                                        \
+    if (a.x_bf16) {                                       \
+      if (a.out_bf16) RH_MANY(D / 16, 8, true, true)      \
+      else RH_MANY(D / 16, 8, true, false)                \
+    } else {                                              \
+      if (a.out_bf16) RH_MANY(D / 8, 4, false, true)      \
+      else RH_MANY(D / 8, 4, false, false)                \
+    }                                                     \
+  }
+    RH_LANES(32)
+    RH_LANES(64)
+    RH_LANES(128)
+    RH_LANES(256)
 #undef RH_LANES
+#undef RH_MANY
 #undef RH_ROPE
+  }
   return hipGetLastError();
 }
 

@@ -5,11 +5,12 @@
 #include "rowops.h"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace rh {
 
 constexpr int kRopeThreads = 256;
-constexpr int kRopeItems = 4;    // heads' chunks of a thread whose loads are in flight together
+constexpr int kRopeItems = 4;    // the most heads of a thread, whose loads are in flight together
 constexpr int kRopePairs = 512;  // cosines and sines that a workgroup holds
 
 __device__ __forceinline__ int rope_used(const RopeArgs& p) {
@@ -27,94 +28,99 @@ struct RopeHead {
   }
 };
 
-// Rows of a workgroup: kRopeItems chunks for each thread where there are rows enough for two
-// workgroups a CU, as far as their cosines fit.
-inline int rope_group(const RopeArgs& a, int lanes) {
-  const long long nh = (long long)a.heads + a.kv_heads + a.v_heads;
-  long long g = kRopeThreads * kRopeItems / std::max(1LL, nh * lanes);
-  g = std::min(g, (long long)kRopePairs / a.turn.pairs);
-  g = std::min(g, ((long long)a.rows + 511) / 512);
-  return (int)std::max(1LL, g);
+// How rows are given to workgroups: `sets` threads' heads a row, kRopeItems or one each; a workgroup
+// has `group` rows, of each one of `slices` ranges of `each` sets.
+struct RopeShare {
+  int many, sets, each, slices, group;
+  int first;  // row of the first workgroup
+  long long blocks(int rows) const { return (rows + (group - 1LL)) / group * slices; }
+};
+// Four heads a thread, whose cosines it then reads once, where two workgroups a CU remain; as
+// many rows as fill the workgroup's threads and as far as their cosines fit.
+inline RopeShare rope_share(const RopeArgs& a, int lanes) {
+  const long long nh = std::max(1LL, (long long)a.heads + a.kv_heads + a.v_heads);
+  RopeShare s;
+  s.many = nh * lanes * a.rows >= kRopeItems * 512LL * kRopeThreads;
+  s.sets = (int)(s.many ? (nh + kRopeItems - 1) / kRopeItems : nh);
+  s.each = std::min(s.sets, kRopeThreads / lanes);
+  s.slices = (s.sets + s.each - 1) / s.each;
+  s.group = std::max(1, std::min(kRopeThreads / (s.each * lanes), kRopePairs / a.turn.pairs));
+  s.group = std::min(s.group, a.rows / 512 + 1);
+  s.first = 0;
+  return s;
 }
 
-// A lane takes P pairs of a head, LPH lanes a head; a workgroup `group` rows at a time, whose
-// cosines and sines it puts into LDS once for all heads. lds: 2 * kRopePairs + 4 * LPH * P floats.
-template <int LPH, int P, bool XB, bool OB>
-__device__ __forceinline__ void rope_rows(const RopeArgs& p, int group, unsigned block,
-                                          unsigned blocks, float* lds) {
+// A lane takes P pairs of a head, 16 bytes of each half, LPH lanes a head; a thread ITEMS heads of
+// a row. The rows' cosines and sines are in LDS once for all heads. lds: 2 * kRopePairs +
+// 4 * LPH * P floats, 16-byte aligned.
+template <int LPH, int P, bool XB, bool OB, int ITEMS>
+__device__ __forceinline__ void rope_rows(const RopeArgs& p, const RopeShare& share, unsigned block,
+                                          float* lds) {
+  static_assert(P == (XB ? 8 : 4), "16 bytes");
   constexpr int DH = LPH * 2 * P;
   float *s_cos = lds, *s_sin = lds + kRopePairs, *s_w = lds + 2 * kRopePairs;
   const int tid = threadIdx.x, l = tid % LPH;
   const int nh = p.heads + p.kv_heads + p.v_heads, pairs = p.turn.pairs;
   const int used = rope_used(p);
+  const int r0 = share.first + (int)(block / share.slices) * share.group;
+  const int nr = min(share.group, used - r0);
+  if (nr <= 0) return;
   const RopePlace<P> at(p.turn, l);
-  for (int i = tid; i < 2 * DH; i += kRopeThreads) {
-    const float* w = i < DH ? p.q_norm.weight : p.k_norm.weight;
-    s_w[i] = w ? w[i % DH] : 1.0f;
+  // the thread's row of these, and its heads set, set + sets, ..
+  const int unit = tid / LPH, row = unit / share.each;
+  const int set = (int)(block % share.slices) * share.each + unit - row * share.each;
+  const bool mine = row < nr && set < share.sets;
+  using S = std::conditional_t<XB, __bf16, float>;
+  const S* x = static_cast<const S*>(p.x) + (size_t)(r0 + min(row, nr - 1)) * p.ldx;
+  v4i a[ITEMS], b[ITEMS];
+#pragma unroll
+  for (int k = 0; k < ITEMS; k++) {  // behind the last head: that one, not used
+    const int from = RopeHead(p, min(set + k * share.sets, nh - 1), DH).in;
+    a[k] = *reinterpret_cast<const v4i*>(x + from + at.a);
+    b[k] = *reinterpret_cast<const v4i*>(x + from + at.b);
   }
-  for (long long r0 = (long long)block * group; r0 < used; r0 += (long long)blocks * group) {
-    const int nr = min(group, used - (int)r0);
-    const unsigned slots = (unsigned)nr * nh;  // heads of these rows
-    float a[kRopeItems][P], b[kRopeItems][P];
-    auto load = [&](unsigned base) {
-#pragma unroll
-      for (int k = 0; k < kRopeItems; k++) {
-        const unsigned slot = base + (tid + k * kRopeThreads) / LPH;
-#pragma unroll
-        for (int i = 0; i < P; i++) a[k][i] = b[k][i] = 0.0f;
-        if (slot < slots) {
-          const unsigned row = slot / (unsigned)nh;
-          const RopeHead h(p, (int)(slot - row * nh), DH);
-          const size_t from = (size_t)(r0 + row) * p.ldx + h.in;
-          load_values<P, XB>(p.x, from + at.a, a[k]);
-          load_values<P, XB>(p.x, from + at.b, b[k]);
-        }
-      }
-    };
-    load(0);
-    for (int i = tid; i < nr * pairs; i += kRopeThreads) {
-      const int row = i / pairs;
-      turn_cos_sin(turn_at(p.turn.freq[i - row * pairs], p.pos[r0 + row]), p.turn.amp, s_cos[i],
-                   s_sin[i]);
+  if (p.q_norm.on || p.k_norm.on)
+    for (int i = tid; i < 2 * DH; i += kRopeThreads) {
+      const float* w = i < DH ? p.q_norm.weight : p.k_norm.weight;
+      s_w[i] = w ? w[i % DH] : 1.0f;
     }
-    __syncthreads();
-    for (unsigned base = 0; base < slots; base += kRopeThreads / LPH * kRopeItems) {
-      if (base) load(base);
+  for (int i = tid; i < nr * pairs; i += kRopeThreads) {
+    const int t = i / pairs;
+    turn_cos_sin(turn_at(p.turn.freq[i - t * pairs], p.pos[r0 + t]), p.turn.amp, s_cos[i], s_sin[i]);
+  }
+  __syncthreads();
+  if (!mine) return;
+  float c[P], s[P];
+  if (at.turns) {
+    load_floats(s_cos + row * pairs + l * P, c);
+    load_floats(s_sin + row * pairs + l * P, s);
+  }
 #pragma unroll
-      for (int k = 0; k < kRopeItems; k++) {
-        const unsigned slot = base + (tid + k * kRopeThreads) / LPH;
-        const unsigned row = slot / (unsigned)nh;
-        const RopeHead h(p, (int)(slot - row * nh), DH);
-        const HeadNorm& norm = h.part == 0 ? p.q_norm : p.k_norm;
-        float ss = 0.0f;
+  for (int k = 0; k < ITEMS; k++) {
+    const int h = set + k * share.sets;
+    if (h >= nh) return;
+    const RopeHead head(p, h, DH);
+    const HeadNorm& norm = head.part == 0 ? p.q_norm : p.k_norm;
+    float y[P], z[P];
+    widen<XB>(a[k], y);
+    widen<XB>(b[k], z);
+    if (head.part < 2 && norm.on) {
+      float ss = 0.0f;
 #pragma unroll
-        for (int i = 0; i < P; i++) ss += a[k][i] * a[k][i] + b[k][i] * b[k][i];
-        ss = group_sum<LPH>(ss);
-        if (slot >= slots) continue;
-        if (h.part < 2 && norm.on) {
-          const float inv = 1.0f / sqrtf(ss / (float)DH + norm.eps);
-          const float* w = s_w + (h.part ? DH : 0);
+      for (int i = 0; i < P; i++) ss += y[i] * y[i] + z[i] * z[i];
+      const float inv = inverse_root(group_sum<LPH>(ss) / (float)DH + norm.eps);
+      float w[P];
+      load_floats(s_w + (head.part ? DH : 0) + at.a, w);
 #pragma unroll
-          for (int i = 0; i < P; i++) {
-            a[k][i] = a[k][i] * inv * w[at.a + i];
-            b[k][i] = b[k][i] * inv * w[at.b + i];
-          }
-        }
-        if (h.part < 2 && at.turns) {
-          float c[P], s[P];
+      for (int i = 0; i < P; i++) y[i] = y[i] * inv * w[i];
+      load_floats(s_w + (head.part ? DH : 0) + at.b, w);
 #pragma unroll
-          for (int i = 0; i < P; i++) {
-            c[i] = s_cos[row * pairs + l * P + i];
-            s[i] = s_sin[row * pairs + l * P + i];
-          }
-          rope_turn<P>(a[k], b[k], c, s, p.turn.halves);
-        }
-        const size_t to = (size_t)(r0 + row) * p.ldout + h.out;
-        store_values<P, OB>(p.out, to + at.a, a[k]);
-        store_values<P, OB>(p.out, to + at.b, b[k]);
-      }
+      for (int i = 0; i < P; i++) z[i] = z[i] * inv * w[i];
     }
-    __syncthreads();
+    if (head.part < 2 && at.turns) rope_turn<P>(y, z, c, s, p.turn.halves);
+    const size_t to = (size_t)(r0 + row) * p.ldout + head.out;
+    store_values<P, OB>(p.out, to + at.a, y);
+    store_values<P, OB>(p.out, to + at.b, z);
   }
 }
 

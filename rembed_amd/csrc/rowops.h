@@ -80,6 +80,39 @@ __device__ __forceinline__ void store_values(void* base, size_t at, const float 
   }
 }
 
+// 16 bytes of a row as values, and 16 (4 aligned floats) of LDS.
+template <bool BF16, int N>
+__device__ __forceinline__ void widen(const v4i& raw, float (&v)[N], int at = 0) {
+  if constexpr (BF16) {
+    const v8bf x = __builtin_bit_cast(v8bf, raw);
+#pragma unroll
+    for (int e = 0; e < 8; e++) v[at + e] = (float)x[e];
+  } else {
+    const v4f x = __builtin_bit_cast(v4f, raw);
+#pragma unroll
+    for (int e = 0; e < 4; e++) v[at + e] = x[e];
+  }
+}
+template <int N>
+__device__ __forceinline__ void load_floats(const float* lds, float (&v)[N]) {
+#pragma unroll
+  for (int j = 0; j < N; j += 4) {
+    const v4f x = *reinterpret_cast<const v4f*>(lds + j);
+#pragma unroll
+    for (int e = 0; e < 4; e++) v[j + e] = x[e];
+  }
+}
+
+// 1 / sqrt(a), within 0.6 steps: the hardware's (within one) and a correction with the product's
+// own rounding taken along, where that neither under- nor overflows.
+__device__ __forceinline__ float inverse_root(float a) {
+  if (!(a >= 0x1p-100f && a <= 0x1p100f)) return 1.0f / sqrtf(a);
+  const float r = __builtin_amdgcn_rsqf(a);
+  const float h = a * r, low = __builtin_fmaf(a, r, -h);
+  const float e = __builtin_fmaf(-low, r, __builtin_fmaf(-h, r, 1.0f));  // 1 - a r r
+  return __builtin_fmaf(0.5f * r, e, r);
+}
+
 // ---- the turn ---------------------------------------------------------------------------
 struct RopeTurn {
   const uint64_t* freq;  // [pairs] 2^64 times the turns a position
