@@ -178,7 +178,7 @@ __global__ __launch_bounds__(256) void residual_norm_kernel(ResidualArgs p, int 
         v2i q;
         q[0] = fp8_pack4(v[e][0] * f, v[e][1] * f, v[e][2] * f, v[e][3] * f);
         q[1] = fp8_pack4(v[e][4] * f, v[e][5] * f, v[e][6] * f, v[e][7] * f);
-        *reinterpret_cast<v2i*>(p.qa + (size_t)row * p.ldq + c) = q;
+        __builtin_nontemporal_store(q, reinterpret_cast<v2i*>(p.qa + (size_t)row * p.ldq + c));
         if (t % 16 == 0)
           p.sa[fp8_scale_at((int)row, c / kFp8Block, (p.m + 127) / 128)] = (uint8_t)x;
       }

@@ -70,13 +70,13 @@ __device__ __forceinline__ void store_values(void* base, size_t at, const float 
       T x;
 #pragma unroll
       for (int e = 0; e < W; e++) x[e] = (__bf16)v[j + e];
-      *reinterpret_cast<T*>(static_cast<__bf16*>(base) + at + j) = x;
+      __builtin_nontemporal_store(x, reinterpret_cast<T*>(static_cast<__bf16*>(base) + at + j));
     }
   } else {
 #pragma unroll
     for (int j = 0; j < N; j += 4)
-      *reinterpret_cast<v4f*>(static_cast<float*>(base) + at + j) =
-          (v4f){v[j], v[j + 1], v[j + 2], v[j + 3]};
+      __builtin_nontemporal_store((v4f){v[j], v[j + 1], v[j + 2], v[j + 3]},
+                                  reinterpret_cast<v4f*>(static_cast<float*>(base) + at + j));
   }
 }
 
