@@ -570,23 +570,36 @@ __global__ __launch_bounds__(kAppendThreads) void cache_append_kernel(CacheAppen
   append_block<DH, BF16, false>(p, RopeArgs{}, blockIdx.x, s_k, s_v, s_max, nullptr);
 }
 
-// Workgroups for blocks of K and V, then ones for rows of q, which are shorter: one launch for
-// both, and K never as rows.
+// Workgroups for blocks of K and V and ones for rows of q, in one launch, and K never as rows. The
+// first kind computes more and takes longer, the second one is bound by its bytes. So that a CU
+// has both and the first kind is begun early, of each w workgroups w * kBlockShare are that kind
+// while there are both. The golden section, because a fixed turn would meet the round robin over
+// XCDs and CUs (22.8k tokens of 16 + 8 heads of 128: one kind after the other 75 µs, in turns of
+// one or of eight 78), and a share in proportion begins the last blocks late (2.5k tokens of 3 + 1
+// heads of 256: 12 µs, in proportion 18 to 23).
+constexpr uint64_t kBlockShare = 0x9E3779BA;  // times 2^32
+// How many of the first w workgroups are blocks.
+__device__ __forceinline__ unsigned blocks_before(unsigned w, unsigned blocks, unsigned rows) {
+  const unsigned turn = min(blocks, (unsigned)(w * kBlockShare >> 32));
+  return w > rows ? max(turn, w - rows) : turn;
+}
+
 template <int DH, bool BF16, bool OB, int ITEMS>
 __global__ __launch_bounds__(kAppendThreads) void rope_append_kernel(CacheAppendArgs p,
-                                                                     RopeArgs rope,
-                                                                     unsigned blocks, RopeShare share) {
+                                                                     RopeArgs rope, unsigned blocks,
+                                                                     RopeShare share) {
   constexpr int P = BF16 ? 8 : 4;
   __shared__ __attribute__((aligned(16))) uint8_t s_two[2 * kPage * DH];
   __shared__ uint32_t s_max[kAppendThreads / 64][2];
   __shared__ __attribute__((aligned(16))) AppendTurn s_turn;
   static_assert((2 * kRopePairs + 2 * DH) * sizeof(float) <= sizeof s_two, "the turns' LDS");
   static_assert(kAppendThreads == kRopeThreads, "workgroups of one size");
-  if (blockIdx.x < blocks)
-    append_block<DH, BF16, true>(p, rope, blockIdx.x, s_two, s_two + kPage * DH, s_max,
-                                   &s_turn);
+  const unsigned w = blockIdx.x, rows = gridDim.x - blocks;
+  const unsigned before = blocks_before(w, blocks, rows);
+  if (blocks_before(w + 1, blocks, rows) != before)
+    append_block<DH, BF16, true>(p, rope, before, s_two, s_two + kPage * DH, s_max, &s_turn);
   else
-    rope_rows<DH / 2 / P, P, BF16, OB, ITEMS>(rope, share, blockIdx.x - blocks,
+    rope_rows<DH / 2 / P, P, BF16, OB, ITEMS>(rope, share, w - before,
                                               reinterpret_cast<float*>(s_two));
 }
 

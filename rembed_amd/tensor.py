@@ -413,7 +413,7 @@ class Rope:
             self.h = None
 
     def __del__(self):
-        if sys.is_finalizing():
+        if sys is None or sys.is_finalizing():
             return  # the HIP runtime may already be torn down
         try:
             self.close()
