@@ -373,7 +373,7 @@ __device__ __forceinline__ void append_block(const CacheAppendArgs& p, const Rop
 #pragma unroll
         for (int i = 0; i < 8; i++) {
           if (!mine) turned[j][half][i] = 0.0f;
-          ss += turned[j][half][i] * turned[j][half][i];
+          ss = __builtin_fmaf(turned[j][half][i], turned[j][half][i], ss);
         }
       }
 #if defined(__HIP_DEVICE_COMPILE__)

@@ -10,10 +10,10 @@
 
 #include "rowops.h"
 
-// The frequencies of a turn, 2^64 times the turns a position.
+// The frequencies of a turn in HBM.
 struct rh_rope {
   rh_context* ctx = nullptr;
-  uint64_t* d_freq = nullptr;
+  rh::RopeFreq* d_freq = nullptr;
   int pairs = 0, halves = 0;
   float amp = 1.0f;
 };
@@ -236,10 +236,11 @@ int rh_rope_create(rh_context* ctx, const rh_rope_config* cfg, rh_rope** out) {
     double amp = 1.0;
     if (int st = rope_frequencies(cfg, f, amp)) return st;
     // whole turns a position change nothing: positions are whole numbers
-    std::vector<uint64_t> turns(f.size());
+    std::vector<RopeFreq> turns(f.size());
     for (size_t i = 0; i < f.size(); i++) {
       const long double t = f[i] / (2 * acosl(-1.0L)), x = roundl((t - floorl(t)) * 0x1p64L);
-      turns[i] = x >= 0x1p64L ? 0 : (uint64_t)x;
+      const uint64_t u = x >= 0x1p64L ? 0 : (uint64_t)x;
+      turns[i] = RopeFreq{(int32_t)(uint32_t)u, (int32_t)(uint32_t)((u + 0x80000000u) >> 32)};
     }
     CTX_GUARD(ctx);
     std::unique_ptr<rh_rope, void (*)(rh_rope*)> r(new rh_rope(), destroy_rope);
@@ -247,8 +248,8 @@ int rh_rope_create(rh_context* ctx, const rh_rope_config* cfg, rh_rope** out) {
     r->pairs = (int)f.size();
     r->halves = cfg->layout == RH_ROPE_HALVES;
     r->amp = (float)amp;
-    RH_HIP(hipMalloc((void**)&r->d_freq, turns.size() * sizeof(uint64_t)));
-    RH_HIP(hipMemcpy(r->d_freq, turns.data(), turns.size() * sizeof(uint64_t),
+    RH_HIP(hipMalloc((void**)&r->d_freq, turns.size() * sizeof(RopeFreq)));
+    RH_HIP(hipMemcpy(r->d_freq, turns.data(), turns.size() * sizeof(RopeFreq),
                      hipMemcpyHostToDevice));
     ctx_retain(ctx);
     *out = r.release();

@@ -107,7 +107,7 @@ __device__ __forceinline__ void rope_rows(const RopeArgs& p, const RopeShare& sh
     if (head.part < 2 && norm.on) {
       float ss = 0.0f;
 #pragma unroll
-      for (int i = 0; i < P; i++) ss += y[i] * y[i] + z[i] * z[i];
+      for (int i = 0; i < P; i++) ss = __builtin_fmaf(y[i], y[i], __builtin_fmaf(z[i], z[i], ss));
       const float inv = inverse_root(group_sum<LPH>(ss) / (float)DH + norm.eps);
       float w[P];
       load_floats(s_w + (head.part ? DH : 0) + at.a, w);

@@ -5,8 +5,8 @@
 //   a' = m (a cos(t f) - b sin(t f)),   b' = m (b cos(t f) + a sin(t f)).
 // Positions are whole numbers, so whole turns of f drop out: f is kept as a 64-bit fraction of a
 // turn, t f mod 1 is a product mod 2^64, exact but for f's own rounding (2^-65 of a turn a
-// position; 2^-34 at 2^31), and no table limits how long a text is. fp32 angles would be off
-// by 2^-24 of the angle itself: 0.004 rad at position 65536.
+// position; 2^-34 at 2^31) and the 32 bits that are kept, and no table limits how long a text is.
+// fp32 angles would be off by 2^-24 of the angle itself: 0.004 rad at position 65536.
 #pragma once
 
 #include "fp8.h"
@@ -114,36 +114,39 @@ __device__ __forceinline__ float inverse_root(float a) {
 }
 
 // ---- the turn ---------------------------------------------------------------------------
+// A pair's turns a position: t -> t * high + (t * low >> 32) is the 32-bit fraction of a turn at
+// position t. low is signed, what it lacks is in high.
+struct RopeFreq {
+  int32_t low, high;
+};
 struct RopeTurn {
-  const uint64_t* freq;  // [pairs] 2^64 times the turns a position
+  const RopeFreq* freq;  // [pairs]
   int pairs;             // rot / 2: the head's leading 2 * pairs values turn
   int halves;            // pair i is (i, i + pairs); else (2i, 2i + 1)
   float amp;             // cos and sin are multiplied by it
 };
-// The 32-bit fraction of a turn at position t.
-__device__ __forceinline__ uint32_t turn_at(uint64_t freq, int t) {
-  const uint32_t lo = (uint32_t)freq, hi = (uint32_t)(freq >> 32), u = (uint32_t)t;
-  return __umulhi(u, lo) + u * hi - (t < 0 ? lo : 0u);
+__device__ __forceinline__ uint32_t turn_at(const RopeFreq& f, int t) {
+  return (uint32_t)__mulhi(t, f.low) + (uint32_t)t * (uint32_t)f.high;
 }
-// cos and sin of a fraction of a turn: its distance from the nearest quarter (at most pi / 4) by
-// Taylor's polynomials (rests under 2e-9 and 2e-10), off by at most 1.5e-7 with the roundings.
+// cos and sin of a fraction of a turn: of its distance x from the nearest quarter, at most
+// pi / 4, by polynomials whose largest error is least (found by exchange; sin 1.8e-9, cos
+// 5.4e-11), then the quarter's exchange and signs. Off by at most 1.5e-7 with the roundings.
 __device__ __forceinline__ void turn_cos_sin(uint32_t turn, float amp, float& c, float& s) {
-  const uint32_t q = (turn + 0x20000000u) >> 30;
-  const float x = (float)(int)(turn - (q << 30)) * 1.46291807926715968e-9f;  // 2 pi / 2^32
+  const uint32_t u = turn + 0x20000000u;  // its upper two bits: the quarter
+  const float x = (float)(int)(turn << 2) * 3.6572951981678993e-10f;  // 2 pi / 2^34
   const float x2 = x * x;
-  float u = __builtin_fmaf(x2, 1.0f / 362880, -1.0f / 5040);
-  u = __builtin_fmaf(x2, u, 1.0f / 120);
-  u = __builtin_fmaf(x2, u, -1.0f / 6);
-  const float sn = __builtin_fmaf(x * x2, u, x);
-  float w = __builtin_fmaf(x2, -1.0f / 3628800, 1.0f / 40320);
-  w = __builtin_fmaf(x2, w, -1.0f / 720);
-  w = __builtin_fmaf(x2, w, 1.0f / 24);
-  w = __builtin_fmaf(x2, w, -0.5f);
-  const float cs = __builtin_fmaf(x2, w, 1.0f);
+  float p = __builtin_fmaf(x2, -0.0001949563619f, 0.008331978663f);
+  p = __builtin_fmaf(x2, p, -0.1666665067f);
+  const float sn = __builtin_fmaf(x * x2, p, x);
+  float q = __builtin_fmaf(x2, 2.439045066e-05f, -0.001388676379f);
+  q = __builtin_fmaf(x2, q, 0.04166662332f);
+  q = __builtin_fmaf(x2, q, -0.4999999973f);
+  const float cs = __builtin_fmaf(x2, q, 1.0f);
   // quarters 0..3: (c, s), (-s, c), (-c, -s), (s, -c)
-  const float a = q & 1 ? sn : cs, b = q & 1 ? cs : sn;
-  c = ((q + 1) & 2 ? -a : a) * amp;
-  s = (q & 2 ? -b : b) * amp;
+  const bool odd = u & 0x40000000u;
+  const uint32_t a = __float_as_uint(odd ? sn : cs), b = __float_as_uint(odd ? cs : sn);
+  c = __uint_as_float(a ^ ((u + 0x40000000u) & 0x80000000u)) * amp;
+  s = __uint_as_float(b ^ (u & 0x80000000u)) * amp;
 }
 
 // Where chunk l of P pairs of a head lies: its two runs of P values. Behind the pairs that turn
