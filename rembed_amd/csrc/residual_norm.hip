@@ -11,156 +11,206 @@
 #include "rowops.h"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace rh {
 
-// T threads a row (a wave, or the workgroup's four), V chunks of eight consecutive values each:
-// chunk e of thread t is values 8 (t + T e) .. + 7, so 16 lanes have a block of 128.
+// T threads a row (a wave, or the workgroup), V chunks of eight consecutive values each: chunk e of
+// thread t is values 8 (t + T e) .. + 7, so 16 lanes have a block of 128. Rows and weights are
+// all asked for at once, before anything is summed: a row's time is one latency of the memory, its
+// reductions (at most four, a barrier each where a row has several waves) and its stores, and
+// whole lines leave past the L2.
 template <int T>
 struct RowSum {
-  float (*slot)[4];  // of the workgroup: a place for each wave, for each sum of a row
+  static constexpr int kWaves = T / 64;
+  float (*slot)[kWaves];  // of the workgroup: a place for each wave, for each sum of a row
   int k = 0;
   __device__ __forceinline__ float operator()(float v) {
     v = group_sum<64>(v);
     if constexpr (T == 64) return v;
     if ((threadIdx.x & 63) == 0) slot[k][threadIdx.x >> 6] = v;
     __syncthreads();
-    v = (slot[k][0] + slot[k][1]) + (slot[k][2] + slot[k][3]);
+    v = slot[k][threadIdx.x % kWaves];
     k++;
-    return v;
+    return group_sum<kWaves>(v);
   }
 };
 
-template <bool VEC, bool BF16>
+enum Type : int { kNone, kF32, kBF16 };
+
+// Eight values; WHOLE: 16-byte aligned, in the row or behind it; else of any alignment (memory
+// takes 16 bytes at any address), the row's last ones by themselves.
+template <bool WHOLE, Type K>
 __device__ __forceinline__ void load_chunk(const void* base, size_t at, int c, int n, float (&v)[8]) {
 #pragma unroll
   for (int i = 0; i < 8; i++) v[i] = 0.0f;
-  if constexpr (VEC) {
-    if (c < n) load_values<8, BF16>(base, at + c, v);
+  if constexpr (WHOLE) {
+    if (c < n) load_values<8, K == kBF16>(base, at + c, v);
   } else {
+    using S = std::conditional_t<K == kBF16, __bf16, float>;
+    typedef S W __attribute__((ext_vector_type(16 / sizeof(S)), aligned(sizeof(S))));
+    constexpr int kW = 16 / sizeof(S);
+    const S* p = static_cast<const S*>(base) + at + c;
+    if (c + 8 <= n) {
 #pragma unroll
-    for (int i = 0; i < 8; i++)
-      if (c + i < n)
-        v[i] = BF16 ? (float)static_cast<const __bf16*>(base)[at + c + i]
-                    : static_cast<const float*>(base)[at + c + i];
+      for (int j = 0; j < 8; j += kW) {
+        const W x = *reinterpret_cast<const W*>(p + j);
+#pragma unroll
+        for (int i = 0; i < kW; i++) v[j + i] = (float)x[i];
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; i++)
+        if (c + i < n) v[i] = (float)p[i];
+    }
   }
 }
-template <bool VEC, bool BF16>
+template <bool WHOLE, Type K>
 __device__ __forceinline__ void store_chunk(void* base, size_t at, int c, int n, const float (&v)[8]) {
-  if constexpr (VEC) {
-    if (c < n) store_values<8, BF16>(base, at + c, v);
+  if constexpr (WHOLE) {
+    if (c < n) store_values<8, K == kBF16>(base, at + c, v);
   } else {
+    using S = std::conditional_t<K == kBF16, __bf16, float>;
+    typedef S W __attribute__((ext_vector_type(16 / sizeof(S)), aligned(sizeof(S))));
+    constexpr int kW = 16 / sizeof(S);
+    S* p = static_cast<S*>(base) + at + c;
+    if (c + 8 <= n) {
 #pragma unroll
-    for (int i = 0; i < 8; i++)
-      if (c + i < n) {
-        if constexpr (BF16) static_cast<__bf16*>(base)[at + c + i] = (__bf16)v[i];
-        else static_cast<float*>(base)[at + c + i] = v[i];
+      for (int j = 0; j < 8; j += kW) {
+        W x;
+#pragma unroll
+        for (int i = 0; i < kW; i++) x[i] = (S)v[j + i];
+        *reinterpret_cast<W*>(p + j) = x;
       }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; i++)
+        if (c + i < n) p[i] = (S)v[i];
+    }
   }
 }
 
+// A norm's weights, as the row's chunks.
+template <int V, int T, bool WHOLE>
+struct NormWeights {
+  float w[V][8], b[V][8];
+  __device__ __forceinline__ void load(const rh_norm& norm, int n, int t) {
+    if (norm.weight) {
+#pragma unroll
+      for (int e = 0; e < V; e++) load_chunk<WHOLE, kF32>(norm.weight, 0, (t + T * e) * 8, n, w[e]);
+    }
+    if (norm.bias) {
+#pragma unroll
+      for (int e = 0; e < V; e++) load_chunk<WHOLE, kF32>(norm.bias, 0, (t + T * e) * 8, n, b[e]);
+    }
+  }
+};
+
 // v normed in place; values past n are zeros before, and anything after.
-template <int V, int T, bool VEC>
-__device__ __forceinline__ void norm_row(float (&v)[V][8], const rh_norm& norm, int n, int t,
+template <int V, int T, bool WHOLE>
+__device__ __forceinline__ void norm_row(float (&v)[V][8], const rh_norm& norm,
+                                         const NormWeights<V, T, WHOLE>& by, int n, int t,
                                          RowSum<T>& sum) {
-  float mean = 0.0f, ss = 0.0f;
   if (norm.kind == RH_NORM_LAYER) {
     float s = 0.0f;
 #pragma unroll
     for (int e = 0; e < V; e++)
 #pragma unroll
       for (int i = 0; i < 8; i++) s += v[e][i];
-    mean = sum(s) / (float)n;
-  }
-#pragma unroll
-  for (int e = 0; e < V; e++)
-#pragma unroll
-    for (int i = 0; i < 8; i++) {
-      v[e][i] -= mean;
-      const bool in = VEC ? (t + T * e) * 8 < n : (t + T * e) * 8 + i < n;
-      ss += in ? v[e][i] * v[e][i] : 0.0f;
-    }
-  const float inv = inverse_root(sum(ss) / (float)n + norm.eps);
-#pragma unroll
-  for (int e = 0; e < V; e++) {
-    const int c = (t + T * e) * 8;
-    float w[8], b[8];
-    if (norm.weight) load_chunk<VEC, false>(norm.weight, 0, c, n, w);
-    if (norm.bias) load_chunk<VEC, false>(norm.bias, 0, c, n, b);
-#pragma unroll
-    for (int i = 0; i < 8; i++) {
-      v[e][i] *= inv;
-      if (norm.weight) v[e][i] *= w[i];
-      if (norm.bias) v[e][i] += b[i];
-    }
-  }
-}
-
-template <int V, int T, bool VEC>
-__global__ __launch_bounds__(256) void residual_norm_kernel(ResidualArgs p, int r0) {
-  __shared__ float s_sum[4][4];
-  const int t = threadIdx.x % T;
-  const long long row = r0 + (long long)blockIdx.x * (256 / T) + threadIdx.x / T;
-  const int used = p.used ? min(*p.used, p.m) : p.m;
-  if (row >= used) return;  // whole waves; with T = 256 the whole workgroup
-  const int n = p.n;
-  RowSum<T> sum{s_sum};
-  float v[V][8], w[V][8];
-#pragma unroll
-  for (int e = 0; e < V; e++) {
-    const int c = (t + T * e) * 8;
-    if (p.x_bf16) load_chunk<VEC, true>(p.x, (size_t)row * p.ldx, c, n, v[e]);
-    else load_chunk<VEC, false>(p.x, (size_t)row * p.ldx, c, n, v[e]);
-  }
-  if (p.y) {
-#pragma unroll
-    for (int e = 0; e < V; e++) {
-      const int c = (t + T * e) * 8;
-      if (p.y_bf16) load_chunk<VEC, true>(p.y, (size_t)row * p.ldy, c, n, w[e]);
-      else load_chunk<VEC, false>(p.y, (size_t)row * p.ldy, c, n, w[e]);
-    }
-    if (p.post.kind != RH_NORM_NONE) norm_row<V, T, VEC>(w, p.post, n, t, sum);
-#pragma unroll
-    for (int e = 0; e < V; e++) {
-      float g[8];
-      if (p.gate)
-        load_chunk<VEC, false>(p.gate, (size_t)row * p.ldg, (t + T * e) * 8, n, g);
-#pragma unroll
-      for (int i = 0; i < 8; i++) {
-        if (p.gate) w[e][i] *= g[i];
-        v[e][i] = __builtin_fmaf(v[e][i], p.x_scale, w[e][i] * p.y_scale);
-      }
-    }
-  } else {
+    const float mean = sum(s) / (float)n;
 #pragma unroll
     for (int e = 0; e < V; e++)
 #pragma unroll
-      for (int i = 0; i < 8; i++) v[e][i] *= p.x_scale;
+      for (int i = 0; i < 8; i++) {
+        const int c = (t + T * e) * 8;
+        v[e][i] = (WHOLE ? c < n : c + i < n) ? v[e][i] - mean : 0.0f;
+      }
+  }
+  float ss = 0.0f;
+#pragma unroll
+  for (int e = 0; e < V; e++)
+#pragma unroll
+    for (int i = 0; i < 8; i++) ss = __builtin_fmaf(v[e][i], v[e][i], ss);
+  const float inv = inverse_root(sum(ss) / (float)n + norm.eps);
+#pragma unroll
+  for (int e = 0; e < V; e++)
+#pragma unroll
+    for (int i = 0; i < 8; i++) v[e][i] *= inv;
+  if (norm.weight) {
+#pragma unroll
+    for (int e = 0; e < V; e++)
+#pragma unroll
+      for (int i = 0; i < 8; i++) v[e][i] *= by.w[e][i];
+  }
+  if (norm.bias) {
+#pragma unroll
+    for (int e = 0; e < V; e++)
+#pragma unroll
+      for (int i = 0; i < 8; i++) v[e][i] += by.b[e][i];
+  }
+}
+
+template <int V, int T, bool WHOLE, Type X, Type Y>
+__global__ __launch_bounds__(T == 64 ? 256 : T) void residual_norm_kernel(ResidualArgs p, int r0) {
+  constexpr int kRows = T == 64 ? 4 : 1;
+  __shared__ float s_sum[4][RowSum<T>::kWaves];
+  const int t = threadIdx.x % T;
+  const long long row = r0 + (long long)blockIdx.x * kRows + threadIdx.x / T;
+  const int used = p.used ? min(*p.used, p.m) : p.m;
+  if (row >= used) return;  // whole waves; a workgroup of one row as a whole
+  const int n = p.n;
+  RowSum<T> sum{s_sum};
+  float v[V][8], w[V][8], g[V][8];
+  NormWeights<V, T, WHOLE> post, pre;
+#pragma unroll
+  for (int e = 0; e < V; e++)
+    load_chunk<WHOLE, X>(p.x, (size_t)row * p.ldx, (t + T * e) * 8, n, v[e]);
+  if constexpr (Y != kNone) {
+#pragma unroll
+    for (int e = 0; e < V; e++)
+      load_chunk<WHOLE, Y>(p.y, (size_t)row * p.ldy, (t + T * e) * 8, n, w[e]);
+    if (p.gate) {
+#pragma unroll
+      for (int e = 0; e < V; e++)
+        load_chunk<WHOLE, kF32>(p.gate, (size_t)row * p.ldg, (t + T * e) * 8, n, g[e]);
+    }
+    post.load(p.post, n, t);
+  }
+  if constexpr (V == 1) pre.load(p.pre, n, t);
+  if constexpr (Y != kNone) {
+    if (p.post.kind != RH_NORM_NONE) norm_row<V, T, WHOLE>(w, p.post, post, n, t, sum);
+    if (p.gate) {
+#pragma unroll
+      for (int e = 0; e < V; e++)
+#pragma unroll
+        for (int i = 0; i < 8; i++) w[e][i] *= g[e][i];
+    }
   }
 #pragma unroll
   for (int e = 0; e < V; e++) {
     const int c = (t + T * e) * 8;
 #pragma unroll
-    for (int i = 0; i < 8; i++)  // post's bias reaches past the row
-      if (VEC ? c >= n : c + i >= n) v[e][i] = 0.0f;
-    if (p.sum) {
-      if (p.x_bf16) store_chunk<VEC, true>(p.sum, (size_t)row * p.ldsum, c, n, v[e]);
-      else store_chunk<VEC, false>(p.sum, (size_t)row * p.ldsum, c, n, v[e]);
+    for (int i = 0; i < 8; i++) {
+      if constexpr (Y != kNone) v[e][i] = __builtin_fmaf(v[e][i], p.x_scale, w[e][i] * p.y_scale);
+      else v[e][i] *= p.x_scale;
+      if (WHOLE ? c >= n : c + i >= n) v[e][i] = 0.0f;  // what a norm left past the row
     }
+    if (p.sum) store_chunk<WHOLE, X>(p.sum, (size_t)row * p.ldsum, c, n, v[e]);
   }
-  if (p.pre.kind != RH_NORM_NONE) norm_row<V, T, VEC>(v, p.pre, n, t, sum);
+  if constexpr (V > 1) pre.load(p.pre, n, t);  // registers: late
+  if (p.pre.kind != RH_NORM_NONE) norm_row<V, T, WHOLE>(v, p.pre, pre, n, t, sum);
 #pragma unroll
   for (int e = 0; e < V; e++) {
     const int c = (t + T * e) * 8;
     if (p.out) {
-      if (p.out_bf16) store_chunk<VEC, true>(p.out, (size_t)row * p.ldout, c, n, v[e]);
-      else store_chunk<VEC, false>(p.out, (size_t)row * p.ldout, c, n, v[e]);
+      if (p.out_bf16) store_chunk<WHOLE, kBF16>(p.out, (size_t)row * p.ldout, c, n, v[e]);
+      else store_chunk<WHOLE, kF32>(p.out, (size_t)row * p.ldout, c, n, v[e]);
     }
     if (p.qa) {
       uint32_t u = 0;
 #pragma unroll
       for (int i = 0; i < 8; i++) {
-        if (VEC ? c >= n : c + i >= n) v[e][i] = 0.0f;
+        if (WHOLE ? c >= n : c + i >= n) v[e][i] = 0.0f;
         u = max(u, finite_abs_bits(v[e][i]));
       }
 #if defined(__HIP_DEVICE_COMPILE__)
@@ -198,30 +248,41 @@ static bool by_chunks(const ResidualArgs& a) {
          fits(a.pre.weight, 0, 0) && fits(a.pre.bias, 0, 0);
 }
 
-hipError_t launch_residual_norm(const ResidualArgs& a, hipStream_t s) {
-  if (a.m <= 0) return hipSuccess;
-  const bool vec = by_chunks(a);
-  const bool wide = a.n > 1024 || (a.n > 512 && a.m < 1024);  // a workgroup for a row
-  const int chunks = ceil_div(a.n, wide ? 2048 : 512);
-  const int per = wide ? 1 : 4, most = 1 << 23;  // a launch holds fewer than 2^32 threads
-  for (int r0 = 0; r0 < a.m; r0 += std::min(most * per, a.m - r0)) {
-    const int rows = std::min(most * per, a.m - r0);
-    const dim3 grid(ceil_div(rows, per)), block(256);
-#define RH_RN(V, T)                                                                              \
-  {                                                                                              \
-    if (vec) hipLaunchKernelGGL((residual_norm_kernel<V, T, true>), grid, block, 0, s, a, r0);   \
-    else hipLaunchKernelGGL((residual_norm_kernel<V, T, false>), grid, block, 0, s, a, r0);      \
+template <int V, int T, bool WHOLE>
+static void launch_rows(const ResidualArgs& a, int r0, int rows, hipStream_t s) {
+  constexpr int kThreads = T == 64 ? 256 : T;
+  const dim3 grid(ceil_div(rows, kThreads / T)), block(kThreads);
+#define RH_RN(X, Y) \
+  hipLaunchKernelGGL((residual_norm_kernel<V, T, WHOLE, X, Y>), grid, block, 0, s, a, r0)
+  if (a.x_bf16) {
+    if (!a.y) RH_RN(kBF16, kNone);
+    else if (a.y_bf16) RH_RN(kBF16, kBF16);
+    else RH_RN(kBF16, kF32);
+  } else {
+    if (!a.y) RH_RN(kF32, kNone);
+    else if (a.y_bf16) RH_RN(kF32, kBF16);
+    else RH_RN(kF32, kF32);
   }
-    if (wide) {
-      if (chunks <= 1) RH_RN(1, 256)
-      else if (chunks <= 2) RH_RN(2, 256)
-      else if (chunks <= 4) RH_RN(4, 256)
-      else RH_RN(8, 256)
-    } else {
-      if (chunks <= 1) RH_RN(1, 64)
-      else RH_RN(2, 64)
-    }
 #undef RH_RN
+}
+
+template <bool WHOLE>
+static void launch_part(const ResidualArgs& a, int r0, int rows, hipStream_t s) {
+  if (a.n <= 512) launch_rows<1, 64, WHOLE>(a, r0, rows, s);
+  else if (a.n <= 1024) launch_rows<1, 128, WHOLE>(a, r0, rows, s);
+  else if (a.n <= 2048) launch_rows<1, 256, WHOLE>(a, r0, rows, s);
+  else if (a.n <= 4096) launch_rows<1, 512, WHOLE>(a, r0, rows, s);
+  else if (a.n <= 8192) launch_rows<1, 1024, WHOLE>(a, r0, rows, s);
+  else launch_rows<2, 1024, WHOLE>(a, r0, rows, s);
+}
+
+hipError_t launch_residual_norm(const ResidualArgs& a, hipStream_t s) {
+  const bool whole = by_chunks(a);
+  constexpr int kMost = 1 << 21;  // a launch holds fewer than 2^32 threads
+  for (int r0 = 0; r0 < a.m; r0 += std::min(kMost, a.m - r0)) {
+    const int rows = std::min(kMost, a.m - r0);
+    if (whole) launch_part<true>(a, r0, rows, s);
+    else launch_part<false>(a, r0, rows, s);
   }
   return hipGetLastError();
 }
