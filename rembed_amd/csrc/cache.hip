@@ -660,7 +660,7 @@ hipError_t launch_cache_append(const CacheAppendArgs& a, hipStream_t s) {
 // first[b] .. first[b] + count - 1 go to rows cu[b] + position - first[b]. K's 16-byte pieces are
 // runs of a token's values; V's are 16 tokens of one column, so its block goes through LDS
 // (16 more bytes behind every 128: a wave's words then meet all banks) and a thread takes
-// eight columns of four tokens. A code times its power of two is exact in fp32, and in bf16 from
+// eight columns (four of fp32 rows) of four tokens. A code times its power of two is exact in fp32, and in bf16 from
 // its smallest normal value on.
 // Requests are found without a table of their blocks: request b starts at unit
 // cu[b] / 64 + 2 b, which leaves room for the blocks that its count can touch.
@@ -703,10 +703,11 @@ __global__ __launch_bounds__(256) void cache_read_kernel(CacheReadArgs p) {
   const bool here = page >= 0 && page < p.cache.pages;
   const size_t at = here ? (size_t)page * heads + h : 0;
 
-  constexpr int kChunks = DH / 8, kPieces = kBytes / 16 / 256;
-  constexpr int kLoads = kPage * kChunks / 256;  // eight values of K each
-  typedef int v2i __attribute__((ext_vector_type(2)));
-  v2i k[kLoads];
+  constexpr int N = OB ? 8 : 4;  // values of a row: 16 bytes of the output, beside each other's
+  constexpr int kChunks = DH / N, kPieces = kBytes / 16 / 256;
+  constexpr int kLoads = kPage * kChunks / 256;  // N values of K each
+  typedef int W __attribute__((ext_vector_type(N / 4)));
+  W k[kLoads];
   v4i v[kPieces];
   float fk = 0.0f, fv = 0.0f;
   if (here) {
@@ -717,8 +718,8 @@ __global__ __launch_bounds__(256) void cache_read_kernel(CacheReadArgs p) {
       v[i] = *reinterpret_cast<const v4i*>(gv + (tid + i * 256) * 16);
 #pragma unroll
     for (int i = 0; i < kLoads; i++)
-      k[i] = *reinterpret_cast<const v2i*>(
-          gk + k_at(tid / kChunks + i * (256 / kChunks), tid % kChunks * 8));
+      k[i] = *reinterpret_cast<const W*>(
+          gk + k_at(tid / kChunks + i * (256 / kChunks), tid % kChunks * N));
     fk = fp8_power(p.cache.k_exp[at]);
     fv = fp8_power(p.cache.v_exp[at]);
 #pragma unroll
@@ -728,17 +729,17 @@ __global__ __launch_bounds__(256) void cache_read_kernel(CacheReadArgs p) {
     }
   }
   __syncthreads();
-  auto store = [&](int t, int col, const float (&x)[8]) {
-    if (t >= lo && t <= hi) store_values<8, OB>(p.out, (row0 + t) * p.ldout + col, x);
+  auto store = [&](int t, int col, const float (&x)[N]) {
+    if (t >= lo && t <= hi) store_values<N, OB>(p.out, (row0 + t) * p.ldout + col, x);
   };
 #pragma unroll
   for (int i = 0; i < kLoads; i++) {
-    const int t = tid / kChunks + i * (256 / kChunks), d = tid % kChunks * 8;
-    float x[8] = {};
+    const int t = tid / kChunks + i * (256 / kChunks), d = tid % kChunks * N;
+    float x[N] = {};
     if (here) {
       float y[4];
 #pragma unroll
-      for (int w = 0; w < 2; w++) {
+      for (int w = 0; w < N / 4; w++) {
         fp8_unpack4(k[i][w], y);
 #pragma unroll
         for (int e = 0; e < 4; e++) x[4 * w + e] = y[e] * fk;
@@ -747,11 +748,11 @@ __global__ __launch_bounds__(256) void cache_read_kernel(CacheReadArgs p) {
     store(t, p.k_off + h * DH + d, x);
   }
   for (int task = tid; task < kChunks * (kPage / 4); task += 256) {
-    const int d = task % kChunks * 8, t0 = task / kChunks * 4;
-    float x[4][8] = {};
+    const int d = task % kChunks * N, t0 = task / kChunks * 4;
+    float x[4][N] = {};
     if (here) {
 #pragma unroll
-      for (int i = 0; i < 8; i++) {
+      for (int i = 0; i < N; i++) {
         const int byte = v_at(t0, d + i);
         float y[4];
         fp8_unpack4(*reinterpret_cast<const int*>(s_v + byte + byte / 128 * 16), y);

@@ -38,99 +38,120 @@ struct RowSum {
 
 enum Type : int { kNone, kF32, kBF16 };
 
-// Eight values; WHOLE: 16-byte aligned, in the row or behind it; else of any alignment (memory
-// takes 16 bytes at any address), the row's last ones by themselves.
-template <bool WHOLE, Type K>
-__device__ __forceinline__ void load_chunk(const void* base, size_t at, int c, int n, float (&v)[8]) {
-#pragma unroll
-  for (int i = 0; i < 8; i++) v[i] = 0.0f;
-  if constexpr (WHOLE) {
-    if (c < n) load_values<8, K == kBF16>(base, at + c, v);
-  } else {
-    using S = std::conditional_t<K == kBF16, __bf16, float>;
-    typedef S W __attribute__((ext_vector_type(16 / sizeof(S)), aligned(sizeof(S))));
-    constexpr int kW = 16 / sizeof(S);
-    const S* p = static_cast<const S*>(base) + at + c;
-    if (c + 8 <= n) {
-#pragma unroll
-      for (int j = 0; j < 8; j += kW) {
-        const W x = *reinterpret_cast<const W*>(p + j);
-#pragma unroll
-        for (int i = 0; i < kW; i++) v[j + i] = (float)x[i];
+// A thread's eight values: WHOLE: from column c on, 16-byte aligned, in the row or behind it. Else
+// rows of any length and alignment (memory takes 16 bytes at any address): the row's last chunk
+// begins `twice` columns early, so that it ends with the row; what it shares with the chunk before
+// is computed and stored by both, alike, and summed by that one. Rows of under eight values are
+// taken one by one.
+template <bool WHOLE>
+struct Chunk {
+  int from, twice, n;
+  bool here;
+  Chunk() = default;
+  __device__ __forceinline__ Chunk(int c, int n) : from(c), twice(0), n(n), here(c < n) {
+    if constexpr (!WHOLE) {
+      if (here && n >= 8 && c + 8 > n) {
+        from = n - 8;
+        twice = c - from;
       }
-    } else {
-#pragma unroll
-      for (int i = 0; i < 8; i++)
-        if (c + i < n) v[i] = (float)p[i];
     }
   }
-}
-template <bool WHOLE, Type K>
-__device__ __forceinline__ void store_chunk(void* base, size_t at, int c, int n, const float (&v)[8]) {
-  if constexpr (WHOLE) {
-    if (c < n) store_values<8, K == kBF16>(base, at + c, v);
-  } else {
-    using S = std::conditional_t<K == kBF16, __bf16, float>;
-    typedef S W __attribute__((ext_vector_type(16 / sizeof(S)), aligned(sizeof(S))));
-    constexpr int kW = 16 / sizeof(S);
-    S* p = static_cast<S*>(base) + at + c;
-    if (c + 8 <= n) {
+  __device__ __forceinline__ bool inside(int i) const { return here && (WHOLE || i < n); }
+  __device__ __forceinline__ bool counts(int i) const { return inside(i) && (WHOLE || i >= twice); }
+  template <Type K>
+  __device__ __forceinline__ void load(const void* base, size_t at, float (&v)[8]) const {
 #pragma unroll
-      for (int j = 0; j < 8; j += kW) {
-        W x;
-#pragma unroll
-        for (int i = 0; i < kW; i++) x[i] = (S)v[j + i];
-        *reinterpret_cast<W*>(p + j) = x;
-      }
+    for (int i = 0; i < 8; i++) v[i] = 0.0f;
+    if (!here) return;
+    if constexpr (WHOLE) {
+      load_values<8, K == kBF16>(base, at + from, v);
     } else {
+      using S = std::conditional_t<K == kBF16, __bf16, float>;
+      constexpr int kW = 16 / sizeof(S);
+      typedef S W __attribute__((ext_vector_type(kW), aligned(sizeof(S))));
+      const S* p = static_cast<const S*>(base) + at + from;
+      if (n >= 8) {
 #pragma unroll
-      for (int i = 0; i < 8; i++)
-        if (c + i < n) p[i] = (S)v[i];
+        for (int j = 0; j < 8; j += kW) {
+          const W x = *reinterpret_cast<const W*>(p + j);
+#pragma unroll
+          for (int i = 0; i < kW; i++) v[j + i] = (float)x[i];
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < 7; i++)
+          if (i < n) v[i] = (float)p[i];
+      }
     }
   }
-}
-
-// A norm's weights, as the row's chunks.
-template <int V, int T, bool WHOLE>
-struct NormWeights {
-  float w[V][8], b[V][8];
-  __device__ __forceinline__ void load(const rh_norm& norm, int n, int t) {
-    if (norm.weight) {
+  template <Type K>
+  __device__ __forceinline__ void store(void* base, size_t at, const float (&v)[8]) const {
+    if (!here) return;
+    if constexpr (WHOLE) {
+      store_values<8, K == kBF16>(base, at + from, v);
+    } else {
+      using S = std::conditional_t<K == kBF16, __bf16, float>;
+      constexpr int kW = 16 / sizeof(S);
+      typedef S W __attribute__((ext_vector_type(kW), aligned(sizeof(S))));
+      S* p = static_cast<S*>(base) + at + from;
+      if (n >= 8) {
 #pragma unroll
-      for (int e = 0; e < V; e++) load_chunk<WHOLE, kF32>(norm.weight, 0, (t + T * e) * 8, n, w[e]);
-    }
-    if (norm.bias) {
+        for (int j = 0; j < 8; j += kW) {
+          W x;
 #pragma unroll
-      for (int e = 0; e < V; e++) load_chunk<WHOLE, kF32>(norm.bias, 0, (t + T * e) * 8, n, b[e]);
+          for (int i = 0; i < kW; i++) x[i] = (S)v[j + i];
+          __builtin_nontemporal_store(x, reinterpret_cast<W*>(p + j));
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < 7; i++)
+          if (i < n) p[i] = (S)v[i];
+      }
     }
   }
 };
 
-// v normed in place; values past n are zeros before, and anything after.
+// A norm's weights, as the row's chunks.
+template <int V, bool WHOLE>
+struct NormWeights {
+  float w[V][8], b[V][8];
+  __device__ __forceinline__ void load(const rh_norm& norm, const Chunk<WHOLE>* at) {
+    if (norm.weight) {
+#pragma unroll
+      for (int e = 0; e < V; e++) at[e].template load<kF32>(norm.weight, 0, w[e]);
+    }
+    if (norm.bias) {
+#pragma unroll
+      for (int e = 0; e < V; e++) at[e].template load<kF32>(norm.bias, 0, b[e]);
+    }
+  }
+};
+
+// v normed in place; values outside the row are zeros before, and anything after.
 template <int V, int T, bool WHOLE>
 __device__ __forceinline__ void norm_row(float (&v)[V][8], const rh_norm& norm,
-                                         const NormWeights<V, T, WHOLE>& by, int n, int t,
-                                         RowSum<T>& sum) {
+                                         const NormWeights<V, WHOLE>& by, const Chunk<WHOLE>* at,
+                                         int n, RowSum<T>& sum) {
   if (norm.kind == RH_NORM_LAYER) {
     float s = 0.0f;
 #pragma unroll
     for (int e = 0; e < V; e++)
 #pragma unroll
-      for (int i = 0; i < 8; i++) s += v[e][i];
+      for (int i = 0; i < 8; i++) s += at[e].counts(i) ? v[e][i] : 0.0f;
     const float mean = sum(s) / (float)n;
 #pragma unroll
     for (int e = 0; e < V; e++)
 #pragma unroll
-      for (int i = 0; i < 8; i++) {
-        const int c = (t + T * e) * 8;
-        v[e][i] = (WHOLE ? c < n : c + i < n) ? v[e][i] - mean : 0.0f;
-      }
+      for (int i = 0; i < 8; i++) v[e][i] -= mean;
   }
   float ss = 0.0f;
 #pragma unroll
   for (int e = 0; e < V; e++)
 #pragma unroll
-    for (int i = 0; i < 8; i++) ss = __builtin_fmaf(v[e][i], v[e][i], ss);
+    for (int i = 0; i < 8; i++) {
+      const float x = at[e].counts(i) ? v[e][i] : 0.0f;
+      ss = __builtin_fmaf(x, x, ss);
+    }
   const float inv = inverse_root(sum(ss) / (float)n + norm.eps);
 #pragma unroll
   for (int e = 0; e < V; e++)
@@ -160,25 +181,27 @@ __global__ __launch_bounds__(T == 64 ? 256 : T) void residual_norm_kernel(Residu
   if (row >= used) return;  // whole waves; a workgroup of one row as a whole
   const int n = p.n;
   RowSum<T> sum{s_sum};
-  float v[V][8], w[V][8], g[V][8];
-  NormWeights<V, T, WHOLE> post, pre;
+  Chunk<WHOLE> at[V];
 #pragma unroll
-  for (int e = 0; e < V; e++)
-    load_chunk<WHOLE, X>(p.x, (size_t)row * p.ldx, (t + T * e) * 8, n, v[e]);
+  for (int e = 0; e < V; e++) at[e] = Chunk<WHOLE>((t + T * e) * 8, n);
+  float v[V][8], w[V][8], g[V][8];
+  NormWeights<V, WHOLE> post, pre;
+#pragma unroll
+  for (int e = 0; e < V; e++) at[e].template load<X>(p.x, (size_t)row * p.ldx, v[e]);
   if constexpr (Y != kNone) {
 #pragma unroll
-    for (int e = 0; e < V; e++)
-      load_chunk<WHOLE, Y>(p.y, (size_t)row * p.ldy, (t + T * e) * 8, n, w[e]);
+    for (int e = 0; e < V; e++) at[e].template load<Y>(p.y, (size_t)row * p.ldy, w[e]);
     if (p.gate) {
 #pragma unroll
-      for (int e = 0; e < V; e++)
-        load_chunk<WHOLE, kF32>(p.gate, (size_t)row * p.ldg, (t + T * e) * 8, n, g[e]);
+      for (int e = 0; e < V; e++) at[e].template load<kF32>(p.gate, (size_t)row * p.ldg, g[e]);
     }
-    post.load(p.post, n, t);
+    post.load(p.post, at);
   }
-  if constexpr (V == 1) pre.load(p.pre, n, t);
+  if constexpr (V == 1) pre.load(p.pre, at);
+  // a chunk's shared values may be another wave's to store, where an output lies on its input
+  if constexpr (!WHOLE && T > 64) __syncthreads();
   if constexpr (Y != kNone) {
-    if (p.post.kind != RH_NORM_NONE) norm_row<V, T, WHOLE>(w, p.post, post, n, t, sum);
+    if (p.post.kind != RH_NORM_NONE) norm_row<V, T, WHOLE>(w, p.post, post, at, n, sum);
     if (p.gate) {
 #pragma unroll
       for (int e = 0; e < V; e++)
@@ -188,30 +211,29 @@ __global__ __launch_bounds__(T == 64 ? 256 : T) void residual_norm_kernel(Residu
   }
 #pragma unroll
   for (int e = 0; e < V; e++) {
-    const int c = (t + T * e) * 8;
 #pragma unroll
     for (int i = 0; i < 8; i++) {
       if constexpr (Y != kNone) v[e][i] = __builtin_fmaf(v[e][i], p.x_scale, w[e][i] * p.y_scale);
       else v[e][i] *= p.x_scale;
-      if (WHOLE ? c >= n : c + i >= n) v[e][i] = 0.0f;  // what a norm left past the row
+      if (!at[e].inside(i)) v[e][i] = 0.0f;  // what a norm left there
     }
-    if (p.sum) store_chunk<WHOLE, X>(p.sum, (size_t)row * p.ldsum, c, n, v[e]);
+    if (p.sum) at[e].template store<X>(p.sum, (size_t)row * p.ldsum, v[e]);
   }
-  if constexpr (V > 1) pre.load(p.pre, n, t);  // registers: late
-  if (p.pre.kind != RH_NORM_NONE) norm_row<V, T, WHOLE>(v, p.pre, pre, n, t, sum);
+  if constexpr (V > 1) pre.load(p.pre, at);  // registers: late
+  if (p.pre.kind != RH_NORM_NONE) norm_row<V, T, WHOLE>(v, p.pre, pre, at, n, sum);
 #pragma unroll
   for (int e = 0; e < V; e++) {
     const int c = (t + T * e) * 8;
     if (p.out) {
-      if (p.out_bf16) store_chunk<WHOLE, kBF16>(p.out, (size_t)row * p.ldout, c, n, v[e]);
-      else store_chunk<WHOLE, kF32>(p.out, (size_t)row * p.ldout, c, n, v[e]);
+      if (p.out_bf16) at[e].template store<kBF16>(p.out, (size_t)row * p.ldout, v[e]);
+      else at[e].template store<kF32>(p.out, (size_t)row * p.ldout, v[e]);
     }
     if (p.qa) {
       uint32_t u = 0;
 #pragma unroll
       for (int i = 0; i < 8; i++) {
-        if (WHOLE ? c >= n : c + i >= n) v[e][i] = 0.0f;
-        u = max(u, finite_abs_bits(v[e][i]));
+        if (!at[e].inside(i)) v[e][i] = 0.0f;
+        if (at[e].counts(i)) u = max(u, finite_abs_bits(v[e][i]));
       }
 #if defined(__HIP_DEVICE_COMPILE__)
 #define RH_ROR(n) u = max(u, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)u, 0x120 + n, 0xF, 0xF, true))
@@ -224,11 +246,10 @@ __global__ __launch_bounds__(T == 64 ? 256 : T) void residual_norm_kernel(Residu
       if (c < p.ldq) {  // a multiple of 128: whole groups of 16 lanes
         const int x = fp8_exponent(u);
         const float f = fp8_inverse(x);
-        typedef int v2i __attribute__((ext_vector_type(2)));
-        v2i q;
-        q[0] = fp8_pack4(v[e][0] * f, v[e][1] * f, v[e][2] * f, v[e][3] * f);
-        q[1] = fp8_pack4(v[e][4] * f, v[e][5] * f, v[e][6] * f, v[e][7] * f);
-        __builtin_nontemporal_store(q, reinterpret_cast<v2i*>(p.qa + (size_t)row * p.ldq + c));
+        uint64_t q = (uint32_t)fp8_pack4(v[e][4] * f, v[e][5] * f, v[e][6] * f, v[e][7] * f);
+        q = q << 32 | (uint32_t)fp8_pack4(v[e][0] * f, v[e][1] * f, v[e][2] * f, v[e][3] * f);
+        if constexpr (!WHOLE) q >>= 8 * at[e].twice;  // and zeros behind the row
+        __builtin_nontemporal_store(q, reinterpret_cast<uint64_t*>(p.qa + (size_t)row * p.ldq + c));
         if (t % 16 == 0)
           p.sa[fp8_scale_at((int)row, c / kFp8Block, (p.m + 127) / 128)] = (uint8_t)x;
       }

@@ -7,6 +7,7 @@
 #include "rope_rows.h"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace rh {
 
@@ -16,62 +17,75 @@ __global__ __launch_bounds__(kRopeThreads) void rope_rows_kernel(RopeArgs p, Rop
   rope_rows<LPH, P, XB, OB, ITEMS>(p, share, blockIdx.x, lds);
 }
 
-// Heads of any even size, rows of any alignment: a wave takes a head at a time, a lane the pairs
-// lane and lane + 64.
-template <bool XB, bool OB>
-__global__ __launch_bounds__(256) void rope_any_kernel(RopeArgs p) {
+// Heads of any even size, rows of any alignment: a wave takes ITEMS heads of a row, a lane the
+// pairs lane and (E = 2) lane + 64 of them, one value a load, and their cosines once.
+template <bool XB, bool OB, int E, int ITEMS>
+__global__ __launch_bounds__(256) void rope_any_kernel(RopeArgs p, int sets) {
+  using X = std::conditional_t<XB, __bf16, float>;
+  using Y = std::conditional_t<OB, __bf16, float>;
   const int lane = threadIdx.x & 63;
-  const int nh = p.heads + p.kv_heads + p.v_heads;
-  const long long items = (long long)rope_used(p) * nh, step = (long long)gridDim.x * 4;
-  for (long long it = (long long)blockIdx.x * 4 + (threadIdx.x >> 6); it < items; it += step) {
-    const int row = (int)(it / nh), h = (int)(it - (long long)row * nh);
-    const RopeHead at(p, h, p.dh);
-    const size_t in = (size_t)row * p.ldx + at.in, out = (size_t)row * p.ldout + at.out;
-    float a[2], b[2], ss = 0.0f;
-    int ia[2], ib[2];
+  const int nh = p.heads + p.kv_heads + p.v_heads, used = rope_used(p);
+  const long long units = (long long)used * sets, step = (long long)gridDim.x * 4;
+  int ia[E], ib[E];
+  bool in[E];
 #pragma unroll
-    for (int e = 0; e < 2; e++) {
+  for (int e = 0; e < E; e++) {
+    const int j = lane + 64 * e;
+    const bool apart = p.turn.halves && j < p.turn.pairs;
+    in[e] = j < p.dh / 2;
+    ia[e] = !in[e] ? 0 : apart ? j : 2 * j;
+    ib[e] = !in[e] ? 0 : apart ? j + p.turn.pairs : 2 * j + 1;
+  }
+  for (long long u = (long long)blockIdx.x * 4 + (threadIdx.x >> 6); u < units; u += step) {
+    const int row = (int)(u / sets), set = (int)(u - (long long)row * sets);
+    const X* x = static_cast<const X*>(p.x) + (size_t)row * p.ldx;
+    Y* y = static_cast<Y*>(p.out) + (size_t)row * p.ldout;
+    float a[ITEMS][E], b[ITEMS][E];
+#pragma unroll
+    for (int k = 0; k < ITEMS; k++) {  // behind the last head: that one, not used
+      const int from = RopeHead(p, min(set + k * sets, nh - 1), p.dh).in;
+#pragma unroll
+      for (int e = 0; e < E; e++) {
+        a[k][e] = (float)x[from + ia[e]];
+        b[k][e] = (float)x[from + ib[e]];
+      }
+    }
+    const int t = p.pos[row];
+    float c[E], s[E];
+#pragma unroll
+    for (int e = 0; e < E; e++) {
       const int j = lane + 64 * e;
-      const bool apart = p.turn.halves && j < p.turn.pairs;
-      ia[e] = apart ? j : 2 * j;
-      ib[e] = apart ? j + p.turn.pairs : 2 * j + 1;
-      a[e] = b[e] = 0.0f;
-      if (j < p.dh / 2) {
-        if constexpr (XB) {
-          a[e] = (float)static_cast<const __bf16*>(p.x)[in + ia[e]];
-          b[e] = (float)static_cast<const __bf16*>(p.x)[in + ib[e]];
-        } else {
-          a[e] = static_cast<const float*>(p.x)[in + ia[e]];
-          b[e] = static_cast<const float*>(p.x)[in + ib[e]];
+      c[e] = 1.0f;
+      s[e] = 0.0f;
+      if (j < p.turn.pairs) turn_cos_sin(turn_at(p.turn.freq[j], t), p.turn.amp, c[e], s[e]);
+    }
+#pragma unroll
+    for (int k = 0; k < ITEMS; k++) {
+      if (set + k * sets >= nh) break;
+      const RopeHead at(p, set + k * sets, p.dh);
+      const HeadNorm& norm = at.part == 0 ? p.q_norm : p.k_norm;
+      if (at.part < 2 && norm.on) {
+        float ss = 0.0f;
+#pragma unroll
+        for (int e = 0; e < E; e++)
+          if (in[e]) ss = __builtin_fmaf(a[k][e], a[k][e], __builtin_fmaf(b[k][e], b[k][e], ss));
+        const float inv = inverse_root(group_sum<64>(ss) / (float)p.dh + norm.eps);
+#pragma unroll
+        for (int e = 0; e < E; e++) {
+          a[k][e] = a[k][e] * inv * (norm.weight ? norm.weight[ia[e]] : 1.0f);
+          b[k][e] = b[k][e] * inv * (norm.weight ? norm.weight[ib[e]] : 1.0f);
         }
       }
-      ss += a[e] * a[e] + b[e] * b[e];
-    }
-    const HeadNorm norm = at.part == 0 ? p.q_norm : p.k_norm;
-    const bool normed = at.part < 2 && norm.on;
-    const float inv = inverse_root(group_sum<64>(ss) / (float)p.dh + norm.eps);
-    const int t = p.pos[row];
 #pragma unroll
-    for (int e = 0; e < 2; e++) {
-      const int j = lane + 64 * e;
-      if (j >= p.dh / 2) continue;
-      if (normed) {
-        a[e] = a[e] * inv * (norm.weight ? norm.weight[ia[e]] : 1.0f);
-        b[e] = b[e] * inv * (norm.weight ? norm.weight[ib[e]] : 1.0f);
-      }
-      if (at.part < 2 && j < p.turn.pairs) {
-        float c, s;
-        turn_cos_sin(turn_at(p.turn.freq[j], t), p.turn.amp, c, s);
-        const float x = a[e], y = b[e];
-        a[e] = __builtin_fmaf(x, c, -(y * s));
-        b[e] = __builtin_fmaf(y, c, x * s);
-      }
-      if constexpr (OB) {
-        static_cast<__bf16*>(p.out)[out + ia[e]] = (__bf16)a[e];
-        static_cast<__bf16*>(p.out)[out + ib[e]] = (__bf16)b[e];
-      } else {
-        static_cast<float*>(p.out)[out + ia[e]] = a[e];
-        static_cast<float*>(p.out)[out + ib[e]] = b[e];
+      for (int e = 0; e < E; e++) {
+        if (!in[e]) continue;
+        float v = a[k][e], w = b[k][e];
+        if (at.part < 2 && lane + 64 * e < p.turn.pairs) {
+          v = __builtin_fmaf(a[k][e], c[e], -(b[k][e] * s[e]));
+          w = __builtin_fmaf(b[k][e], c[e], a[k][e] * s[e]);
+        }
+        y[at.out + ia[e]] = (Y)v;
+        y[at.out + ib[e]] = (Y)w;
       }
     }
   }
@@ -94,15 +108,29 @@ hipError_t launch_rope_rows(const RopeArgs& a, hipStream_t s) {
   const long long nh = (long long)a.heads + a.kv_heads + a.v_heads;
   if (a.rows <= 0 || nh == 0) return hipSuccess;
   if (!rope_by_lanes(a)) {
-    const unsigned wgs = (unsigned)std::min((nh * a.rows + 3) / 4, 1LL << 20);
-#define RH_ANY(X, O) hipLaunchKernelGGL((rope_any_kernel<X, O>), dim3(wgs), dim3(256), 0, s, a)
+    const bool many = nh * a.rows >= kRopeItems * 2048LL;  // waves: as rope_share
+    const int sets = (int)(many ? (nh + kRopeItems - 1) / kRopeItems : nh);
+    const unsigned wgs = (unsigned)std::min(((long long)sets * a.rows + 3) / 4, 1LL << 20);
+#define RH_ANY(X, O, E, I) \
+  hipLaunchKernelGGL((rope_any_kernel<X, O, E, I>), dim3(wgs), dim3(256), 0, s, a, sets)
+#define RH_PAIRS(X, O)                                   \
+  {                                                      \
+    if (a.dh > 128) {                                    \
+      if (many) RH_ANY(X, O, 2, kRopeItems);             \
+      else RH_ANY(X, O, 2, 1);                           \
+    } else {                                             \
+      if (many) RH_ANY(X, O, 1, kRopeItems);             \
+      else RH_ANY(X, O, 1, 1);                           \
+    }                                                    \
+  }
     if (a.x_bf16) {
-      if (a.out_bf16) RH_ANY(true, true);
-      else RH_ANY(true, false);
+      if (a.out_bf16) RH_PAIRS(true, true)
+      else RH_PAIRS(true, false)
     } else {
-      if (a.out_bf16) RH_ANY(false, true);
-      else RH_ANY(false, false);
+      if (a.out_bf16) RH_PAIRS(false, true)
+      else RH_PAIRS(false, false)
     }
+#undef RH_PAIRS
 #undef RH_ANY
     return hipGetLastError();
   }
