@@ -42,22 +42,49 @@ inline RopeShare rope_share(const RopeArgs& a, int lanes) {
   RopeShare s;
   s.many = nh * lanes * a.rows >= kRopeItems * 512LL * kRopeThreads;
   s.sets = (int)(s.many ? (nh + kRopeItems - 1) / kRopeItems : nh);
-  s.each = std::min(s.sets, kRopeThreads / lanes);
-  s.slices = (s.sets + s.each - 1) / s.each;
+  s.slices = (s.sets - 1) / (kRopeThreads / lanes) + 1;
+  s.each = (s.sets - 1) / s.slices + 1;  // slices of one size
   s.group = std::max(1, std::min(kRopeThreads / (s.each * lanes), kRopePairs / a.turn.pairs));
   s.group = std::min(s.group, a.rows / 512 + 1);
   s.first = 0;
   return s;
 }
 
-// A lane takes P pairs of a head, 16 bytes of each half, LPH lanes a head; a thread ITEMS heads of
-// a row. The rows' cosines and sines are in LDS once for all heads. lds: 2 * kRopePairs +
-// 4 * LPH * P floats, 16-byte aligned.
-template <int LPH, int P, bool XB, bool OB, int ITEMS>
+// P values of a row as loaded. ANY: of any alignment, else 16 bytes.
+template <int P, bool BF16, bool ANY>
+struct RopeRun {
+  using S = std::conditional_t<BF16, __bf16, float>;
+  typedef S W __attribute__((ext_vector_type(P), aligned(ANY ? sizeof(S) : 16)));
+  W raw;
+  __device__ __forceinline__ void load(const S* p) { raw = *reinterpret_cast<const W*>(p); }
+  __device__ __forceinline__ void widen(float (&v)[P]) const {
+#pragma unroll
+    for (int i = 0; i < P; i++) v[i] = (float)raw[i];
+  }
+};
+template <int P, bool BF16, bool ANY>
+__device__ __forceinline__ void store_run(void* base, size_t at, const float (&v)[P]) {
+  if constexpr (!ANY) {
+    store_values<P, BF16>(base, at, v);
+  } else {
+    using S = std::conditional_t<BF16, __bf16, float>;
+    typedef S W __attribute__((ext_vector_type(P), aligned(sizeof(S))));
+    W x;
+#pragma unroll
+    for (int i = 0; i < P; i++) x[i] = (S)v[i];
+    __builtin_nontemporal_store(x, reinterpret_cast<W*>(static_cast<S*>(base) + at));
+  }
+}
+
+// A lane takes P pairs of a head, LPH lanes a head; a thread ITEMS heads of a row. The rows'
+// cosines and sines are in LDS once for all heads. ANY: heads of up to LPH * 2 P values and rows of
+// any alignment; else heads of so many, and a lane's halves are 16 bytes each. lds:
+// 2 * kRopePairs + 4 * LPH * P floats, 16-byte aligned.
+template <int LPH, int P, bool XB, bool OB, int ITEMS, bool ANY = false>
 __device__ __forceinline__ void rope_rows(const RopeArgs& p, const RopeShare& share, unsigned block,
                                           float* lds) {
-  static_assert(P == (XB ? 8 : 4), "16 bytes");
-  constexpr int DH = LPH * 2 * P;
+  static_assert(ANY || P == (XB ? 8 : 4), "16 bytes");
+  const int DH = ANY ? p.dh : LPH * 2 * P;
   float *s_cos = lds, *s_sin = lds + kRopePairs, *s_w = lds + 2 * kRopePairs;
   const int tid = threadIdx.x, l = tid % LPH;
   const int nh = p.heads + p.kv_heads + p.v_heads, pairs = p.turn.pairs;
@@ -65,24 +92,26 @@ __device__ __forceinline__ void rope_rows(const RopeArgs& p, const RopeShare& sh
   const int r0 = share.first + (int)(block / share.slices) * share.group;
   const int nr = min(share.group, used - r0);
   if (nr <= 0) return;
-  const RopePlace<P> at(p.turn, l);
+  const bool in = !ANY || l * 2 * P < DH;
+  const RopePlace<P> at(p.turn, in ? l : 0);
   // the thread's row of these, and its heads set, set + sets, ..
   const int unit = tid / LPH, row = unit / share.each;
   const int set = (int)(block % share.slices) * share.each + unit - row * share.each;
   const bool mine = row < nr && set < share.sets;
   using S = std::conditional_t<XB, __bf16, float>;
   const S* x = static_cast<const S*>(p.x) + (size_t)(r0 + min(row, nr - 1)) * p.ldx;
-  v4i a[ITEMS], b[ITEMS];
+  RopeRun<P, XB, ANY> a[ITEMS], b[ITEMS];
 #pragma unroll
   for (int k = 0; k < ITEMS; k++) {  // behind the last head: that one, not used
     const int from = RopeHead(p, min(set + k * share.sets, nh - 1), DH).in;
-    a[k] = *reinterpret_cast<const v4i*>(x + from + at.a);
-    b[k] = *reinterpret_cast<const v4i*>(x + from + at.b);
+    a[k].load(x + from + at.a);
+    b[k].load(x + from + at.b);
   }
   if (p.q_norm.on || p.k_norm.on)
     for (int i = tid; i < 2 * DH; i += kRopeThreads) {
-      const float* w = i < DH ? p.q_norm.weight : p.k_norm.weight;
-      s_w[i] = w ? w[i % DH] : 1.0f;
+      const bool q = i < DH;
+      const float* w = q ? p.q_norm.weight : p.k_norm.weight;
+      s_w[i] = w ? w[q ? i : i - DH] : 1.0f;
     }
   for (int i = tid; i < nr * pairs; i += kRopeThreads) {
     const int t = i / pairs;
@@ -92,8 +121,8 @@ __device__ __forceinline__ void rope_rows(const RopeArgs& p, const RopeShare& sh
   if (!mine) return;
   float c[P], s[P];
   if (at.turns) {
-    load_floats(s_cos + row * pairs + l * P, c);
-    load_floats(s_sin + row * pairs + l * P, s);
+    load_floats(s_cos + row * pairs + at.chunk * P, c);
+    load_floats(s_sin + row * pairs + at.chunk * P, s);
   }
 #pragma unroll
   for (int k = 0; k < ITEMS; k++) {
@@ -102,12 +131,13 @@ __device__ __forceinline__ void rope_rows(const RopeArgs& p, const RopeShare& sh
     const RopeHead head(p, h, DH);
     const HeadNorm& norm = head.part == 0 ? p.q_norm : p.k_norm;
     float y[P], z[P];
-    widen<XB>(a[k], y);
-    widen<XB>(b[k], z);
+    a[k].widen(y);
+    b[k].widen(z);
     if (head.part < 2 && norm.on) {
       float ss = 0.0f;
 #pragma unroll
       for (int i = 0; i < P; i++) ss = __builtin_fmaf(y[i], y[i], __builtin_fmaf(z[i], z[i], ss));
+      if (!in) ss = 0.0f;
       const float inv = inverse_root(group_sum<LPH>(ss) / (float)DH + norm.eps);
       float w[P];
       load_floats(s_w + (head.part ? DH : 0) + at.a, w);
@@ -118,9 +148,11 @@ __device__ __forceinline__ void rope_rows(const RopeArgs& p, const RopeShare& sh
       for (int i = 0; i < P; i++) z[i] = z[i] * inv * w[i];
     }
     if (head.part < 2 && at.turns) rope_turn<P>(y, z, c, s, p.turn.halves);
-    const size_t to = (size_t)(r0 + row) * p.ldout + head.out;
-    store_values<P, OB>(p.out, to + at.a, y);
-    store_values<P, OB>(p.out, to + at.b, z);
+    if (in) {
+      const size_t to = (size_t)(r0 + row) * p.ldout + head.out;
+      store_run<P, OB, ANY>(p.out, to + at.a, y);
+      store_run<P, OB, ANY>(p.out, to + at.b, z);
+    }
   }
 }
 

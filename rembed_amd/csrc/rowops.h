@@ -80,7 +80,7 @@ __device__ __forceinline__ void store_values(void* base, size_t at, const float 
   }
 }
 
-// 16 bytes of a row as values, and 16 (4 aligned floats) of LDS.
+// 16 bytes of a row as values, and N aligned floats of LDS.
 template <bool BF16, int N>
 __device__ __forceinline__ void widen(const v4i& raw, float (&v)[N], int at = 0) {
   if constexpr (BF16) {
@@ -95,11 +95,13 @@ __device__ __forceinline__ void widen(const v4i& raw, float (&v)[N], int at = 0)
 }
 template <int N>
 __device__ __forceinline__ void load_floats(const float* lds, float (&v)[N]) {
+  constexpr int W = N < 4 ? N : 4;
+  typedef float T __attribute__((ext_vector_type(W)));
 #pragma unroll
-  for (int j = 0; j < N; j += 4) {
-    const v4f x = *reinterpret_cast<const v4f*>(lds + j);
+  for (int j = 0; j < N; j += W) {
+    const T x = *reinterpret_cast<const T*>(lds + j);
 #pragma unroll
-    for (int e = 0; e < 4; e++) v[j + e] = x[e];
+    for (int e = 0; e < W; e++) v[j + e] = x[e];
   }
 }
 
@@ -153,9 +155,9 @@ __device__ __forceinline__ void turn_cos_sin(uint32_t turn, float amp, float& c,
 // a chunk is 2 P consecutive values, of either layout.
 template <int P>
 struct RopePlace {
-  int a, b;
+  int chunk, a, b;
   bool turns;
-  __device__ __forceinline__ RopePlace(const RopeTurn& t, int l) {
+  __device__ __forceinline__ RopePlace(const RopeTurn& t, int l) : chunk(l) {
     turns = l * P < t.pairs;
     const bool apart = turns && t.halves;
     a = apart ? l * P : 2 * l * P;
