@@ -277,27 +277,42 @@ __device__ __forceinline__ int spread(int at) {
 }
 
 // What a turning workgroup holds of K's norm and, of few tokens, their cosines and sines: those
-// are then made by all threads rather than by the tokens' own four.
+// are then made by all threads rather than by the tokens' own.
 struct AppendTurn {
   static constexpr int kPairs = 256;
   float w[256], c[kPairs], s[kPairs];
 };
 
-// TURN: K's heads are normed and turned (rope.h) on the way, in fp32. Four lanes have a token
-// here too, each every fourth chunk of eight pairs.
+// TURN: K's heads are normed and turned (rowops.h) on the way, in fp32, a thread every PARTS-th
+// chunk of eight pairs of its token. Heads of 256 take eight threads a token there: with four, 200
+// registers left a CU two workgroups (22.8k tokens of 4 kv heads: 46.4 µs, with eight 40.6; 48
+// single tokens of one: 8.7, with eight 6.4).
+template <int DH, bool TURN>
+constexpr int kAppendParts = TURN && DH == 256 ? 8 : 4;  // threads of a token
 template <int DH, bool BF16, bool TURN>
 __device__ __forceinline__ void append_block(const CacheAppendArgs& p, const RopeArgs& rope,
                                              unsigned block, uint8_t* s_k, uint8_t* s_v,
                                              uint32_t (*s_max)[2], AppendTurn* s_turn) {
-  constexpr int kBytes = kPage * DH, E = DH / 4;  // a head's block; values per thread
+  constexpr int PARTS = kAppendParts<DH, TURN>, THREADS = 64 * PARTS;
+  constexpr int kBytes = kPage * DH, E = DH / PARTS;  // a head's block; values per thread
   const int tid = threadIdx.x;
   const int heads = p.cache.kv_heads;
   const int seg = block / heads, h = block % heads;
+  // of few tokens, thread by thread: the pair, and its token if that is of the request's first block
+  RopeFreq freq{};
+  int turn_token = 0;
+  if constexpr (TURN) {
+    turn_token = tid / rope.turn.pairs;
+    freq = rope.turn.freq[tid - turn_token * rope.turn.pairs];
+    if (rope.k_norm.on && tid < DH) s_turn->w[tid] = rope.k_norm.weight ? rope.k_norm.weight[tid] : 1.0f;
+  }
   const int b = append_request(p.blocks, p.batch, seg, tid & 63);
   if (seg >= p.blocks[p.batch]) return;
   const int j = seg - p.blocks[b];
   const int r0 = p.cu[b], fresh = p.cu[b + 1] - r0;
   if (r0 < 0 || fresh <= 0 || r0 + (long long)fresh > p.rows) return;
+  int turn_pos = 0;
+  if constexpr (TURN) turn_pos = rope.pos[r0 + min(turn_token, fresh - 1)];
   // a row of this block, wherever in its first block the request starts
   const int probe = j > (fresh - 1) / kPage ? fresh - 1 : j * kPage;
   int64_t start = p.slots[r0];
@@ -309,9 +324,9 @@ __device__ __forceinline__ void append_block(const CacheAppendArgs& p, const Rop
   const int cnt = min(kPage - off, fresh - first);
   if (cnt <= 0) return;
 
-  // every fourth 16 bytes of its token's K and V to a thread (so a load of a token's four takes 64
-  // bytes at a time); four lanes beside each other have the four tokens of one word of V
-  const int tok = tid / 16 * 4 + tid % 4, quarter = tid / 4 % 4;
+  // every fourth (PARTS-th) 16 bytes of its token's K and V to a thread (so a load of a token's four
+  // takes 64 bytes at a time); four lanes beside each other have the four tokens of one word of V
+  const int tok = tid / (4 * PARTS) * 4 + tid % 4, part = tid / 4 % PARTS;
   const bool mine = tok >= off && tok < off + cnt;
   using T = std::conditional_t<BF16, v8bf, v4f>;  // 16 bytes of a row, widened when used
   constexpr int kStep = BF16 ? 8 : 4;
@@ -321,14 +336,14 @@ __device__ __forceinline__ void append_block(const CacheAppendArgs& p, const Rop
   const int row_at = r0 + first + tok - off;
   int pos = 0;
   if (mine) {
-    const size_t at = (size_t)row_at * p.ldkv + h * DH + quarter * kStep;
+    const size_t at = (size_t)row_at * p.ldkv + h * DH + part * kStep;
     using S = std::conditional_t<BF16, __bf16, float>;
     const S* row = static_cast<const S*>(p.kv) + at;
     if constexpr (TURN) pos = rope.pos[row_at];
 #pragma unroll
     for (int e = 0; e < E / kStep; e++) {
-      if constexpr (!TURN) k[e] = *reinterpret_cast<const T*>(row + p.k_off + e * 4 * kStep);
-      v[e] = *reinterpret_cast<const T*>(row + p.v_off + e * 4 * kStep);
+      if constexpr (!TURN) k[e] = *reinterpret_cast<const T*>(row + p.k_off + e * PARTS * kStep);
+      v[e] = *reinterpret_cast<const T*>(row + p.v_off + e * PARTS * kStep);
     }
   }
   constexpr int kRaw = BF16 ? 1 : 2;  // 16 bytes each, of eight values
@@ -340,7 +355,7 @@ __device__ __forceinline__ void append_block(const CacheAppendArgs& p, const Rop
       const S* x = static_cast<const S*>(p.kv) + (size_t)row_at * p.ldkv + p.k_off + h * DH;
 #pragma unroll
       for (int j = 0; j < E / 16; j++) {
-        const RopePlace<8> to(rope.turn, quarter + 4 * j);
+        const RopePlace<8> to(rope.turn, part + PARTS * j);
 #pragma unroll
         for (int i = 0; i < kRaw; i++) {
           raw[j][0][i] = *reinterpret_cast<const v4i*>(x + to.a + i * kStep);
@@ -348,12 +363,10 @@ __device__ __forceinline__ void append_block(const CacheAppendArgs& p, const Rop
         }
       }
     }
-    if (rope.k_norm.on && tid < DH) s_turn->w[tid] = rope.k_norm.weight ? rope.k_norm.weight[tid] : 1.0f;
     few_turns = cnt * rope.turn.pairs <= AppendTurn::kPairs;
-    if (few_turns && tid < cnt * rope.turn.pairs) {
-      const int t = tid / rope.turn.pairs;
-      turn_cos_sin(turn_at(rope.turn.freq[tid - t * rope.turn.pairs], rope.pos[r0 + first + t]),
-                   rope.turn.amp, s_turn->c[tid], s_turn->s[tid]);
+    if (few_turns && turn_token < cnt) {
+      if (first) turn_pos = rope.pos[r0 + first + turn_token];
+      turn_cos_sin(turn_at(freq, turn_pos), rope.turn.amp, s_turn->c[tid], s_turn->s[tid]);
     }
     __syncthreads();
   }
@@ -379,15 +392,16 @@ __device__ __forceinline__ void append_block(const CacheAppendArgs& p, const Rop
 #if defined(__HIP_DEVICE_COMPILE__)
 #define RH_ROR(n)                                                                                 \
   ss += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(ss), 0x120 + n, 0xF, 0xF, true))
-    RH_ROR(4);  // the token's four lanes
+    RH_ROR(4);  // the token's lanes
     RH_ROR(8);
 #undef RH_ROR
 #endif
+    if constexpr (PARTS == 8) ss += __shfl_xor(ss, 16, 64);
     if (mine) {
       const float inv = inverse_root(ss / (float)DH + rope.k_norm.eps);
 #pragma unroll
       for (int j = 0; j < E / 16; j++) {
-        const int chunk = quarter + 4 * j;
+        const int chunk = part + PARTS * j;
         const RopePlace<8> to(rope.turn, chunk);
         if (rope.k_norm.on) {
 #pragma unroll
@@ -428,6 +442,7 @@ __device__ __forceinline__ void append_block(const CacheAppendArgs& p, const Rop
   int bad = mk >= 0x7F800000u || mv >= 0x7F800000u;
   bad |= __shfl_xor(bad, 4, 64);
   bad |= __shfl_xor(bad, 8, 64);
+  if constexpr (PARTS == 8) bad |= __shfl_xor(bad, 16, 64);
   if (bad) mk = mv = 0;
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) {
@@ -441,7 +456,7 @@ __device__ __forceinline__ void append_block(const CacheAppendArgs& p, const Rop
   if (!here) return;  // the whole workgroup
   __syncthreads();
 #pragma unroll
-  for (int w = 0; w < kAppendThreads / 64; w++) {
+  for (int w = 0; w < THREADS / 64; w++) {
     mk = max(mk, s_max[w][0]);
     mv = max(mv, s_max[w][1]);
   }
@@ -455,7 +470,7 @@ __device__ __forceinline__ void append_block(const CacheAppendArgs& p, const Rop
   };
   if (off == 0) {
     if (cnt < kPage) {
-      for (int i = tid * 16; i < kBytes; i += kAppendThreads * 16) {
+      for (int i = tid * 16; i < kBytes; i += THREADS * 16) {
         *reinterpret_cast<v4i*>(s_k + i) = v4i{0, 0, 0, 0};
         *reinterpret_cast<v4i*>(s_v + i) = v4i{0, 0, 0, 0};
       }
@@ -466,7 +481,7 @@ __device__ __forceinline__ void append_block(const CacheAppendArgs& p, const Rop
     whole_v = xv > ov;
     xk = max(xk, ok);
     xv = max(xv, ov);
-    for (int i = tid * 16; i < kBytes && (whole_k || whole_v); i += kAppendThreads * 16) {
+    for (int i = tid * 16; i < kBytes && (whole_k || whole_v); i += THREADS * 16) {
       v4i a, c;
       if (whole_k) a = *reinterpret_cast<const v4i*>(gk + i);
       if (whole_v) c = *reinterpret_cast<const v4i*>(gv + i);
@@ -498,7 +513,7 @@ __device__ __forceinline__ void append_block(const CacheAppendArgs& p, const Rop
       }
     }
     // value e of the thread lies at this one of the row
-    auto place = [&](int e) { return (e / kStep * 4 + quarter) * kStep + e % kStep; };
+    auto place = [&](int e) { return (e / kStep * PARTS + part) * kStep + e % kStep; };
     constexpr int kRun = TURN ? 8 : kStep;  // values of K beside each other
     typedef int W __attribute__((ext_vector_type(kRun / 4)));
 #pragma unroll
@@ -508,7 +523,7 @@ __device__ __forceinline__ void append_block(const CacheAppendArgs& p, const Rop
       for (int i = 0; i < kRun / 4; i++) w[i] = wk[e / 4 + i];
       int d = place(e);
       if constexpr (TURN) {
-        const RopePlace<8> to(rope.turn, quarter + e / 16 * 4);
+        const RopePlace<8> to(rope.turn, part + e / 16 * PARTS);
         d = e / 8 % 2 ? to.b : to.a;
       }
       *reinterpret_cast<W*>((whole_k ? s_k : gk) + k_at(tok, d)) = w;
@@ -544,11 +559,11 @@ __device__ __forceinline__ void append_block(const CacheAppendArgs& p, const Rop
   }
   if (few) {
     __syncthreads();
-    for (int i = tid; i < cnt * DH; i += kAppendThreads) gv[v_at(off + i / DH, i % DH)] = s_v[i];
+    for (int i = tid; i < cnt * DH; i += THREADS) gv[v_at(off + i / DH, i % DH)] = s_v[i];
   }
   if (!whole_k && !whole_v) return;  // the scales stay as well
   __syncthreads();
-  for (int i = tid * 16; i < kBytes; i += kAppendThreads * 16) {
+  for (int i = tid * 16; i < kBytes; i += THREADS * 16) {
     // whole lines, past the L2, whose own would be written back at the kernel's end
     if (whole_k)
       __builtin_nontemporal_store(*reinterpret_cast<const v4i*>(s_k + i),
@@ -585,22 +600,21 @@ __device__ __forceinline__ unsigned blocks_before(unsigned w, unsigned blocks, u
 }
 
 template <int DH, bool BF16, bool OB, int ITEMS>
-__global__ __launch_bounds__(kAppendThreads) void rope_append_kernel(CacheAppendArgs p,
-                                                                     RopeArgs rope, unsigned blocks,
-                                                                     RopeShare share) {
+__global__ __launch_bounds__((64 * kAppendParts<DH, true>)) void rope_append_kernel(
+    CacheAppendArgs p, RopeArgs rope, unsigned blocks, RopeShare share) {
   constexpr int P = BF16 ? 8 : 4;
   __shared__ __attribute__((aligned(16))) uint8_t s_two[2 * kPage * DH];
-  __shared__ uint32_t s_max[kAppendThreads / 64][2];
+  constexpr int THREADS = 64 * kAppendParts<DH, true>;
+  __shared__ uint32_t s_max[THREADS / 64][2];
   __shared__ __attribute__((aligned(16))) AppendTurn s_turn;
-  static_assert((2 * kRopePairs + 2 * DH) * sizeof(float) <= sizeof s_two, "the turns' LDS");
-  static_assert(kAppendThreads == kRopeThreads, "workgroups of one size");
+  static_assert(rope_lds(DH) * sizeof(float) <= sizeof s_two, "the turns' LDS");
   const unsigned w = blockIdx.x, rows = gridDim.x - blocks;
   const unsigned before = blocks_before(w, blocks, rows);
   if (blocks_before(w + 1, blocks, rows) != before)
     append_block<DH, BF16, true>(p, rope, before, s_two, s_two + kPage * DH, s_max, &s_turn);
   else
-    rope_rows<DH / 2 / P, P, BF16, OB, ITEMS>(rope, share, w - before,
-                                              reinterpret_cast<float*>(s_two));
+    rope_rows<DH / 2 / P, P, BF16, OB, ITEMS, false, THREADS>(rope, share, w - before,
+                                                              reinterpret_cast<float*>(s_two));
 }
 
 // Every touched block holds a new row, and each request has at most two partly new blocks.
@@ -611,9 +625,10 @@ static long long append_blocks(const CacheAppendArgs& a) {
 
 hipError_t launch_rope_append(const CacheAppendArgs& a, const RopeArgs& rope, hipStream_t s) {
   const unsigned blocks = (unsigned)append_blocks(a);
-  const RopeShare share = rope_share(rope, a.cache.dh / (a.in_bf16 ? 16 : 8));
+  const int threads = 64 * (a.cache.dh == 256 ? kAppendParts<256, true> : kAppendParts<64, true>);
+  const RopeShare share = rope_share(rope, a.cache.dh / (a.in_bf16 ? 16 : 8), a.cache.dh, threads);
   const unsigned more = rope.heads ? (unsigned)share.blocks(rope.rows) : 0;
-  const dim3 grid(blocks + more), block(kAppendThreads);
+  const dim3 grid(blocks + more), block(threads);
   if (grid.x == 0) return hipSuccess;
 #define RH_APPEND(D, X, O, I) \
   hipLaunchKernelGGL((rope_append_kernel<D, X, O, I>), grid, block, 0, s, a, rope, blocks, share)

@@ -13,7 +13,7 @@ namespace rh {
 
 template <int LPH, int P, bool XB, bool OB, int ITEMS, bool ANY>
 __global__ __launch_bounds__(kRopeThreads) void rope_rows_kernel(RopeArgs p, RopeShare share) {
-  __shared__ __attribute__((aligned(16))) float lds[2 * kRopePairs + 4 * LPH * P];
+  __shared__ __attribute__((aligned(16))) float lds[rope_lds(LPH * 2 * P)];
   rope_rows<LPH, P, XB, OB, ITEMS, ANY>(p, share, blockIdx.x, lds);
 }
 
@@ -106,7 +106,7 @@ static bool rope_by_lanes(const RopeArgs& a) {
 
 template <int LPH, int P, bool XB, bool OB, bool ANY>
 static void launch_lanes(const RopeArgs& a, hipStream_t s) {
-  RopeShare share = rope_share(a, LPH);
+  RopeShare share = rope_share(a, LPH, LPH * 2 * P, kRopeThreads);
   // a launch holds fewer than 2^32 threads
   const int most = std::max(1, (1 << 23) / share.slices) * share.group;
   for (; share.first < a.rows; share.first += std::min(most, a.rows - share.first)) {

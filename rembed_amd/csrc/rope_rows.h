@@ -11,7 +11,11 @@ namespace rh {
 
 constexpr int kRopeThreads = 256;
 constexpr int kRopeItems = 4;    // the most heads of a thread, whose loads are in flight together
-constexpr int kRopePairs = 512;  // cosines and sines that a workgroup holds
+// Cosines and sines that a workgroup holds, of heads of dh: eight rows', so that few large heads
+// (a row of 4 heads of 256 is 16 threads) leave no threads without a row.
+__host__ __device__ constexpr int rope_pairs(int dh) { return 8 * dh; }
+// Floats of LDS: those, and q's and k's norm weights.
+__host__ __device__ constexpr int rope_lds(int dh) { return 2 * rope_pairs(dh) + 2 * dh; }
 
 __device__ __forceinline__ int rope_used(const RopeArgs& p) {
   return p.used ? min(*p.used, p.rows) : p.rows;
@@ -37,14 +41,14 @@ struct RopeShare {
 };
 // Four heads a thread, whose cosines it then reads once, where two workgroups a CU remain; as
 // many rows as fill the workgroup's threads and as far as their cosines fit.
-inline RopeShare rope_share(const RopeArgs& a, int lanes) {
+inline RopeShare rope_share(const RopeArgs& a, int lanes, int most_dh, int threads) {
   const long long nh = std::max(1LL, (long long)a.heads + a.kv_heads + a.v_heads);
   RopeShare s;
   s.many = nh * lanes * a.rows >= kRopeItems * 512LL * kRopeThreads;
   s.sets = (int)(s.many ? (nh + kRopeItems - 1) / kRopeItems : nh);
-  s.slices = (s.sets - 1) / (kRopeThreads / lanes) + 1;
+  s.slices = (s.sets - 1) / (threads / lanes) + 1;
   s.each = (s.sets - 1) / s.slices + 1;  // slices of one size
-  s.group = std::max(1, std::min(kRopeThreads / (s.each * lanes), kRopePairs / a.turn.pairs));
+  s.group = std::max(1, std::min(threads / (s.each * lanes), rope_pairs(most_dh) / a.turn.pairs));
   s.group = std::min(s.group, a.rows / 512 + 1);
   s.first = 0;
   return s;
@@ -79,13 +83,14 @@ __device__ __forceinline__ void store_run(void* base, size_t at, const float (&v
 // A lane takes P pairs of a head, LPH lanes a head; a thread ITEMS heads of a row. The rows'
 // cosines and sines are in LDS once for all heads. ANY: heads of up to LPH * 2 P values and rows of
 // any alignment; else heads of so many, and a lane's halves are 16 bytes each. lds:
-// 2 * kRopePairs + 4 * LPH * P floats, 16-byte aligned.
-template <int LPH, int P, bool XB, bool OB, int ITEMS, bool ANY = false>
+// rope_lds(LPH * 2 * P) floats, 16-byte aligned.
+template <int LPH, int P, bool XB, bool OB, int ITEMS, bool ANY = false, int THREADS = kRopeThreads>
 __device__ __forceinline__ void rope_rows(const RopeArgs& p, const RopeShare& share, unsigned block,
                                           float* lds) {
   static_assert(ANY || P == (XB ? 8 : 4), "16 bytes");
   const int DH = ANY ? p.dh : LPH * 2 * P;
-  float *s_cos = lds, *s_sin = lds + kRopePairs, *s_w = lds + 2 * kRopePairs;
+  constexpr int kPairs = rope_pairs(LPH * 2 * P);
+  float *s_cos = lds, *s_sin = lds + kPairs, *s_w = lds + 2 * kPairs;
   const int tid = threadIdx.x, l = tid % LPH;
   const int nh = p.heads + p.kv_heads + p.v_heads, pairs = p.turn.pairs;
   const int used = rope_used(p);
@@ -108,12 +113,12 @@ __device__ __forceinline__ void rope_rows(const RopeArgs& p, const RopeShare& sh
     b[k].load(x + from + at.b);
   }
   if (p.q_norm.on || p.k_norm.on)
-    for (int i = tid; i < 2 * DH; i += kRopeThreads) {
+    for (int i = tid; i < 2 * DH; i += THREADS) {
       const bool q = i < DH;
       const float* w = q ? p.q_norm.weight : p.k_norm.weight;
       s_w[i] = w ? w[q ? i : i - DH] : 1.0f;
     }
-  for (int i = tid; i < nr * pairs; i += kRopeThreads) {
+  for (int i = tid; i < nr * pairs; i += THREADS) {
     const int t = i / pairs;
     turn_cos_sin(turn_at(p.turn.freq[i - t * pairs], p.pos[r0 + t]), p.turn.amp, s_cos[i], s_sin[i]);
   }
