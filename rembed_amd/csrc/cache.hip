@@ -284,16 +284,12 @@ struct AppendTurn {
 };
 
 // TURN: K's heads are normed and turned (rowops.h) on the way, in fp32, a thread every PARTS-th
-// chunk of eight pairs of its token. Heads of 256 take eight threads a token there: with four, 200
-// registers left a CU two workgroups (22.8k tokens of 4 kv heads: 46.4 µs, with eight 40.6; 48
-// single tokens of one: 8.7, with eight 6.4).
-template <int DH, bool TURN>
-constexpr int kAppendParts = TURN && DH == 256 ? 8 : 4;  // threads of a token
-template <int DH, bool BF16, bool TURN>
+// chunk of eight pairs of its token; PARTS threads have a token.
+template <int DH, bool BF16, bool TURN, int PARTS>
 __device__ __forceinline__ void append_block(const CacheAppendArgs& p, const RopeArgs& rope,
                                              unsigned block, uint8_t* s_k, uint8_t* s_v,
                                              uint32_t (*s_max)[2], AppendTurn* s_turn) {
-  constexpr int PARTS = kAppendParts<DH, TURN>, THREADS = 64 * PARTS;
+  constexpr int THREADS = 64 * PARTS;
   constexpr int kBytes = kPage * DH, E = DH / PARTS;  // a head's block; values per thread
   const int tid = threadIdx.x;
   const int heads = p.cache.kv_heads;
@@ -582,7 +578,7 @@ template <int DH, bool BF16>
 __global__ __launch_bounds__(kAppendThreads) void cache_append_kernel(CacheAppendArgs p) {
   __shared__ __attribute__((aligned(16))) uint8_t s_k[kPage * DH], s_v[kPage * DH];
   __shared__ uint32_t s_max[kAppendThreads / 64][2];
-  append_block<DH, BF16, false>(p, RopeArgs{}, blockIdx.x, s_k, s_v, s_max, nullptr);
+  append_block<DH, BF16, false, 4>(p, RopeArgs{}, blockIdx.x, s_k, s_v, s_max, nullptr);
 }
 
 // Workgroups for blocks of K and V and ones for rows of q, in one launch, and K never as rows. The
@@ -599,19 +595,19 @@ __device__ __forceinline__ unsigned blocks_before(unsigned w, unsigned blocks, u
   return w > rows ? max(turn, w - rows) : turn;
 }
 
-template <int DH, bool BF16, bool OB, int ITEMS>
-__global__ __launch_bounds__((64 * kAppendParts<DH, true>)) void rope_append_kernel(
+template <int DH, bool BF16, bool OB, int ITEMS, int PARTS>
+__global__ __launch_bounds__(64 * PARTS) void rope_append_kernel(
     CacheAppendArgs p, RopeArgs rope, unsigned blocks, RopeShare share) {
   constexpr int P = BF16 ? 8 : 4;
   __shared__ __attribute__((aligned(16))) uint8_t s_two[2 * kPage * DH];
-  constexpr int THREADS = 64 * kAppendParts<DH, true>;
+  constexpr int THREADS = 64 * PARTS;
   __shared__ uint32_t s_max[THREADS / 64][2];
   __shared__ __attribute__((aligned(16))) AppendTurn s_turn;
   static_assert(rope_lds(DH) * sizeof(float) <= sizeof s_two, "the turns' LDS");
   const unsigned w = blockIdx.x, rows = gridDim.x - blocks;
   const unsigned before = blocks_before(w, blocks, rows);
   if (blocks_before(w + 1, blocks, rows) != before)
-    append_block<DH, BF16, true>(p, rope, before, s_two, s_two + kPage * DH, s_max, &s_turn);
+    append_block<DH, BF16, true, PARTS>(p, rope, before, s_two, s_two + kPage * DH, s_max, &s_turn);
   else
     rope_rows<DH / 2 / P, P, BF16, OB, ITEMS, false, THREADS>(rope, share, w - before,
                                                               reinterpret_cast<float*>(s_two));
@@ -623,36 +619,44 @@ static long long append_blocks(const CacheAppendArgs& a) {
   return segs * a.cache.kv_heads;
 }
 
-hipError_t launch_rope_append(const CacheAppendArgs& a, const RopeArgs& rope, hipStream_t s) {
-  const unsigned blocks = (unsigned)append_blocks(a);
-  const int threads = 64 * (a.cache.dh == 256 ? kAppendParts<256, true> : kAppendParts<64, true>);
-  const RopeShare share = rope_share(rope, a.cache.dh / (a.in_bf16 ? 16 : 8), a.cache.dh, threads);
+template <int DH, bool BF16, int PARTS>
+static void launch_turning(const CacheAppendArgs& a, const RopeArgs& rope, unsigned blocks,
+                           hipStream_t s) {
+  const RopeShare share = rope_share(rope, DH / (BF16 ? 16 : 8), DH, 64 * PARTS);
   const unsigned more = rope.heads ? (unsigned)share.blocks(rope.rows) : 0;
-  const dim3 grid(blocks + more), block(threads);
-  if (grid.x == 0) return hipSuccess;
-#define RH_APPEND(D, X, O, I) \
-  hipLaunchKernelGGL((rope_append_kernel<D, X, O, I>), grid, block, 0, s, a, rope, blocks, share)
-#define RH_MANY(D, X, O)                              \
-  {                                                   \
-    if (share.many) RH_APPEND(D, X, O, kRopeItems);   \
-    else RH_APPEND(D, X, O, 1);                       \
+  const dim3 grid(blocks + more);
+  if (grid.x == 0) return;
+#define RH_APPEND(O, I)                                                                        \
+  hipLaunchKernelGGL((rope_append_kernel<DH, BF16, O, I, PARTS>), grid, dim3(64 * PARTS), 0, s, \
+                     a, rope, blocks, share)
+  if (rope.out_bf16) {
+    if (share.many) RH_APPEND(true, kRopeItems);
+    else RH_APPEND(true, 1);
+  } else {
+    if (share.many) RH_APPEND(false, kRopeItems);
+    else RH_APPEND(false, 1);
   }
-#define RH_DIM(D)                               \
-  if (a.cache.dh == D) {                        \
-    if (a.in_bf16) {                            \
-      if (rope.out_bf16) RH_MANY(D, true, true) \
-      else RH_MANY(D, true, false)              \
-    } else {                                    \
-      if (rope.out_bf16) RH_MANY(D, false, true) \
-      else RH_MANY(D, false, false)             \
-    }                                           \
-  }
-  RH_DIM(64)
-  RH_DIM(128)
-  RH_DIM(256)
-#undef RH_DIM
-#undef RH_MANY
 #undef RH_APPEND
+}
+
+// Heads of 128 take eight threads a token where the blocks are up to two workgroups a CU, which
+// shortens a block's time, and four where they are more, which takes fewer instructions in all (µs
+// with eight and with four, 8 kv heads, bf16: 48 single tokens 5.7, 6.5; 500 tokens 7.0, 7.9; 2000
+// 10.2, 10.5; 4000 16.4, 14.8; 16000 54.8, 51.4). Heads of 256 take eight: four leave a CU two
+// workgroups for their registers (22.8k tokens of 4 kv heads 46.4, with eight 40.6), sixteen only
+// more instructions (500 tokens of one kv head 9.3, 9.2; 8000 12.6, 13.8).
+template <bool BF16>
+static void launch_dims(const CacheAppendArgs& a, const RopeArgs& rope, hipStream_t s) {
+  const unsigned blocks = (unsigned)append_blocks(a);
+  if (a.cache.dh == 64) launch_turning<64, BF16, 4>(a, rope, blocks, s);
+  else if (a.cache.dh == 256) launch_turning<256, BF16, 8>(a, rope, blocks, s);
+  else if (blocks <= 512) launch_turning<128, BF16, 8>(a, rope, blocks, s);
+  else launch_turning<128, BF16, 4>(a, rope, blocks, s);
+}
+
+hipError_t launch_rope_append(const CacheAppendArgs& a, const RopeArgs& rope, hipStream_t s) {
+  if (a.in_bf16) launch_dims<true>(a, rope, s);
+  else launch_dims<false>(a, rope, s);
   return hipGetLastError();
 }
 
