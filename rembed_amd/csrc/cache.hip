@@ -276,6 +276,19 @@ __device__ __forceinline__ int spread(int at) {
   return at ^ (at >> 9 & 1) << 6;
 }
 
+// Where chunk l of eight pairs of a head lies: its two runs of eight values. Behind the pairs that
+// turn, and of neighbours, a chunk is 16 consecutive values.
+struct RopePlace {
+  int a, b;
+  bool turns;
+  __device__ __forceinline__ RopePlace(const RopeTurn& t, int l) {
+    turns = l * 8 < t.pairs;
+    const bool apart = turns && t.halves;
+    a = apart ? l * 8 : 16 * l;
+    b = apart ? l * 8 + t.pairs : 16 * l + 8;
+  }
+};
+
 // What a turning workgroup holds of K's norm and, of few tokens, their cosines and sines: those
 // are then made by all threads rather than by the tokens' own.
 struct AppendTurn {
@@ -351,7 +364,7 @@ __device__ __forceinline__ void append_block(const CacheAppendArgs& p, const Rop
       const S* x = static_cast<const S*>(p.kv) + (size_t)row_at * p.ldkv + p.k_off + h * DH;
 #pragma unroll
       for (int j = 0; j < E / 16; j++) {
-        const RopePlace<8> to(rope.turn, part + PARTS * j);
+        const RopePlace to(rope.turn, part + PARTS * j);
 #pragma unroll
         for (int i = 0; i < kRaw; i++) {
           raw[j][0][i] = *reinterpret_cast<const v4i*>(x + to.a + i * kStep);
@@ -398,12 +411,12 @@ __device__ __forceinline__ void append_block(const CacheAppendArgs& p, const Rop
 #pragma unroll
       for (int j = 0; j < E / 16; j++) {
         const int chunk = part + PARTS * j;
-        const RopePlace<8> to(rope.turn, chunk);
+        const RopePlace to(rope.turn, chunk);
         if (rope.k_norm.on) {
 #pragma unroll
           for (int half = 0; half < 2; half++) {
             float w[8];
-            load_floats(s_turn->w + (half ? to.b : to.a), w);
+            load_floats<8>(s_turn->w + (half ? to.b : to.a), w);
 #pragma unroll
             for (int i = 0; i < 8; i++) turned[j][half][i] = turned[j][half][i] * inv * w[i];
           }
@@ -411,14 +424,19 @@ __device__ __forceinline__ void append_block(const CacheAppendArgs& p, const Rop
         if (to.turns) {
           float c[8], sn[8];
           if (few_turns) {
-            load_floats(s_turn->c + (tok - off) * rope.turn.pairs + chunk * 8, c);
-            load_floats(s_turn->s + (tok - off) * rope.turn.pairs + chunk * 8, sn);
+            load_floats<8>(s_turn->c + (tok - off) * rope.turn.pairs + chunk * 8, c);
+            load_floats<8>(s_turn->s + (tok - off) * rope.turn.pairs + chunk * 8, sn);
           } else {
 #pragma unroll
             for (int i = 0; i < 8; i++)
               turn_cos_sin(turn_at(rope.turn.freq[chunk * 8 + i], pos), rope.turn.amp, c[i], sn[i]);
           }
-          rope_turn<8>(turned[j][0], turned[j][1], c, sn, rope.turn.halves);
+          if (rope.turn.halves) {
+            turn_halves<8>(turned[j][0], turned[j][1], c, sn);
+          } else {
+            turn_pairs<8>(turned[j][0], c, sn);
+            turn_pairs<8>(turned[j][1], c + 4, sn + 4);
+          }
         }
       }
     }
@@ -519,7 +537,7 @@ __device__ __forceinline__ void append_block(const CacheAppendArgs& p, const Rop
       for (int i = 0; i < kRun / 4; i++) w[i] = wk[e / 4 + i];
       int d = place(e);
       if constexpr (TURN) {
-        const RopePlace<8> to(rope.turn, part + e / 16 * PARTS);
+        const RopePlace to(rope.turn, part + e / 16 * PARTS);
         d = e / 8 % 2 ? to.b : to.a;
       }
       *reinterpret_cast<W*>((whole_k ? s_k : gk) + k_at(tok, d)) = w;

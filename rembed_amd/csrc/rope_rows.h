@@ -54,6 +54,31 @@ inline RopeShare rope_share(const RopeArgs& a, int lanes, int most_dh, int threa
   return s;
 }
 
+// What lane l of a head has: two runs of P values, beside the other lanes' (so that a store takes
+// whole lines), and the cosines of their pairs.
+//   halves: P pairs (a + i, b + i), with P cosines from l P; behind the pairs that turn, the
+//           first and the second half of the rest;
+//   pairs:  the first and the second half of the head, P / 2 pairs each, with P / 2 cosines.
+template <int P>
+struct RopeLane {
+  int a, b;
+  bool turns, second;  // the first run (and with it b's of halves), b's pairs
+  __device__ __forceinline__ RopeLane(const RopeTurn& t, int l, int dh) {
+    if (t.halves) {
+      const int chunks = t.pairs / P, rest = (dh - 2 * t.pairs) / 2;
+      turns = l < chunks;
+      second = false;
+      a = turns ? l * P : 2 * t.pairs + (l - chunks) * P;
+      b = a + (turns ? t.pairs : rest);
+    } else {
+      a = l * P;
+      b = a + dh / 2;
+      turns = a < 2 * t.pairs;
+      second = b < 2 * t.pairs;
+    }
+  }
+};
+
 // P values of a row as loaded. ANY: of any alignment, else 16 bytes.
 template <int P, bool BF16, bool ANY>
 struct RopeRun {
@@ -98,7 +123,7 @@ __device__ __forceinline__ void rope_rows(const RopeArgs& p, const RopeShare& sh
   const int nr = min(share.group, used - r0);
   if (nr <= 0) return;
   const bool in = !ANY || l * 2 * P < DH;
-  const RopePlace<P> at(p.turn, in ? l : 0);
+  const RopeLane<P> at(p.turn, in ? l : 0, DH);
   // the thread's row of these, and its heads set, set + sets, ..
   const int unit = tid / LPH, row = unit / share.each;
   const int set = (int)(block % share.slices) * share.each + unit - row * share.each;
@@ -125,9 +150,21 @@ __device__ __forceinline__ void rope_rows(const RopeArgs& p, const RopeShare& sh
   __syncthreads();
   if (!mine) return;
   float c[P], s[P];
-  if (at.turns) {
-    load_floats(s_cos + row * pairs + at.chunk * P, c);
-    load_floats(s_sin + row * pairs + at.chunk * P, s);
+  const float *cos = s_cos + row * pairs, *sin = s_sin + row * pairs;
+  if (p.turn.halves) {
+    if (at.turns) {
+      load_floats<P>(cos + at.a, c);
+      load_floats<P>(sin + at.a, s);
+    }
+  } else {
+    if (at.turns) {
+      load_floats<P / 2>(cos + at.a / 2, c);
+      load_floats<P / 2>(sin + at.a / 2, s);
+    }
+    if (at.second) {
+      load_floats<P / 2>(cos + at.b / 2, c + P / 2);
+      load_floats<P / 2>(sin + at.b / 2, s + P / 2);
+    }
   }
 #pragma unroll
   for (int k = 0; k < ITEMS; k++) {
@@ -145,14 +182,21 @@ __device__ __forceinline__ void rope_rows(const RopeArgs& p, const RopeShare& sh
       if (!in) ss = 0.0f;
       const float inv = inverse_root(group_sum<LPH>(ss) / (float)DH + norm.eps);
       float w[P];
-      load_floats(s_w + (head.part ? DH : 0) + at.a, w);
+      load_floats<P>(s_w + (head.part ? DH : 0) + at.a, w);
 #pragma unroll
       for (int i = 0; i < P; i++) y[i] = y[i] * inv * w[i];
-      load_floats(s_w + (head.part ? DH : 0) + at.b, w);
+      load_floats<P>(s_w + (head.part ? DH : 0) + at.b, w);
 #pragma unroll
       for (int i = 0; i < P; i++) z[i] = z[i] * inv * w[i];
     }
-    if (head.part < 2 && at.turns) rope_turn<P>(y, z, c, s, p.turn.halves);
+    if (head.part < 2 && at.turns) {
+      if (p.turn.halves) {
+        turn_halves<P>(y, z, c, s);
+      } else {
+        turn_pairs<P>(y, c, s);
+        if (at.second) turn_pairs<P>(z, c + P / 2, s + P / 2);
+      }
+    }
     if (in) {
       const size_t to = (size_t)(r0 + row) * p.ldout + head.out;
       store_run<P, OB, ANY>(p.out, to + at.a, y);

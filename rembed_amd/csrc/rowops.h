@@ -94,7 +94,7 @@ __device__ __forceinline__ void widen(const v4i& raw, float (&v)[N], int at = 0)
   }
 }
 template <int N>
-__device__ __forceinline__ void load_floats(const float* lds, float (&v)[N]) {
+__device__ __forceinline__ void load_floats(const float* lds, float* v) {
   constexpr int W = N < 4 ? N : 4;
   typedef float T __attribute__((ext_vector_type(W)));
 #pragma unroll
@@ -151,38 +151,23 @@ __device__ __forceinline__ void turn_cos_sin(uint32_t turn, float amp, float& c,
   s = __uint_as_float(b ^ (u & 0x80000000u)) * amp;
 }
 
-// Where chunk l of P pairs of a head lies: its two runs of P values. Behind the pairs that turn
-// a chunk is 2 P consecutive values, of either layout.
+// Pairs (a[i], b[i]) turned by c and s, and pairs (v[2 i], v[2 i + 1]).
 template <int P>
-struct RopePlace {
-  int chunk, a, b;
-  bool turns;
-  __device__ __forceinline__ RopePlace(const RopeTurn& t, int l) : chunk(l) {
-    turns = l * P < t.pairs;
-    const bool apart = turns && t.halves;
-    a = apart ? l * P : 2 * l * P;
-    b = apart ? l * P + t.pairs : 2 * l * P + P;
+__device__ __forceinline__ void turn_halves(float* a, float* b, const float* c, const float* s) {
+#pragma unroll
+  for (int i = 0; i < P; i++) {
+    const float x = a[i], y = b[i];
+    a[i] = __builtin_fmaf(x, c[i], -(y * s[i]));
+    b[i] = __builtin_fmaf(y, c[i], x * s[i]);
   }
-};
-// The chunk's pairs turned by c and s.
+}
 template <int P>
-__device__ __forceinline__ void rope_turn(float (&a)[P], float (&b)[P], const float (&c)[P],
-                                          const float (&s)[P], bool halves) {
-  if (halves) {
+__device__ __forceinline__ void turn_pairs(float* v, const float* c, const float* s) {
 #pragma unroll
-    for (int i = 0; i < P; i++) {
-      const float x = a[i], y = b[i];
-      a[i] = __builtin_fmaf(x, c[i], -(y * s[i]));
-      b[i] = __builtin_fmaf(y, c[i], x * s[i]);
-    }
-  } else {
-    auto at = [&](int e) -> float& { return e < P ? a[e] : b[e - P]; };
-#pragma unroll
-    for (int i = 0; i < P; i++) {
-      const float x = at(2 * i), y = at(2 * i + 1);
-      at(2 * i) = __builtin_fmaf(x, c[i], -(y * s[i]));
-      at(2 * i + 1) = __builtin_fmaf(y, c[i], x * s[i]);
-    }
+  for (int i = 0; i < P / 2; i++) {
+    const float x = v[2 * i], y = v[2 * i + 1];
+    v[2 * i] = __builtin_fmaf(x, c[i], -(y * s[i]));
+    v[2 * i + 1] = __builtin_fmaf(y, c[i], x * s[i]);
   }
 }
 
