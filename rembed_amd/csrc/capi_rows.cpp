@@ -173,7 +173,7 @@ int rh_residual_norm(rh_context* ctx, const rh_residual* r, const void* x, int x
       return fail(RH_ERR_INVALID, "misaligned buffer");
     const Rows rx = rows_of(x, x_bf16, n, ldx), ry = rows_of(y, y_bf16, n, ldy);
     const Rows rs = rows_of(sum, x_bf16, n, ldsum), ro = rows_of(out, out_bf16, n, ldout);
-    const Rows rg = rows_of(r->ldg ? r->gate : nullptr, 0, n, r->ldg);
+    const Rows rg = rows_of(r->gate, 0, n, r->ldg);
     const Rows rq{qa, 1, (size_t)ldq, (size_t)ldq};
     const size_t bytes = qa ? rh_fp8_scale_bytes(m, n) : 0;
     auto scales_meet = [&](const Rows& o) {
@@ -187,6 +187,11 @@ int rh_residual_norm(rh_context* ctx, const rh_residual* r, const void* x, int x
         scales_meet(rx) || scales_meet(ry) || scales_meet(rg) || scales_meet(rs) ||
         scales_meet(ro) || scales_meet(rq))
       return fail(RH_ERR_INVALID, "an output overlaps another buffer");
+    for (const float* w : {r->post.weight, r->post.bias, r->pre.weight, r->pre.bias}) {
+      const Rows rw = rows_of(w, 0, n, 0);
+      if (share(rs, rw, m) || share(ro, rw, m) || share(rq, rw, m) || scales_meet(rw))
+        return fail(RH_ERR_INVALID, "an output overlaps a norm's weights");
+    }
     CTX_GUARD(ctx);
     ResidualArgs a{};
     a.x = x;

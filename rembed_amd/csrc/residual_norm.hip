@@ -251,7 +251,7 @@ __global__ __launch_bounds__(T == 64 ? 256 : T) void residual_norm_kernel(Residu
         if constexpr (!WHOLE) q >>= 8 * at[e].twice;  // and zeros behind the row
         __builtin_nontemporal_store(q, reinterpret_cast<uint64_t*>(p.qa + (size_t)row * p.ldq + c));
         if (t % 16 == 0)
-          p.sa[fp8_scale_at((int)row, c / kFp8Block, (p.m + 127) / 128)] = (uint8_t)x;
+          p.sa[fp8_scale_at((int)row, c / kFp8Block, (p.m - 1) / 128 + 1)] = (uint8_t)x;
       }
     }
   }

@@ -140,6 +140,10 @@ def test_residual_refusals():
     no(L.RH_ERR_INVALID, a15=at((1 << 20) + 1024))
     no(L.RH_ERR_INVALID, a15=at((5 << 20) + 256))
     no(L.RH_ERR_INVALID, dict(gate=3 << 20, ldg=256))
+    no(L.RH_ERR_INVALID, dict(gate=(3 << 20) + 1024))
+    no(L.RH_ERR_INVALID, dict(pre=L.NormDesc(1, 0, (4 << 20) + 512, None)))
+    no(L.RH_ERR_INVALID, dict(pre=L.NormDesc(2, 0, None, 5 << 20)))
+    no(L.RH_ERR_INVALID, dict(post=L.NormDesc(1, 0, 6 << 20, None)))
 
 
 def test_rotary_refusals_without_a_handle():
