@@ -130,20 +130,23 @@ struct RopeTurn {
 __device__ __forceinline__ uint32_t turn_at(const RopeFreq& f, int t) {
   return (uint32_t)__mulhi(t, f.low) + (uint32_t)t * (uint32_t)f.high;
 }
-// cos and sin of a fraction of a turn: of its distance x from the nearest quarter, at most
-// pi / 4, by polynomials whose largest error is least (found by exchange; sin 1.8e-9, cos
-// 5.4e-11), then the quarter's exchange and signs. Off by at most 1.5e-7 with the roundings.
+// cos and sin of a fraction of a turn: of its distance t from the nearest quarter, at most 1/8
+// turn, by polynomials in t whose largest error is least (found by exchange; sin 1.8e-9, cos
+// 5.4e-11; 2 pi in two parts, so that the angle itself is not rounded again), then the quarter's
+// exchange and signs. Off by at most 7.2e-8 before amp, 2e-8 in the mean: K's codes flip between
+// two values no more often than an exact angle's would.
 __device__ __forceinline__ void turn_cos_sin(uint32_t turn, float amp, float& c, float& s) {
   const uint32_t u = turn + 0x20000000u;  // its upper two bits: the quarter
-  const float x = (float)(int)(turn << 2) * 3.6572951981678993e-10f;  // 2 pi / 2^34
-  const float x2 = x * x;
-  float p = __builtin_fmaf(x2, -0.0001949563619f, 0.008331978663f);
-  p = __builtin_fmaf(x2, p, -0.1666665067f);
-  const float sn = __builtin_fmaf(x * x2, p, x);
-  float q = __builtin_fmaf(x2, 2.439045066e-05f, -0.001388676379f);
-  q = __builtin_fmaf(x2, q, 0.04166662332f);
-  q = __builtin_fmaf(x2, q, -0.4999999973f);
-  const float cs = __builtin_fmaf(x2, q, 1.0f);
+  const float t = (float)(int)(turn << 2) * 0x1p-34f;
+  const float t2 = t * t;
+  float p = __builtin_fmaf(t2, -75.36964857f, 81.59198349f);
+  p = __builtin_fmaf(t2, p, -41.34166256f);
+  p = __builtin_fmaf(t2, p, -1.74845553e-7f);
+  const float sn = __builtin_fmaf(t, 6.2831854820251465f, t * p);
+  float q = __builtin_fmaf(t2, 59.24596417f, -85.44374173f);
+  q = __builtin_fmaf(t2, q, 64.93932647f);
+  q = __builtin_fmaf(t2, q, -19.73920869f);
+  const float cs = __builtin_fmaf(t2, q, 1.0f);
   // quarters 0..3: (c, s), (-s, c), (-c, -s), (s, -c)
   const bool odd = u & 0x40000000u;
   const uint32_t a = __float_as_uint(odd ? sn : cs), b = __float_as_uint(odd ? cs : sn);

@@ -9,8 +9,8 @@ import numpy as np
 import test_fp8_operators as F
 
 U = 2.0 ** -24
-# cos and sin of the kernels: Taylor's rest 2e-9, the angle's roundings 2 u pi/4, six fused steps
-# of which the last weighs most (u each), amp's product u
+# cos and sin of the kernels: the polynomials' rest 2e-9, the angle's roundings (2 u pi/4 at most), the
+# fused steps, of which the last weighs most (u each), amp's product u
 TURN = 2e-9 + 8 * U
 
 
