@@ -30,9 +30,15 @@ struct RowSum {
     if constexpr (T == 64) return v;
     if ((threadIdx.x & 63) == 0) slot[k][threadIdx.x >> 6] = v;
     __syncthreads();
-    v = slot[k][threadIdx.x % kWaves];
+    if constexpr (kWaves & (kWaves - 1)) {
+      v = slot[k][0];
+#pragma unroll
+      for (int w = 1; w < kWaves; w++) v += slot[k][w];
+    } else {
+      v = group_sum<kWaves>(slot[k][threadIdx.x % kWaves]);
+    }
     k++;
-    return group_sum<kWaves>(v);
+    return v;
   }
 };
 
@@ -287,13 +293,20 @@ static void launch_rows(const ResidualArgs& a, int r0, int rows, hipStream_t s) 
 #undef RH_RN
 }
 
+// The fewest threads of these that have eight values each: waves that sit out a row's end cost
+// their share (2272 rows of 5520 values: 32.5 µs with 1024 threads, 26.8 with 768; 8192 of 2560:
+// 37.6 with 512, 35.0 with 384).
 template <bool WHOLE>
 static void launch_part(const ResidualArgs& a, int r0, int rows, hipStream_t s) {
-  if (a.n <= 512) launch_rows<1, 64, WHOLE>(a, r0, rows, s);
-  else if (a.n <= 1024) launch_rows<1, 128, WHOLE>(a, r0, rows, s);
-  else if (a.n <= 2048) launch_rows<1, 256, WHOLE>(a, r0, rows, s);
-  else if (a.n <= 4096) launch_rows<1, 512, WHOLE>(a, r0, rows, s);
-  else if (a.n <= 8192) launch_rows<1, 1024, WHOLE>(a, r0, rows, s);
+  const int waves = (a.n + 511) / 512;
+  if (waves <= 1) launch_rows<1, 64, WHOLE>(a, r0, rows, s);
+  else if (waves <= 2) launch_rows<1, 128, WHOLE>(a, r0, rows, s);
+  else if (waves <= 3) launch_rows<1, 192, WHOLE>(a, r0, rows, s);
+  else if (waves <= 4) launch_rows<1, 256, WHOLE>(a, r0, rows, s);
+  else if (waves <= 6) launch_rows<1, 384, WHOLE>(a, r0, rows, s);
+  else if (waves <= 8) launch_rows<1, 512, WHOLE>(a, r0, rows, s);
+  else if (waves <= 12) launch_rows<1, 768, WHOLE>(a, r0, rows, s);
+  else if (waves <= 16) launch_rows<1, 1024, WHOLE>(a, r0, rows, s);
   else launch_rows<2, 1024, WHOLE>(a, r0, rows, s);
 }
 

@@ -17,7 +17,7 @@ __global__ __launch_bounds__(kRopeThreads) void rope_rows_kernel(RopeArgs p, Rop
   rope_rows<LPH, P, XB, OB, ITEMS, ANY>(p, share, blockIdx.x, lds);
 }
 
-// An odd number of pairs, or a head size that is no multiple of 4: a wave takes ITEMS heads of a row, a lane the
+// An odd number of pairs of halves, or a head size that is no multiple of 4: a wave takes ITEMS heads of a row, a lane the
 // pairs lane and (E = 2) lane + 64 of them, one value a load, and their cosines once.
 template <bool XB, bool OB, int E, int ITEMS>
 __global__ __launch_bounds__(256) void rope_any_kernel(RopeArgs p, int sets) {
@@ -91,13 +91,18 @@ __global__ __launch_bounds__(256) void rope_any_kernel(RopeArgs p, int sets) {
   }
 }
 
+// Whether the pairs that turn are whole runs of `run` values.
+static bool runs_fit(const RopeArgs& a, int run) {
+  return (a.turn.halves ? a.turn.pairs : 2 * a.turn.pairs) % run == 0;
+}
+
 // Whether rope_rows may take these rows: P pairs a lane (8 of bf16 rows, 4 of fp32 ones), 16-byte
 // loads, 16-byte stores (8 from fp32 to bf16).
 static bool rope_by_lanes(const RopeArgs& a) {
   const int P = a.x_bf16 ? 8 : 4, to = a.out_bf16 ? P * 2 : 16, in = a.x_bf16 ? 8 : 4;
   const int out = to / (a.out_bf16 ? 2 : 4);
   if (a.dh != 32 && a.dh != 64 && a.dh != 128 && a.dh != 256) return false;
-  if (a.turn.pairs % P) return false;
+  if (!runs_fit(a, P)) return false;
   if ((uintptr_t)a.x % 16 || (uintptr_t)a.out % to || a.ldx % in || a.ldout % out) return false;
   if (a.heads && (a.q_off % in || a.q_out % out)) return false;
   if (a.kv_heads && (a.k_off % in || a.k_out % out)) return false;
@@ -145,7 +150,7 @@ static void launch_types(const RopeArgs& a, hipStream_t s) {
     else launch_lanes<128 / P, P, XB, OB, false>(a, s);
     return;
   }
-  auto whole = [&](int run) { return a.turn.pairs % run == 0 && a.dh / 2 % run == 0; };
+  auto whole = [&](int run) { return runs_fit(a, run) && a.dh / 2 % run == 0; };
   if (whole(P)) {
     if (a.dh <= 64) launch_lanes<32 / P, P, XB, OB, true>(a, s);
     else if (a.dh <= 128) launch_lanes<64 / P, P, XB, OB, true>(a, s);

@@ -231,6 +231,9 @@ ROPE = [  # rows, heads, kv, dh, rot, layout, columns before / behind / more in 
     (8, 2, 2, 254, 250, 0, 0, 0, 0), (12, 1, 2, 64, 2, 1, 0, 0, 0), (2, 40, 20, 128, 128, 1, 0, 0, 0),
     (1100, 2, 1, 64, 64, 0, 0, 0, 0), (2, 1, 1, 32, 24, 0, 0, 0, 0), (3, 300, 8, 32, 32, 0, 0, 0, 0),
     (700, 6, 1, 256, 128, 0, 0, 0, 0), (2, 2, 1, 128, 100, 0, 0, 0, 4),
+    # neighbours in runs of 2 and 4 of which one half turns in part, halves of an odd number of pairs
+    (5, 2, 1, 128, 14, 1, 0, 0, 0), (9, 2, 2, 128, 68, 1, 8, 0, 0), (4, 2, 1, 36, 18, 1, 2, 0, 0),
+    (700, 4, 1, 36, 18, 0, 0, 0, 0), (700, 4, 2, 200, 120, 0, 4, 0, 0), (900, 4, 1, 96, 50, 1, 0, 0, 0),
 ]
 
 
