@@ -395,7 +395,7 @@ int rh_cache_attention(rh_context *ctx, const void *q, int q_bf16, int ldq, int 
  * What a decoder layer on the operators above runs around its linears and its attention.
  * Like them, none of these calls allocates or waits (rh_rope_create apart), and each may be
  * captured into a HIP graph. Arithmetic is fp32 on unrounded values, with one rounding where a
- * value is stored; sums of squares are fp32, so values from 2^63 on overflow them. `used` may
+ * value is stored (rows or heads whose squares sum to 2^128 and more become 0 in a norm). `used` may
  * name a device integer (a plan's cu + batch, status + 1): rows from it on are left as they
  * are; NULL: all rows are taken. An output may lie exactly on an input of its own type and
  * stride, as said; other overlaps are refused. Rows and columns have no alignment beyond
@@ -445,7 +445,7 @@ int rh_residual_norm(rh_context *ctx, const rh_residual *r, const void *x, int x
  *              whole i around those; amp = 0.1 ln(factor) + 1
  *   WAVELENGTH the same with a mean linear in the turns themselves; fast 0: 4, slow 0: 1; amp 1
  *   GIVEN      f_i = freq[i]
- * Angles are exact to 2^-33 of a turn at every 32-bit position, negative ones turn back. */
+ * Angles are exact to 2^-31 of a turn at every 32-bit position, negative ones turn back. */
 #define RH_ROPE_HALVES 0
 #define RH_ROPE_PAIRS 1
 #define RH_ROPE_PLAIN 0
@@ -487,7 +487,8 @@ int rh_rope_rows(rh_context *ctx, const rh_rope *rope, const void *x, int x_bf16
  * 0 where those or V are no numbers), q's heads to q [rows][ldq], head h at h*dh (fp32 or bf16;
  * may be x + q_off with x's type and stride). heads may be 0. pos, cu, blocks and slots are a
  * plan's; rows of q behind cu[batch] are left as they are. rot a multiple of 16; x and q 16-byte
- * aligned, ldx, ldq and the offsets multiples of 8. */
+ * aligned, ldx, ldq and the offsets multiples of 8. A call holds under 2^23 workgroups (one for a
+ * block and kv head, one for some rows of q), else RH_ERR_SHAPE. */
 int rh_rope_append(rh_context *ctx, const rh_rope *rope, const rh_kv_cache *cache, const void *x,
                    int x_bf16, int ldx, int q_off, int k_off, int v_off, void *q, int q_bf16,
                    int ldq, int heads, const int32_t *pos, const int32_t *cu,
@@ -499,7 +500,7 @@ int rh_rope_append(rh_context *ctx, const rh_rope *rope, const rh_kv_cache *cach
  * to other positions: read it, turn K by the difference, append it elsewhere. Values are what the
  * codes stand for, exactly (bf16: below 2^-126 rounded). Positions without a page of the cache
  * are zeros; rows behind cu[batch] are left as they are. out 16-byte aligned, ldout and the
- * offsets multiples of 8. */
+ * offsets multiples of 8; (rows / 64 + 2 batch) * kv_heads under 2^24. */
 int rh_cache_read(rh_context *ctx, const rh_kv_cache *cache, const int32_t *table, int ldt,
                   const int32_t *cu, const int32_t *first, int batch, int rows, void *out,
                   int out_bf16, int ldout, int k_off, int v_off);

@@ -638,12 +638,27 @@ static long long append_blocks(const CacheAppendArgs& a) {
   return segs * a.cache.kv_heads;
 }
 
+// Threads of a token. Heads of 128 take eight where the blocks are up to two workgroups a CU, which
+// shortens a block's time, and four where they are more, which takes fewer instructions in all (µs
+// with eight and with four, 8 kv heads, bf16: 48 single tokens 5.7, 6.5; 500 tokens 7.0, 7.9; 2000
+// 10.2, 10.5; 4000 16.4, 14.8; 16000 54.8, 51.4). Heads of 256 take eight: four leave a CU two
+// workgroups for their registers (22.8k tokens of 4 kv heads 46.4, with eight 40.6), sixteen only
+// more instructions (500 tokens of one kv head 9.3, 9.2; 8000 12.6, 13.8).
+static int append_parts(const CacheAppendArgs& a) {
+  return a.cache.dh == 256 || (a.cache.dh == 128 && append_blocks(a) <= 512) ? 8 : 4;
+}
+static RopeShare append_share(const CacheAppendArgs& a, const RopeArgs& rope) {
+  return rope_share(rope, a.cache.dh / (a.in_bf16 ? 16 : 8), a.cache.dh, 64 * append_parts(a));
+}
+long long rope_append_grid(const CacheAppendArgs& a, const RopeArgs& rope) {
+  return append_blocks(a) + (rope.heads ? append_share(a, rope).blocks(rope.rows) : 0);
+}
+
 template <int DH, bool BF16, int PARTS>
-static void launch_turning(const CacheAppendArgs& a, const RopeArgs& rope, unsigned blocks,
-                           hipStream_t s) {
-  const RopeShare share = rope_share(rope, DH / (BF16 ? 16 : 8), DH, 64 * PARTS);
-  const unsigned more = rope.heads ? (unsigned)share.blocks(rope.rows) : 0;
-  const dim3 grid(blocks + more);
+static void launch_turning(const CacheAppendArgs& a, const RopeArgs& rope, hipStream_t s) {
+  const RopeShare share = append_share(a, rope);
+  const unsigned blocks = (unsigned)append_blocks(a);
+  const dim3 grid((unsigned)rope_append_grid(a, rope));
   if (grid.x == 0) return;
 #define RH_APPEND(O, I)                                                                        \
   hipLaunchKernelGGL((rope_append_kernel<DH, BF16, O, I, PARTS>), grid, dim3(64 * PARTS), 0, s, \
@@ -658,19 +673,12 @@ static void launch_turning(const CacheAppendArgs& a, const RopeArgs& rope, unsig
 #undef RH_APPEND
 }
 
-// Heads of 128 take eight threads a token where the blocks are up to two workgroups a CU, which
-// shortens a block's time, and four where they are more, which takes fewer instructions in all (µs
-// with eight and with four, 8 kv heads, bf16: 48 single tokens 5.7, 6.5; 500 tokens 7.0, 7.9; 2000
-// 10.2, 10.5; 4000 16.4, 14.8; 16000 54.8, 51.4). Heads of 256 take eight: four leave a CU two
-// workgroups for their registers (22.8k tokens of 4 kv heads 46.4, with eight 40.6), sixteen only
-// more instructions (500 tokens of one kv head 9.3, 9.2; 8000 12.6, 13.8).
 template <bool BF16>
 static void launch_dims(const CacheAppendArgs& a, const RopeArgs& rope, hipStream_t s) {
-  const unsigned blocks = (unsigned)append_blocks(a);
-  if (a.cache.dh == 64) launch_turning<64, BF16, 4>(a, rope, blocks, s);
-  else if (a.cache.dh == 256) launch_turning<256, BF16, 8>(a, rope, blocks, s);
-  else if (blocks <= 512) launch_turning<128, BF16, 8>(a, rope, blocks, s);
-  else launch_turning<128, BF16, 4>(a, rope, blocks, s);
+  if (a.cache.dh == 64) launch_turning<64, BF16, 4>(a, rope, s);
+  else if (a.cache.dh == 256) launch_turning<256, BF16, 8>(a, rope, s);
+  else if (append_parts(a) == 8) launch_turning<128, BF16, 8>(a, rope, s);
+  else launch_turning<128, BF16, 4>(a, rope, s);
 }
 
 hipError_t launch_rope_append(const CacheAppendArgs& a, const RopeArgs& rope, hipStream_t s) {

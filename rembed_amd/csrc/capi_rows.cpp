@@ -70,7 +70,8 @@ static int rope_frequencies(const rh_rope_config* c, std::vector<long double>& f
     long double hi = std::min(ceill(pair_of(slow)), rot - 1);
     if (lo == hi) hi += 0.001L;
     for (int i = 0; i < pairs; i++) {
-      const long double stay = yarn ? 1 - (i - lo) / (hi - lo) : (n * f[i] / pi2 - slow) / (fast - slow);
+      long double stay = yarn ? 1 - (i - lo) / (hi - lo) : (n * f[i] / pi2 - slow) / (fast - slow);
+      if (yarn && hi < lo) stay = hi < 0 ? 0 : 1;  // every pair turns under `slow` or over `fast` times
       const long double w = std::min(std::max(stay, 0.0L), 1.0L);
       f[i] = f[i] / s * (1 - w) + f[i] * w;
     }
@@ -361,9 +362,6 @@ int rh_rope_append(rh_context* ctx, const rh_rope* rope, const rh_kv_cache* cach
              : share(out, rows_of(x, x_bf16, end, ldx), rows))
       return fail(RH_ERR_INVALID, "q overlaps x without being its own columns");
     const long long segs = std::min((long long)rows, (long long)rows / RH_CACHE_BLOCK + 2LL * batch);
-    // workgroups for blocks, and (eight heads of a row each, or more) for rows of q
-    if (segs * cache->kv_heads > 1 << 23 || rows * (heads / 8 + 1LL) > 1 << 23)
-      return fail(RH_ERR_SHAPE, "too many rows for one call");
     CTX_GUARD(ctx);
     if (batch == 0 || rows == 0) return RH_OK;
     CacheAppendArgs c{*cache, x, x_bf16 ? 1 : 0, ldx, k_off, v_off, cu, blocks, slots, batch,
@@ -381,6 +379,7 @@ int rh_rope_append(rh_context* ctx, const rh_rope* rope, const rh_kv_cache* cach
     a.pos = pos;
     a.used = cu + batch;
     a.rows = rows;
+    if (rope_append_grid(c, a) >= 1 << 23) return fail(RH_ERR_SHAPE, "too many rows for one call");
     RH_HIP(launch_rope_append(c, a, ctx->stream));
     return RH_OK;
   });
@@ -400,8 +399,8 @@ int rh_cache_read(rh_context* ctx, const rh_kv_cache* cache, const int32_t* tabl
     if (columns_meet(k_off, width, v_off, width)) return fail(RH_ERR_SHAPE, "K and V share columns");
     if (ldout % 8 || k_off % 8 || v_off % 8 || !aligned(out, 16))
       return fail(RH_ERR_SHAPE, "rows and offsets must be multiples of 8 values, out 16-byte aligned");
-    if (((long long)rows / RH_CACHE_BLOCK + 2LL * batch) * cache->kv_heads > 1 << 23)
-      return fail(RH_ERR_SHAPE, "too many blocks for one call");
+    if (((long long)rows / RH_CACHE_BLOCK + 2LL * batch) * cache->kv_heads >= 1 << 24)
+      return fail(RH_ERR_SHAPE, "too many blocks for one call");  // 2^32 threads
     CTX_GUARD(ctx);
     if (batch == 0 || rows == 0) return RH_OK;
     CacheReadArgs a{*cache, table, ldt, cu, first, batch, rows, out, out_bf16 ? 1 : 0, ldout,

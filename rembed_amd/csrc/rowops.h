@@ -197,6 +197,8 @@ hipError_t launch_rope_rows(const RopeArgs& a, hipStream_t s);
 // The append with K's heads normed and turned on the way (append.kv: the q|k|v rows), and q's heads
 // as rows (rope: x, q_off, heads; rows behind cu[batch] are left as they are).
 hipError_t launch_rope_append(const CacheAppendArgs& append, const RopeArgs& rope, hipStream_t s);
+// Its workgroups, of 512 threads at most.
+long long rope_append_grid(const CacheAppendArgs& append, const RopeArgs& rope);
 
 struct CacheReadArgs {
   rh_kv_cache cache;

@@ -36,6 +36,16 @@ def test_rope_frequencies(rot, kw):
         assert f[0] == 1.0 and abs(f[-1] - 10000.0 ** (2.0 / rot - 1)) < 1e-15
 
 
+def test_rope_frequencies_all_fast_or_all_slow():
+    """YaRN where every pair turns over `fast` times, or under `slow`: none, all are scaled."""
+    from rembed_amd import tensor as T
+    plain, _ = T.rope_frequencies(16, theta=1.5)
+    same, _ = T.rope_frequencies(16, theta=1.5, scaling=3, factor=8.0, original=1 << 30)
+    assert np.array_equal(same, plain)
+    all_, _ = T.rope_frequencies(16, theta=1.5, scaling=3, factor=8.0, original=1)
+    assert np.allclose(all_, plain / 8, rtol=1e-15)
+
+
 def test_rope_frequencies_given():
     from rembed_amd import _lib as L
     from rembed_amd import tensor as T
@@ -193,7 +203,8 @@ def test_read_refusals():
     no(L.RH_ERR_SHAPE, a10=260)
     no(L.RH_ERR_SHAPE, a11=4, a10=264, a12=136)
     no(L.RH_ERR_SHAPE, a8=at((1 << 20) + 8))
-    no(L.RH_ERR_SHAPE, a6=1 << 23)
+    no(L.RH_ERR_SHAPE, a6=1 << 22)
+    no(L.RH_ERR_SHAPE, a7=1 << 29, a6=0, a1=F.desc(heads=2))
 
 
 # ---- GPU: helpers -----------------------------------------------------------------------
@@ -439,6 +450,7 @@ def test_rope_refusals(gpu_ctx):
                        (7, -8, L.RH_ERR_SHAPE), (8, 136, L.RH_ERR_SHAPE), (11, 56, L.RH_ERR_SHAPE),
                        (3, buf.ptr + 8, L.RH_ERR_SHAPE), (9, far.ptr + 8, L.RH_ERR_SHAPE),
                        (13, buf.ptr + 2, L.RH_ERR_INVALID), (16, buf.ptr + 4, L.RH_ERR_INVALID),
+                       (18, 2 ** 31 - 1, L.RH_ERR_SHAPE),
                        (9, buf.ptr + 16, L.RH_ERR_INVALID), (7, 0, L.RH_ERR_INVALID)):
         a = list(args)
         a[i] = v
