@@ -385,7 +385,7 @@ __device__ __forceinline__ void append_block(const CacheAppendArgs& p, const Rop
   uint8_t* gv = p.cache.v + unit * kBytes;
   const int ok = p.cache.k_exp[unit], ov = p.cache.v_exp[unit];
   if constexpr (TURN) {
-    float ss = 0.0f;
+    float ss = 0.0f;  // a token's lanes have one or none: what they hold without one stays theirs
 #pragma unroll
     for (int j = 0; j < E / 16; j++)
 #pragma unroll
@@ -393,10 +393,8 @@ __device__ __forceinline__ void append_block(const CacheAppendArgs& p, const Rop
 #pragma unroll
         for (int i = 0; i < kRaw; i++) widen<BF16>(raw[j][half][i], turned[j][half], i * kStep);
 #pragma unroll
-        for (int i = 0; i < 8; i++) {
-          if (!mine) turned[j][half][i] = 0.0f;
+        for (int i = 0; i < 8; i++)
           ss = __builtin_fmaf(turned[j][half][i], turned[j][half][i], ss);
-        }
       }
 #if defined(__HIP_DEVICE_COMPILE__)
 #define RH_ROR(n)                                                                                 \

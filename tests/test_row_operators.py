@@ -454,6 +454,8 @@ def test_rope_refusals(gpu_ctx):
                        (9, buf.ptr + 16, L.RH_ERR_INVALID), (7, 0, L.RH_ERR_INVALID)):
         a = list(args)
         a[i] = v
+        if i == 18:                                  # too many blocks, without q
+            a[9], a[12] = None, 0
         if i == 7 and v == 0:                        # q on its columns of x, which are k's too
             a[9], a[11] = buf.ptr, 192
         F.refused(code, "rh_rope_append", *a)
@@ -799,6 +801,34 @@ def test_rope_append_of_what_has_no_page_or_is_no_number(gpu_ctx):
     none = T.KVCache(gpu_ctx, 0, kv, dh)                        # a cache of no pages: q alone
     got, left = go(none, cu, blk, slots)
     assert np.array_equal(got[:8], x[:8, :64]) and left[8:].all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dh", [64, 128, 256])
+@pytest.mark.parametrize("n", [1, 70])
+def test_rope_append_of_zeros_and_extremes(gpu_ctx, dh, n):
+    """Heads of zeros (whose 1 / rms is 1 / sqrt(eps)), tiny and huge ones, alone in their blocks and
+    together: the codes of the rows that rh_rope_rows gives."""
+    from rembed_amd import tensor as T
+    rng = np.random.default_rng(dh + n)
+    rope, norm = T.Rope(gpu_ctx, dh), T.Norm(None, 1e-6)
+    for scale in (0.0, 1e-30, 2.0 ** -140, 1e15, None):
+        x = rng.standard_normal((n, 2 * dh))
+        x[:, :dh] *= np.exp(rng.uniform(-60, 30, (n, 1))) if scale is None else scale
+        img, val = F.typed(x, "f32")
+        c = O.Cache(2, 1, dh)
+        dev = F.device_cache(gpu_ctx, c)
+        cu, blk, lens, slots, pos, _ = O.plan([0], [n], [1, 0], np.zeros((1, 2), I32), n)
+        d, dpos = gpu_ctx.upload(img), gpu_ctx.upload(pos)
+        turned, read = marked(gpu_ctx, n, 2 * dh, False)
+        T.RopeRows(gpu_ctx, rope, d, False, 2 * dh, turned, False, 2 * dh, 0, 0, -1, 0, 1, dh, dpos, n, None,
+                   norm)
+        T.RopeAppend(gpu_ctx, rope, dev, d, False, 2 * dh, 0, 0, dh, None, False, 0, 0, dpos,
+                     gpu_ctx.upload(cu), gpu_ctx.upload(blk), gpu_ctx.upload(slots), 1, n, None, norm)
+        k = read()[0][:, :dh].reshape(n, 1, dh).astype(np.float64)
+        assert np.isfinite(k).all() and (scale != 0.0 or not k.any())
+        c.append(k, val[:, dh:].reshape(n, 1, dh).astype(np.float64), cu, slots)
+        same_but_for_norms(dev, c, None)
 
 
 def filled(rng, ctx, pages, kv, dh):
