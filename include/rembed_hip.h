@@ -414,8 +414,8 @@ typedef struct {
   const float *bias;   /* dev [n], RH_NORM_LAYER only; NULL: zeros */
 } rh_norm;
 
-/* A block's end and the next one's beginning (Add and the norms around it, tensor.go:383-389;
- * Gemma's norm sandwich, gemma3.go:357,376):
+/* A block's end and the next one's beginning (Add and the norms around it, tensor.go:383-387;
+ * Gemma's post-norms, gemma3.go:357,376):
  *   sum = x_scale * x + y_scale * gate * post(y),   out = pre(sum). */
 typedef struct {
   rh_norm post;      /* of the block's output y; RH_NORM_NONE: as it is */
@@ -434,7 +434,7 @@ int rh_residual_norm(rh_context *ctx, const rh_residual *r, const void *x, int x
                      int out_bf16, int ldout, uint8_t *qa, int ldq, uint8_t *sa, int m, int n,
                      const int32_t *used);
 
-/* Rotary positions (the RoPE table and applyRoPE, modernbert.go:111-143). The leading `rot`
+/* Rotary positions (ropeTable and applyRoPE, modernbert.go:108-143). The leading `rot`
  * values of a head are pairs, (i, i + rot/2) or (2i, 2i + 1), that turn by pos * f_i:
  *   a' = amp * (a cos - b sin),  b' = amp * (b cos + a sin);  the rest of the head passes.
  * f_i = theta^(-2i/rot) radians a position, scaled for texts longer than trained on:
@@ -476,8 +476,8 @@ void rh_rope_destroy(rh_rope *rope);
  * NULL: not) and turned at pos[row], to the same columns of out [rows][ldout] (fp32 or bf16; may
  * be x itself). q head h starts at column q_off + h*dh, k head h at k_off + h*dh; heads or
  * kv_heads may be 0. v_off >= 0: the kv_heads heads from there are copied as well (converted;
- * with out on x they are left); -1: not. dh even, 2..256, rot <= dh. Replaces the QK-norm and
- * RoPE loops of qwen3.go:483-505, gemma3.go:293-316. */
+ * with out on x they are left); -1: not. dh even, 2..256, rot <= dh. Replaces
+ * applyRoPE over a text's rows and heads (modernbert.go:130-143). */
 int rh_rope_rows(rh_context *ctx, const rh_rope *rope, const void *x, int x_bf16, int ldx,
                  void *out, int out_bf16, int ldout, int q_off, int k_off, int v_off, int heads,
                  int kv_heads, int dh, const int32_t *pos, int rows, const rh_norm *q_norm,

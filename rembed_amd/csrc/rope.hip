@@ -2,7 +2,7 @@
 //
 // For each pair: y = x * w / sqrt(mean(x^2) + eps) where a head norm is given, then
 // rowops.h's turn; one rounding, at the end. The reference keeps a table of
-// cosines and turns fp32 rows in place (applyRoPE, modernbert.go:130-143; qwen3.go:319-390); the
+// cosines and turns fp32 rows in place (ropeTable, applyRoPE, modernbert.go:108-143); the
 // model forwards here have a pass of their own for that (kernels_dec.hip).
 //
 // Every value is read and written once, and that bounds it: 16384 rows of 16 + 8 heads of 128, 201
@@ -20,8 +20,9 @@ __global__ __launch_bounds__(kRopeThreads) void rope_rows_kernel(RopeArgs p, Rop
   rope_rows<LPH, P, XB, OB, ITEMS, ANY>(p, share, blockIdx.x, lds);
 }
 
-// An odd number of pairs of halves, or a head size that is no multiple of 4: a wave takes ITEMS heads of a row, a lane the
-// pairs lane and (E = 2) lane + 64 of them, one value a load, and their cosines once.
+// An odd number of pairs of halves, or a head size that is no multiple of 4: a wave takes ITEMS
+// heads of a row, a lane the pairs lane and (E = 2) lane + 64 of them, one value a load, and their
+// cosines once.
 template <bool XB, bool OB, int E, int ITEMS>
 __global__ __launch_bounds__(256) void rope_any_kernel(RopeArgs p, int sets) {
   using X = std::conditional_t<XB, __bf16, float>;
