@@ -46,31 +46,36 @@ struct RowSum {
 
 enum Type : int { kNone, kF32, kBF16 };
 
-// A thread's eight values: WHOLE: from column c on, 16-byte aligned, in the row or behind it. Else
-// rows of any length and alignment (memory takes 16 bytes at any address): the row's last chunk
-// begins `twice` columns early, so that it ends with the row; what it shares with the chunk before
-// is computed and stored by both, alike, and summed by that one. Rows of under eight values are
-// taken one by one.
+// A thread's eight values: WHOLE: from column c on, 16-byte aligned. Else rows of any length and
+// alignment (memory takes 16 bytes at any address): the row's last chunk begins `twice` columns
+// early, so that it ends with the row; what it shares with the chunk before is computed and stored
+// by both, alike, and summed by that one. Threads behind the row (not `here`) read the row's last
+// values as well, and neither sum nor store them. Rows of under eight values are taken one by one.
 template <bool WHOLE>
 struct Chunk {
   int from, twice, n;
   bool here;
   Chunk() = default;
-  __device__ __forceinline__ Chunk(int c, int n) : from(c), twice(0), n(n), here(c < n) {
-    if constexpr (!WHOLE) {
-      if (here && n >= 8 && c + 8 > n) {
-        from = n - 8;
-        twice = c - from;
-      }
+  __device__ __forceinline__ Chunk(int c, int n) : from(min(c, max(n - 8, 0))), n(n), here(c < n) {
+    twice = here ? c - from : 8;
+  }
+  __device__ __forceinline__ bool counts(int i) const { return i >= twice && i < n; }
+  // a sum over the values that count, of x(value)
+  template <class F>
+  __device__ __forceinline__ float over(const float (&v)[8], float s, F&& add) const {
+    if constexpr (WHOLE) {
+      float own = s;
+#pragma unroll
+      for (int i = 0; i < 8; i++) own = add(own, v[i]);
+      return here ? own : s;
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; i++) s = add(s, counts(i) ? v[i] : 0.0f);
+      return s;
     }
   }
-  __device__ __forceinline__ bool inside(int i) const { return here && (WHOLE || i < n); }
-  __device__ __forceinline__ bool counts(int i) const { return inside(i) && (WHOLE || i >= twice); }
   template <Type K>
   __device__ __forceinline__ void load(const void* base, size_t at, float (&v)[8]) const {
-#pragma unroll
-    for (int i = 0; i < 8; i++) v[i] = 0.0f;
-    if (!here) return;
     if constexpr (WHOLE) {
       load_values<8, K == kBF16>(base, at + from, v);
     } else {
@@ -87,8 +92,7 @@ struct Chunk {
         }
       } else {
 #pragma unroll
-        for (int i = 0; i < 7; i++)
-          if (i < n) v[i] = (float)p[i];
+        for (int i = 0; i < 8; i++) v[i] = i < n ? (float)p[i < n ? i : 0] : 0.0f;
       }
     }
   }
@@ -135,7 +139,7 @@ struct NormWeights {
   }
 };
 
-// v normed in place; values outside the row are zeros before, and anything after.
+// v normed in place.
 template <int V, int T, bool WHOLE>
 __device__ __forceinline__ void norm_row(float (&v)[V][8], const rh_norm& norm,
                                          const NormWeights<V, WHOLE>& by, const Chunk<WHOLE>* at,
@@ -143,9 +147,7 @@ __device__ __forceinline__ void norm_row(float (&v)[V][8], const rh_norm& norm,
   if (norm.kind == RH_NORM_LAYER) {
     float s = 0.0f;
 #pragma unroll
-    for (int e = 0; e < V; e++)
-#pragma unroll
-      for (int i = 0; i < 8; i++) s += at[e].counts(i) ? v[e][i] : 0.0f;
+    for (int e = 0; e < V; e++) s = at[e].over(v[e], s, [](float a, float x) { return a + x; });
     const float mean = sum(s) / (float)n;
 #pragma unroll
     for (int e = 0; e < V; e++)
@@ -155,11 +157,7 @@ __device__ __forceinline__ void norm_row(float (&v)[V][8], const rh_norm& norm,
   float ss = 0.0f;
 #pragma unroll
   for (int e = 0; e < V; e++)
-#pragma unroll
-    for (int i = 0; i < 8; i++) {
-      const float x = at[e].counts(i) ? v[e][i] : 0.0f;
-      ss = __builtin_fmaf(x, x, ss);
-    }
+    ss = at[e].over(v[e], ss, [](float a, float x) { return __builtin_fmaf(x, x, a); });
   const float inv = inverse_root(sum(ss) / (float)n + norm.eps);
 #pragma unroll
   for (int e = 0; e < V; e++)
@@ -184,9 +182,11 @@ __global__ __launch_bounds__(T == 64 ? 256 : T) void residual_norm_kernel(Residu
   constexpr int kRows = T == 64 ? 4 : 1;
   __shared__ float s_sum[4][RowSum<T>::kWaves];
   const int t = threadIdx.x % T;
-  const long long row = r0 + (long long)blockIdx.x * kRows + threadIdx.x / T;
+  // of the wave, and so a scalar; unsigned: behind the last row it may pass 2^31
+  const unsigned row = (unsigned)r0 + blockIdx.x * kRows +
+                       (T == 64 ? __builtin_amdgcn_readfirstlane(threadIdx.x / 64) : 0);
   const int used = p.used ? min(*p.used, p.m) : p.m;
-  if (row >= used) return;  // whole waves; a workgroup of one row as a whole
+  if (row >= (unsigned)max(used, 0)) return;  // whole waves; a workgroup of one row as a whole
   const int n = p.n;
   RowSum<T> sum{s_sum};
   Chunk<WHOLE> at[V];
@@ -217,13 +217,20 @@ __global__ __launch_bounds__(T == 64 ? 256 : T) void residual_norm_kernel(Residu
         for (int i = 0; i < 8; i++) w[e][i] *= g[e][i];
     }
   }
+  if constexpr (Y != kNone) {
+    if (p.y_scale != 1.0f) {
+#pragma unroll
+      for (int e = 0; e < V; e++)
+#pragma unroll
+        for (int i = 0; i < 8; i++) w[e][i] *= p.y_scale;
+    }
+  }
 #pragma unroll
   for (int e = 0; e < V; e++) {
 #pragma unroll
     for (int i = 0; i < 8; i++) {
-      if constexpr (Y != kNone) v[e][i] = __builtin_fmaf(v[e][i], p.x_scale, w[e][i] * p.y_scale);
+      if constexpr (Y != kNone) v[e][i] = __builtin_fmaf(v[e][i], p.x_scale, w[e][i]);
       else v[e][i] *= p.x_scale;
-      if (!at[e].inside(i)) v[e][i] = 0.0f;  // what a norm left there
     }
     if (p.sum) at[e].template store<X>(p.sum, (size_t)row * p.ldsum, v[e]);
   }
@@ -239,10 +246,15 @@ __global__ __launch_bounds__(T == 64 ? 256 : T) void residual_norm_kernel(Residu
     if (p.qa) {
       uint32_t u = 0;
 #pragma unroll
-      for (int i = 0; i < 8; i++) {
-        if (!at[e].inside(i)) v[e][i] = 0.0f;
-        if (at[e].counts(i)) u = max(u, finite_abs_bits(v[e][i]));
+      for (int i = 0; i < 8; i++)
+        if (WHOLE || at[e].counts(i)) u = max(u, __float_as_uint(v[e][i]) & 0x7FFFFFFFu);
+      if (u >= 0x7F800000u) {  // infinities and NaN set no scale
+        u = 0;
+#pragma unroll
+        for (int i = 0; i < 8; i++)
+          if (WHOLE || at[e].counts(i)) u = max(u, finite_abs_bits(v[e][i]));
       }
+      if (!at[e].here) u = 0;
 #if defined(__HIP_DEVICE_COMPILE__)
 #define RH_ROR(n) u = max(u, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)u, 0x120 + n, 0xF, 0xF, true))
       RH_ROR(8);
@@ -256,7 +268,11 @@ __global__ __launch_bounds__(T == 64 ? 256 : T) void residual_norm_kernel(Residu
         const float f = fp8_inverse(x);
         uint64_t q = (uint32_t)fp8_pack4(v[e][4] * f, v[e][5] * f, v[e][6] * f, v[e][7] * f);
         q = q << 32 | (uint32_t)fp8_pack4(v[e][0] * f, v[e][1] * f, v[e][2] * f, v[e][3] * f);
-        if constexpr (!WHOLE) q >>= 8 * at[e].twice;  // and zeros behind the row
+        if constexpr (!WHOLE) {  // and zeros behind the row
+          q >>= 8 * (at[e].twice & 7);
+          if (n < 8) q &= (1ull << 8 * n) - 1;
+        }
+        if (!at[e].here) q = 0;
         __builtin_nontemporal_store(q, reinterpret_cast<uint64_t*>(p.qa + (size_t)row * p.ldq + c));
         if (t % 16 == 0)
           p.sa[fp8_scale_at((int)row, c / kFp8Block, (p.m - 1) / 128 + 1)] = (uint8_t)x;
