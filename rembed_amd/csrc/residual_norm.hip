@@ -6,8 +6,8 @@
 //   layer: (v - mean(v)) * w / sqrt(mean((v - mean(v))^2) + eps) + b
 // Statistics are fp32 sums over values in registers, the layer norm's variance around its mean; s
 // reaches `pre` unrounded, whatever type it is stored in, and codes are those of fp32 values.
-// Every row is read and written once: 8192 rows of 4096, 235 MB, take 49.5 µs, 4.7 TB/s; 2111 of
-// 768 4.8, of which a launch is 4.0; odd rows (1213 of 1001) 6.2.
+// Every row is read and written once: 8192 rows of 4096, 235 MB, take 48 µs, 4.9 TB/s; 2111 of 768
+// 4.9, of which a launch is 4.0; odd rows (1213 of 1001) 6.2.
 // Covers what the model forwards do in passes of their own (Add and the norms, tensor.go:383-387,
 // 433-471; Gemma's post-norms, gemma3.go:357,376).
 #include "rowops.h"

@@ -11,7 +11,7 @@ namespace rh {
 
 constexpr int kRopeThreads = 256;
 constexpr int kRopeItems = 4;    // the most heads of a thread, whose loads are in flight together
-// Cosines and sines that a workgroup holds, of heads of dh: eight rows', so that few large heads
+// Cosines and sines that a workgroup holds, of heads of dh: sixteen rows', so that few large heads
 // (a row of 4 heads of 256 is 16 threads) leave no threads without a row.
 __host__ __device__ constexpr int rope_pairs(int dh) { return 8 * dh; }
 // Floats of LDS: those, and q's and k's norm weights.
