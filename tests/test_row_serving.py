@@ -394,3 +394,39 @@ def test_rows_past_32_bits(gpu_ctx):
     for a, b in zip(*got):
         assert np.array_equal(a, b)
     assert got[0][4].any()
+
+
+def test_rows_of_more_than_a_launch(gpu_ctx):
+    """More rows than a launch's threads reach: the last ones are as those of a small call."""
+    from rembed_amd import tensor as T
+    rng = np.random.default_rng(4)
+    norm = T.Norm(None, 1e-6)
+    # residual norms: 2^21 rows a launch
+    m, n = (1 << 21) + 5, 24
+    x = rng.standard_normal((8, n)).astype(np.float32)
+    buf, out, want = gpu_ctx.alloc(m * n * 4), gpu_ctx.alloc(m * n * 4), gpu_ctx.alloc(8 * n * 4)
+    put(gpu_ctx, buf.ptr + (m - 8) * n * 4, x)
+    res = T.Residual(None, norm)
+    T.ResidualNorm(gpu_ctx, res, buf, False, n, None, False, 0, None, 0, out, False, n, None, 0, None, m, n)
+    T.ResidualNorm(gpu_ctx, res, gpu_ctx.upload(x), False, n, None, False, 0, None, 0, want, False, n, None, 0,
+                   None, 8, n)
+    gpu_ctx.sync()
+    assert np.array_equal(get(gpu_ctx, out.ptr + (m - 8) * n * 4, np.float32, (8, n)),
+                          want.download(np.float32, (8, n)))
+    # rotary rows, in place: sixteen rows of one head of 32 a workgroup, 2^23 workgroups a launch;
+    # and heads of 6, taken value by value, in more steps of a grid than one
+    for m, dh in (((1 << 27) + 3, 32), ((1 << 22) + (1 << 20) + 3, 6)):
+        x = rng.standard_normal((8, dh)).astype(np.float32)
+        bits, pos = F.bf16(x)[1], rng.integers(0, 9999, 8).astype(I32)
+        buf, dpos = gpu_ctx.alloc(m * dh * 2), gpu_ctx.alloc(m * 4)
+        put(gpu_ctx, buf.ptr + (m - 8) * dh * 2, bits)
+        put(gpu_ctx, dpos.ptr + (m - 8) * 4, pos)
+        want = gpu_ctx.upload(bits)
+        rope = T.Rope(gpu_ctx, dh)
+        T.RopeRows(gpu_ctx, rope, buf, True, dh, buf, True, dh, 0, 0, -1, 1, 0, dh, dpos, m, norm)
+        T.RopeRows(gpu_ctx, rope, want, True, dh, want, True, dh, 0, 0, -1, 1, 0, dh, gpu_ctx.upload(pos), 8,
+                   norm)
+        gpu_ctx.sync()
+        assert np.array_equal(get(gpu_ctx, buf.ptr + (m - 8) * dh * 2, np.uint16, (8, dh)),
+                              want.download(np.uint16, (8, dh)))
+        del buf, dpos
