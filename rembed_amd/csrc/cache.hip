@@ -399,8 +399,10 @@ __device__ __forceinline__ void append_block(const CacheAppendArgs& p, const Rop
 #if defined(__HIP_DEVICE_COMPILE__)
 #define RH_ROR(n)                                                                                 \
   ss += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(ss), 0x120 + n, 0xF, 0xF, true))
-    RH_ROR(4);  // the token's lanes
+    // the token's lanes: by 8 first, so that every lane adds the same two sums to the same bits (by
+    // 4 first, neighbours would add others, and the head have two factors a step apart)
     RH_ROR(8);
+    RH_ROR(4);
 #undef RH_ROR
 #endif
     if constexpr (PARTS == 8) ss += __shfl_xor(ss, 16, 64);

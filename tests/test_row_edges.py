@@ -1,0 +1,52 @@
+"""Edges of the row operators (residual norms, rotary rows, the rotary append, the cache read
+back): one factor for a whole head, many heads at document sizes, what is refused, frequencies of
+any size, codes next to a border. Against numpy in 64 bits (row_oracle, fp8_oracle).
+"""
+import numpy as np
+import pytest
+
+import fp8_oracle as O
+import test_fp8_operators as F
+
+I32 = np.int32
+
+
+# ---- GPU: the rotary append's norm of K ---------------------------------------------------
+
+def cached_k(ctx, rope, norm, x, kv, dh):
+    """K rows [n][kv][dh] (fp32, v zeros), a request and page each, at position 0, through the
+    rotary append: the codes [n][kv][dh]."""
+    from rembed_amd import tensor as T
+    n = x.shape[0]
+    rows = np.concatenate([x.reshape(n, -1), np.zeros((n, kv * dh))], 1).astype(np.float32)
+    cu, blk, _, slots, pos, _ = O.plan([0] * n, [1] * n, list(range(n)), np.zeros((n, 1), I32), n)
+    c = O.Cache(n, kv, dh)
+    dev = F.device_cache(ctx, c)
+    T.RopeAppend(ctx, rope, dev, ctx.upload(rows), False, rows.shape[1], 0, 0, kv * dh, None, False, 0,
+                 0, ctx.upload(pos), ctx.upload(cu), ctx.upload(blk), ctx.upload(slots), n, n, None, norm)
+    ctx.sync()
+    k = dev.k.download(np.uint8, c.k.shape)
+    return k[:, :, O.places(O.k_at, dh)[0]]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dh,kv,parts", [(64, 1, 4), (128, 2, 4), (128, 1, 8), (256, 1, 8)])
+def test_rope_append_norms_a_head_by_one_factor(gpu_ctx, dh, kv, parts):
+    """Equal values of a head have equal codes, whichever of the token's threads has them. The values
+    stand within four steps of fp32 of the place where their normed values change codes, so that
+    factors a step apart give other codes."""
+    from rembed_amd import tensor as T
+    rng = np.random.default_rng(dh + parts)
+    n = 300                       # 300 blocks of two heads are over 512 workgroups: four threads a token
+    x = rng.standard_normal((n, kv, dh)).astype(np.float32).astype(np.float64)
+    at = 8 * np.arange(parts)[:, None] + np.arange(8)  # eight values of each thread
+    x[..., at] = 0
+    border = 0.53125              # between the codes 0.5 and 0.5625, and 2^-k of them
+    mean = (x * x).sum(-1) / dh / (1 - 8 * parts * border ** 2 / dh)
+    near = (border * np.sqrt(mean + 1e-6)).astype(np.float32)
+    steps = np.arange(-4, 4)
+    x[..., at] = (near.view(I32)[..., None] + steps).astype(I32).view(np.float32)[:, :, None]
+    codes = cached_k(gpu_ctx, T.Rope(gpu_ctx, dh), T.Norm(None, 1e-6), x, kv, dh)[..., at]
+    assert (codes == codes[:, :, :1]).all()
+    below = (codes[:, :, 0, 0] != codes[:, :, 0, 7]).mean()
+    assert below > 0.5            # the border is among them
