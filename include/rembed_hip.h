@@ -408,7 +408,7 @@ int rh_cache_attention(rh_context *ctx, const void *q, int q_bf16, int ldq, int 
 #define RH_NORM_RMS 1
 #define RH_NORM_LAYER 2
 typedef struct {
-  int kind;
+  int kind;            /* RH_NORM_NONE: the other fields are not looked at */
   float eps;           /* >= 0 */
   const float *weight; /* dev [n]; NULL: ones */
   const float *bias;   /* dev [n], RH_NORM_LAYER only; NULL: zeros */

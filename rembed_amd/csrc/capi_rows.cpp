@@ -106,21 +106,27 @@ static bool share(const Rows& a, const Rows& b, int m) {
   return a.p && b.p && m > 0 && rows_overlap(a.p, a.wide, a.ld, b.p, b.wide, b.ld, m);
 }
 
-static int check_norm(const rh_norm& n, const char* what) {
+// Checks a norm. One of RH_NORM_NONE names no memory: what its other fields hold is not looked at.
+static int take_norm(const rh_norm& n, rh_norm& to) {
+  to = rh_norm{};
   if (n.kind < RH_NORM_NONE || n.kind > RH_NORM_LAYER) return fail(RH_ERR_INVALID, "unknown norm");
   if (n.kind == RH_NORM_NONE) return RH_OK;
   if (!std::isfinite(n.eps) || n.eps < 0) return fail(RH_ERR_INVALID, "eps must be finite, >= 0");
   if (n.bias && n.kind != RH_NORM_LAYER) return fail(RH_ERR_INVALID, "only a layer norm has a bias");
-  if (!aligned(n.weight, 4) || !aligned(n.bias, 4)) return fail(RH_ERR_INVALID, what);
+  if (!aligned(n.weight, 4) || !aligned(n.bias, 4))
+    return fail(RH_ERR_INVALID, "misaligned norm weight");
+  to = n;
   return RH_OK;
 }
 
 static int check_head_norm(const rh_norm* n, HeadNorm& to) {
   to = HeadNorm{};
-  if (!n || n->kind == RH_NORM_NONE) return RH_OK;
-  if (int st = check_norm(*n, "misaligned norm weight")) return st;
-  if (n->kind != RH_NORM_RMS) return fail(RH_ERR_INVALID, "heads take an RMS norm");
-  to = HeadNorm{1, n->eps, n->weight};
+  rh_norm own{};
+  if (!n) return RH_OK;
+  if (int st = take_norm(*n, own)) return st;
+  if (own.kind == RH_NORM_NONE) return RH_OK;
+  if (own.kind != RH_NORM_RMS) return fail(RH_ERR_INVALID, "heads take an RMS norm");
+  to = HeadNorm{1, own.eps, own.weight};
   return RH_OK;
 }
 
@@ -153,11 +159,12 @@ int rh_residual_norm(rh_context* ctx, const rh_residual* r, const void* x, int x
     if (!r) return fail(RH_ERR_INVALID, "null residual");
     if (m < 0 || n < 1) return fail(RH_ERR_INVALID, "bad m/n");
     if (n > 16384) return fail(RH_ERR_SHAPE, "n must be at most 16384");
-    if (int st = check_norm(r->post, "misaligned norm weight")) return st;
-    if (int st = check_norm(r->pre, "misaligned norm weight")) return st;
+    rh_norm post, pre;
+    if (int st = take_norm(r->post, post)) return st;
+    if (int st = take_norm(r->pre, pre)) return st;
     if (!std::isfinite(r->x_scale) || !std::isfinite(r->y_scale))
       return fail(RH_ERR_INVALID, "scales must be finite");
-    if (!y && (r->post.kind != RH_NORM_NONE || r->gate))
+    if (!y && (post.kind != RH_NORM_NONE || r->gate))
       return fail(RH_ERR_INVALID, "a post norm or gate needs y");
     if (r->gate && r->ldg != 0 && r->ldg < n)
       return fail(RH_ERR_SHAPE, "ldg must be 0 or cover the columns");
@@ -188,7 +195,7 @@ int rh_residual_norm(rh_context* ctx, const rh_residual* r, const void* x, int x
         scales_meet(rx) || scales_meet(ry) || scales_meet(rg) || scales_meet(rs) ||
         scales_meet(ro) || scales_meet(rq))
       return fail(RH_ERR_INVALID, "an output overlaps another buffer");
-    for (const float* w : {r->post.weight, r->post.bias, r->pre.weight, r->pre.bias}) {
+    for (const float* w : {post.weight, post.bias, pre.weight, pre.bias}) {
       const Rows rw = rows_of(w, 0, n, 0);
       if (share(rs, rw, m) || share(ro, rw, m) || share(rq, rw, m) || scales_meet(rw))
         return fail(RH_ERR_INVALID, "an output overlaps a norm's weights");
@@ -209,8 +216,8 @@ int rh_residual_norm(rh_context* ctx, const rh_residual* r, const void* x, int x
     a.qa = qa;
     a.sa = sa;
     a.ldq = ldq;
-    a.post = r->post;
-    a.pre = r->pre;
+    a.post = post;
+    a.pre = pre;
     a.gate = r->gate;
     a.ldg = r->ldg;
     a.x_scale = r->x_scale;

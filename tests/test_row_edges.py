@@ -2,6 +2,8 @@
 back): one factor for a whole head, many heads at document sizes, what is refused, frequencies of
 any size, codes next to a border. Against numpy in 64 bits (row_oracle, fp8_oracle).
 """
+import ctypes
+
 import numpy as np
 import pytest
 
@@ -9,6 +11,55 @@ import fp8_oracle as O
 import test_fp8_operators as F
 
 I32 = np.int32
+
+
+# ---- a norm that is none -------------------------------------------------------------------
+
+def at(p):
+    return ctypes.c_void_p(p)
+
+
+def passes(fn, *args):
+    """The call's checks let it through as far as to the context, which there is none."""
+    from rembed_amd import _lib as L
+    F.refused(L.RH_ERR_INVALID, fn, None, *args)
+    assert b"null context" in L.lib.rh_last_error(), L.lib.rh_last_error()
+
+
+def test_a_norm_that_is_none_names_no_memory():
+    from rembed_amd import _lib as L
+    rows = [at(1 << 20), 0, 256, at(2 << 20), 0, 256, at(3 << 20), 256, at(4 << 20), 1, 256, None, 0, None,
+            9, 256, None]
+    stale = L.NormDesc(0, float("nan"), 3 << 20, 1 + (4 << 20))  # on the outputs, and at odd bytes
+    none = L.NormDesc()
+    for post, pre in ((stale, none), (none, stale), (stale, stale)):
+        passes("rh_residual_norm", L.ResidualDesc(post, pre, None, 0, 1.0, 1.0), *rows)
+    rows[3] = None                                               # no y: a post norm of a kind is refused
+    passes("rh_residual_norm", L.ResidualDesc(stale, none, None, 0, 1.0, 1.0), *rows)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n", [1024, 1001, 16384])
+def test_a_norm_that_is_none_is_not_read(gpu_ctx, n):
+    """Weights of NaN that a norm of no kind names, at bytes that no 16-byte load takes: the bits
+    of null ones."""
+    from rembed_amd import _lib as L
+    from rembed_amd import tensor as T
+    rng = np.random.default_rng(n)
+    m = 5
+    x, y = (gpu_ctx.upload(rng.standard_normal((m, n)).astype(np.float32)) for _ in "xy")
+    nan = gpu_ctx.upload(np.full(n + 1, np.nan, np.float32))
+    got = []
+    for w in (None, nan.ptr + 4):
+        out, total = gpu_ctx.alloc(m * n * 4), gpu_ctx.alloc(m * n * 4)
+        res = T.Residual()
+        for norm in (res.desc.post, res.desc.pre):
+            norm.kind, norm.eps, norm.weight, norm.bias = L.RH_NORM_NONE, 1e-6, w, w
+        T.ResidualNorm(gpu_ctx, res, x, False, n, y, False, n, total, n, out, False, n, None, 0, None, m, n)
+        gpu_ctx.sync()
+        got.append([b.download(np.uint32, (m, n)) for b in (out, total)])
+    for a, b in zip(*got):
+        assert np.array_equal(a, b) and np.isfinite(a.view(np.float32)).all()
 
 
 # ---- GPU: the rotary append's norm of K ---------------------------------------------------
