@@ -81,6 +81,35 @@ static int rope_frequencies(const rh_rope_config* c, std::vector<long double>& f
   return RH_OK;
 }
 
+// 1 / (2 pi) in binary, 64 bits a word: behind the point as many as the largest double's fraction of
+// a turn takes.
+static const uint64_t kInvTwoPi[18] = {
+    0x28BE60DB9391054A, 0x7F09D5F47D4D3770, 0x36D8A5664F10E410, 0x7F9458EAF7AEF158, 0x6DC91B8E909374B8,
+    0x01924BBA82746487, 0x3F877AC72C4A69CF, 0xBA208D7D4BAED121, 0x3A671C09AD17DF90, 0x4E64758E60D4CE7D,
+    0x272117E2EF7E4A0E, 0xC7FE25FFF7816603, 0xFBCBC462D6829B47, 0xDB4D9FB3C9F2C26D, 0xD3D18FD9A797FA8B,
+    0x5D49EEB1FAF97C5E, 0xCF41CE7DE294A4BA, 0x9AFED7EC47E35742};
+
+// f radians in turns, mod 1, rounded to 64 bits: |f| = m 2^e with m whole, and only the bits of
+// 1 / (2 pi) from 2^(-e - 1) on give m 2^e / (2 pi) a fraction, of which the first 192 leave out under
+// 2^-128 of a turn. A quotient of long doubles instead would be off by up to 2^-64 of its own size:
+// at f = 50 and position 2^31 by 2^-30 of a turn, and by whole turns from f = 2^67 on.
+static uint64_t turns_of(long double f) {
+  int e;
+  const uint64_t m = (uint64_t)ldexpl(frexpl(fabsl(f), &e), 64);
+  e -= 64;
+  auto bits = [](int from) -> uint64_t {  // 64 of 1 / (2 pi), behind the first `from`
+    if (from <= -64) return 0;
+    if (from < 0) return kInvTwoPi[0] >> -from;
+    auto word = [](int i) -> uint64_t { return i < 18 ? kInvTwoPi[i] : 0; };
+    const int i = from / 64, s = from % 64;
+    return s ? word(i) << s | word(i + 1) >> (64 - s) : word(i);
+  };
+  using u128 = unsigned __int128;
+  const u128 low = (u128)m * bits(e + 64) + (uint64_t)((u128)m * bits(e + 128) >> 64);
+  const uint64_t u = m * bits(e) + (uint64_t)(low >> 64) + ((uint64_t)low >> 63);
+  return f < 0 ? 0 - u : u;
+}
+
 static void destroy_rope(rh_rope* r) {
   if (r->d_freq) (void)hipFree(r->d_freq);
   delete r;
@@ -251,8 +280,7 @@ int rh_rope_create(rh_context* ctx, const rh_rope_config* cfg, rh_rope** out) {
     // whole turns a position change nothing: positions are whole numbers
     std::vector<RopeFreq> turns(f.size());
     for (size_t i = 0; i < f.size(); i++) {
-      const long double t = f[i] / (2 * acosl(-1.0L)), x = roundl((t - floorl(t)) * 0x1p64L);
-      const uint64_t u = x >= 0x1p64L ? 0 : (uint64_t)x;
+      const uint64_t u = turns_of(f[i]);
       turns[i] = RopeFreq{(int32_t)(uint32_t)u, (int32_t)(uint32_t)((u + 0x80000000u) >> 32)};
     }
     CTX_GUARD(ctx);

@@ -5,7 +5,8 @@
 //   a' = m (a cos(t f) - b sin(t f)),   b' = m (b cos(t f) + a sin(t f)).
 // Positions are whole numbers, so whole turns of f drop out: f is kept as a 64-bit fraction of a
 // turn, t f mod 1 is a product mod 2^64, exact but for f's own rounding (2^-65 of a turn a
-// position; 2^-34 at 2^31) and the 32 bits that are kept, and no table limits how long a text is.
+// position, 2^-34 at 2^31, whatever f's size; a computed f, at most 1, is off by as much again) and
+// the 32 bits that are kept, and no table limits how long a text is.
 // fp32 angles would be off by 2^-24 of the angle itself: 0.004 rad at position 65536.
 #pragma once
 

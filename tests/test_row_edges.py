@@ -8,6 +8,7 @@ import numpy as np
 import pytest
 
 import fp8_oracle as O
+import row_oracle as R
 import test_fp8_operators as F
 
 I32 = np.int32
@@ -60,6 +61,63 @@ def test_a_norm_that_is_none_is_not_read(gpu_ctx, n):
         got.append([b.download(np.uint32, (m, n)) for b in (out, total)])
     for a, b in zip(*got):
         assert np.array_equal(a, b) and np.isfinite(a.view(np.float32)).all()
+
+
+# ---- GPU: frequencies of any size ------------------------------------------------------------
+
+BITS = 1400
+
+
+def machin():
+    """pi * 2^BITS in whole numbers: 16 arctan(1/5) - 4 arctan(1/239)."""
+    def arctan(n):
+        x = (1 << BITS) // n
+        total, i = 0, 1
+        while x:
+            total += x // i if i % 4 == 1 else -(x // i)
+            x //= n * n
+            i += 2
+        return total
+    return 16 * arctan(5) - 4 * arctan(239)
+
+
+def turn_fraction(pos, freq, pi):
+    """pos * freq / (2 pi) less the nearest whole number, within 2^-63."""
+    n, d = float(freq).as_integer_ratio()
+    u = (pos * n << BITS + 64) // (2 * d * pi) % (1 << 64)
+    return (u - (1 << 64) if u >> 63 else u) / 2.0 ** 64
+
+
+@pytest.mark.gpu
+def test_rope_of_given_frequencies_of_any_size(gpu_ctx):
+    """Angles within 2^-31 of a turn at every position: a sine near a whole turn shows them. Sine and
+    cosine are those of pi from whole numbers."""
+    from rembed_amd import tensor as T
+    rng = np.random.default_rng(0)
+    pi = machin()
+    assert abs(pi / (1 << BITS) - np.pi) < 1e-15
+    freq = [0.0, 5e-324, 1e-30, 2.0 ** -40, 0.37, 1.0, np.pi, 2 * np.pi, 50.0, -50.0, 1e3, -12345.678, 1e6, 2.0 ** 53,
+            1e16, -3e18, 2.0 ** 63, 2.0 ** 64, 1e20, -1e25, 1e30, 1.7e38, 2.0 ** 127, 1e50, -1e77, 1e100, 1e150, 2.0 ** 640,
+            1e200, -1e250, 1e300, np.finfo(np.float64).max]
+    n, dh = len(freq), 2 * len(freq)
+    pos = np.concatenate([[0, 1, -1, 2, 2 ** 31 - 1, -2 ** 31], rng.integers(-2 ** 31, 2 ** 31, 2000)])
+    # those whose angle of one of the frequencies is next to a whole turn, and some others
+    frac = np.array([[turn_fraction(int(p), f, pi) for f in freq] for p in pos])
+    pick = np.unique(np.concatenate([np.arange(60), np.abs(np.where(frac == 0, 1, frac)).argmin(0)]))
+    pos, frac = pos[pick].astype(I32), frac[pick]
+    x = np.zeros((len(pos), dh), np.float32)
+    x[:, :n] = 1.0                                 # (1, 0) becomes (cos, sin)
+    rope = T.Rope(gpu_ctx, dh, scaling=5, freq=freq)
+    out = gpu_ctx.alloc(x.nbytes)
+    T.RopeRows(gpu_ctx, rope, gpu_ctx.upload(x), False, dh, out, False, dh, 0, 0, -1, 1, 0, dh,
+               gpu_ctx.upload(pos), len(pos))
+    gpu_ctx.sync()
+    got = out.download(np.float32, x.shape).astype(np.float64)
+    c, s = np.cos(2 * np.pi * frac), np.sin(2 * np.pi * frac)
+    off = 2 * np.pi * 2.0 ** -31
+    # relative where the sine is small: its polynomial, t itself and two products round it
+    assert (np.abs(got[:, n:] - s) <= off + R.TURN * np.abs(s)).all()
+    assert (np.abs(got[:, :n] - c) <= off * np.abs(s) + off ** 2 + R.TURN).all()
 
 
 # ---- GPU: the rotary append's norm of K ---------------------------------------------------
