@@ -398,7 +398,8 @@ int rh_cache_attention(rh_context *ctx, const void *q, int q_bf16, int ldq, int 
  * value is stored (rows or heads whose squares sum to 2^128 and more become 0 in a norm). `used` may
  * name a device integer (a plan's cu + batch, status + 1): rows from it on are left as they
  * are; NULL: all rows are taken. An output may lie exactly on an input of its own type and
- * stride, as said; other overlaps are refused. Rows and columns have no alignment beyond
+ * stride, as said; one on other bytes that the call reads or writes (rows, gates, norms' weights,
+ * positions, tables, `used`, the cache) is refused. Rows and columns have no alignment beyond
  * their type's unless said; 16-byte aligned rows of whole 16-byte groups are read faster. */
 
 /* A norm of rows or heads: v * weight / sqrt(mean(v^2) + eps) (RMSNorm, tensor.go:459-471), or

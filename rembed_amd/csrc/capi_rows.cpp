@@ -4,7 +4,9 @@
 // Like the rest of the ABI every entry point checks its arguments, returns an RH_* status and
 // enqueues on the context's stream. None but rh_rope_create allocates or waits.
 #include <algorithm>
+#include <array>
 #include <cmath>
+#include <initializer_list>
 #include <memory>
 #include <vector>
 
@@ -135,6 +137,38 @@ static bool share(const Rows& a, const Rows& b, int m) {
   return a.p && b.p && m > 0 && rows_overlap(a.p, a.wide, a.ld, b.p, b.wide, b.ld, m);
 }
 
+// A stretch of memory that a call reads, or writes as a whole.
+struct Bytes {
+  const void* p;
+  size_t n;
+};
+static bool meet(const Bytes& a, const Bytes& b) {
+  const uintptr_t x = (uintptr_t)a.p, y = (uintptr_t)b.p;
+  return a.p && b.p && a.n && b.n && x < y + b.n && y < x + a.n;
+}
+// Whether a stretch shares bytes with m rows; what lies between two rows is none of theirs.
+static bool meet(const Rows& r, int m, const Bytes& a) {
+  if (!r.p || !a.p || m <= 0 || !r.wide || !a.n) return false;
+  const uintptr_t x = (uintptr_t)r.p, y = (uintptr_t)a.p;
+  size_t i = 0;  // the first row that ends behind a's beginning
+  if (y >= x + r.wide) {
+    if (!r.ld) return false;  // one row for all
+    i = (y - x - r.wide) / r.ld + 1;
+  }
+  return i < (size_t)m && x + i * r.ld < y + a.n;
+}
+// Whether an output's rows lie on one of the stretches.
+static bool on_any(const Rows& out, int m, std::initializer_list<Bytes> all) {
+  return std::any_of(all.begin(), all.end(), [&](const Bytes& a) { return meet(out, m, a); });
+}
+static Bytes ints(const int32_t* p, long long n) { return {p, (size_t)n * sizeof(int32_t)}; }
+static Bytes floats(const float* p, int n) { return {p, (size_t)n * sizeof(float)}; }
+// What a cache holds: K, V and their scale bytes.
+static std::array<Bytes, 4> buffers_of(const rh_kv_cache& c) {
+  const size_t heads = (size_t)c.pages * c.kv_heads, codes = heads * RH_CACHE_BLOCK * c.dh;
+  return {Bytes{c.k, codes}, Bytes{c.v, codes}, Bytes{c.k_exp, heads}, Bytes{c.v_exp, heads}};
+}
+
 // Checks a norm. One of RH_NORM_NONE names no memory: what its other fields hold is not looked at.
 static int take_norm(const rh_norm& n, rh_norm& to) {
   to = rh_norm{};
@@ -212,23 +246,17 @@ int rh_residual_norm(rh_context* ctx, const rh_residual* r, const void* x, int x
     const Rows rs = rows_of(sum, x_bf16, n, ldsum), ro = rows_of(out, out_bf16, n, ldout);
     const Rows rg = rows_of(r->gate, 0, n, r->ldg);
     const Rows rq{qa, 1, (size_t)ldq, (size_t)ldq};
-    const size_t bytes = qa ? rh_fp8_scale_bytes(m, n) : 0;
-    auto scales_meet = [&](const Rows& o) {
-      if (!sa || !o.p || m <= 0) return false;
-      const uintptr_t a = (uintptr_t)sa, b = (uintptr_t)o.p;
-      return a < b + (size_t)(m - 1) * o.ld + o.wide && b < a + bytes;
-    };
+    const Bytes scales{sa, rh_fp8_scale_bytes(m, n)};
     if (clash(rs, rx, m) || clash(rs, ry, m) || share(rs, rg, m) || clash(ro, rx, m) ||
         clash(ro, ry, m) || share(ro, rg, m) || share(rs, ro, m) || share(rq, rx, m) ||
-        share(rq, ry, m) || share(rq, rg, m) || share(rq, rs, m) || share(rq, ro, m) ||
-        scales_meet(rx) || scales_meet(ry) || scales_meet(rg) || scales_meet(rs) ||
-        scales_meet(ro) || scales_meet(rq))
+        share(rq, ry, m) || share(rq, rg, m) || share(rq, rs, m) || share(rq, ro, m))
       return fail(RH_ERR_INVALID, "an output overlaps another buffer");
-    for (const float* w : {post.weight, post.bias, pre.weight, pre.bias}) {
-      const Rows rw = rows_of(w, 0, n, 0);
-      if (share(rs, rw, m) || share(ro, rw, m) || share(rq, rw, m) || scales_meet(rw))
-        return fail(RH_ERR_INVALID, "an output overlaps a norm's weights");
-    }
+    for (const Rows& rows : {rx, ry, rg, rs, ro, rq})
+      if (meet(rows, m, scales)) return fail(RH_ERR_INVALID, "an output overlaps another buffer");
+    for (const Bytes& b : {floats(post.weight, n), floats(post.bias, n), floats(pre.weight, n),
+                           floats(pre.bias, n), ints(used, 1)})
+      if (meet(rs, m, b) || meet(ro, m, b) || meet(rq, m, b) || meet(scales, b))
+        return fail(RH_ERR_INVALID, "an output overlaps a norm's weights or used");
     CTX_GUARD(ctx);
     ResidualArgs a{};
     a.x = x;
@@ -342,6 +370,14 @@ int rh_rope_rows(rh_context* ctx, const rh_rope* rope, const void* x, int x_bf16
       return fail(RH_ERR_INVALID, "misaligned buffer");
     if (!on_x && share(rows_of(out, out_bf16, end, ldout), rows_of(x, x_bf16, end, ldx), rows))
       return fail(RH_ERR_INVALID, "out overlaps x without being it");
+    a.v_heads = wv && !on_x ? kv_heads : 0;
+    auto written = [&](int off, long long wide) {
+      return rows_of(static_cast<char*>(out) + (size_t)off * (out_bf16 ? 2 : 4), out_bf16, wide, ldout);
+    };
+    for (const Rows& r : {written(q_off, wq), written(k_off, wk), written(v_off, a.v_heads ? wv : 0)})
+      if (on_any(r, rows, {floats(a.q_norm.weight, dh), floats(a.k_norm.weight, dh), ints(pos, rows),
+                           ints(used, 1)}))
+        return fail(RH_ERR_INVALID, "out overlaps a norm's weights, pos or used");
     CTX_GUARD(ctx);
     a.turn = turn_of(rope);
     a.x = x;
@@ -355,7 +391,6 @@ int rh_rope_rows(rh_context* ctx, const rh_rope* rope, const void* x, int x_bf16
     a.v_off = a.v_out = v_off;
     a.heads = heads;
     a.kv_heads = kv_heads;
-    a.v_heads = wv && !on_x ? kv_heads : 0;
     a.dh = dh;
     a.pos = pos;
     a.used = used;
@@ -397,8 +432,6 @@ int rh_rope_append(rh_context* ctx, const rh_rope* rope, const rh_kv_cache* cach
              : share(out, rows_of(x, x_bf16, end, ldx), rows))
       return fail(RH_ERR_INVALID, "q overlaps x without being its own columns");
     const long long segs = std::min((long long)rows, (long long)rows / RH_CACHE_BLOCK + 2LL * batch);
-    CTX_GUARD(ctx);
-    if (batch == 0 || rows == 0) return RH_OK;
     CacheAppendArgs c{*cache, x, x_bf16 ? 1 : 0, ldx, k_off, v_off, cu, blocks, slots, batch,
                       cache->pages ? rows : 0};
     a.turn = turn_of(rope);
@@ -414,7 +447,24 @@ int rh_rope_append(rh_context* ctx, const rh_rope* rope, const rh_kv_cache* cach
     a.pos = pos;
     a.used = cu + batch;
     a.rows = rows;
-    if (rope_append_grid(c, a) >= 1 << 23) return fail(RH_ERR_SHAPE, "too many rows for one call");
+    if (batch > 0 && rope_append_grid(c, a) >= 1 << 23)
+      return fail(RH_ERR_SHAPE, "too many rows for one call");
+    if (batch > 0 && rows > 0) {
+      const auto read = {ints(pos, rows), ints(cu, batch + 1LL), ints(blocks, batch + 1LL),
+                         Bytes{slots, (size_t)rows * sizeof(int64_t)},
+                         floats(a.q_norm.weight, cache->dh), floats(a.k_norm.weight, cache->dh)};
+      if (on_any(out, rows, read)) return fail(RH_ERR_INVALID, "q overlaps what the call reads");
+      const Rows in = rows_of(x, x_bf16, end, ldx);
+      for (const Bytes& held : buffers_of(*cache)) {
+        if (meet(out, rows, held)) return fail(RH_ERR_INVALID, "q overlaps the cache");
+        if (meet(in, rows, held) || std::any_of(read.begin(), read.end(), [&](const Bytes& b) {
+              return meet(held, b);
+            }))
+          return fail(RH_ERR_INVALID, "the cache overlaps what the call reads");
+      }
+    }
+    CTX_GUARD(ctx);
+    if (batch == 0 || rows == 0) return RH_OK;
     RH_HIP(launch_rope_append(c, a, ctx->stream));
     return RH_OK;
   });
@@ -436,6 +486,17 @@ int rh_cache_read(rh_context* ctx, const rh_kv_cache* cache, const int32_t* tabl
       return fail(RH_ERR_SHAPE, "rows and offsets must be multiples of 8 values, out 16-byte aligned");
     if (((long long)rows / RH_CACHE_BLOCK + 2LL * batch) * cache->kv_heads >= 1 << 24)
       return fail(RH_ERR_SHAPE, "too many blocks for one call");  // 2^32 threads
+    if (batch > 0 && rows > 0) {
+      const size_t each = out_bf16 ? 2 : 4;
+      for (int off : {k_off, v_off}) {
+        const Rows r = rows_of(static_cast<char*>(out) + off * each, out_bf16, width, ldout);
+        if (on_any(r, rows, {ints(table, (long long)batch * ldt), ints(cu, batch + 1LL),
+                             ints(first, batch)}))
+          return fail(RH_ERR_INVALID, "out overlaps what the call reads");
+        for (const Bytes& held : buffers_of(*cache))
+          if (meet(r, rows, held)) return fail(RH_ERR_INVALID, "out overlaps the cache");
+      }
+    }
     CTX_GUARD(ctx);
     if (batch == 0 || rows == 0) return RH_OK;
     CacheReadArgs a{*cache, table, ldt, cu, first, batch, rows, out, out_bf16 ? 1 : 0, ldout,

@@ -63,6 +63,140 @@ def test_a_norm_that_is_none_is_not_read(gpu_ctx, n):
         assert np.array_equal(a, b) and np.isfinite(a.view(np.float32)).all()
 
 
+# ---- outputs on what a call reads -------------------------------------------------------------
+
+def test_residual_overlaps():
+    """An output that holds the weights, the gate, the count or the scales is refused to the byte;
+    what lies between an output's rows, or next to them, is not."""
+    from rembed_amd import _lib as L
+    out, codes, scales = 4 << 20, 5 << 20, 6 << 20   # 9 rows of 256 values, 512 apart; codes; 2 * 128 bytes
+    n, m, ld = 256, 9, 512
+    end = out + 8 * ld * 4 + n * 4
+
+    def call(post=L.NormDesc(), pre=L.NormDesc(), gate=None, ldg=0, used=None, sa=scales):
+        return ["rh_residual_norm", L.ResidualDesc(post, pre, gate, ldg, 1.0, 1.0), at(1 << 20), 0, n,
+                at(2 << 20), 0, n, None, 0, at(out), 0, ld, at(codes), n, at(sa), m, n, used]
+
+    def no(**kw):
+        fn, *args = call(**kw)
+        F.refused(L.RH_ERR_INVALID, fn, None, *args)
+        assert b"overlaps" in L.lib.rh_last_error()
+
+    gaps = [out + i * ld * 4 + n * 4 for i in range(m)]
+    for p in gaps + [out - n * 4, end, codes - n * 4, codes + m * n, scales - n * 4, scales + 256]:
+        for norm in (L.NormDesc(1, 0, p, None), L.NormDesc(2, 0, None, p)):
+            passes(*call(pre=norm))
+            passes(*call(post=norm))
+        passes(*call(used=at(p)))
+    for p in [out, end - 4, codes, codes + m * n - 4, scales, scales + 252] + [g - 4 for g in gaps]:
+        for norm in (L.NormDesc(1, 0, p, None), L.NormDesc(2, 0, None, p), L.NormDesc(1, 0, p - n * 4 + 4, None)):
+            no(pre=norm)
+            no(post=norm)
+        no(used=at(p))
+    no(pre=L.NormDesc(1, 0, gaps[0] + 4, None))      # on the next row's first value
+    no(gate=out + 4 * ld, ldg=ld)
+    no(gate=scales + 252)
+    for p in gaps:
+        passes(*call(sa=p))
+    for p in (out, gaps[3] - 4, end - 4, codes + 4, 1 << 20, (2 << 20) + m * n * 4 - 4):
+        no(sa=p)
+
+
+def test_read_overlaps():
+    """Rows of K and V on the cache, the table, the offsets or the first positions."""
+    from rembed_amd import _lib as L
+    k, v, ke, ve, table, cu, first, out = (i << 20 for i in range(1, 9))
+    codes, rows, batch, ldt = 4 * 2 * 64 * 64, 9, 2, 4   # 4 pages of 2 heads of 64; rows of 8 + 2 * 128, 300 apart
+
+    def call(**kw):
+        p = dict(k=k, v=v, ke=ke, ve=ve, table=table, cu=cu, first=first)
+        p.update(kw)
+        return ["rh_cache_read", F.desc(4, 2, 64, p["k"], p["v"], p["ke"], p["ve"]), at(p["table"]), ldt,
+                at(p["cu"]), at(p["first"]), batch, rows, at(out), 0, 304, 8, 136]
+
+    sizes = dict(k=codes, v=codes, ke=8, ve=8, table=batch * ldt * 4, cu=12, first=8)
+    end = out + (8 * 304 + 264) * 4
+    for name, size in sizes.items():
+        # in front of the first row's columns, behind the last's, between two rows where it fits
+        near = [out + 32 - (size + 15) // 16 * 16, end] + [out + (i * 304 + 264) * 4 for i in range(8) if size <= 160]
+        for p in near:
+            passes(*call(**{name: p}))
+        for p in (out + 32, end - 16, out + (3 * 304 + 260) * 4, out + (4 * 304 + 136) * 4):
+            fn, *args = call(**{name: p})
+            F.refused(L.RH_ERR_INVALID, fn, None, *args)
+            assert b"overlaps" in L.lib.rh_last_error(), name
+
+
+@pytest.mark.gpu
+def test_rotary_overlaps(gpu_ctx):
+    """Rotary rows and the rotary append: outputs on weights, positions, tables, the cache. Every
+    refusal is the host's."""
+    from rembed_amd import _lib as L
+    from rembed_amd import tensor as T
+    rope, buf = T.Rope(gpu_ctx, 32), gpu_ctx.upload(np.zeros(1 << 23, np.uint8))
+    x, out, pos, used, w = (buf.ptr + (i << 20) for i in range(5))
+    rms = lambda p: L.NormDesc(1, 0, p, None)
+
+    def rows(pos=pos, used=used, q=rms(w), k=rms(w + 256)):
+        return [gpu_ctx.h, rope.h, x, 1, 528, out, 0, 528, 8, 264, 392, 4, 2, 64, pos, 9, q, k, used]
+
+    last = out + (8 * 528 + 392 + 128) * 4               # behind v's last value
+    inside = [out + 32, out + 264 * 4, last - 4, out + (528 + 8) * 4]
+    for p in inside:
+        for kw in (dict(pos=p), dict(used=p), dict(q=rms(p)), dict(k=rms(p)), dict(pos=p - 32), dict(k=rms(p - 252))):
+            F.refused(L.RH_ERR_INVALID, "rh_rope_rows", *rows(**kw))
+            assert b"overlaps" in L.lib.rh_last_error()
+
+    k, v, ke, ve, cu, blk, slots = (buf.ptr + (5 << 20) + (i << 17) for i in range(7))
+    codes = 2 * 64 * 64                                  # two pages of one head
+
+    def app(k=k, v=v, ke=ke, ve=ve, cu=cu, blk=blk, slots=slots, pos=pos, qn=rms(w), kn=rms(w + 256)):
+        return [gpu_ctx.h, rope.h, F.desc(2, 1, 64, k, v, ke, ve), x, 1, 512, 8, 264, 392, out, 1, 512, 4, pos,
+                cu, blk, slots, 2, 9, qn, kn]
+
+    q_end = out + (8 * 512 + 256) * 2
+    for name in ("k", "v", "ke", "ve", "cu", "blk", "slots", "pos", "qn", "kn"):
+        take = rms if name in ("qn", "kn") else int
+        on_q = [out, out + 16, q_end - 16, out + 512 * 2 * 3 + 496]
+        on_x = [x, x + (8 * 512 + 448) * 2] if name in ("k", "v", "ke", "ve") else []
+        on_cache = [] if name in ("k", "v", "ke", "ve") else [k, v + codes - 8, ke, ve]
+        for p in on_q + on_x + on_cache:
+            F.refused(L.RH_ERR_INVALID, "rh_rope_append", *app(**{name: take(p)}))
+            assert b"overlaps" in L.lib.rh_last_error(), (name, p)
+
+
+@pytest.mark.gpu
+def test_rotary_rows_beside_what_they_read(gpu_ctx):
+    """Weights, positions and the count between the output's rows: the bits of other places."""
+    from rembed_amd import tensor as T
+    rng = np.random.default_rng(5)
+    rope, n, dh = T.Rope(gpu_ctx, 64), 7, 64
+    ld = 2 * dh + 96                                     # 96 values between two rows
+    img = rng.standard_normal((n, 2 * dh)).astype(np.float32)
+    x = gpu_ctx.upload(img)
+    pos, w = rng.integers(0, 999, n).astype(I32), rng.uniform(0.5, 1.5, dh).astype(np.float32)
+
+    class At:
+        def __init__(self, buf, value):
+            self.ptr = buf.ptr + 4 * value
+
+    got = []
+    for inside in (False, True):
+        host = np.zeros((n, ld), np.float32)
+        host[0, 2 * dh:2 * dh + n] = pos.view(np.float32)
+        host[1, 2 * dh + 32:] = w
+        host[2, 2 * dh + 5] = np.array([n - 1], I32).view(np.float32)[0]
+        buf = gpu_ctx.upload(host)
+        place = buf if inside else gpu_ctx.upload(host)
+        norm = T.Norm(At(place, ld + 2 * dh + 32), 1e-6)
+        T.RopeRows(gpu_ctx, rope, x, False, 2 * dh, buf, False, ld, 0, dh, -1, 1, 1, dh, At(place, 2 * dh), n,
+                   norm, norm, At(place, 2 * ld + 2 * dh + 5))
+        gpu_ctx.sync()
+        got.append(buf.download(np.uint32, (n, ld)))
+        assert np.array_equal(got[-1][:, 2 * dh:], host.view(np.uint32)[:, 2 * dh:]) and not got[-1][n - 1, :2 * dh].any()
+    assert np.array_equal(*got) and got[0][:n - 1, :2 * dh].any(1).all()
+
+
 # ---- GPU: frequencies of any size ------------------------------------------------------------
 
 BITS = 1400
