@@ -423,7 +423,8 @@ int rh_rope_append(rh_context* ctx, const rh_rope* rope, const rh_kv_cache* cach
     if (ldx % 8 || q_off % 8 || k_off % 8 || v_off % 8 || !aligned(x, 16) ||
         (heads && (ldq % 8 || !aligned(q, 16))))
       return fail(RH_ERR_SHAPE, "rows and offsets must be multiples of 8 values, x and q 16-byte aligned");
-    if (!aligned(pos, 4) || !aligned(slots, 8)) return fail(RH_ERR_INVALID, "misaligned buffer");
+    if (!aligned(pos, 4) || !aligned(slots, 8) || !aligned(cu, 4) || !aligned(blocks, 4))
+      return fail(RH_ERR_INVALID, "misaligned buffer");
     // q may lie on its own columns of x, and nowhere else among the rows
     const size_t each = x_bf16 ? 2 : 4;
     const bool on_x = x && q == static_cast<const char*>(x) + q_off * each && !x_bf16 == !q_bf16 && ldq == ldx;
@@ -431,7 +432,6 @@ int rh_rope_append(rh_context* ctx, const rh_rope* rope, const rh_kv_cache* cach
     if (on_x ? columns_meet(q_off, wq, k_off, wk) || columns_meet(q_off, wq, v_off, wk)
              : share(out, rows_of(x, x_bf16, end, ldx), rows))
       return fail(RH_ERR_INVALID, "q overlaps x without being its own columns");
-    const long long segs = std::min((long long)rows, (long long)rows / RH_CACHE_BLOCK + 2LL * batch);
     CacheAppendArgs c{*cache, x, x_bf16 ? 1 : 0, ldx, k_off, v_off, cu, blocks, slots, batch,
                       cache->pages ? rows : 0};
     a.turn = turn_of(rope);
@@ -484,6 +484,8 @@ int rh_cache_read(rh_context* ctx, const rh_kv_cache* cache, const int32_t* tabl
     if (columns_meet(k_off, width, v_off, width)) return fail(RH_ERR_SHAPE, "K and V share columns");
     if (ldout % 8 || k_off % 8 || v_off % 8 || !aligned(out, 16))
       return fail(RH_ERR_SHAPE, "rows and offsets must be multiples of 8 values, out 16-byte aligned");
+    if (!aligned(table, 4) || !aligned(cu, 4) || !aligned(first, 4))
+      return fail(RH_ERR_INVALID, "misaligned buffer");
     if (((long long)rows / RH_CACHE_BLOCK + 2LL * batch) * cache->kv_heads >= 1 << 24)
       return fail(RH_ERR_SHAPE, "too many blocks for one call");  // 2^32 threads
     if (batch > 0 && rows > 0) {

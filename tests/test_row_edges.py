@@ -197,6 +197,33 @@ def test_rotary_rows_beside_what_they_read(gpu_ctx):
     assert np.array_equal(*got) and got[0][:n - 1, :2 * dh].any(1).all()
 
 
+def test_misaligned_tables_of_a_read():
+    from rembed_amd import _lib as L
+    ok = [None, F.desc(), F.P, 4, F.P, None, 2, 9, at(1 << 20), 1, 256, 0, 128]
+    for i in (2, 4, 5):
+        a = list(ok)
+        a[i] = at(4098)
+        F.refused(L.RH_ERR_INVALID, "rh_cache_read", *a)
+        assert b"misaligned" in L.lib.rh_last_error()
+
+
+@pytest.mark.gpu
+def test_misaligned_tables_of_a_rotary_append(gpu_ctx):
+    from rembed_amd import _lib as L
+    from rembed_amd import tensor as T
+    rope, buf = T.Rope(gpu_ctx, 32), gpu_ctx.upload(np.zeros(1 << 20, np.uint8))
+    p = [buf.ptr + (i << 16) for i in range(10)]
+    ok = [gpu_ctx.h, rope.h, F.desc(2, 1, 64, p[0], p[1], p[2], p[3]), p[4], 1, 192, 0, 64, 128, p[5], 1, 64, 1,
+          p[6], p[7], p[8], p[9], 1, 4, None, None]
+    for i in (14, 15):
+        a = list(ok)
+        a[i] += 2
+        F.refused(L.RH_ERR_INVALID, "rh_rope_append", *a)
+        assert b"misaligned" in L.lib.rh_last_error()
+    assert L.lib.rh_rope_append(*ok) == 0                # of no rows: every offset is 0
+    gpu_ctx.sync()
+
+
 # ---- GPU: frequencies of any size ------------------------------------------------------------
 
 BITS = 1400
