@@ -463,7 +463,7 @@ typedef struct {
   double theta;       /* > 1 (GIVEN: unused) */
   double factor;      /* >= 1 */
   double fast, slow;
-  double amp;         /* 0: the method's own */
+  double amp;         /* 0: the method's own; finite in fp32 */
   const double *freq; /* GIVEN: host [rot/2], finite */
 } rh_rope_config;
 /* f_i [rot/2] and amp, on the host (either may be NULL). */

@@ -33,7 +33,8 @@ static int rope_frequencies(const rh_rope_config* c, std::vector<long double>& f
     return fail(RH_ERR_SHAPE, "rot must be even, 2 to 256");
   if (c->scaling < RH_ROPE_PLAIN || c->scaling > RH_ROPE_GIVEN)
     return fail(RH_ERR_INVALID, "unknown rope scaling");
-  if (!std::isfinite(c->amp) || c->amp < 0) return fail(RH_ERR_INVALID, "amp must be finite, >= 0");
+  if (!std::isfinite((float)c->amp) || c->amp < 0)
+    return fail(RH_ERR_INVALID, "amp must be finite in fp32, >= 0");
   const int pairs = c->rot / 2;
   f.resize(pairs);
   amp = 1.0;

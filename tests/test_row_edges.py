@@ -249,6 +249,16 @@ def turn_fraction(pos, freq, pi):
     return (u - (1 << 64) if u >> 63 else u) / 2.0 ** 64
 
 
+def test_rope_amp_that_fp32_does_not_hold():
+    from rembed_amd import _lib as L
+    from rembed_amd import tensor as T
+    big = float(np.finfo(np.float32).max)
+    assert T.rope_frequencies(8, amp=big)[1] == big
+    for amp in (2.0 ** 128, 1e300):
+        with pytest.raises(L.RembedError):
+            T.rope_frequencies(8, amp=amp)
+
+
 @pytest.mark.gpu
 def test_rope_of_given_frequencies_of_any_size(gpu_ctx):
     """Angles within 2^-31 of a turn at every position: a sine near a whole turn shows them. Sine and
