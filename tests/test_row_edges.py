@@ -10,6 +10,7 @@ import pytest
 import fp8_oracle as O
 import row_oracle as R
 import test_fp8_operators as F
+import test_row_operators as W
 
 I32 = np.int32
 
@@ -330,3 +331,205 @@ def test_rope_append_norms_a_head_by_one_factor(gpu_ctx, dh, kv, parts):
     assert (codes == codes[:, :, :1]).all()
     below = (codes[:, :, 0, 0] != codes[:, :, 0, 7]).mean()
     assert below > 0.5            # the border is among them
+
+
+# ---- GPU: many heads at document sizes -----------------------------------------------------
+
+# rows, heads, kv, dh, rot, layout, dtype, out, in place, normed. Four heads a thread from heads * threads a head
+# * rows = 2^19 on (value by value: from 8192 heads), the heads no multiple of four in most.
+MANY = [
+    (3000, 16, 8, 128, 128, 0, "bf16", "bf16", False, True), (5100, 5, 4, 128, 64, 1, "bf16", "f32", False, True),
+    (2100, 9, 4, 128, 128, 0, "f32", "bf16", False, False), (2600, 9, 4, 128, 32, 0, "f32", "f32", True, True),
+    (9500, 9, 5, 64, 64, 1, "bf16", "bf16", True, True), (3300, 11, 5, 64, 32, 0, "f32", "f32", False, True),
+    (9100, 17, 6, 32, 32, 0, "bf16", "bf16", False, False), (5600, 4, 1, 256, 128, 0, "bf16", "bf16", False, True),
+    (2800, 3, 2, 256, 256, 1, "f32", "bf16", False, True),
+    # odd heads: runs of 8, 4 and 2 values, and value by value
+    (9400, 5, 2, 80, 80, 0, "bf16", "bf16", True, True), (3400, 5, 4, 72, 72, 0, "bf16", "f32", False, False),
+    (2100, 5, 2, 96, 50, 1, "bf16", "bf16", False, True), (2400, 5, 2, 36, 20, 0, "f32", "f32", True, True),
+    (1100, 5, 2, 36, 18, 0, "bf16", "bf16", False, True), (1200, 6, 1, 254, 250, 0, "f32", "bf16", False, True),
+    (1250, 5, 2, 254, 250, 0, "bf16", "bf16", True, False),
+]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("i", range(len(MANY)), ids=lambda i: "%dx%d+%d-%d-%d-%d-%s-%s" % MANY[i][:8])
+def test_rope_rows_of_many_heads(gpu_ctx, i):
+    """Every q and k head of every row against 64 bits, v's copied (in place: left), what lies around
+    the heads left as it was."""
+    from rembed_amd import tensor as T
+    rows, heads, kv, dh, rot, layout, dtype, out, place, normed = MANY[i]
+    rng = np.random.default_rng(100 + i)
+    front, nh = 8, heads + 2 * kv
+    ld = front + nh * dh + 8
+    x = rng.standard_normal((rows, ld)) * np.exp(rng.uniform(-3, 3, (rows, 1)))
+    img, val = F.typed(x, dtype)
+    pos = rng.integers(0, 200000, rows).astype(I32)
+    w = [rng.uniform(0.5, 1.5, dh).astype(np.float32) for _ in "qk"]
+    norms = [T.Norm(gpu_ctx.upload(a), e) for a, e in zip(w, (1e-6, 1e-3))] if normed else [None, None]
+    rope = T.Rope(gpu_ctx, rot, layout=layout)
+    src = gpu_ctx.upload(img)
+    if place:
+        buf, read = src, lambda: (gpu_ctx.sync(), src.download(img.dtype, (rows, ld)))[1]
+    else:
+        buf, read = W.marked(gpu_ctx, rows + 1, ld, out == "bf16")
+    at_ = (front, front + heads * dh, front + (heads + kv) * dh)
+    T.RopeRows(gpu_ctx, rope, src, dtype == "bf16", ld, buf, out == "bf16", ld, *at_, heads, kv, dh,
+               gpu_ctx.upload(pos), rows, *norms)
+    if place:
+        bits = read()
+        got = F.from_bf16(bits) if dtype == "bf16" else bits
+        same = bits == img
+        assert same[:, :front].all() and same[:, at_[2]:].all()
+    else:
+        got, left = read()
+        assert left[rows:].all() and left[:, :front].all() and left[:, front + nh * dh:].all()
+        got = got[:rows]
+        v = val[:, at_[2]:front + nh * dh]
+        v = F.bf16(v)[0] if out == "bf16" else v
+        assert np.array_equal(got[:, at_[2]:front + nh * dh], v)
+    heads_of = lambda a: a[:, front:at_[2]].astype(np.float64).reshape(rows, heads + kv, dh)
+    W.check_heads(heads_of(got), heads_of(val), heads, kv, dh, rot, layout, {}, pos, w if normed else None,
+                  out == "bf16")
+
+
+# batch, lengths up to, cached before up to, heads, kv, dh, rot, layout, dtype, q in place. Threads of a token of heads of
+# 128: eight up to 512 blocks, then four; heads of a thread's q: four from heads * threads a head * rows = 2^19 on.
+APPENDS = [
+    (40, 12, 130, 16, 8, 128, 128, 0, "bf16", False),      # four threads a token, one head a thread
+    (7, 800, 90, 18, 8, 128, 128, 0, "bf16", False),       # four and four
+    (19, 160, 70, 17, 8, 128, 64, 1, "f32", False),
+    (9, 700, 100, 16, 8, 128, 128, 1, "bf16", True),
+    (4, 2100, 50, 11, 1, 128, 128, 0, "bf16", False),      # eight and four
+    (3, 3300, 70, 19, 2, 64, 64, 0, "bf16", False), (5, 1100, 0, 17, 3, 64, 32, 1, "f32", False),
+    (3, 2300, 40, 7, 1, 256, 256, 0, "bf16", False), (3, 1200, 300, 6, 2, 256, 64, 1, "f32", False),
+]
+
+
+def append_case(ctx, i, normed):
+    """A step behind cached beginnings: K and V as numbers, the cache before and after, q's rows."""
+    from rembed_amd import tensor as T
+    batch, most, before, heads, kv, dh, rot, layout, dtype, place = APPENDS[i]
+    rng = np.random.default_rng(200 + i)
+    fresh = rng.integers(most // 2 + 1, most + 1, batch)
+    fresh[0] = most
+    past = rng.integers(0, before + 1, batch)
+    rows = int(fresh.sum())
+    pages, table, _, _, _, _ = F.batch_of(rng, [0] * batch, past + fresh)
+    free = [int(table[b, j]) for b in range(batch)
+            for j in range(-(-past[b] // 64), -(-(past[b] + fresh[b]) // 64))]
+    cu, blk, _, slots, pos, _ = O.plan(past, fresh, free, table.copy(), rows + 2)
+    c = O.Cache(pages, kv, dh)
+    c.k, c.v = (rng.integers(0, 127, a.shape).astype(np.uint8) | rng.integers(0, 2, a.shape).astype(np.uint8) << 7
+                for a in (c.k, c.v))
+    c.k_exp, c.v_exp = (rng.integers(112, 124, a.shape).astype(np.uint8) for a in (c.k_exp, c.v_exp))
+    dev = F.device_cache(ctx, c)
+    width = (heads + 2 * kv) * dh + 8
+    x = rng.standard_normal((rows + 2, width)) * np.exp(rng.uniform(-2, 2, (rows + 2, 1)))
+    img, val = F.typed(x, dtype)
+    w = [rng.uniform(0.5, 1.5, dh).astype(np.float32) for _ in "qk"]
+    norms = [T.Norm(ctx.upload(a), e) for a, e in zip(w, (1e-6, 1e-3))] if normed else [None, None]
+    rope, src, bf = T.Rope(ctx, rot, layout=layout), ctx.upload(img), dtype == "bf16"
+    if place:
+        q, ldq, q_bf = W.At(src, 8 * img.itemsize), width, bf
+    else:
+        ldq, q_bf = heads * dh + 8, True
+        q, read = W.marked(ctx, rows + 2, ldq, True)
+    T.RopeAppend(ctx, rope, dev, src, bf, width, 8, 8 + heads * dh, 8 + (heads + kv) * dh, q, q_bf, ldq, heads,
+                 ctx.upload(pos), ctx.upload(cu), ctx.upload(blk), ctx.upload(slots), batch, rows + 2, *norms)
+    ctx.sync()
+    if place:
+        bits = src.download(img.dtype, img.shape)
+        assert np.array_equal(bits[rows:], img[rows:]) and np.array_equal(bits[:, :8], img[:, :8])
+        assert np.array_equal(bits[:, 8 + heads * dh:], img[:, 8 + heads * dh:])
+        got = F.from_bf16(bits)[:rows, 8:8 + heads * dh]
+    else:
+        got, left = read()
+        assert left[rows:].all() and left[:, heads * dh:].all()
+        got = got[:rows, :heads * dh]
+    val = val[:rows, 8:].astype(np.float64).reshape(rows, -1, dh)
+    W.check_heads(got.reshape(rows, heads, dh), val[:, :heads], heads, 0, dh, rot, layout, {}, pos[:rows],
+                  w if normed else None, q_bf)
+    k, off = val[:, heads:heads + kv], np.zeros((rows, kv, dh))
+    if normed:
+        k, off = R.head_norm(k, w[1], 1e-3)
+    k, off = R.turn(k, off, pos[:rows], *R.frequencies(rot), layout == 0)
+    check_appended(dev, c, k, off, val[:, heads + kv:], cu, slots)
+
+
+def check_appended(dev, c, k, off, v, cu, slots):
+    """The device's cache is c with K (each within `off`) and V appended: V's bytes, scales of K that its
+    largest value can have, codes of K that its values can have, kept codes and zeros exactly."""
+    before = [a.copy() for a in (c.k, c.k_exp)]
+    c.append(k, v, cu, slots)
+    assert np.array_equal(dev.v.download(np.uint8, c.v.shape) & 127 != 0, c.v & 127 != 0)
+    assert np.array_equal(O.CODES[dev.v.download(np.uint8, c.v.shape)], O.CODES[c.v])
+    assert np.array_equal(dev.v_exp.download(np.uint8, c.v_exp.shape), c.v_exp)
+    codes = dev.k.download(np.uint8, c.k.shape)[..., O.places(O.k_at, c.dh)]
+    exps = dev.k_exp.download(np.uint8, c.k_exp.shape).astype(np.int64)
+    old, old_exps = before[0][..., O.places(O.k_at, c.dh)], before[1].astype(np.int64)
+    touched = np.zeros(c.pages, bool)
+    differ = total = other = 0
+    for b in range(len(cu) - 1):
+        r = cu[b]
+        while r < cu[b + 1]:
+            page, at_ = divmod(int(slots[r]), 64)
+            n = min(64 - at_, cu[b + 1] - r)
+            touched[page] = True
+            x, o = k[r:r + n].transpose(1, 0, 2), off[r:r + n].transpose(1, 0, 2)
+            lo, hi = (np.abs(x) - o).clip(0).max((1, 2)), (np.abs(x) + o).max((1, 2))
+            e = exps[page]
+            floor = old_exps[page] if at_ else 0
+            assert (np.maximum(O.exponent(lo), floor) <= e).all() and (e <= np.maximum(O.exponent(hi), floor)).all()
+            other += (e != np.maximum(O.exponent(np.abs(x).max((1, 2))), floor)).sum()
+            s = O.two(e)[:, None, None]
+            got = O.CODES[codes[page][:, at_:at_ + n]]
+            value = lambda y: O.CODES[O.encode(np.clip(y / s, -448, 448))]
+            assert (value(x - o) <= got).all() and (got <= value(x + o)).all()
+            differ += (got != value(x)).sum()
+            total += got.size
+            kept = np.zeros((c.heads, 64, c.dh))
+            if at_:
+                kept = O.CODES[O.encode(O.CODES[old[page]] * O.two(127 + floor - e)[:, None, None])]
+            rest = np.r_[0:at_, at_ + n:64]
+            assert np.array_equal(O.CODES[codes[page][:, rest]], kept[:, rest])
+            r += n
+    assert np.array_equal(codes[~touched], old[~touched]) and np.array_equal(exps[~touched], old_exps[~touched])
+    # values of up to 30 u beside a border, of which there is one in 2^-4 of a value: 2 * 30 u / 2^-4 = 6e-5
+    assert differ <= 6e-5 * total + 3 and other <= 1
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("normed", [False, True])
+@pytest.mark.parametrize("i", range(len(APPENDS)), ids=lambda i: "%dx%d+%d-%dx%d-%d-%d-%d-%s" % APPENDS[i][:9])
+def test_rope_append_of_many(gpu_ctx, i, normed):
+    append_case(gpu_ctx, i, normed)
+
+
+# ---- GPU: row offsets that are none ----------------------------------------------------------
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("out", ["bf16", "f32"])
+def test_cache_read_of_row_offsets_that_are_none(gpu_ctx, out):
+    """Requests whose offsets fall, begin before the rows or end behind them write nothing; the
+    others write exactly their rows."""
+    from rembed_amd import tensor as T
+    rng = np.random.default_rng(6)
+    rows, guard, dh = 40, 30, 64
+    c, dev = W.filled(rng, gpu_ctx, 4, 1, dh)
+    c.k, c.v = c.k & 0x77, c.v & 0x77                # no NaN
+    dev = F.device_cache(gpu_ctx, c)
+    table = gpu_ctx.upload(np.array([[0], [1], [2], [3]], I32))
+    for cu, done in (([0, 0, 0, 0, rows + 1], []), ([9, 4, 4, 4, 4], []), ([0, -5, 10, 10, 10], []),
+                     ([-3, 5, 9, 9, 9], [(1, 5, 9)]), ([2, 7, 7, rows, rows + 20], [(0, 2, 7), (2, 7, rows)]),
+                     ([3, 8, rows + 1, rows + 1, rows + 5], [(0, 3, 8)]), ([0, 5, 5, 5, 5], [(0, 0, 5)])):
+        buf, read = W.marked(gpu_ctx, rows + guard, 2 * dh, out == "bf16")
+        T.CacheRead(gpu_ctx, dev, table, 1, gpu_ctx.upload(np.array(cu, I32)), None, 4, rows, buf, out == "bf16",
+                    2 * dh, 0, dh)
+        got, left = read()
+        written = np.zeros(rows + guard, bool)
+        for b, lo, hi in done:
+            written[lo:hi] = True
+            for x, col in zip(c.rows([b], hi - lo), (0, dh)):
+                want = x[:, 0] if out == "f32" else F.bf16(x[:, 0])[0]
+                assert np.array_equal(got[lo:hi, col:col + dh], want.astype(np.float32)), cu
+        assert left[~written].all(), cu
