@@ -395,12 +395,13 @@ int rh_cache_attention(rh_context *ctx, const void *q, int q_bf16, int ldq, int 
  * What a decoder layer on the operators above runs around its linears and its attention.
  * Like them, none of these calls allocates or waits (rh_rope_create apart), and each may be
  * captured into a HIP graph. Arithmetic is fp32 on unrounded values, with one rounding where a
- * value is stored (rows or heads whose squares sum to 2^128 and more become 0 in a norm). `used` may
- * name a device integer (a plan's cu + batch, status + 1): rows from it on are left as they
- * are; NULL: all rows are taken. An output may lie exactly on an input of its own type and
- * stride, as said; one on other bytes that the call reads or writes (rows, gates, norms' weights,
- * positions, tables, `used`, the cache) is refused. Rows and columns have no alignment beyond
- * their type's unless said; 16-byte aligned rows of whole 16-byte groups are read faster. */
+ * value is stored (in a norm, rows or heads whose squares sum to 2^128 and more become 0, and with
+ * eps 0 those whose squares all round to 0 become infinite or NaN, as zeros do). `used` may name
+ * a device integer (a plan's cu + batch, status + 1): rows from it on are left as they are; NULL:
+ * all rows are taken. An output may lie exactly on an input of its own type and stride, as said;
+ * one on other bytes that the call reads or writes (rows, gates, norms' weights, positions, tables,
+ * `used`, the cache) is refused. Rows and columns have no alignment beyond their type's unless
+ * said; 16-byte aligned rows of whole 16-byte groups are read faster. */
 
 /* A norm of rows or heads: v * weight / sqrt(mean(v^2) + eps) (RMSNorm, tensor.go:459-471), or
  * (v - mean) * weight / sqrt(var + eps) + bias with the biased variance (LayerNorm,
@@ -468,7 +469,8 @@ typedef struct {
 } rh_rope_config;
 /* f_i [rot/2] and amp, on the host (either may be NULL). */
 int rh_rope_frequencies(const rh_rope_config *cfg, double *freq, double *amp);
-/* A turn's frequencies in HBM, used with the context that made it. */
+/* A turn's frequencies in HBM, used with the context that made it; kept as long as graphs that
+ * hold its calls are replayed. */
 typedef struct rh_rope rh_rope;
 int rh_rope_create(rh_context *ctx, const rh_rope_config *cfg, rh_rope **out);
 void rh_rope_destroy(rh_rope *rope);

@@ -7,7 +7,10 @@
 // Statistics are fp32 sums over values in registers, the layer norm's variance around its mean; s
 // reaches `pre` unrounded, whatever type it is stored in, and codes are those of fp32 values.
 // Every row is read and written once: 8192 rows of 4096, 235 MB, take 48 µs, 4.9 TB/s; 2111 of 768
-// 4.9, of which a launch is 4.0; odd rows (1213 of 1001) 6.2.
+// 4.9, of which a launch is 4.0; odd rows (1213 of 1001) 6.1. Rows of over 8192 values have two chunks
+// a thread, whose registers (86 to 113) leave a CU one workgroup: nothing else is loaded while a row is
+// summed, and 2048 rows of 16384 (235 MB, e4m3 out) take 56 µs, 4.2 TB/s, 1024 fp32 rows of 12288 with a
+// norm on both sides (201 MB) 50, 4.0 TB/s.
 // Covers what the model forwards do in passes of their own (Add and the norms, tensor.go:383-387,
 // 433-471; Gemma's post-norms, gemma3.go:357,376).
 #include "rowops.h"

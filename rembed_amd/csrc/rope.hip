@@ -6,7 +6,7 @@
 // model forwards here have a pass of their own for that (kernels_dec.hip).
 //
 // Every value is read and written once, and that bounds it: 16384 rows of 16 + 8 heads of 128, 201
-// MB of bf16, take 36.8 µs, 5.5 TB/s (vector units 45 % busy); 48 rows 4.5, a launch.
+// MB of bf16, take 37 µs, 5.4 TB/s (vector units 45 % busy); 48 rows 4.5, a launch.
 #include "rope_rows.h"
 
 #include <algorithm>
@@ -142,8 +142,8 @@ static void launch_any(const RopeArgs& a, hipStream_t s) {
 }
 
 // The widest run of values that both the pairs and the head are whole numbers of: 16 bytes (8 or 4
-// values), half or a quarter of that. 4096 rows of 16 + 4 heads of 80, bf16: 22.6 µs a value at a
-// time, 8.8 in runs of 8; the leading 20 of 128 turning: 18.5, 11.9 in runs of 2.
+// values), half or a quarter of that. 4096 rows of 16 + 4 heads of 80, bf16, normed: 22.7 µs a value
+// at a time, 9.0 in runs of 8; heads of 128 whose leading 20 turn, not normed: 18.5, 12.1 in runs of 2.
 template <bool XB, bool OB>
 static void launch_types(const RopeArgs& a, hipStream_t s) {
   constexpr int P = XB ? 8 : 4;

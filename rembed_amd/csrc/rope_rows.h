@@ -42,7 +42,8 @@ struct RopeShare {
 // Four heads a thread, whose cosines it then reads once and whose loads are in flight together, where
 // two workgroups a CU remain (16384 rows of 24 heads of 128: 36.8 µs, with one head a thread 42.2;
 // begun at half as many rows, 2000 take 7.5 for 6.0, at twice as many 3000 take 9.0 for 9.2 and 1500
-// in fp32 8.5 for 8.1); as many rows as fill the workgroup's threads and as far as their cosines
+// in fp32 8.5 for 8.1), counted with the lanes that hold no values (heads of 80 have some in five of
+// eight, so they begin at five eighths of the work); as many rows as fill the workgroup's threads and as far as their cosines
 // fit, and slices of one size where a row is more than a workgroup.
 inline RopeShare rope_share(const RopeArgs& a, int lanes, int most_dh, int threads) {
   const long long nh = std::max(1LL, (long long)a.heads + a.kv_heads + a.v_heads);

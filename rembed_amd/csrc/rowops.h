@@ -134,8 +134,9 @@ __device__ __forceinline__ uint32_t turn_at(const RopeFreq& f, int t) {
 // cos and sin of a fraction of a turn: of its distance t from the nearest quarter, at most 1/8
 // turn, by polynomials in t whose largest error is least (found by exchange; sin 1.8e-9, cos
 // 5.4e-11; 2 pi in two parts, so that the angle itself is not rounded again), then the quarter's
-// exchange and signs. Off by at most 7.2e-8 before amp, 2e-8 in the mean: K's codes flip between
-// two values no more often than an exact angle's would.
+// exchange and signs. Over all fractions of a turn the cosine is off by at most 7.6e-8 before amp, the
+// sine by 6.1e-8, both by 1.4e-8 in the mean: K's codes flip between two values no more often than
+// those of cosines in 64 bits, rounded.
 __device__ __forceinline__ void turn_cos_sin(uint32_t turn, float amp, float& c, float& s) {
   const uint32_t u = turn + 0x20000000u;  // its upper two bits: the quarter
   const float t = (float)(int)(turn << 2) * 0x1p-34f;
