@@ -250,8 +250,8 @@ hipError_t launch_cache_plan(const CachePlanArgs& a, hipStream_t s) {
 // reach queries that must not see it through V). It sets no scale.
 // Single tokens are bound by latency, so a request is found by a 64-way search (one load of
 // a wave per level; a binary search took 3 µs of 7.6 for 48 requests) and its rows are
-// asked for once its first slot is there, before their page's scales: 48 single tokens of 8 heads of 128
-// take 5.5 µs. Many
+// asked for once its first slot is there, before their page's scales: 48 single tokens of 8 heads of
+// 128 take 5.5 µs. Many
 // tokens are bound by their bytes: 22k tokens, 140 MB, take 28.6 µs, 4.9 TB/s, what a large copy
 // reaches (a thread's loads one after the other in a row instead of 64 bytes by four threads:
 // 30.7; stores that stay in the L2: 36.2).
@@ -704,8 +704,9 @@ hipError_t launch_cache_append(const CacheAppendArgs& a, hipStream_t s) {
 
 // ---- read back --------------------------------------------------------------------------
 // Bound by its bytes: 76.7k tokens of 8 heads of 128, 471 MB, take 94 µs, 5.0 TB/s, as fp32 rows, 785
-// MB, 147; of 4 heads of 256 96 and 150; 640 tokens 4.0, a launch. A workgroup takes one block of a request and one kv head: the block's tokens among
-// first[b] .. first[b] + count - 1 go to rows cu[b] + position - first[b]. K's 16-byte pieces are
+// MB, 147; of 4 heads of 256 96 and 150; 640 tokens 4.0, a launch. A workgroup takes one block of a
+// request and one kv head: the block's tokens among first[b] .. first[b] + count - 1 go to rows
+// cu[b] + position - first[b]. K's 16-byte pieces are
 // runs of a token's values; V's are 16 tokens of one column, so its block goes through LDS
 // (16 more bytes behind every 128: a wave's words then meet all banks) and a thread takes
 // eight columns (four of fp32 rows) of four tokens. A code times its power of two is exact in fp32, and in bf16 from

@@ -194,7 +194,8 @@ def test_rotary_rows_beside_what_they_read(gpu_ctx):
                    norm, norm, At(place, 2 * ld + 2 * dh + 5))
         gpu_ctx.sync()
         got.append(buf.download(np.uint32, (n, ld)))
-        assert np.array_equal(got[-1][:, 2 * dh:], host.view(np.uint32)[:, 2 * dh:]) and not got[-1][n - 1, :2 * dh].any()
+        assert np.array_equal(got[-1][:, 2 * dh:], host.view(np.uint32)[:, 2 * dh:])
+        assert not got[-1][n - 1, :2 * dh].any()
     assert np.array_equal(*got) and got[0][:n - 1, :2 * dh].any(1).all()
 
 
@@ -268,9 +269,9 @@ def test_rope_of_given_frequencies_of_any_size(gpu_ctx):
     rng = np.random.default_rng(0)
     pi = machin()
     assert abs(pi / (1 << BITS) - np.pi) < 1e-15
-    freq = [0.0, 5e-324, 1e-30, 2.0 ** -40, 0.37, 1.0, np.pi, 2 * np.pi, 50.0, -50.0, 1e3, -12345.678, 1e6, 2.0 ** 53,
-            1e16, -3e18, 2.0 ** 63, 2.0 ** 64, 1e20, -1e25, 1e30, 1.7e38, 2.0 ** 127, 1e50, -1e77, 1e100, 1e150, 2.0 ** 640,
-            1e200, -1e250, 1e300, np.finfo(np.float64).max]
+    freq = [0.0, 5e-324, 1e-30, 2.0 ** -40, 0.37, 1.0, np.pi, 2 * np.pi, 50.0, -50.0, 1e3, -12345.678, 1e6,
+            2.0 ** 53, 1e16, -3e18, 2.0 ** 63, 2.0 ** 64, 1e20, -1e25, 1e30, 1.7e38, 2.0 ** 127, 1e50, -1e77,
+            1e100, 1e150, 2.0 ** 640, 1e200, -1e250, 1e300, np.finfo(np.float64).max]
     n, dh = len(freq), 2 * len(freq)
     pos = np.concatenate([[0, 1, -1, 2, 2 ** 31 - 1, -2 ** 31], rng.integers(-2 ** 31, 2 ** 31, 2000)])
     # those whose angle of one of the frequencies is next to a whole turn, and some others
@@ -392,8 +393,9 @@ def test_rope_rows_of_many_heads(gpu_ctx, i):
                   out == "bf16")
 
 
-# batch, lengths up to, cached before up to, heads, kv, dh, rot, layout, dtype, q in place. Threads of a token of heads of
-# 128: eight up to 512 blocks, then four; heads of a thread's q: four from heads * threads a head * rows = 2^19 on.
+# batch, lengths up to, cached before up to, heads, kv, dh, rot, layout, dtype, q in place. Threads of a
+# token of heads of 128: eight up to 512 blocks, then four; heads of a thread's q: four from
+# heads * threads a head * rows = 2^19 on.
 APPENDS = [
     (40, 12, 130, 16, 8, 128, 128, 0, "bf16", False),      # four threads a token, one head a thread
     (7, 800, 90, 18, 8, 128, 128, 0, "bf16", False),       # four and four
